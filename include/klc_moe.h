@@ -479,6 +479,79 @@ int klc_attn_step(const klc_attn_step_args* args, void* stream);
  * limit_us microseconds have passed (0). */
 int klc_attn_step_wait(const void* host_record, int64_t tag, int64_t limit_us);
 
+/* ---- Attention of many sequences ---------------------------------------------
+ * Serving several requests at once: prompts in one pass, a paged cache that
+ * sequences share, a decode batch that reads it.  No counterpart in the
+ * reference, which feeds a prompt token by token through one sequence's cache
+ * (streamed_attention.py:101-152); the mathematics, sinks and window are that
+ * call's.  The cache's pools are [n_pages][page_size][n_kv][head_dim] of
+ * kv_dtype (KLC_DTYPE_F16 or KLC_DTYPE_BF16), page_size a power of two from
+ * 16 to 4096; slot i is token i % page_size of page i / page_size.  head_dim
+ * is a multiple of 8 up to 128; query head h reads KV head h / (n_heads / n_kv). */
+
+/* Causal attention of whole prompts, packed one behind the other: sequence s
+ * is tokens starts[s] up to starts[s + 1] (int32 [n_seq + 1], ascending, on the
+ * device; clamped to [0, tokens]) of q [tokens][n_heads][head_dim], k and v
+ * [tokens][n_kv][head_dim], all of `dtype`; token strides in elements
+ * (multiples of 8), heads contiguous.  Token i of a sequence sees its keys
+ * max(0, i - window + 1)..i (window 0: all up to i); softmax of scale * q . k
+ * over them and, if sinks (bfloat16 [n_heads]) is not NULL, the sink logit,
+ * which has no value.  Scores, statistics and sums are float32; probabilities
+ * are rounded to `dtype` before the value product, which the sum of the
+ * rounded ones normalises.  Rows of out [tokens][n_heads][head_dim] outside
+ * every sequence are not written.  What a row must not see does not reach it,
+ * NaN and infinities included.  q, k, v and out 16-byte aligned; tokens *
+ * n_heads / n_kv < 2^30. */
+int klc_attn_prompt(const void* q, const void* k, const void* v, const int32_t* starts, const void* sinks,
+                    int64_t tokens, int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t q_stride,
+                    int64_t k_stride, int64_t v_stride, int64_t window, float scale, int dtype, void* out,
+                    void* stream);
+
+/* Rotation and append of `tokens` tokens (klc_rope_append for many): bfloat16
+ * q, k, v rows as in klc_attn_prompt; the token at position p is rotated by
+ * row p of cos_half / sin_half (bfloat16 [n_positions][head_dim / 2]), in
+ * float32 with one rounding (klc_rope_append rounds every bfloat16 operation),
+ * and its key and value are stored to slot slots[t] of k_pages / v_pages.
+ * q_out [tokens][n_heads][head_dim] and, if not NULL, k_out
+ * [tokens][n_kv][head_dim] receive the rotated rows in bfloat16.  A slot
+ * outside [0, n_slots) stores nothing; a position outside [0, n_positions)
+ * gives NaN.  Slots of one call are distinct. */
+int klc_kv_append(const void* q, const void* k, const void* v, const void* cos_half, const void* sin_half,
+                  const int32_t* positions, const int32_t* slots, int64_t tokens, int64_t n_positions,
+                  int64_t n_slots, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t q_stride,
+                  int64_t k_stride, int64_t v_stride, int kv_dtype, void* q_out, void* k_out, void* k_pages,
+                  void* v_pages, void* stream);
+
+/* Copies page src[i] to page dst[i] in each of n_pools pools (consecutive,
+ * each n_pages pages of page_bytes, a multiple of 16) for i < n: the forks and
+ * the compaction of a paged cache.  src and dst are HOST arrays, read before
+ * the call returns; no destination may be another move's source or
+ * destination (the moves run at once). */
+int klc_kv_copy_pages(void* pools, int64_t n_pools, int64_t n_pages, int64_t page_bytes, const int32_t* src,
+                      const int32_t* dst, int64_t n, void* stream);
+
+/* Attention of one token of each of n_seq sequences over pages.  Sequence b's
+ * keys are the first prefix_len tokens of the pages in prefix_table (int32
+ * [ceil(prefix_len / page_size)]; the same for every sequence, read once for
+ * all of them) and then lengths[b] (int32) tokens of its own, in the pages of
+ * row b of tables (int32 [n_seq][table_width]); the token itself is the last.
+ * It sees the last `window` of them (0: all).  q rows are bfloat16
+ * [n_heads][head_dim], q_stride elements apart; softmax as klc_attn_prompt,
+ * probabilities rounded to kv_dtype; out [n_seq][n_heads][head_dim] bfloat16.
+ * lengths[b] < 0: no sequence, zeros.  A page number outside [0, n_pages) or a
+ * length past table_width * page_size makes the sequence's output NaN (of the
+ * prefix: every sequence's); nothing outside the pools is read.  n_heads / n_kv <= 32, n_seq <= 65535.
+ * workspace: klc_attn_batch_workspace_bytes with max_own = table_width *
+ * page_size, 16-byte aligned, no initialisation; calls that may overlap need
+ * one each. */
+int64_t klc_attn_batch_workspace_bytes(int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t head_dim,
+                                       int64_t prefix_len, int64_t max_own, int64_t window);
+int klc_attn_batch(const void* q, const void* k_pages, const void* v_pages, const int32_t* tables,
+                   const int32_t* lengths, const int32_t* prefix_table, const void* sinks, int64_t n_seq,
+                   int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t q_stride, int64_t n_pages,
+                   int64_t page_size, int64_t table_width, int64_t prefix_len, int64_t window, float scale,
+                   int kv_dtype, void* workspace, int64_t workspace_bytes, void* out, void* stream);
+
 /* ---- Synthetic inputs -------------------------------------------------------
  * Counter-based SplitMix64 stream, identical to klcquant_amd/synth.py:
  * mode 0: n random bytes; mode 1: n bytes uniform in [lo, hi]. */

@@ -12,6 +12,7 @@ import ctypes
 import math
 from typing import NamedTuple
 
+import numpy as np
 import torch
 
 from . import _native as nat
@@ -282,6 +283,211 @@ def pair_norms(gated: torch.Tensor, expert_out: torch.Tensor) -> torch.Tensor:
 
 def workspace_bytes(n_tokens: int, hidden: int, inter: int, n_experts: int, k: int) -> int:
     return nat.call("klc_moe_workspace_bytes", n_tokens, hidden, inter, n_experts, k)
+
+
+# ---- Attention of many sequences ---------------------------------------------------
+
+_KV_CODES = {torch.bfloat16: nat.DTYPE_BF16, torch.float16: nat.DTYPE_F16}
+
+
+def _check_rows(name: str, t: torch.Tensor, dtype: torch.dtype, dev: torch.device) -> int:
+    """``[tokens, heads, head_dim]`` with contiguous heads, a view of a wider row allowed; the token stride."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} must be on a GPU device (there is no CPU implementation), got {t.device}")
+    if t.device != dev:
+        raise ValueError(f"tensors on different devices: {dev} vs {t.device}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != 3 or 0 in t.shape[1:]:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim], got shape {tuple(t.shape)}")
+    _, heads, dim = t.shape
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires grad: this operator has no backward pass")
+    stride = t.stride(0) if t.shape[0] > 1 else heads * dim
+    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim) or stride < heads * dim or stride % 8:
+        raise ValueError(f"{name} needs contiguous heads and a token stride that is a multiple of 8, got strides {t.stride()}")
+    return stride
+
+
+def _check_index(name: str, t: torch.Tensor, ndim: int, dev: torch.device) -> None:
+    _check_gpu(name, t, torch.int32, ndim)
+    if t.device != dev:
+        raise ValueError(f"tensors on different devices: {dev} vs {t.device}")
+
+
+def _check_heads(dev: torch.device, sinks: torch.Tensor | None, n_heads: int, n_kv: int, window: int | None,
+                 scale: float | None, dim: int) -> tuple[int, float]:
+    if n_heads % n_kv:
+        raise ValueError(f"{n_heads} query heads over {n_kv} KV heads")
+    if sinks is not None:
+        _check_gpu("sinks", sinks, torch.bfloat16, 1)
+        if sinks.shape[0] != n_heads or sinks.device != dev:
+            raise ValueError(f"sinks must be [{n_heads}] on {dev}, got {tuple(sinks.shape)} on {sinks.device}")
+        if sinks.requires_grad and torch.is_grad_enabled():
+            raise ValueError("sinks require grad: this operator has no backward pass")
+    if window is not None and window <= 0:
+        raise ValueError(f"window must be positive (None: no window), got {window}")
+    return min(int(window), (1 << 30) - 1) if window else 0, float(scale) if scale is not None else 1.0 / math.sqrt(dim)
+
+
+def _check_out(name: str, out: torch.Tensor | None, shape: tuple, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    _check_gpu(name, out, dtype)
+    if tuple(out.shape) != tuple(shape) or out.device != dev:
+        raise ValueError(f"{name} must be {tuple(shape)} on {dev}, got {tuple(out.shape)} on {out.device}")
+    return out
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor,
+                     sinks: torch.Tensor | None = None, window: int | None = None, scale: float | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of packed prompts (klc_attn_prompt): ``q [T, n_heads, D]``, ``k``, ``v [T, n_kv, D]``, all
+    bfloat16 or all float16 (views with contiguous heads too, such as splits of one projection), sequence ``s`` =
+    tokens ``starts[s]:starts[s + 1]`` (int32 ``[S + 1]`` on the device, ascending) -> ``[T, n_heads, D]``.  A token
+    sees the last ``window`` tokens up to itself (None: all); ``sinks`` bf16 ``[n_heads]``; ``scale`` 1 / sqrt(D)
+    unless given.  Rows outside every sequence are left as ``out`` had them."""
+    if not isinstance(q, torch.Tensor):
+        raise TypeError(f"q must be a torch.Tensor, got {type(q).__name__}")
+    dev, dtype = q.device, q.dtype
+    if dtype not in _KV_CODES:
+        raise TypeError(f"q must be bfloat16 or float16, got {dtype}")
+    strides = [_check_rows(n, t, dtype, dev) for n, t in (("q", q), ("k", k), ("v", v))]
+    tokens, n_heads, dim = q.shape
+    n_kv = k.shape[1]
+    if k.shape != (tokens, n_kv, dim) or v.shape != k.shape:
+        raise ValueError(f"shapes mismatch: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    _check_index("starts", starts, 1, dev)
+    if starts.shape[0] < 1:
+        raise ValueError("starts must hold the sequences' starts and the end of the last one")
+    window, scale = _check_heads(dev, sinks, n_heads, n_kv, window, scale, dim)
+    out = _check_out("out", out, (tokens, n_heads, dim), dtype, dev)
+    if tokens == 0 or starts.shape[0] == 1:
+        return out
+    with torch.cuda.device(dev):
+        nat.call("klc_attn_prompt", _ptr(q), _ptr(k), _ptr(v), _ptr(starts), _ptr(sinks), tokens, starts.shape[0] - 1,
+                 n_heads, n_kv, dim, *strides, window, scale, _KV_CODES[dtype], _ptr(out), _stream(dev))
+    return out
+
+
+def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, dev: torch.device) -> tuple[int, int, int, int]:
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        _check_gpu(name, t, None, 4)
+        if t.dtype not in _KV_CODES:
+            raise TypeError(f"{name} must be bfloat16 or float16, got {t.dtype}")
+    if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+        raise ValueError(f"page pools mismatch: {k_pages.dtype} {tuple(k_pages.shape)}, {v_pages.dtype} {tuple(v_pages.shape)}")
+    if k_pages.device != dev or v_pages.device != dev:
+        raise ValueError(f"tensors on different devices: {dev} vs {k_pages.device}, {v_pages.device}")
+    n_pages, page, n_kv, dim = k_pages.shape
+    if n_pages == 0 or page < 16 or page > 4096 or page & (page - 1):
+        raise ValueError(f"pages must hold a power of two of tokens, 16 to 4096, got {n_pages} of {page}")
+    return n_pages, page, n_kv, dim
+
+
+def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                 positions: torch.Tensor, slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                 want_keys: bool = True):
+    """Rotates bf16 ``q [T, n_heads, D]`` and ``k [T, n_kv, D]`` by rows ``positions`` of the bf16 tables ``cos`` and
+    ``sin [n, D / 2]`` and stores the keys and ``v [T, n_kv, D]`` to ``slots`` (int32 ``[T]``, distinct; page * page
+    size + offset, negative: stored nowhere) of the pools ``[n_pages, page, n_kv, D]`` (klc_kv_append).  Returns the
+    rotated bf16 ``(q, k)``, ``k`` None unless ``want_keys``."""
+    if not isinstance(q, torch.Tensor):
+        raise TypeError(f"q must be a torch.Tensor, got {type(q).__name__}")
+    dev = q.device
+    strides = [_check_rows(n, t, torch.bfloat16, dev) for n, t in (("q", q), ("k", k), ("v", v))]
+    tokens, n_heads, dim = q.shape
+    n_pages, page, n_kv, page_dim = _check_pages(k_pages, v_pages, dev)
+    if k.shape != (tokens, n_kv, dim) or v.shape != k.shape or page_dim != dim:
+        raise ValueError(f"shapes mismatch: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, pages {tuple(k_pages.shape)}")
+    for name, t in (("cos", cos), ("sin", sin)):
+        _check_gpu(name, t, torch.bfloat16, 2)
+        if t.shape[1] * 2 != dim or t.shape != cos.shape or t.shape[0] == 0 or t.device != dev:
+            raise ValueError(f"{name} must be [positions, {dim // 2}] on {dev}, got {tuple(t.shape)} on {t.device}")
+    for name, t in (("positions", positions), ("slots", slots)):
+        _check_index(name, t, 1, dev)
+        if t.shape[0] != tokens:
+            raise ValueError(f"{name} of {t.shape[0]} tokens, not {tokens}")
+    q_out = torch.empty((tokens, n_heads, dim), dtype=torch.bfloat16, device=dev)
+    k_out = torch.empty((tokens, n_kv, dim), dtype=torch.bfloat16, device=dev) if want_keys else None
+    if tokens:
+        with torch.cuda.device(dev):
+            nat.call("klc_kv_append", _ptr(q), _ptr(k), _ptr(v), _ptr(cos), _ptr(sin), _ptr(positions), _ptr(slots),
+                     tokens, cos.shape[0], n_pages * page, n_heads, n_kv, dim, *strides, _KV_CODES[k_pages.dtype],
+                     _ptr(q_out), _ptr(k_out), _ptr(k_pages), _ptr(v_pages), _stream(dev))
+    return q_out, k_out
+
+
+def copy_pages(pools: torch.Tensor, src, dst) -> None:
+    """``pools[:, dst[i]] = pools[:, src[i]]`` for every i (klc_kv_copy_pages), for contiguous ``pools [n, n_pages,
+    ...]`` and page numbers on the host (sequences or int32 arrays).  The moves run at once: a destination is no other
+    move's source or destination."""
+    _check_gpu("pools", pools)
+    if pools.dim() < 3 or pools.numel() == 0:
+        raise ValueError(f"pools must be [pools, pages, ...], got shape {tuple(pools.shape)}")
+    src, dst = (np.ascontiguousarray(x, dtype=np.int64) for x in (src, dst))
+    if src.ndim != 1 or src.shape != dst.shape:
+        raise ValueError(f"source and destination pages mismatch: {src.shape} and {dst.shape}")
+    n_pages = pools.shape[1]
+    if not src.size:
+        return
+    if min(src.min(), dst.min()) < 0 or max(src.max(), dst.max()) >= n_pages:
+        raise ValueError(f"page numbers must be in [0, {n_pages})")
+    once = np.zeros(n_pages, dtype=bool)
+    once[dst] = True
+    if int(once.sum()) != dst.size or once[src].any():
+        raise ValueError("a destination page is another move's source or destination")
+    page_bytes = math.prod(pools.shape[2:]) * pools.element_size()
+    src, dst = src.astype(np.int32), dst.astype(np.int32)
+    with torch.cuda.device(pools.device):
+        nat.call("klc_kv_copy_pages", _ptr(pools), pools.shape[0], n_pages, page_bytes, ctypes.c_void_p(src.ctypes.data),
+                 ctypes.c_void_p(dst.ctypes.data), src.size, _stream(pools.device))
+
+
+def batch_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor,
+                    lengths: torch.Tensor, prefix_table: torch.Tensor | None = None, prefix_len: int = 0,
+                    sinks: torch.Tensor | None = None, window: int | None = None, scale: float | None = None,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one token of each of B sequences over pages (klc_attn_batch): bf16 ``q [B, n_heads, D]``; sequence
+    b's keys are the first ``prefix_len`` tokens of the pages ``prefix_table`` (int32, shared by all sequences and read
+    once) and then ``lengths[b]`` of the pages ``tables[b]`` (int32 ``[B, width]``), the token's own last.  ``lengths[b]
+    < 0``: no sequence, zeros.  Other arguments as :func:`prompt_attention`; returns bf16 ``[B, n_heads, D]``."""
+    if not isinstance(q, torch.Tensor):
+        raise TypeError(f"q must be a torch.Tensor, got {type(q).__name__}")
+    dev = q.device
+    stride = _check_rows("q", q, torch.bfloat16, dev)
+    count, n_heads, dim = q.shape
+    n_pages, page, n_kv, page_dim = _check_pages(k_pages, v_pages, dev)
+    if page_dim != dim:
+        raise ValueError(f"shapes mismatch: q {tuple(q.shape)}, pages {tuple(k_pages.shape)}")
+    _check_index("tables", tables, 2, dev)
+    _check_index("lengths", lengths, 1, dev)
+    if tables.shape[0] != count or lengths.shape[0] != count:
+        raise ValueError(f"tables {tuple(tables.shape)} and lengths {tuple(lengths.shape)} for {count} sequences")
+    prefix_len = int(prefix_len)
+    if prefix_len < 0:
+        raise ValueError(f"prefix_len must not be negative, got {prefix_len}")
+    if prefix_len:
+        if prefix_table is None:
+            raise ValueError("prefix_len without a prefix_table")
+        _check_index("prefix_table", prefix_table, 1, dev)
+        if prefix_table.shape[0] * page < prefix_len:
+            raise ValueError(f"prefix of {prefix_len} tokens in {prefix_table.shape[0]} pages of {page}")
+    window, scale = _check_heads(dev, sinks, n_heads, n_kv, window, scale, dim)
+    out = _check_out("out", out, (count, n_heads, dim), torch.bfloat16, dev)
+    if not count:
+        return out
+    width = tables.shape[1]
+    nbytes = nat.call("klc_attn_batch_workspace_bytes", count, n_heads, n_kv, dim, prefix_len, width * page, window)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        nat.call("klc_attn_batch", _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(tables if width else None), _ptr(lengths),
+                 _ptr(prefix_table if prefix_len else None), _ptr(sinks), count, n_heads, n_kv, dim, stride, n_pages,
+                 page, width, prefix_len, window, scale, _KV_CODES[k_pages.dtype], _ptr(workspace), nbytes, _ptr(out),
+                 _stream(dev))
+    return out
 
 
 def synth_fill(dst: torch.Tensor, seed: int, mode: int = 0, lo: int = 0, hi: int = 255) -> torch.Tensor:
