@@ -502,10 +502,15 @@ int klc_attn_step_wait(const void* host_record, int64_t tag, int64_t limit_us);
  * every sequence are not written.  What a row must not see does not reach it,
  * NaN and infinities included.  q, k, v and out 16-byte aligned; tokens *
  * n_heads / n_kv < 2^30. */
-int klc_attn_prompt(const void* q, const void* k, const void* v, const int32_t* starts, const void* sinks,
-                    int64_t tokens, int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t q_stride,
-                    int64_t k_stride, int64_t v_stride, int64_t window, float scale, int dtype, void* out,
-                    void* stream);
+typedef struct klc_attn_prompt_args {
+  const void *q, *k, *v;  /* [tokens][heads][head_dim] of dtype */
+  const void* starts;     /* int32 [n_seq + 1] */
+  const void* sinks;      /* bfloat16 [n_heads], or NULL */
+  void* out;
+  int64_t tokens, n_seq, n_heads, n_kv, head_dim, q_stride, k_stride, v_stride, window, dtype;
+  double scale;
+} klc_attn_prompt_args;
+int klc_attn_prompt(const klc_attn_prompt_args* args, void* stream);
 
 /* Rotation and append of `tokens` tokens (klc_rope_append for many): bfloat16
  * q, k, v rows as in klc_attn_prompt; the token at position p is rotated by
@@ -516,11 +521,13 @@ int klc_attn_prompt(const void* q, const void* k, const void* v, const int32_t* 
  * [tokens][n_kv][head_dim] receive the rotated rows in bfloat16.  A slot
  * outside [0, n_slots) stores nothing; a position outside [0, n_positions)
  * gives NaN.  Slots of one call are distinct. */
-int klc_kv_append(const void* q, const void* k, const void* v, const void* cos_half, const void* sin_half,
-                  const int32_t* positions, const int32_t* slots, int64_t tokens, int64_t n_positions,
-                  int64_t n_slots, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t q_stride,
-                  int64_t k_stride, int64_t v_stride, int kv_dtype, void* q_out, void* k_out, void* k_pages,
-                  void* v_pages, void* stream);
+typedef struct klc_kv_append_args {
+  const void *q, *k, *v, *cos_half, *sin_half;
+  const void *positions, *slots;  /* int32 [tokens] */
+  void *q_out, *k_out, *k_pages, *v_pages;
+  int64_t tokens, n_positions, n_slots, n_heads, n_kv, head_dim, q_stride, k_stride, v_stride, kv_dtype;
+} klc_kv_append_args;
+int klc_kv_append(const klc_kv_append_args* args, void* stream);
 
 /* Copies page src[i] to page dst[i] in each of n_pools pools (consecutive,
  * each n_pages pages of page_bytes, a multiple of 16) for i < n: the forks and
@@ -542,15 +549,20 @@ int klc_kv_copy_pages(void* pools, int64_t n_pools, int64_t n_pages, int64_t pag
  * length past table_width * page_size makes the sequence's output NaN (of the
  * prefix: every sequence's); nothing outside the pools is read.  n_heads / n_kv <= 32, n_seq <= 65535.
  * workspace: klc_attn_batch_workspace_bytes with max_own = table_width *
- * page_size, 16-byte aligned, no initialisation; calls that may overlap need
- * one each. */
+ * page_size (0: none needed), 16-byte aligned, no initialisation; calls that
+ * may overlap need one each. */
 int64_t klc_attn_batch_workspace_bytes(int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t head_dim,
                                        int64_t prefix_len, int64_t max_own, int64_t window);
-int klc_attn_batch(const void* q, const void* k_pages, const void* v_pages, const int32_t* tables,
-                   const int32_t* lengths, const int32_t* prefix_table, const void* sinks, int64_t n_seq,
-                   int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t q_stride, int64_t n_pages,
-                   int64_t page_size, int64_t table_width, int64_t prefix_len, int64_t window, float scale,
-                   int kv_dtype, void* workspace, int64_t workspace_bytes, void* out, void* stream);
+typedef struct klc_attn_batch_args {
+  const void *q, *k_pages, *v_pages;
+  const void *tables, *lengths, *prefix_table;  /* int32; tables may be NULL if table_width is 0, prefix_table if prefix_len is */
+  const void* sinks;
+  void *workspace, *out;
+  int64_t n_seq, n_heads, n_kv, head_dim, q_stride, n_pages, page_size, table_width, prefix_len, window, kv_dtype,
+      workspace_bytes;
+  double scale;
+} klc_attn_batch_args;
+int klc_attn_batch(const klc_attn_batch_args* args, void* stream);
 
 /* ---- Synthetic inputs -------------------------------------------------------
  * Counter-based SplitMix64 stream, identical to klcquant_amd/synth.py:

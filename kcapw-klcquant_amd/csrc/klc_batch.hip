@@ -1,11 +1,17 @@
 // Attention of a decode batch over a paged KV cache (gfx950): one token of
 // each sequence, whose first tokens may be a prefix that all sequences share.
 //
-// The prefix's keys are read once for the whole batch: its query rows are
-// (sequence, head of the group) pairs, many rows to a tile of keys, split
-// over the keys.  Each sequence's own keys are read by the workgroups of that
-// sequence.  Every part leaves its sum, maximum and normaliser in float32 and
-// a last kernel joins them.
+// One launch with two kinds of workgroups, so that the compute-bound prefix
+// and the sequences' own keys, a stream from HBM, share the chip:
+//   shared  a KV head, 128 query rows (sequence, head of the group) and a
+//           range of the prefix: 4 waves x 32 rows over one ring of tiles, the
+//           prefix's keys read once for the batch
+//   own     a KV head of one sequence and a range of its own keys (with a
+//           window, or a prefix not worth the pass above, of all its keys):
+//           its waves take tiles in turn, each through a ring of its own with
+//           no barrier, and join their sums in LDS
+// Parts are float32 (sum, maximum, normaliser) and a second launch joins
+// them; where a row has one part, the own workgroup writes the result itself.
 #include <math.h>
 
 #include "klc_flash.h"
@@ -13,13 +19,16 @@
 namespace klc {
 namespace {
 
-constexpr int kOwnTile = 32;      // keys of a tile of the sequences' own parts
-constexpr int kOwnRing = 3;
-constexpr int kSharedTile = 64;
-constexpr int kSharedRing = 3;
-constexpr int kSharedWaves = 4;
+constexpr int kWaves = 4;
+constexpr int kOwnTile = 32;      // keys of a tile of an own wave
+constexpr int kOwnRing = 2;
 constexpr int kBatchGroup = 32;   // most query heads of a KV head: the columns of a wave's matrix instruction
 constexpr int kPrefixAlign = 64;  // own keys start at a multiple of this in a sequence's list of keys
+// a shared tile is 16 KB of K and V, four of them the LDS of a head size of 64
+template <int DP>
+constexpr int kSharedTile = DP == 64 ? 64 : 32;
+template <int DP>
+constexpr int kBatchLds = kWaves * kOwnRing * 2 * kOwnTile * 2 * DP;
 
 struct BatchArgs {
   const uint16_t* q;                   // bfloat16 [n_seq] rows
@@ -31,7 +40,7 @@ struct BatchArgs {
   float* part_o;                       // [n_seq * n_heads][splits][d]
   float2* part_ml;                     // [n_seq * n_heads][splits]
   int64_t q_stride;
-  int n_seq, n_heads, n_kv, d, n_pages, page_log2, width, prefix, window, shared_splits, own_splits, shared_tiles;
+  int n_seq, n_heads, n_kv, d, n_pages, page_log2, width, prefix, window, shared_splits, own_splits, shared_tiles, shared_wgs;
   float c2;
 };
 
@@ -72,23 +81,6 @@ __device__ __forceinline__ float load_query(u32x4_t (&q)[F::kSteps], const uint1
   return ldexpf(1.f, ex);
 }
 
-template <int DP, int RB, class F>
-__device__ __forceinline__ void store_part(const BatchArgs& a, const F& f, int rb, int64_t row, int split, bool bad) {
-  const int lane = threadIdx.x % kWave, splits = a.shared_splits + a.own_splits;
-  const float sum = add_halves(f.l[rb]);
-  const int64_t at = row * splits + split;
-  if (lane < 32) a.part_ml[at] = make_float2(f.m[rb], bad ? __uint_as_float(0x7fc00000u) : sum);
-  float* dst = a.part_o + at * a.d + 4 * (lane / 32);
-#pragma unroll
-  for (int db = 0; db < F::kDimBlocks; ++db)
-#pragma unroll
-    for (int e = 0; e < 16; e += 4) {
-      const int dim = 32 * db + 2 * e;
-      if (dim + 4 * (lane / 32) >= a.d) continue;
-      *reinterpret_cast<float4*>(dst + dim) = make_float4(f.o[rb][db][e], f.o[rb][db][e + 1], f.o[rb][db][e + 2], f.o[rb][db][e + 3]);
-    }
-}
-
 // A lane's source row of a load instruction: `key` is the instruction's first
 // key (its rows lie in one page).  Keys outside the visible first..last take
 // the nearest visible one's row, so that only its pages are asked for.
@@ -123,16 +115,17 @@ __device__ __forceinline__ void clear_values(lds_u8 stage, int from, int to, int
   }
 }
 
-// The prefix's part: workgroup (KV head, tile of rows, split of the keys).
+// The prefix's part of 128 query rows: workgroup (KV head, tile of rows,
+// split of the keys).
 template <int DP, bool kF16, bool kFull>
-__global__ __launch_bounds__(64 * kSharedWaves) void batch_shared_kernel(BatchArgs a) {
-  using F = Flash<DP, kF16, kFull, 1, kSharedTile>;
-  constexpr int KT = kSharedTile, W = kSharedWaves, kLoads = 2 * F::kDmas / W;
-  __shared__ __align__(1024) uint8_t ring_mem[kSharedRing * F::kStage];
-  const lds_u8 ring = (lds_u8)ring_mem;
+__device__ __forceinline__ void shared_part(const BatchArgs& a, int wg, lds_u8 ring) {
+  constexpr int KT = kSharedTile<DP>, W = kWaves;
+  using F = Flash<DP, kF16, kFull, 1, KT>;
+  constexpr int kRing = kBatchLds<DP> / F::kStage, kLoads = 2 * F::kDmas / W;
+  static_assert(F::kDmas % W == 0 && kRing >= 3, "the tile's loads split evenly over the waves");
   const int g = a.n_heads / a.n_kv, rows = a.n_seq * g;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int kvh = blockIdx.x % a.n_kv, row_tile = blockIdx.x / a.n_kv, split = blockIdx.y;
+  const int kvh = wg % a.n_kv, split = wg / a.n_kv % a.shared_splits, row_tile = wg / (a.n_kv * a.shared_splits);
   const int first = split * a.shared_tiles, end_tile = min(first + a.shared_tiles, (a.prefix + KT - 1) / KT);
   const int w_row = (row_tile * W + wave) * 32;
   const bool w_live = w_row < rows;
@@ -143,7 +136,7 @@ __global__ __launch_bounds__(64 * kSharedWaves) void batch_shared_kernel(BatchAr
   const int64_t kv_stride = (int64_t)a.n_kv * a.d;
   bool bad = false;
   auto load = [&](int j) {
-    const lds_u8 stage = ring + ((j - first) % kSharedRing) * F::kStage;
+    const lds_u8 stage = ring + ((j - first) % kRing) * F::kStage;
 #pragma unroll
     for (int i = 0; i < F::kDmas / W; ++i) {
       const int n = wave + i * W, r = F::dma_row(n);
@@ -156,15 +149,15 @@ __global__ __launch_bounds__(64 * kSharedWaves) void batch_shared_kernel(BatchAr
     }
   };
 #pragma unroll
-  for (int i = 0; i < kSharedRing - 1; ++i)
+  for (int i = 0; i < kRing - 1; ++i)
     if (first + i < end_tile) load(first + i);
   for (int j = first; j < end_tile; ++j) {
-    if (j + 1 < end_tile)
-      tile_wait<kLoads*(kSharedRing - 2), true>();
+    if (j + kRing - 2 < end_tile)
+      tile_wait<kLoads*(kRing - 2), true>();
     else
       tile_wait<0, true>();
-    if (j + kSharedRing - 1 < end_tile) load(j + kSharedRing - 1);
-    const int stage = ((j - first) % kSharedRing) * F::kStage;
+    if (j + kRing - 1 < end_tile) load(j + kRing - 1);
+    const int stage = ((j - first) % kRing) * F::kStage;
     const int left = a.prefix - j * KT;
     if (left < KT) {
       clear_values<F, KT>(ring + stage, 0, left, threadIdx.x, 64 * W);
@@ -184,44 +177,57 @@ __global__ __launch_bounds__(64 * kSharedWaves) void batch_shared_kernel(BatchAr
     f.softmax(0, sc[0], c2, p[0]);
     f.values(stage, p);
   }
-  const bool any_bad = __syncthreads_or(bad);
-  if (w_row + lane % 32 < rows) store_part<DP, 1>(a, f, 0, (int64_t)b * a.n_heads + head, split, any_bad);
+  bad = __syncthreads_or(bad);
+  const float sum = add_halves(f.l[0]);
+  if (w_row + lane % 32 >= rows) return;
+  const int64_t at = ((int64_t)b * a.n_heads + head) * (a.shared_splits + a.own_splits) + split;
+  if (lane < 32) a.part_ml[at] = make_float2(f.m[0], bad ? __uint_as_float(0x7fc00000u) : sum);
+  float* dst = a.part_o + at * a.d + 4 * (lane / 32);
+#pragma unroll
+  for (int db = 0; db < F::kDimBlocks; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int dim = 32 * db + 2 * e;
+      if (!kFull && dim + 4 * (lane / 32) >= a.d) continue;
+      *reinterpret_cast<float4*>(dst + dim) = make_float4(f.o[0][db][e], f.o[0][db][e + 1], f.o[0][db][e + 2], f.o[0][db][e + 3]);
+    }
 }
 
-// A sequence's own part, and with a window or no shared pass its part of the
-// prefix: a wave takes (sequence, KV head, split of the keys).  The keys are
-// listed as [prefix, padded to kPrefixAlign][own].
+// A sequence's own part, and without a shared pass its part of the prefix.
+// The keys are listed as [prefix, padded to kPrefixAlign][own].
 template <int DP, bool kF16, bool kFull>
-__global__ __launch_bounds__(64) void batch_own_kernel(BatchArgs a) {
+__device__ __forceinline__ void own_part(const BatchArgs& a, int wg, lds_u8 lds, float2 (&wave_ml)[kWaves][kBatchGroup]) {
   using F = Flash<DP, kF16, kFull, 1, kOwnTile>;
   constexpr int KT = kOwnTile, kLoads = 2 * F::kDmas;
-  __shared__ __align__(1024) uint8_t ring_mem[kOwnRing * F::kStage];
-  const lds_u8 ring = (lds_u8)ring_mem;
-  const int g = a.n_heads / a.n_kv, lane = threadIdx.x;
-  const int kvh = blockIdx.x % a.n_kv, split = blockIdx.x / a.n_kv, b = blockIdx.y;
-  int n = a.lengths[b];
-  n = __builtin_amdgcn_readfirstlane(n);
-  if (n < 0) return;  // no sequence: the join writes its zeros
+  const int g = a.n_heads / a.n_kv, lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int kvh = wg % a.n_kv, split = wg / a.n_kv % a.own_splits, b = wg / (a.n_kv * a.own_splits);
+  const int splits = a.shared_splits + a.own_splits;
+  int n = table_at(a.lengths, b);
+  if (n < 0) {  // no sequence: zeros, here or from the join
+    if (splits == 1)
+      for (int i = threadIdx.x; i < g * a.d; i += kWaves * kWave) a.out[((int64_t)b * a.n_heads + kvh * g) * a.d + i] = 0;
+    return;
+  }
+  const lds_u8 ring = lds + wave * kOwnRing * F::kStage;
   const int64_t room = (int64_t)a.width << a.page_log2;
   bool bad = n > room;
   n = (int)min((int64_t)n, room);
   const int pad = (a.prefix + kPrefixAlign - 1) / kPrefixAlign * kPrefixAlign;
-  const bool shared = a.shared_splits > 0;
-  // first visible key, and the lists' visible range
+  // the list's visible range: from `begin` on, up to the prefix's end in its tiles and `end` in the others
   const int seen = a.window > 0 ? min(a.window, a.prefix + n) : a.prefix + n, low = a.prefix + n - seen;
-  const int begin = shared || low >= a.prefix ? pad + max(0, low - a.prefix) : low;
+  const int begin = a.shared_splits > 0 || low >= a.prefix ? pad + max(0, low - a.prefix) : low;
   const int end = n > 0 ? pad + n : a.prefix;
   const int first_tile = begin / KT, n_tiles = begin < end ? (end - 1) / KT + 1 - first_tile : 0;
-  const int per = max((n_tiles + a.own_splits - 1) / a.own_splits, 1);
-  const int first = first_tile + split * per, end_tile = min(first + per, first_tile + n_tiles);
+  const int per = (n_tiles + a.own_splits - 1) / a.own_splits;
+  const int end_tile = first_tile + min((split + 1) * per, n_tiles), first = first_tile + split * per + wave;
   const int col = min(lane % 32, g - 1), head = kvh * g + col;
   F f;
   f.init(ring, a.d);
   const float c2 = a.c2 * load_query<F, kF16>(f.q[0], a.q + b * a.q_stride + (int64_t)head * a.d, a.d);
   const int64_t kv_stride = (int64_t)a.n_kv * a.d;
   const int32_t* own_table = a.tables + (int64_t)b * a.width;
-  auto load = [&](int j) {
-    const lds_u8 stage = ring + ((j - first) % kOwnRing) * F::kStage;
+  auto load = [&](int j, int slot) {
+    const lds_u8 stage = ring + slot * F::kStage;
     const bool own = j * KT >= pad;
     const int base = own ? j * KT - pad : j * KT, last = own ? n - 1 : a.prefix - 1;
     const int visible = own ? max(begin - pad, 0) : begin;
@@ -236,109 +242,210 @@ __global__ __launch_bounds__(64) void batch_own_kernel(BatchArgs a) {
       __builtin_amdgcn_global_load_lds(a.v_pages + at, (lds_void)(stage + F::kMatBytes + i * 1024), 16, 0, 0);
     }
   };
-#pragma unroll
-  for (int i = 0; i < kOwnRing - 1; ++i)
-    if (first + i < end_tile) load(first + i);
-  for (int j = first; j < end_tile; ++j) {
-    if (j + 1 < end_tile)
-      tile_wait<kLoads*(kOwnRing - 2), false>();
+  if (first < end_tile) load(first, 0);
+  if (first + kWaves < end_tile) load(first + kWaves, 1);
+  int slot = 0;
+  for (int j = first; j < end_tile; j += kWaves) {
+    if (j + kWaves < end_tile)
+      tile_wait<kLoads, false>();
     else
       tile_wait<0, false>();
-    if (j + kOwnRing - 1 < end_tile) load(j + kOwnRing - 1);
-    const int stage = ((j - first) % kOwnRing) * F::kStage;
+    const int stage = slot * F::kStage;
     const int from = max(0, begin - j * KT), to = min(KT, (j * KT >= pad ? end : a.prefix) - j * KT);
     const bool part = from > 0 || to < KT;
     if (part) {
-      clear_values<F, KT>(ring + stage, from, to, lane, 64);
+      clear_values<F, KT>(ring + stage, from, to, lane, kWave);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     f32x16_t sc[1][KT / 32];
     f.scores(stage, sc);
     if (part) {
 #pragma unroll
-      for (int kb = 0; kb < KT / 32; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int key = 32 * kb + 8 * (e / 4) + e % 4 + 4 * (lane / 32);
-          if (key < from || key >= to) sc[0][kb][e] = -INFINITY;
-        }
+      for (int e = 0; e < 16; ++e) {
+        const int key = 8 * (e / 4) + e % 4 + 4 * (lane / 32);
+        if (key < from || key >= to) sc[0][0][e] = -INFINITY;
+      }
     }
     u32x4_t p[1][KT / 16];
     f.softmax(0, sc[0], c2, p[0]);
     f.values(stage, p);
+    if (j + 2 * kWaves < end_tile) {
+      tile_wait<63, false>();  // the slot's reads are done
+      load(j + 2 * kWaves, slot);
+    }
+    slot ^= 1;
   }
-  if (lane % 32 < g) store_part<DP, 1>(a, f, 0, (int64_t)b * a.n_heads + head, a.shared_splits + split, __any(bad));
-}
 
-// out[row] = sum over the splits, a wave per row: lane l joins dims l and l + 64.
-__global__ __launch_bounds__(256) void batch_join_kernel(BatchArgs a) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
-  if (row >= (int64_t)a.n_seq * a.n_heads) return;
-  const int lane = threadIdx.x % kWave, splits = a.shared_splits + a.own_splits;
-  const bool absent = a.lengths[row / a.n_heads] < 0;
-  const float2* ml = a.part_ml + row * splits;
-  const float sink = a.sinks != nullptr ? sink_log2(a.sinks[row % a.n_heads]) : -INFINITY;
-  float o[2] = {0.f, 0.f}, sum = 0.f;
-  if (!absent) {
-    float top = sink;
-    for (int s = 0; s < splits; ++s) top = fmaxf(top, ml[s].x);
-    const float base = top == -INFINITY ? 0.f : top;
-    if (sink != -INFINITY) sum = exp2f(sink - base);
-    for (int s = 0; s < splits; ++s) {
-      const float2 x = ml[s];
-      if (x.x == -INFINITY && x.y == 0.f) continue;  // a split without keys
-      const float w = exp2f(x.x - base);
-      sum += w * x.y;
+  // the waves' sums: [wave][head of the group][d], rows 16 bytes apart from a multiple of the banks
+  __syncthreads();
+  const int stride = a.d + 4;
+  typedef __attribute__((address_space(3))) float* lds_f32;
+  typedef __attribute__((address_space(3))) f32x4_t* lds_f32x4;
+  const lds_f32 sums = (lds_f32)lds;
+  const float sum = add_halves(f.l[0]);
+  if (lane % 32 < g) {
+    if (lane < 32) wave_ml[wave][lane] = make_float2(f.m[0], bad ? __uint_as_float(0x7fc00000u) : sum);
+    const lds_f32 dst = sums + (wave * g + lane % 32) * stride + 4 * (lane / 32);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (lane + 64 * i < a.d) o[i] += w * a.part_o[(row * splits + s) * a.d + lane + 64 * i];
+    for (int db = 0; db < F::kDimBlocks; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int dim = 32 * db + 2 * e;
+        if (!kFull && dim + 4 * (lane / 32) >= a.d) continue;
+        *(lds_f32x4)(dst + dim) = f32x4_t{f.o[0][db][e], f.o[0][db][e + 1], f.o[0][db][e + 2], f.o[0][db][e + 3]};
+      }
+  }
+  __syncthreads();
+  const int quads = a.d / 4;
+  for (int i = threadIdx.x; i < g * quads; i += kWaves * kWave) {
+    const int h = i / quads, dim = 4 * (i - h * quads);
+    float2 ml[kWaves];
+    float top = -INFINITY, sink = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      ml[w] = wave_ml[w][h];
+      top = fmaxf(top, ml[w].x);
+    }
+    if (splits == 1 && a.sinks != nullptr) top = fmaxf(top, sink = sink_log2(a.sinks[kvh * g + h]));
+    const float base = top == -INFINITY ? 0.f : top;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float x = __builtin_amdgcn_exp2f(ml[w].x - base);
+      const f32x4_t y = *(lds_f32x4)(sums + (w * g + h) * stride + dim);
+      l = fmaf(x, ml[w].y, l);
+      o.x = fmaf(x, y.x, o.x), o.y = fmaf(x, y.y, o.y), o.z = fmaf(x, y.z, o.z), o.w = fmaf(x, y.w, o.w);
+    }
+    const int64_t row = (int64_t)b * a.n_heads + kvh * g + h;
+    if (splits == 1) {
+      if (sink != -INFINITY) l += __builtin_amdgcn_exp2f(sink - base);
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      *reinterpret_cast<u32x2_t*>(a.out + row * a.d + dim) = u32x2_t{pack2<false>(o.x * inv, o.y * inv), pack2<false>(o.z * inv, o.w * inv)};
+    } else {
+      const int64_t at = row * splits + a.shared_splits + split;
+      *reinterpret_cast<float4*>(a.part_o + at * a.d + dim) = o;
+      if (dim == 0) a.part_ml[at] = make_float2(top, l);
     }
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+}
+
+template <int DP, bool kF16, bool kFull>
+__global__ __launch_bounds__(kWave * kWaves, DP == 64 ? 2 : 1) void batch_attention_kernel(BatchArgs a) {
+  __shared__ __align__(1024) uint8_t lds[kBatchLds<DP>];
+  __shared__ float2 wave_ml[kWaves][kBatchGroup];
+  if ((int)blockIdx.x < a.shared_wgs)
+    shared_part<DP, kF16, kFull>(a, blockIdx.x, (lds_u8)lds);
+  else
+    own_part<DP, kF16, kFull>(a, blockIdx.x - a.shared_wgs, (lds_u8)lds, wave_ml);
+}
+
+// out[row] = sum over the splits.  W waves a row; in a wave, lanes take 4 dims
+// each and the groups of lanes that this leaves take splits in turn.
+template <int W>
+__global__ __launch_bounds__(256) void batch_join_kernel(BatchArgs a) {
+  __shared__ float4 wave_o[4][32];
+  __shared__ float wave_l[4];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int64_t row = (int64_t)blockIdx.x * (4 / W) + wave / W, rows = (int64_t)a.n_seq * a.n_heads;
+  const bool live = row < rows;
+  const int64_t r = live ? row : rows - 1;
+  const int splits = a.shared_splits + a.own_splits;
+  const int lanes = a.d <= 32 ? 8 : a.d <= 64 ? 16 : 32, groups = kWave / lanes, grp = lane / lanes;
+  const int dim = min(4 * (lane % lanes), a.d - 4);
+  const bool absent = a.lengths[r / a.n_heads] < 0;
+  const float2* ml = a.part_ml + r * splits;
+  const float sink = a.sinks != nullptr ? sink_log2(a.sinks[r % a.n_heads]) : -INFINITY;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+  if (!absent) {
+    float top = sink;
+    for (int s = lane; s < splits; s += kWave) top = fmaxf(top, ml[s].x);
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (lane + 64 * i < a.d) a.out[row * a.d + lane + 64 * i] = (uint16_t)f32_to_bf16_rne(o[i] * inv);
+    for (int off = kWave / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+    const float base = top == -INFINITY ? 0.f : top;
+    constexpr int kAhead = 4;
+    const int step = groups * W;
+    for (int s0 = (wave % W) * groups + grp; s0 < splits; s0 += kAhead * step) {
+      float4 y[kAhead];
+      float2 x[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int s = min(s0 + i * step, splits - 1);
+        y[i] = *reinterpret_cast<const float4*>(a.part_o + (r * splits + s) * a.d + dim);
+        x[i] = ml[s];
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (s0 + i * step >= splits) break;
+        const float w = __builtin_amdgcn_exp2f(x[i].x - base);
+        l = fmaf(w, x[i].y, l);
+        o.x = fmaf(w, y[i].x, o.x), o.y = fmaf(w, y[i].y, o.y), o.z = fmaf(w, y[i].z, o.z), o.w = fmaf(w, y[i].w, o.w);
+      }
+    }
+    for (int off = lanes; off < kWave; off <<= 1) {
+      l += __shfl_xor(l, off);
+      o.x += __shfl_xor(o.x, off), o.y += __shfl_xor(o.y, off), o.z += __shfl_xor(o.z, off), o.w += __shfl_xor(o.w, off);
+    }
+    if (wave % W == 0 && sink != -INFINITY) l += __builtin_amdgcn_exp2f(sink - base);
+  }
+  if constexpr (W > 1) {
+    if (lane < lanes) wave_o[wave][lane] = o;
+    if (lane == 0) wave_l[wave] = l;
+    __syncthreads();
+    if (wave % W != 0) return;
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      const float4 y = wave_o[wave + w][lane % lanes];
+      l += wave_l[wave + w];
+      o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (live && lane < a.d / 4)
+    *reinterpret_cast<u32x2_t*>(a.out + row * a.d + dim) = u32x2_t{pack2<false>(o.x * inv, o.y * inv), pack2<false>(o.z * inv, o.w * inv)};
 }
 
 struct BatchPlan {
   int64_t shared_splits, shared_tiles, row_tiles, own_splits;
   int64_t splits() const { return shared_splits + own_splits; }
 };
-BatchPlan batch_plan(int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t prefix, int64_t max_own, int64_t window) {
+BatchPlan batch_plan(int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t d, int64_t prefix, int64_t max_own, int64_t window) {
   BatchPlan p{};
   const int64_t rows = n_seq * (n_heads / n_kv);
-  p.row_tiles = (rows + 32 * kSharedWaves - 1) / (32 * kSharedWaves);
+  p.row_tiles = (rows + 32 * kWaves - 1) / (32 * kWaves);
   const bool shared = prefix > 0 && window == 0 && n_seq > 1;
   int64_t keys = max_own + (shared ? 0 : prefix);
   if (window > 0 && window < keys) keys = window;
   if (shared) {
-    const int64_t tiles = (prefix + kSharedTile - 1) / kSharedTile;
+    const int64_t tile = d <= 64 ? kSharedTile<64> : kSharedTile<128>;
+    const int64_t tiles = (prefix + tile - 1) / tile;
     const int64_t want = (256 + n_kv * p.row_tiles - 1) / (n_kv * p.row_tiles);
     p.shared_tiles = (tiles + want - 1) / want;
     p.shared_splits = (tiles + p.shared_tiles - 1) / p.shared_tiles;
   }
   const int64_t own_tiles = keys / kOwnTile + 2;
-  const int64_t want = (1024 + n_seq * n_kv - 1) / (n_seq * n_kv), most = (own_tiles + 3) / 4;
+  const int64_t want = (512 + n_seq * n_kv - 1) / (n_seq * n_kv), most = (own_tiles + 2 * kWaves - 1) / (2 * kWaves);
   p.own_splits = want < most ? want : most;
   return p;
 }
 
+// a row of one part needs none
 int64_t batch_bytes(const BatchPlan& p, int64_t n_seq, int64_t n_heads, int64_t d) {
-  return n_seq * n_heads * p.splits() * (4 * d + 8);
+  return p.splits() == 1 ? 0 : n_seq * n_heads * p.splits() * (4 * d + 8);
 }
 
 template <int DP, bool kF16, bool kFull>
 int launch_batch(const BatchArgs& a, const BatchPlan& p, hipStream_t st) {
-  int rc;
-  if (p.shared_splits > 0) {
-    const dim3 grid((unsigned)(a.n_kv * p.row_tiles), (unsigned)p.shared_splits);
-    batch_shared_kernel<DP, kF16, kFull><<<grid, 64 * kSharedWaves, 0, st>>>(a);
-    if ((rc = check_launch("batch_shared_kernel"))) return rc;
-  }
-  const dim3 grid((unsigned)(a.n_kv * p.own_splits), (unsigned)a.n_seq);
-  batch_own_kernel<DP, kF16, kFull><<<grid, 64, 0, st>>>(a);
-  if ((rc = check_launch("batch_own_kernel"))) return rc;
-  batch_join_kernel<<<(unsigned)(((int64_t)a.n_seq * a.n_heads + 3) / 4), 256, 0, st>>>(a);
+  const int64_t wgs = a.shared_wgs + (int64_t)a.n_seq * a.n_kv * p.own_splits;
+  batch_attention_kernel<DP, kF16, kFull><<<(unsigned)wgs, kWave * kWaves, 0, st>>>(a);
+  const int rc = check_launch("batch_attention_kernel");
+  if (rc || p.splits() == 1) return rc;
+  const int64_t rows = (int64_t)a.n_seq * a.n_heads;
+  if (p.splits() > 16)
+    batch_join_kernel<4><<<(unsigned)rows, 256, 0, st>>>(a);
+  else
+    batch_join_kernel<1><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(a);
   return check_launch("batch_join_kernel");
 }
 
@@ -364,48 +471,50 @@ extern "C" int64_t klc_attn_batch_workspace_bytes(int64_t n_seq, int64_t n_heads
                                                   int64_t prefix_len, int64_t max_own, int64_t window) {
   const int rc = check_sizes("klc_attn_batch_workspace_bytes", n_seq, n_heads, n_kv, head_dim, prefix_len, max_own, window);
   if (rc) return rc;
-  return batch_bytes(batch_plan(n_seq, n_heads, n_kv, prefix_len, max_own, window), n_seq, n_heads, head_dim);
+  return batch_bytes(batch_plan(n_seq, n_heads, n_kv, head_dim, prefix_len, max_own, window), n_seq, n_heads, head_dim);
 }
 
-extern "C" int klc_attn_batch(const void* q, const void* k_pages, const void* v_pages, const int32_t* tables,
-                              const int32_t* lengths, const int32_t* prefix_table, const void* sinks, int64_t n_seq,
-                              int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t q_stride, int64_t n_pages,
-                              int64_t page_size, int64_t table_width, int64_t prefix_len, int64_t window, float scale,
-                              int kv_dtype, void* workspace, int64_t workspace_bytes, void* out, void* stream) {
-  KLC_REQUIRE(q && k_pages && v_pages && lengths && out && workspace, KLC_ERR_ARGUMENT, "klc_attn_batch: null pointer");
-  KLC_REQUIRE((tables || table_width == 0) && (prefix_table || prefix_len == 0), KLC_ERR_ARGUMENT,
+extern "C" int klc_attn_batch(const klc_attn_batch_args* args, void* stream) {
+  KLC_REQUIRE(args != nullptr, KLC_ERR_ARGUMENT, "klc_attn_batch: null pointer");
+  const klc_attn_batch_args& x = *args;
+  KLC_REQUIRE(x.q && x.k_pages && x.v_pages && x.lengths && x.out, KLC_ERR_ARGUMENT, "klc_attn_batch: null pointer");
+  KLC_REQUIRE((x.tables || x.table_width == 0) && (x.prefix_table || x.prefix_len == 0), KLC_ERR_ARGUMENT,
               "klc_attn_batch: null table");
-  KLC_REQUIRE(page_size >= 16 && page_size <= 4096 && (page_size & (page_size - 1)) == 0 && n_pages > 0 &&
-                  n_pages * page_size < ((int64_t)1 << 31) && table_width >= 0 && table_width < ((int64_t)1 << 25),
+  KLC_REQUIRE(x.page_size >= 16 && x.page_size <= 4096 && (x.page_size & (x.page_size - 1)) == 0 && x.n_pages > 0 &&
+                  x.n_pages < ((int64_t)1 << 31) && x.n_pages * x.page_size < ((int64_t)1 << 31) && x.table_width >= 0 &&
+                  x.table_width < ((int64_t)1 << 25),
               KLC_ERR_SHAPE, "klc_attn_batch: %lld pages of %lld tokens (a power of two, 16..4096), tables of %lld",
-              (long long)n_pages, (long long)page_size, (long long)table_width);
-  const int64_t max_own = table_width * page_size;
-  int rc = check_sizes("klc_attn_batch", n_seq, n_heads, n_kv, head_dim, prefix_len, max_own, window);
+              (long long)x.n_pages, (long long)x.page_size, (long long)x.table_width);
+  const int64_t max_own = x.table_width * x.page_size, d = x.head_dim, rows = x.n_seq * x.n_heads;
+  int rc = check_sizes("klc_attn_batch", x.n_seq, x.n_heads, x.n_kv, d, x.prefix_len, max_own, x.window);
   if (rc) return rc;
-  KLC_REQUIRE(q_stride >= n_heads * head_dim && q_stride % 8 == 0, KLC_ERR_SHAPE,
-              "klc_attn_batch: q stride %lld (a multiple of 8, no overlap)", (long long)q_stride);
-  KLC_REQUIRE(((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)workspace | (uintptr_t)out) % 16 == 0,
+  KLC_REQUIRE(x.q_stride >= x.n_heads * d && x.q_stride % 8 == 0, KLC_ERR_SHAPE,
+              "klc_attn_batch: q stride %lld (a multiple of 8, no overlap)", (long long)x.q_stride);
+  KLC_REQUIRE(((uintptr_t)x.q | (uintptr_t)x.k_pages | (uintptr_t)x.v_pages | (uintptr_t)x.workspace | (uintptr_t)x.out) % 16 == 0,
               KLC_ERR_ARGUMENT, "klc_attn_batch: q, pages, workspace and out must be 16-byte aligned");
-  KLC_REQUIRE(scale > 0.f && scale < INFINITY, KLC_ERR_ARGUMENT, "klc_attn_batch: scale %g", (double)scale);
-  KLC_REQUIRE(kv_dtype == KLC_DTYPE_BF16 || kv_dtype == KLC_DTYPE_F16, KLC_ERR_UNSUPPORTED,
-              "klc_attn_batch: kv_dtype %d (bfloat16 or float16)", kv_dtype);
-  const BatchPlan p = batch_plan(n_seq, n_heads, n_kv, prefix_len, max_own, window);
-  const int64_t need = batch_bytes(p, n_seq, n_heads, head_dim);
-  KLC_REQUIRE(workspace_bytes >= need, KLC_ERR_ARGUMENT, "klc_attn_batch: workspace of %lld bytes, need %lld",
-              (long long)workspace_bytes, (long long)need);
-  auto in = [](const void* x) { return static_cast<const uint16_t*>(x); };
+  KLC_REQUIRE(x.scale > 0 && (float)x.scale > 0.f && (float)x.scale < INFINITY, KLC_ERR_ARGUMENT,
+              "klc_attn_batch: scale %g", x.scale);
+  KLC_REQUIRE(x.kv_dtype == KLC_DTYPE_BF16 || x.kv_dtype == KLC_DTYPE_F16, KLC_ERR_UNSUPPORTED,
+              "klc_attn_batch: kv_dtype %lld (bfloat16 or float16)", (long long)x.kv_dtype);
+  const BatchPlan p = batch_plan(x.n_seq, x.n_heads, x.n_kv, d, x.prefix_len, max_own, x.window);
+  const int64_t need = batch_bytes(p, x.n_seq, x.n_heads, d);
+  KLC_REQUIRE(need == 0 || (x.workspace && x.workspace_bytes >= need), KLC_ERR_ARGUMENT,
+              "klc_attn_batch: workspace of %lld bytes, need %lld", (long long)x.workspace_bytes, (long long)need);
+  auto in = [](const void* v) { return static_cast<const uint16_t*>(v); };
+  auto index = [](const void* v) { return static_cast<const int32_t*>(v); };
   int page_log2 = 0;
-  while ((1 << page_log2) < page_size) ++page_log2;
-  float* part_o = static_cast<float*>(workspace);
-  const BatchArgs a{in(q), in(k_pages), in(v_pages), tables, lengths, prefix_table, in(sinks),
-                    static_cast<uint16_t*>(out), part_o,
-                    reinterpret_cast<float2*>(part_o + n_seq * n_heads * p.splits() * head_dim), q_stride, (int)n_seq,
-                    (int)n_heads, (int)n_kv, (int)head_dim, (int)n_pages, page_log2, (int)table_width, (int)prefix_len,
-                    (int)window, (int)p.shared_splits, (int)p.own_splits, (int)p.shared_tiles, scale * kLog2e};
+  while ((1 << page_log2) < x.page_size) ++page_log2;
+  float* part_o = static_cast<float*>(x.workspace);
+  float2* part_ml = need > 0 ? reinterpret_cast<float2*>(part_o + rows * p.splits() * d) : nullptr;
+  const BatchArgs a{in(x.q), in(x.k_pages), in(x.v_pages), index(x.tables), index(x.lengths), index(x.prefix_table),
+                    in(x.sinks), static_cast<uint16_t*>(x.out), part_o, part_ml, x.q_stride, (int)x.n_seq,
+                    (int)x.n_heads, (int)x.n_kv, (int)d, (int)x.n_pages, page_log2, (int)x.table_width,
+                    (int)x.prefix_len, (int)x.window, (int)p.shared_splits, (int)p.own_splits, (int)p.shared_tiles,
+                    (int)(p.shared_splits * p.row_tiles * x.n_kv), (float)(x.scale * kLog2e)};
   const hipStream_t st = as_stream(stream);
-  const bool f16 = kv_dtype == KLC_DTYPE_F16;
-  if (head_dim == 64) return f16 ? launch_batch<64, true, true>(a, p, st) : launch_batch<64, false, true>(a, p, st);
-  if (head_dim == 128) return f16 ? launch_batch<128, true, true>(a, p, st) : launch_batch<128, false, true>(a, p, st);
-  if (head_dim < 64) return f16 ? launch_batch<64, true, false>(a, p, st) : launch_batch<64, false, false>(a, p, st);
+  const bool f16 = x.kv_dtype == KLC_DTYPE_F16;
+  if (d == 64) return f16 ? launch_batch<64, true, true>(a, p, st) : launch_batch<64, false, true>(a, p, st);
+  if (d == 128) return f16 ? launch_batch<128, true, true>(a, p, st) : launch_batch<128, false, true>(a, p, st);
+  if (d < 64) return f16 ? launch_batch<64, true, false>(a, p, st) : launch_batch<64, false, false>(a, p, st);
   return f16 ? launch_batch<128, true, false>(a, p, st) : launch_batch<128, false, false>(a, p, st);
 }

@@ -1,5 +1,7 @@
 // A paged KV cache of many sequences (gfx950): rotation and append of new
 // tokens, and copies of pages between slots of the pools.
+#include <stdlib.h>
+
 #include "klc_common.h"
 
 namespace klc {
@@ -106,40 +108,40 @@ __global__ __launch_bounds__(kPagedThreads) void copy_pages_kernel(uint8_t* __re
 
 using namespace klc;
 
-extern "C" int klc_kv_append(const void* q, const void* k, const void* v, const void* cos_half, const void* sin_half,
-                             const int32_t* positions, const int32_t* slots, int64_t tokens, int64_t n_positions,
-                             int64_t n_slots, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t q_stride,
-                             int64_t k_stride, int64_t v_stride, int kv_dtype, void* q_out, void* k_out, void* k_pages,
-                             void* v_pages, void* stream) {
-  KLC_REQUIRE(q && k && v && cos_half && sin_half && positions && slots && q_out && k_pages && v_pages,
+extern "C" int klc_kv_append(const klc_kv_append_args* args, void* stream) {
+  KLC_REQUIRE(args != nullptr, KLC_ERR_ARGUMENT, "klc_kv_append: null pointer");
+  const klc_kv_append_args& x = *args;
+  KLC_REQUIRE(x.q && x.k && x.v && x.cos_half && x.sin_half && x.positions && x.slots && x.q_out && x.k_pages && x.v_pages,
               KLC_ERR_ARGUMENT, "klc_kv_append: null pointer");
-  KLC_REQUIRE(n_heads > 0 && n_kv > 0 && n_heads <= 4096 && n_kv <= 4096 && head_dim >= 8 && head_dim % 8 == 0 &&
-                  head_dim <= 128,
+  KLC_REQUIRE(x.n_heads > 0 && x.n_kv > 0 && x.n_heads <= 4096 && x.n_kv <= 4096 && x.head_dim >= 8 &&
+                  x.head_dim % 8 == 0 && x.head_dim <= 128,
               KLC_ERR_SHAPE, "klc_kv_append: heads %lld / %lld, head_dim %lld (8..128, multiple of 8)",
-              (long long)n_heads, (long long)n_kv, (long long)head_dim);
-  KLC_REQUIRE(tokens > 0 && tokens < ((int64_t)1 << 30) && n_positions > 0 && n_positions < ((int64_t)1 << 31) &&
-                  n_slots > 0 && n_slots < ((int64_t)1 << 31),
-              KLC_ERR_ARGUMENT, "klc_kv_append: %lld tokens, %lld positions, %lld slots", (long long)tokens,
-              (long long)n_positions, (long long)n_slots);
-  KLC_REQUIRE(q_stride >= n_heads * head_dim && k_stride >= n_kv * head_dim && v_stride >= n_kv * head_dim &&
-                  (q_stride | k_stride | v_stride) % 8 == 0,
+              (long long)x.n_heads, (long long)x.n_kv, (long long)x.head_dim);
+  KLC_REQUIRE(x.tokens > 0 && x.tokens < ((int64_t)1 << 30) && x.n_positions > 0 &&
+                  x.n_positions < ((int64_t)1 << 31) && x.n_slots > 0 && x.n_slots < ((int64_t)1 << 31),
+              KLC_ERR_ARGUMENT, "klc_kv_append: %lld tokens, %lld positions, %lld slots", (long long)x.tokens,
+              (long long)x.n_positions, (long long)x.n_slots);
+  KLC_REQUIRE(x.q_stride >= x.n_heads * x.head_dim && x.k_stride >= x.n_kv * x.head_dim &&
+                  x.v_stride >= x.n_kv * x.head_dim && (x.q_stride | x.k_stride | x.v_stride) % 8 == 0,
               KLC_ERR_SHAPE, "klc_kv_append: token strides %lld, %lld, %lld (multiples of 8, no overlap)",
-              (long long)q_stride, (long long)k_stride, (long long)v_stride);
-  KLC_REQUIRE(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)cos_half | (uintptr_t)sin_half |
-               (uintptr_t)q_out | (uintptr_t)k_out | (uintptr_t)k_pages | (uintptr_t)v_pages) % 16 == 0,
+              (long long)x.q_stride, (long long)x.k_stride, (long long)x.v_stride);
+  KLC_REQUIRE(((uintptr_t)x.q | (uintptr_t)x.k | (uintptr_t)x.v | (uintptr_t)x.cos_half | (uintptr_t)x.sin_half |
+               (uintptr_t)x.q_out | (uintptr_t)x.k_out | (uintptr_t)x.k_pages | (uintptr_t)x.v_pages) % 16 == 0,
               KLC_ERR_ARGUMENT, "klc_kv_append: tensors must be 16-byte aligned");
-  KLC_REQUIRE(kv_dtype == KLC_DTYPE_BF16 || kv_dtype == KLC_DTYPE_F16, KLC_ERR_UNSUPPORTED,
-              "klc_kv_append: kv_dtype %d (bfloat16 or float16)", kv_dtype);
+  KLC_REQUIRE(x.kv_dtype == KLC_DTYPE_BF16 || x.kv_dtype == KLC_DTYPE_F16, KLC_ERR_UNSUPPORTED,
+              "klc_kv_append: kv_dtype %lld (bfloat16 or float16)", (long long)x.kv_dtype);
   auto in = [](const void* p) { return static_cast<const uint16_t*>(p); };
+  auto index = [](const void* p) { return static_cast<const int32_t*>(p); };
   auto out = [](void* p) { return static_cast<uint16_t*>(p); };
-  const AppendArgs a{in(q), in(k), in(v), in(cos_half), in(sin_half), positions, slots, out(q_out), out(k_out),
-                     out(k_pages), out(v_pages), q_stride, k_stride, v_stride, (int)tokens, (int)n_slots,
-                     (int)n_positions, (int)n_heads, (int)n_kv, (int)head_dim, kv_dtype == KLC_DTYPE_F16};
-  const bool wide = head_dim % 16 == 0;
-  const int64_t items = tokens * (n_heads + 2 * n_kv) * (head_dim / 2 / (wide ? 8 : 4));
+  const AppendArgs a{in(x.q), in(x.k), in(x.v), in(x.cos_half), in(x.sin_half), index(x.positions), index(x.slots),
+                     out(x.q_out), out(x.k_out), out(x.k_pages), out(x.v_pages), x.q_stride, x.k_stride, x.v_stride,
+                     (int)x.tokens, (int)x.n_slots, (int)x.n_positions, (int)x.n_heads, (int)x.n_kv, (int)x.head_dim,
+                     x.kv_dtype == KLC_DTYPE_F16};
+  const bool wide = x.head_dim % 16 == 0;
+  const int64_t items = x.tokens * (x.n_heads + 2 * x.n_kv) * (x.head_dim / 2 / (wide ? 8 : 4));
   const int64_t blocks = (items + kPagedThreads - 1) / kPagedThreads;
-  KLC_REQUIRE(blocks < ((int64_t)1 << 31), KLC_ERR_SHAPE, "klc_kv_append: %lld tokens of %lld heads", (long long)tokens,
-              (long long)n_heads);
+  KLC_REQUIRE(blocks < ((int64_t)1 << 31), KLC_ERR_SHAPE, "klc_kv_append: %lld tokens of %lld heads",
+              (long long)x.tokens, (long long)x.n_heads);
   if (wide)
     paged_append_kernel<8><<<(unsigned)blocks, kPagedThreads, 0, as_stream(stream)>>>(a);
   else
@@ -155,10 +157,25 @@ extern "C" int klc_kv_copy_pages(void* pools, int64_t n_pools, int64_t n_pages, 
               KLC_ERR_ARGUMENT,
               "klc_kv_copy_pages: %lld moves in %lld pools of %lld pages of %lld bytes (a multiple of 16, 16-byte aligned)",
               (long long)n, (long long)n_pools, (long long)n_pages, (long long)page_bytes);
-  for (int64_t i = 0; i < n; ++i)
-    KLC_REQUIRE(src[i] >= 0 && src[i] < n_pages && dst[i] >= 0 && dst[i] < n_pages, KLC_ERR_ARGUMENT,
-                "klc_kv_copy_pages: move %lld from page %d to page %d of %lld", (long long)i, src[i], dst[i],
-                (long long)n_pages);
+  if (n == 0) return KLC_OK;
+  // destinations, a bit a page
+  uint8_t* taken = static_cast<uint8_t*>(calloc((size_t)(n_pages + 7) / 8, 1));
+  KLC_REQUIRE(taken != nullptr, KLC_ERR_ARGUMENT, "klc_kv_copy_pages: no memory to check %lld pages", (long long)n_pages);
+  int64_t bad = -1;
+  bool range = false;
+  for (int64_t i = 0; i < n && bad < 0; ++i) {
+    range = src[i] < 0 || src[i] >= n_pages || dst[i] < 0 || dst[i] >= n_pages;
+    if (range || (taken[dst[i] / 8] >> dst[i] % 8 & 1)) bad = i;
+    else taken[dst[i] / 8] |= (uint8_t)(1 << dst[i] % 8);
+  }
+  for (int64_t i = 0; i < n && bad < 0; ++i)
+    if (taken[src[i] / 8] >> src[i] % 8 & 1) bad = i;
+  free(taken);
+  KLC_REQUIRE(bad < 0 || !range, KLC_ERR_ARGUMENT, "klc_kv_copy_pages: move %lld from page %d to page %d of %lld",
+              (long long)bad, src[bad], dst[bad], (long long)n_pages);
+  KLC_REQUIRE(bad < 0, KLC_ERR_ARGUMENT,
+              "klc_kv_copy_pages: move %lld from page %d to page %d: a destination is another move's source or destination",
+              (long long)bad, src[bad], dst[bad]);
   for (int64_t at = 0; at < n; at += kMovesPerLaunch) {
     const int count = (int)(n - at < kMovesPerLaunch ? n - at : kMovesPerLaunch);
     Moves m;

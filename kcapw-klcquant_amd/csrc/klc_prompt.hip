@@ -217,37 +217,38 @@ int launch_prompt(const PromptArgs& a, hipStream_t st) {
 
 using namespace klc;
 
-extern "C" int klc_attn_prompt(const void* q, const void* k, const void* v, const int32_t* starts, const void* sinks,
-                               int64_t tokens, int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t head_dim,
-                               int64_t q_stride, int64_t k_stride, int64_t v_stride, int64_t window, float scale,
-                               int dtype, void* out, void* stream) {
-  KLC_REQUIRE(q && k && v && starts && out, KLC_ERR_ARGUMENT, "klc_attn_prompt: null pointer");
-  KLC_REQUIRE(n_heads > 0 && n_kv > 0 && n_heads % n_kv == 0 && n_heads <= 4096 && head_dim >= 8 && head_dim % 8 == 0 &&
-                  head_dim <= 128,
+extern "C" int klc_attn_prompt(const klc_attn_prompt_args* args, void* stream) {
+  KLC_REQUIRE(args != nullptr, KLC_ERR_ARGUMENT, "klc_attn_prompt: null pointer");
+  const klc_attn_prompt_args& x = *args;
+  KLC_REQUIRE(x.q && x.k && x.v && x.starts && x.out, KLC_ERR_ARGUMENT, "klc_attn_prompt: null pointer");
+  KLC_REQUIRE(x.n_heads > 0 && x.n_kv > 0 && x.n_heads % x.n_kv == 0 && x.n_heads <= 4096 && x.head_dim >= 8 &&
+                  x.head_dim % 8 == 0 && x.head_dim <= 128,
               KLC_ERR_SHAPE, "klc_attn_prompt: heads %lld / %lld, head_dim %lld (8..128, multiple of 8)",
-              (long long)n_heads, (long long)n_kv, (long long)head_dim);
-  const int64_t g = n_heads / n_kv;
-  KLC_REQUIRE(tokens > 0 && n_seq > 0 && tokens * g < ((int64_t)1 << 30) && n_seq < ((int64_t)1 << 20) &&
-                  (tokens * g / 64 + n_seq) * n_kv < ((int64_t)1 << 31),
+              (long long)x.n_heads, (long long)x.n_kv, (long long)x.head_dim);
+  const int64_t g = x.n_heads / x.n_kv;
+  KLC_REQUIRE(x.tokens > 0 && x.n_seq > 0 && x.tokens < ((int64_t)1 << 30) && x.tokens * g < ((int64_t)1 << 30) &&
+                  x.n_seq < ((int64_t)1 << 20) && (x.tokens * g / 64 + x.n_seq) * x.n_kv < ((int64_t)1 << 31),
               KLC_ERR_ARGUMENT, "klc_attn_prompt: %lld tokens in %lld sequences (tokens * group < 2^30)",
-              (long long)tokens, (long long)n_seq);
-  KLC_REQUIRE(q_stride >= n_heads * head_dim && k_stride >= n_kv * head_dim && v_stride >= n_kv * head_dim &&
-                  (q_stride | k_stride | v_stride) % 8 == 0,
+              (long long)x.tokens, (long long)x.n_seq);
+  KLC_REQUIRE(x.q_stride >= x.n_heads * x.head_dim && x.k_stride >= x.n_kv * x.head_dim &&
+                  x.v_stride >= x.n_kv * x.head_dim && (x.q_stride | x.k_stride | x.v_stride) % 8 == 0,
               KLC_ERR_SHAPE, "klc_attn_prompt: token strides %lld, %lld, %lld (multiples of 8, no overlap)",
-              (long long)q_stride, (long long)k_stride, (long long)v_stride);
-  KLC_REQUIRE(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16 == 0, KLC_ERR_ARGUMENT,
+              (long long)x.q_stride, (long long)x.k_stride, (long long)x.v_stride);
+  KLC_REQUIRE(((uintptr_t)x.q | (uintptr_t)x.k | (uintptr_t)x.v | (uintptr_t)x.out) % 16 == 0, KLC_ERR_ARGUMENT,
               "klc_attn_prompt: q, k, v and out must be 16-byte aligned");
-  KLC_REQUIRE(window >= 0 && window < ((int64_t)1 << 30) && scale > 0.f && scale < INFINITY, KLC_ERR_ARGUMENT,
-              "klc_attn_prompt: window %lld, scale %g", (long long)window, (double)scale);
-  KLC_REQUIRE(dtype == KLC_DTYPE_BF16 || dtype == KLC_DTYPE_F16, KLC_ERR_UNSUPPORTED,
-              "klc_attn_prompt: dtype %d (bfloat16 or float16)", dtype);
+  KLC_REQUIRE(x.window >= 0 && x.window < ((int64_t)1 << 30) && x.scale > 0 && (float)x.scale > 0.f &&
+                  (float)x.scale < INFINITY,
+              KLC_ERR_ARGUMENT, "klc_attn_prompt: window %lld, scale %g", (long long)x.window, x.scale);
+  KLC_REQUIRE(x.dtype == KLC_DTYPE_BF16 || x.dtype == KLC_DTYPE_F16, KLC_ERR_UNSUPPORTED,
+              "klc_attn_prompt: dtype %lld (bfloat16 or float16)", (long long)x.dtype);
   auto in = [](const void* p) { return static_cast<const uint16_t*>(p); };
-  const PromptArgs a{in(q), in(k), in(v), in(sinks), starts, static_cast<uint16_t*>(out), q_stride, k_stride, v_stride,
-                     (int)tokens, (int)n_seq, (int)n_heads, (int)n_kv, (int)head_dim, (int)window, scale * kLog2e};
+  const PromptArgs a{in(x.q), in(x.k), in(x.v), in(x.sinks), static_cast<const int32_t*>(x.starts),
+                     static_cast<uint16_t*>(x.out), x.q_stride, x.k_stride, x.v_stride, (int)x.tokens, (int)x.n_seq,
+                     (int)x.n_heads, (int)x.n_kv, (int)x.head_dim, (int)x.window, (float)(x.scale * kLog2e)};
   const hipStream_t st = as_stream(stream);
-  const bool f16 = dtype == KLC_DTYPE_F16;
-  if (head_dim == 64) return f16 ? launch_prompt<64, true, true>(a, st) : launch_prompt<64, false, true>(a, st);
-  if (head_dim == 128) return f16 ? launch_prompt<128, true, true>(a, st) : launch_prompt<128, false, true>(a, st);
-  if (head_dim < 64) return f16 ? launch_prompt<64, true, false>(a, st) : launch_prompt<64, false, false>(a, st);
+  const bool f16 = x.dtype == KLC_DTYPE_F16;
+  if (x.head_dim == 64) return f16 ? launch_prompt<64, true, true>(a, st) : launch_prompt<64, false, true>(a, st);
+  if (x.head_dim == 128) return f16 ? launch_prompt<128, true, true>(a, st) : launch_prompt<128, false, true>(a, st);
+  if (x.head_dim < 64) return f16 ? launch_prompt<64, true, false>(a, st) : launch_prompt<64, false, false>(a, st);
   return f16 ? launch_prompt<128, true, false>(a, st) : launch_prompt<128, false, false>(a, st);
 }

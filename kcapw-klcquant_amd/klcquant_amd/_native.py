@@ -89,11 +89,11 @@ SIGNATURES: dict[str, tuple] = {
     "klc_attn_step_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64]),
     "klc_attn_step": (_I32, [ctypes.c_char_p, _P]),
     "klc_attn_step_wait": (_I32, [_P, _I64, _I64]),
-    "klc_attn_prompt": (_I32, [_P, _P, _P, _P, _P, *[_I64] * 9, _F32, _I32, _P, _P]),
-    "klc_kv_append": (_I32, [*[_P] * 7, *[_I64] * 9, _I32, _P, _P, _P, _P, _P]),
+    "klc_attn_prompt": (_I32, [ctypes.c_char_p, _P]),
+    "klc_kv_append": (_I32, [ctypes.c_char_p, _P]),
     "klc_kv_copy_pages": (_I32, [_P, _I64, _I64, _I64, _P, _P, _I64, _P]),
     "klc_attn_batch_workspace_bytes": (_I64, [_I64] * 7),
-    "klc_attn_batch": (_I32, [*[_P] * 7, *[_I64] * 10, _F32, _I32, _P, _I64, _P, _P]),
+    "klc_attn_batch": (_I32, [ctypes.c_char_p, _P]),
     "klc_synth_fill": (_I32, [_P, _I64, _U64, _I32, _I32, _I32, _P]),
 }
 

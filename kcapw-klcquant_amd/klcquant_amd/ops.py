@@ -8,8 +8,10 @@ rejected.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
+import struct
 from typing import NamedTuple
 
 import numpy as np
@@ -288,10 +290,22 @@ def workspace_bytes(n_tokens: int, hidden: int, inter: int, n_experts: int, k: i
 # ---- Attention of many sequences ---------------------------------------------------
 
 _KV_CODES = {torch.bfloat16: nat.DTYPE_BF16, torch.float16: nat.DTYPE_F16}
+_TENSORS = (torch.Tensor, torch.nn.Parameter)
+# klc_attn_prompt_args, klc_kv_append_args and klc_attn_batch_args: pointers, sizes, scale
+_PROMPT_ARGS = struct.Struct("=6Q10qd")
+_APPEND_ARGS = struct.Struct("=11Q10q")
+_BATCH_ARGS = struct.Struct("=9Q12qd")
+_batch_bytes: dict = {}  # sizes -> klc_attn_batch's workspace bytes
 
 
-def _check_rows(name: str, t: torch.Tensor, dtype: torch.dtype, dev: torch.device) -> int:
-    """``[tokens, heads, head_dim]`` with contiguous heads, a view of a wider row allowed; the token stride."""
+def _plain(t, dtype: torch.dtype, shape: tuple, index: int) -> bool:
+    """A contiguous tensor of this type and shape on GPU ``index``, with nothing more to look at."""
+    return (type(t) in _TENSORS and t.dtype is dtype and t.shape == shape and t.get_device() == index
+            and t.is_contiguous())
+
+
+def _row_stride(name: str, t: torch.Tensor, dtype: torch.dtype, dev: torch.device) -> int:
+    """The token stride of ``[tokens, heads, head_dim]`` with contiguous heads, a view of wider rows allowed."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
     if t.device.type != "cuda":
@@ -311,34 +325,66 @@ def _check_rows(name: str, t: torch.Tensor, dtype: torch.dtype, dev: torch.devic
     return stride
 
 
-def _check_index(name: str, t: torch.Tensor, ndim: int, dev: torch.device) -> None:
-    _check_gpu(name, t, torch.int32, ndim)
+def _row_strides(rows: tuple, dtype: torch.dtype, dev: torch.device) -> list[int]:
+    """Token strides of the named tensors; the checks in full where one is not a plain contiguous tensor."""
+    index, grad = dev.index, torch.is_grad_enabled()
+    strides = []
+    for name, t in rows:
+        if (type(t) in _TENSORS and t.dtype is dtype and t.get_device() == index and t.dim() == 3 and t.numel()
+                and t.is_contiguous() and not (grad and t.requires_grad)):
+            strides.append(t.shape[1] * t.shape[2])
+        else:
+            strides.append(_row_stride(name, t, dtype, dev))
+    return strides
+
+
+def _check_index(name: str, t: torch.Tensor, shape: tuple, dev: torch.device) -> None:
+    if _plain(t, torch.int32, shape, dev.index):
+        return
+    _check_gpu(name, t, torch.int32, len(shape))
     if t.device != dev:
         raise ValueError(f"tensors on different devices: {dev} vs {t.device}")
+    raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}") if t.shape != shape else TypeError(
+        f"{name} must be a torch.Tensor, got {type(t).__name__}")
 
 
-def _check_heads(dev: torch.device, sinks: torch.Tensor | None, n_heads: int, n_kv: int, window: int | None,
-                 scale: float | None, dim: int) -> tuple[int, float]:
+def _check_heads(sinks: torch.Tensor | None, n_heads: int, n_kv: int, window: int | None, scale: float | None, dim: int,
+                 dev: torch.device) -> tuple[int, int, float]:
+    """The sinks' address, the window as the library takes it, and the scale."""
     if n_heads % n_kv:
         raise ValueError(f"{n_heads} query heads over {n_kv} KV heads")
     if sinks is not None:
-        _check_gpu("sinks", sinks, torch.bfloat16, 1)
-        if sinks.shape[0] != n_heads or sinks.device != dev:
+        if not _plain(sinks, torch.bfloat16, (n_heads,), dev.index):
+            _check_gpu("sinks", sinks, torch.bfloat16, 1)
             raise ValueError(f"sinks must be [{n_heads}] on {dev}, got {tuple(sinks.shape)} on {sinks.device}")
         if sinks.requires_grad and torch.is_grad_enabled():
             raise ValueError("sinks require grad: this operator has no backward pass")
     if window is not None and window <= 0:
         raise ValueError(f"window must be positive (None: no window), got {window}")
-    return min(int(window), (1 << 30) - 1) if window else 0, float(scale) if scale is not None else 1.0 / math.sqrt(dim)
+    return (0 if sinks is None else sinks.data_ptr(), min(int(window), (1 << 30) - 1) if window else 0,
+            dim ** -0.5 if scale is None else float(scale))
 
 
-def _check_out(name: str, out: torch.Tensor | None, shape: tuple, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
+def _result(name: str, out: torch.Tensor | None, shape: tuple, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
     if out is None:
         return torch.empty(shape, dtype=dtype, device=dev)
-    _check_gpu(name, out, dtype)
-    if tuple(out.shape) != tuple(shape) or out.device != dev:
+    if not _plain(out, dtype, shape, dev.index):
+        _check_gpu(name, out, dtype)
         raise ValueError(f"{name} must be {tuple(shape)} on {dev}, got {tuple(out.shape)} on {out.device}")
     return out
+
+
+def _call(name: str, args: bytes, dev: torch.device) -> None:
+    """``name(args, current stream)`` with the tensors' device current."""
+    index = dev.index
+    fn = getattr(nat.load(), name)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
+    if rc < 0:
+        raise nat.KlcError(name, int(rc), nat.last_error())
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor,
@@ -354,36 +400,41 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     dev, dtype = q.device, q.dtype
     if dtype not in _KV_CODES:
         raise TypeError(f"q must be bfloat16 or float16, got {dtype}")
-    strides = [_check_rows(n, t, dtype, dev) for n, t in (("q", q), ("k", k), ("v", v))]
-    tokens, n_heads, dim = q.shape
+    strides = _row_strides((("q", q), ("k", k), ("v", v)), dtype, dev)
+    shape = q.shape
+    tokens, n_heads, dim = shape
     n_kv = k.shape[1]
     if k.shape != (tokens, n_kv, dim) or v.shape != k.shape:
         raise ValueError(f"shapes mismatch: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    _check_index("starts", starts, 1, dev)
-    if starts.shape[0] < 1:
+    n_seq = (starts.shape[0] if isinstance(starts, torch.Tensor) and starts.dim() == 1 else 1) - 1
+    _check_index("starts", starts, (n_seq + 1,), dev)
+    if n_seq < 0:
         raise ValueError("starts must hold the sequences' starts and the end of the last one")
-    window, scale = _check_heads(dev, sinks, n_heads, n_kv, window, scale, dim)
-    out = _check_out("out", out, (tokens, n_heads, dim), dtype, dev)
-    if tokens == 0 or starts.shape[0] == 1:
-        return out
-    with torch.cuda.device(dev):
-        nat.call("klc_attn_prompt", _ptr(q), _ptr(k), _ptr(v), _ptr(starts), _ptr(sinks), tokens, starts.shape[0] - 1,
-                 n_heads, n_kv, dim, *strides, window, scale, _KV_CODES[dtype], _ptr(out), _stream(dev))
+    sink_ptr, window, scale = _check_heads(sinks, n_heads, n_kv, window, scale, dim, dev)
+    out = _result("out", out, shape, dtype, dev)
+    if tokens and n_seq:
+        _call("klc_attn_prompt",
+              _PROMPT_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), starts.data_ptr(), sink_ptr, out.data_ptr(),
+                                tokens, n_seq, n_heads, n_kv, dim, *strides, window, _KV_CODES[dtype], scale), dev)
     return out
 
 
 def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, dev: torch.device) -> tuple[int, int, int, int]:
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        _check_gpu(name, t, None, 4)
-        if t.dtype not in _KV_CODES:
-            raise TypeError(f"{name} must be bfloat16 or float16, got {t.dtype}")
-    if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
-        raise ValueError(f"page pools mismatch: {k_pages.dtype} {tuple(k_pages.shape)}, {v_pages.dtype} {tuple(v_pages.shape)}")
-    if k_pages.device != dev or v_pages.device != dev:
-        raise ValueError(f"tensors on different devices: {dev} vs {k_pages.device}, {v_pages.device}")
+    if not (type(k_pages) in _TENSORS and k_pages.dtype in _KV_CODES and k_pages.dim() == 4 and k_pages.is_contiguous()
+            and k_pages.get_device() == dev.index and _plain(v_pages, k_pages.dtype, k_pages.shape, dev.index)):
+        for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+            _check_gpu(name, t, None, 4)
+            if t.dtype not in _KV_CODES:
+                raise TypeError(f"{name} must be bfloat16 or float16, got {t.dtype}")
+        if k_pages.device != dev or v_pages.device != dev:
+            raise ValueError(f"tensors on different devices: {dev} vs {k_pages.device}, {v_pages.device}")
+        if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+            raise ValueError(f"page pools mismatch: {k_pages.dtype} {tuple(k_pages.shape)}, {v_pages.dtype} {tuple(v_pages.shape)}")
     n_pages, page, n_kv, dim = k_pages.shape
     if n_pages == 0 or page < 16 or page > 4096 or page & (page - 1):
         raise ValueError(f"pages must hold a power of two of tokens, 16 to 4096, got {n_pages} of {page}")
+    if n_kv == 0 or dim == 0:
+        raise ValueError(f"pages of no heads: {tuple(k_pages.shape)}")
     return n_pages, page, n_kv, dim
 
 
@@ -397,27 +448,38 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.T
     if not isinstance(q, torch.Tensor):
         raise TypeError(f"q must be a torch.Tensor, got {type(q).__name__}")
     dev = q.device
-    strides = [_check_rows(n, t, torch.bfloat16, dev) for n, t in (("q", q), ("k", k), ("v", v))]
+    strides = _row_strides((("q", q), ("k", k), ("v", v)), torch.bfloat16, dev)
     tokens, n_heads, dim = q.shape
     n_pages, page, n_kv, page_dim = _check_pages(k_pages, v_pages, dev)
     if k.shape != (tokens, n_kv, dim) or v.shape != k.shape or page_dim != dim:
         raise ValueError(f"shapes mismatch: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, pages {tuple(k_pages.shape)}")
+    n_pos = cos.shape[0] if isinstance(cos, torch.Tensor) and cos.dim() == 2 else 0
     for name, t in (("cos", cos), ("sin", sin)):
-        _check_gpu(name, t, torch.bfloat16, 2)
-        if t.shape[1] * 2 != dim or t.shape != cos.shape or t.shape[0] == 0 or t.device != dev:
+        if not _plain(t, torch.bfloat16, (n_pos, dim // 2), dev.index) or not n_pos:
+            _check_gpu(name, t, torch.bfloat16, 2)
             raise ValueError(f"{name} must be [positions, {dim // 2}] on {dev}, got {tuple(t.shape)} on {t.device}")
-    for name, t in (("positions", positions), ("slots", slots)):
-        _check_index(name, t, 1, dev)
-        if t.shape[0] != tokens:
-            raise ValueError(f"{name} of {t.shape[0]} tokens, not {tokens}")
-    q_out = torch.empty((tokens, n_heads, dim), dtype=torch.bfloat16, device=dev)
-    k_out = torch.empty((tokens, n_kv, dim), dtype=torch.bfloat16, device=dev) if want_keys else None
+    _check_index("positions", positions, (tokens,), dev)
+    _check_index("slots", slots, (tokens,), dev)
+    q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
+    k_out = torch.empty(k.shape, dtype=torch.bfloat16, device=dev) if want_keys else None
     if tokens:
-        with torch.cuda.device(dev):
-            nat.call("klc_kv_append", _ptr(q), _ptr(k), _ptr(v), _ptr(cos), _ptr(sin), _ptr(positions), _ptr(slots),
-                     tokens, cos.shape[0], n_pages * page, n_heads, n_kv, dim, *strides, _KV_CODES[k_pages.dtype],
-                     _ptr(q_out), _ptr(k_out), _ptr(k_pages), _ptr(v_pages), _stream(dev))
+        _call("klc_kv_append",
+              _APPEND_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+                                positions.data_ptr(), slots.data_ptr(), q_out.data_ptr(),
+                                k_out.data_ptr() if want_keys else 0, k_pages.data_ptr(), v_pages.data_ptr(), tokens,
+                                n_pos, n_pages * page, n_heads, n_kv, dim, *strides, _KV_CODES[k_pages.dtype]), dev)
     return q_out, k_out
+
+
+def _page_numbers(x) -> np.ndarray:
+    a = np.asarray(x)
+    if a.dtype != np.int32:
+        if a.size and a.dtype.kind not in "iu":
+            raise TypeError(f"page numbers must be whole numbers, got {a.dtype}")
+        if a.size and (a.min() < 0 or a.max() > 0x7FFFFFFF):
+            raise ValueError("page numbers must be in [0, 2^31)")
+        a = a.astype(np.int32)
+    return np.ascontiguousarray(a)
 
 
 def copy_pages(pools: torch.Tensor, src, dst) -> None:
@@ -427,23 +489,19 @@ def copy_pages(pools: torch.Tensor, src, dst) -> None:
     _check_gpu("pools", pools)
     if pools.dim() < 3 or pools.numel() == 0:
         raise ValueError(f"pools must be [pools, pages, ...], got shape {tuple(pools.shape)}")
-    src, dst = (np.ascontiguousarray(x, dtype=np.int64) for x in (src, dst))
+    src, dst = _page_numbers(src), _page_numbers(dst)
     if src.ndim != 1 or src.shape != dst.shape:
         raise ValueError(f"source and destination pages mismatch: {src.shape} and {dst.shape}")
-    n_pages = pools.shape[1]
-    if not src.size:
-        return
-    if min(src.min(), dst.min()) < 0 or max(src.max(), dst.max()) >= n_pages:
-        raise ValueError(f"page numbers must be in [0, {n_pages})")
-    once = np.zeros(n_pages, dtype=bool)
-    once[dst] = True
-    if int(once.sum()) != dst.size or once[src].any():
-        raise ValueError("a destination page is another move's source or destination")
-    page_bytes = math.prod(pools.shape[2:]) * pools.element_size()
-    src, dst = src.astype(np.int32), dst.astype(np.int32)
-    with torch.cuda.device(pools.device):
-        nat.call("klc_kv_copy_pages", _ptr(pools), pools.shape[0], n_pages, page_bytes, ctypes.c_void_p(src.ctypes.data),
-                 ctypes.c_void_p(dst.ctypes.data), src.size, _stream(pools.device))
+    dev = pools.device
+    n_pools, n_pages = pools.shape[:2]
+    page_bytes = pools.stride(1) * pools.element_size() if n_pages > 1 else pools[0].numel() * pools.element_size()
+    with torch.cuda.device(dev) if torch._C._cuda_getDevice() != dev.index else contextlib.nullcontext():
+        rc = nat.load().klc_kv_copy_pages(pools.data_ptr(), n_pools, n_pages, page_bytes, src.ctypes.data, dst.ctypes.data,
+                                          src.size, torch._C._cuda_getCurrentRawStream(dev.index))
+    if rc == nat.KLC_ERR_ARGUMENT:
+        raise ValueError(nat.last_error())
+    if rc < 0:
+        raise nat.KlcError("klc_kv_copy_pages", int(rc), nat.last_error())
 
 
 def batch_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor,
@@ -457,36 +515,42 @@ def batch_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if not isinstance(q, torch.Tensor):
         raise TypeError(f"q must be a torch.Tensor, got {type(q).__name__}")
     dev = q.device
-    stride = _check_rows("q", q, torch.bfloat16, dev)
-    count, n_heads, dim = q.shape
+    stride, = _row_strides((("q", q),), torch.bfloat16, dev)
+    shape = q.shape
+    count, n_heads, dim = shape
     n_pages, page, n_kv, page_dim = _check_pages(k_pages, v_pages, dev)
     if page_dim != dim:
         raise ValueError(f"shapes mismatch: q {tuple(q.shape)}, pages {tuple(k_pages.shape)}")
-    _check_index("tables", tables, 2, dev)
-    _check_index("lengths", lengths, 1, dev)
-    if tables.shape[0] != count or lengths.shape[0] != count:
-        raise ValueError(f"tables {tuple(tables.shape)} and lengths {tuple(lengths.shape)} for {count} sequences")
+    width = tables.shape[1] if isinstance(tables, torch.Tensor) and tables.dim() == 2 else 0
+    _check_index("tables", tables, (count, width), dev)
+    _check_index("lengths", lengths, (count,), dev)
     prefix_len = int(prefix_len)
     if prefix_len < 0:
         raise ValueError(f"prefix_len must not be negative, got {prefix_len}")
     if prefix_len:
         if prefix_table is None:
             raise ValueError("prefix_len without a prefix_table")
-        _check_index("prefix_table", prefix_table, 1, dev)
-        if prefix_table.shape[0] * page < prefix_len:
-            raise ValueError(f"prefix of {prefix_len} tokens in {prefix_table.shape[0]} pages of {page}")
-    window, scale = _check_heads(dev, sinks, n_heads, n_kv, window, scale, dim)
-    out = _check_out("out", out, (count, n_heads, dim), torch.bfloat16, dev)
+        held = prefix_table.shape[0] if isinstance(prefix_table, torch.Tensor) and prefix_table.dim() == 1 else 0
+        _check_index("prefix_table", prefix_table, (held,), dev)
+        if held * page < prefix_len:
+            raise ValueError(f"prefix of {prefix_len} tokens in {held} pages of {page}")
+    sink_ptr, window, scale = _check_heads(sinks, n_heads, n_kv, window, scale, dim, dev)
+    out = _result("out", out, shape, torch.bfloat16, dev)
     if not count:
         return out
-    width = tables.shape[1]
-    nbytes = nat.call("klc_attn_batch_workspace_bytes", count, n_heads, n_kv, dim, prefix_len, width * page, window)
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        nat.call("klc_attn_batch", _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(tables if width else None), _ptr(lengths),
-                 _ptr(prefix_table if prefix_len else None), _ptr(sinks), count, n_heads, n_kv, dim, stride, n_pages,
-                 page, width, prefix_len, window, scale, _KV_CODES[k_pages.dtype], _ptr(workspace), nbytes, _ptr(out),
-                 _stream(dev))
+    sizes = (count, n_heads, n_kv, dim, prefix_len, width * page, window)
+    nbytes = _batch_bytes.get(sizes)
+    if nbytes is None:
+        if len(_batch_bytes) > 4096:
+            _batch_bytes.clear()
+        nbytes = _batch_bytes[sizes] = nat.call("klc_attn_batch_workspace_bytes", *sizes)
+    # of this call alone: calls on other streams and captured graphs have theirs
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _call("klc_attn_batch",
+          _BATCH_ARGS.pack(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr() if width else 0,
+                           lengths.data_ptr(), prefix_table.data_ptr() if prefix_len else 0, sink_ptr,
+                           workspace.data_ptr() if nbytes else 0, out.data_ptr(), count, n_heads, n_kv, dim, stride,
+                           n_pages, page, width, prefix_len, window, _KV_CODES[k_pages.dtype], nbytes, scale), dev)
     return out
 
 

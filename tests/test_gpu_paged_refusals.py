@@ -101,5 +101,5 @@ def test_copy_refusals(gpu):
             ops.copy_pages(pool, src, dst)
     with pytest.raises(ValueError):
         ops.copy_pages(pool.transpose(0, 1), [0], [1])
-    with pytest.raises(RuntimeError, match="multiple of 16"):
+    with pytest.raises(ValueError, match="multiple of 16"):
         ops.copy_pages(torch.zeros((2, 6, 12), dtype=torch.int8, device=gpu), [0], [1])
