@@ -143,9 +143,8 @@ __device__ __forceinline__ void shared_part(const BatchArgs& a, int wg, lds_u8 r
       const PageRow p = page_row(a.prefix_table, j * KT + n * F::kRowsPerDma, j * KT + r, 0, a.prefix - 1, a.page_log2, a.n_pages);
       bad |= p.bad;
       const int64_t at = p.row * kv_stride + (int64_t)kvh * a.d + 8 * F::dma_chunk(r, a.d);
-      typedef __attribute__((address_space(3))) void* lds_void;
-      __builtin_amdgcn_global_load_lds(a.k_pages + at, (lds_void)(stage + n * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(a.v_pages + at, (lds_void)(stage + F::kMatBytes + n * 1024), 16, 0, 0);
+      load_to_lds(a.k_pages + at, stage + n * 1024);
+      load_to_lds(a.v_pages + at, stage + F::kMatBytes + n * 1024);
     }
   };
 #pragma unroll
@@ -237,9 +236,8 @@ __device__ __forceinline__ void own_part(const BatchArgs& a, int wg, lds_u8 lds,
       const PageRow p = page_row(own ? own_table : a.prefix_table, base + i * F::kRowsPerDma, base + r, visible, last, a.page_log2, a.n_pages);
       bad |= p.bad;
       const int64_t at = p.row * kv_stride + (int64_t)kvh * a.d + 8 * F::dma_chunk(r, a.d);
-      typedef __attribute__((address_space(3))) void* lds_void;
-      __builtin_amdgcn_global_load_lds(a.k_pages + at, (lds_void)(stage + i * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(a.v_pages + at, (lds_void)(stage + F::kMatBytes + i * 1024), 16, 0, 0);
+      load_to_lds(a.k_pages + at, stage + i * 1024);
+      load_to_lds(a.v_pages + at, stage + F::kMatBytes + i * 1024);
     }
   };
   if (first < end_tile) load(first, 0);

@@ -60,6 +60,18 @@ __device__ __forceinline__ float add2(uint32_t p, float acc) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, p), bf16x2_t{(__bf16)1.f, (__bf16)1.f}, acc, false);
 }
 
+// 16 bytes a lane from memory to dst + 16 lane of LDS (dst uniform), counted
+// by vmcnt.  In assembly because the compiler, told of the load, waits for
+// every load in flight before any LDS read that might meet it; the kernels'
+// own waits order them by tile.  It has no output register, nothing reads its
+// LDS before those waits, and nothing else in these kernels uses m0.
+__device__ __forceinline__ void load_to_lds(const uint16_t* src, lds_u8 dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"((uint32_t)(uintptr_t)dst), "v"(src)
+               : "memory");
+}
+
 // the other half's value beside the lane's own: both halves get the same pair
 __device__ __forceinline__ float max_halves(float v) {
   const uint32_t u = __float_as_uint(v);

@@ -83,10 +83,9 @@ __device__ __forceinline__ bool prompt_rows(const PromptArgs& a, const PromptTil
       const int n = wave + i * W, r = F::dma_row(n);
       const int64_t key = min(base + r, t.len - 1);
       const int c = 8 * F::dma_chunk(r, a.d);
-      typedef __attribute__((address_space(3))) void* lds_void;
       const lds_u8 dst = ring + stage + n * 1024;
-      __builtin_amdgcn_global_load_lds(kb + key * a.k_stride + c, (lds_void)dst, 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(vb + key * a.v_stride + c, (lds_void)(dst + F::kMatBytes), 16, 0, 0);
+      load_to_lds(kb + key * a.k_stride + c, dst);
+      load_to_lds(vb + key * a.v_stride + c, dst + F::kMatBytes);
     }
   };
 #pragma unroll
