@@ -3,15 +3,16 @@
 //
 // One launch with two kinds of workgroups, so that the compute-bound prefix
 // and the sequences' own keys, a stream from HBM, share the chip:
-//   shared  a KV head, 128 query rows (sequence, head of the group) and a
-//           range of the prefix: 4 waves x 32 rows over one ring of tiles, the
-//           prefix's keys read once for the batch
+//   shared  a KV head, 64 query rows (sequence, head of the group) and a range
+//           of the prefix: its 4 waves are 2 blocks of 32 rows x 2 halves of
+//           each tile of keys, over one ring of tiles
 //   own     a KV head of one sequence and a range of its own keys (with a
 //           window, or a prefix not worth the pass above, of all its keys):
-//           its waves take tiles in turn, each through a ring of its own with
-//           no barrier, and join their sums in LDS
-// Parts are float32 (sum, maximum, normaliser) and a second launch joins
-// them; where a row has one part, the own workgroup writes the result itself.
+//           1, 2 or 4 waves take its tiles in turn, each through a ring of its
+//           own with no barrier
+// Two workgroups fit a CU by LDS and registers.  Parts are float32 (sum,
+// maximum, normaliser) and a second launch joins them; where a row has one
+// part, the own workgroup writes the result itself.
 #include <math.h>
 
 #include "klc_flash.h"
@@ -20,15 +21,12 @@ namespace klc {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int kOwnTile = 32;      // keys of a tile of an own wave
-constexpr int kOwnRing = 2;
+constexpr int kWaveTile = 32;     // keys that a wave takes at once
+constexpr int kRowBlocks = 2;     // of 32 rows, in a shared workgroup
+constexpr int kKeyParts = kWaves / kRowBlocks;
 constexpr int kBatchGroup = 32;   // most query heads of a KV head: the columns of a wave's matrix instruction
 constexpr int kPrefixAlign = 64;  // own keys start at a multiple of this in a sequence's list of keys
-// a shared tile is 16 KB of K and V, four of them the LDS of a head size of 64
-template <int DP>
-constexpr int kSharedTile = DP == 64 ? 64 : 32;
-template <int DP>
-constexpr int kBatchLds = kWaves * kOwnRing * 2 * kOwnTile * 2 * DP;
+constexpr int kBatchLds = 64 * 1024;
 
 struct BatchArgs {
   const uint16_t* q;                   // bfloat16 [n_seq] rows
@@ -40,7 +38,9 @@ struct BatchArgs {
   float* part_o;                       // [n_seq * n_heads][splits][d]
   float2* part_ml;                     // [n_seq * n_heads][splits]
   int64_t q_stride;
-  int n_seq, n_heads, n_kv, d, n_pages, page_log2, width, prefix, window, shared_splits, own_splits, shared_tiles, shared_wgs;
+  int n_seq, n_heads, n_kv, d, n_pages, page_log2, width, prefix, window;
+  int shared_splits, shared_tiles, shared_wgs;  // parts of the prefix, tiles of one, workgroups
+  int own_splits, own_waves;                    // parts of a sequence's keys, waves of one
   float c2;
 };
 
@@ -50,35 +50,40 @@ __device__ __forceinline__ int32_t table_at(const int32_t* t, int64_t i) {
   return reinterpret_cast<const_i32>(reinterpret_cast<uintptr_t>(t))[i];
 }
 
-// Chunk c of a bfloat16 query row for each of the wave's steps, in the
-// cache's type.  A float16 cache takes the row times a power of two that
-// brings its largest value to [1, 2), which every float16 represents as well
-// as bfloat16 does (what it rounds off lies 2^-24 below that value); the
-// returned factor puts it back.
-template <class F, bool kF16>
-__device__ __forceinline__ float load_query(u32x4_t (&q)[F::kSteps], const uint16_t* src, int d) {
-  const int lane = threadIdx.x % kWave;
+// A lane's chunks of its bfloat16 query row, as they are.
+template <class F>
+__device__ __forceinline__ void load_query(u32x4_t (&q)[F::kSteps], const uint16_t* src, int d) {
 #pragma unroll
   for (int st = 0; st < F::kSteps; ++st) {
-    const int c = 2 * st + lane / 32;
+    const int c = 2 * st + (int)(threadIdx.x % kWave) / 32;
     q[st] = u32x4_t{0, 0, 0, 0};
-    if (8 * c < d) q[st] = *reinterpret_cast<const u32x4_t*>(src + 8 * c);
+    if (F::kWhole || 8 * c < d) q[st] = *reinterpret_cast<const u32x4_t*>(src + 8 * c);
   }
+}
+
+// The row in the cache's type.  A float16 cache takes it times a power of two
+// that brings its largest value to [1, 2): float16 then represents every value
+// as bfloat16 does, but for what lies 2^-24 below that one.  The returned
+// factor puts it back.
+template <class F, bool kF16>
+__device__ __forceinline__ float convert_query(u32x4_t (&q)[F::kSteps]) {
   if constexpr (!kF16) return 1.f;
-  float most = 0.f;
+  uint32_t most = 0;  // bit patterns of positive floats are in their order; NaN and infinity above 0x7f7f
+#pragma unroll
+  for (int st = 0; st < F::kSteps; ++st)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) most = max(most, max(q[st][e] << 16 & 0x7fffffffu, q[st][e] & 0x7fff0000u));
+  const auto both = __builtin_amdgcn_permlane32_swap(most, most, false, false);
+  most = max(both[0], both[1]);
+  int ex = (int)(most >> 23) - 127;
+  if (most >= 0x7f800000u || most == 0) ex = 0;
 #pragma unroll
   for (int st = 0; st < F::kSteps; ++st)
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      most = fmaxf(most, fmaxf(fabsf(__uint_as_float(q[st][e] << 16)), fabsf(__uint_as_float(q[st][e] & 0xffff0000u))));
-  most = max_halves(most);
-  const int ex = most > 0.f && most < INFINITY ? ilogbf(most) : 0;
-#pragma unroll
-  for (int st = 0; st < F::kSteps; ++st)
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      q[st][e] = pack2<true>(ldexpf(__uint_as_float(q[st][e] << 16), -ex), ldexpf(__uint_as_float(q[st][e] & 0xffff0000u), -ex));
-  return ldexpf(1.f, ex);
+      q[st][e] = pack2<true>(__builtin_amdgcn_ldexpf(__uint_as_float(q[st][e] << 16), -ex),
+                             __builtin_amdgcn_ldexpf(__uint_as_float(q[st][e] & 0xffff0000u), -ex));
+  return __builtin_amdgcn_ldexpf(1.f, ex);
 }
 
 // A lane's source row of a load instruction: `key` is the instruction's first
@@ -104,125 +109,139 @@ __device__ __forceinline__ void tile_wait() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
 }
 
-// Clears the V rows of a tile outside [from, to), whose values no query sees
-// (0 * inf would make NaN of them); the caller orders it.
-template <class F, int KT>
-__device__ __forceinline__ void clear_values(lds_u8 stage, int from, int to, int thread, int threads) {
-  for (int i = thread; i < KT * F::kChunks; i += threads) {
-    const int r = i / F::kChunks;
-    if (r < from || r >= to)
-      *reinterpret_cast<__attribute__((address_space(3))) u32x4_t*>(stage + F::kMatBytes + i * 16) = u32x4_t{0, 0, 0, 0};
-  }
+// Four dims of a wave's sums, as its lane holds them: block e of 32 dims / 8.
+template <class F>
+__device__ __forceinline__ f32x4_t quad(const F& f, int i) {
+  const f32x16_t& o = f.o[0][i / 4];
+  const int e = i % 4 * 4;
+  return f32x4_t{o[e], o[e + 1], o[e + 2], o[e + 3]};
 }
+// the first of them
+__device__ __forceinline__ int quad_dim(int i) { return 8 * i + 4 * ((int)(threadIdx.x % kWave) / 32); }
 
-// The prefix's part of 128 query rows: workgroup (KV head, tile of rows,
-// split of the keys).
+// The prefix's part of 64 query rows: workgroup (KV head, split of the keys,
+// tile of rows).
 template <int DP, bool kF16, bool kFull>
 __device__ __forceinline__ void shared_part(const BatchArgs& a, int wg, lds_u8 ring) {
-  constexpr int KT = kSharedTile<DP>, W = kWaves;
-  using F = Flash<DP, kF16, kFull, 1, KT>;
-  constexpr int kRing = kBatchLds<DP> / F::kStage, kLoads = 2 * F::kDmas / W;
-  static_assert(F::kDmas % W == 0 && kRing >= 3, "the tile's loads split evenly over the waves");
+  constexpr int KT = kWaveTile * kKeyParts;
+  using F = Flash<DP, kF16, kFull, 1, kWaveTile>;
+  constexpr int kMat = kKeyParts * F::kMatBytes, kStage = 2 * kMat, kRing = kBatchLds / kStage;
+  constexpr int kDmas = kKeyParts * F::kDmas / kWaves;  // of K, and of V, a wave and tile
+  constexpr int kQuads = 4 * F::kDimBlocks;
   const int g = a.n_heads / a.n_kv, rows = a.n_seq * g;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int kvh = wg % a.n_kv, split = wg / a.n_kv % a.shared_splits, row_tile = wg / (a.n_kv * a.shared_splits);
   const int first = split * a.shared_tiles, end_tile = min(first + a.shared_tiles, (a.prefix + KT - 1) / KT);
-  const int w_row = (row_tile * W + wave) * 32;
+  const int block = wave % kRowBlocks, part = wave / kRowBlocks;
+  const int w_row = (row_tile * kRowBlocks + block) * 32;
   const bool w_live = w_row < rows;
   const int row = min(w_row + lane % 32, rows - 1), b = row / g, head = kvh * g + row - b * g;
   F f;
   f.init(ring, a.d);
-  const float c2 = a.c2 * load_query<F, kF16>(f.q[0], a.q + b * a.q_stride + (int64_t)head * a.d, a.d);
+  load_query<F>(f.q[0], a.q + b * a.q_stride + (int64_t)head * a.d, a.d);
   const int64_t kv_stride = (int64_t)a.n_kv * a.d;
   bool bad = false;
   auto load = [&](int j) {
-    const lds_u8 stage = ring + ((j - first) % kRing) * F::kStage;
+    const lds_u8 stage = ring + ((j - first) % kRing) * kStage;
 #pragma unroll
-    for (int i = 0; i < F::kDmas / W; ++i) {
-      const int n = wave + i * W, r = F::dma_row(n);
+    for (int i = 0; i < kDmas; ++i) {
+      const int n = wave + i * kWaves, r = F::dma_row(n);
       const PageRow p = page_row(a.prefix_table, j * KT + n * F::kRowsPerDma, j * KT + r, 0, a.prefix - 1, a.page_log2, a.n_pages);
       bad |= p.bad;
       const int64_t at = p.row * kv_stride + (int64_t)kvh * a.d + 8 * F::dma_chunk(r, a.d);
       load_to_lds(a.k_pages + at, stage + n * 1024);
-      load_to_lds(a.v_pages + at, stage + F::kMatBytes + n * 1024);
+      load_to_lds(a.v_pages + at, stage + kMat + n * 1024);
     }
   };
 #pragma unroll
   for (int i = 0; i < kRing - 1; ++i)
     if (first + i < end_tile) load(first + i);
+  const float c2 = a.c2 * convert_query<F, kF16>(f.q[0]);
   for (int j = first; j < end_tile; ++j) {
     if (j + kRing - 2 < end_tile)
-      tile_wait<kLoads*(kRing - 2), true>();
+      tile_wait<2 * kDmas * (kRing - 2), true>();
     else
       tile_wait<0, true>();
     if (j + kRing - 1 < end_tile) load(j + kRing - 1);
-    const int stage = ((j - first) % kRing) * F::kStage;
+    const int stage = ((j - first) % kRing) * kStage, mine = part * F::kMatBytes;
     const int left = a.prefix - j * KT;
     if (left < KT) {
-      clear_values<F, KT>(ring + stage, 0, left, threadIdx.x, 64 * W);
+      clear_values<F, KT>(ring + stage + kMat, 0, left, threadIdx.x, kWave * kWaves);
       tile_wait<0, true>();
     }
-    if (!w_live) continue;
-    f32x16_t sc[1][KT / 32];
-    f.scores(stage, sc);
+    if (!w_live || left <= part * kWaveTile) continue;
+    f32x16_t sc[1][1];
+    f.scores(stage + mine, sc);
     if (left < KT) {
 #pragma unroll
-      for (int kb = 0; kb < KT / 32; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (32 * kb + 8 * (e / 4) + e % 4 + 4 * (lane / 32) >= left) sc[0][kb][e] = -INFINITY;
+      for (int e = 0; e < 16; ++e)
+        if (part * kWaveTile + 8 * (e / 4) + e % 4 + 4 * (lane / 32) >= left) sc[0][0][e] = -INFINITY;
     }
-    u32x4_t p[1][KT / 16];
+    u32x4_t p[1][2];
     f.softmax(0, sc[0], c2, p[0]);
-    f.values(stage, p);
+    f.values(stage + kMat + mine, p);
   }
+
+  // the key parts' sums, lane by lane: [block][quad][lane], [block][lane]
+  static_assert(kKeyParts == 2, "one part hands its sums to the other");
   bad = __syncthreads_or(bad);
-  const float sum = add_halves(f.l[0]);
-  if (w_row + lane % 32 >= rows) return;
+  typedef __attribute__((address_space(3))) f32x4_t* lds_f32x4;
+  typedef __attribute__((address_space(3))) f32x2_t* lds_f32x2;
+  const lds_f32x4 sums = (lds_f32x4)ring + block * kQuads * kWave + lane;
+  const lds_f32x2 ml = (lds_f32x2)(ring + kRowBlocks * kQuads * kWave * 16) + block * kWave + lane;
+  float m = f.m[0], l = add_halves(f.l[0]);
+  if (part == 1) {
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) sums[i * kWave] = quad(f, i);
+    *ml = f32x2_t{m, l};
+  }
+  __syncthreads();
+  if (part == 1 || w_row + lane % 32 >= rows) return;
+  const f32x2_t other = *ml;
+  const float top = fmaxf(m, other.x), base = top == -INFINITY ? 0.f : top;
+  const float x = __builtin_amdgcn_exp2f(m - base), y = __builtin_amdgcn_exp2f(other.x - base);
   const int64_t at = ((int64_t)b * a.n_heads + head) * (a.shared_splits + a.own_splits) + split;
-  if (lane < 32) a.part_ml[at] = make_float2(f.m[0], bad ? __uint_as_float(0x7fc00000u) : sum);
-  float* dst = a.part_o + at * a.d + 4 * (lane / 32);
+  if (lane < 32) a.part_ml[at] = make_float2(top, bad ? __uint_as_float(0x7fc00000u) : x * l + y * other.y);
+  float* dst = a.part_o + at * a.d;
 #pragma unroll
-  for (int db = 0; db < F::kDimBlocks; ++db)
-#pragma unroll
-    for (int e = 0; e < 16; e += 4) {
-      const int dim = 32 * db + 2 * e;
-      if (!kFull && dim + 4 * (lane / 32) >= a.d) continue;
-      *reinterpret_cast<float4*>(dst + dim) = make_float4(f.o[0][db][e], f.o[0][db][e + 1], f.o[0][db][e + 2], f.o[0][db][e + 3]);
-    }
+  for (int i = 0; i < kQuads; ++i) {
+    if (!kFull && quad_dim(i) >= a.d) continue;
+    *reinterpret_cast<f32x4_t*>(dst + quad_dim(i)) = x * quad(f, i) + y * sums[i * kWave];
+  }
 }
 
-// A sequence's own part, and without a shared pass its part of the prefix.
-// The keys are listed as [prefix, padded to kPrefixAlign][own].
+// A sequence's own part, and without a shared pass its part of the prefix:
+// own_waves waves take item (KV head, split, sequence).  The keys are listed
+// as [prefix, padded to kPrefixAlign][own].
 template <int DP, bool kF16, bool kFull>
 __device__ __forceinline__ void own_part(const BatchArgs& a, int wg, lds_u8 lds, float2 (&wave_ml)[kWaves][kBatchGroup]) {
-  using F = Flash<DP, kF16, kFull, 1, kOwnTile>;
-  constexpr int KT = kOwnTile, kLoads = 2 * F::kDmas;
+  using F = Flash<DP, kF16, kFull, 1, kWaveTile>;
+  constexpr int KT = kWaveTile, kLoads = 2 * F::kDmas, kRing = kBatchLds / kWaves / F::kStage, kQuads = 4 * F::kDimBlocks;
+  static_assert(kRing == 1 || kRing == 2, "");
   const int g = a.n_heads / a.n_kv, lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int kvh = wg % a.n_kv, split = wg / a.n_kv % a.own_splits, b = wg / (a.n_kv * a.own_splits);
+  const int team = a.own_waves, rank = wave % team;  // the item's waves, and which of them this is
+  const int items = a.n_kv * a.own_splits * a.n_seq, item = min(wg * (kWaves / team) + wave / team, items - 1);
+  const bool spare = wg * (kWaves / team) + wave / team >= items;  // past the last item: nothing to do but the barriers
+  const int kvh = item % a.n_kv, split = item / a.n_kv % a.own_splits, b = item / (a.n_kv * a.own_splits);
   const int splits = a.shared_splits + a.own_splits;
   int n = table_at(a.lengths, b);
-  if (n < 0) {  // no sequence: zeros, here or from the join
-    if (splits == 1)
-      for (int i = threadIdx.x; i < g * a.d; i += kWaves * kWave) a.out[((int64_t)b * a.n_heads + kvh * g) * a.d + i] = 0;
-    return;
-  }
-  const lds_u8 ring = lds + wave * kOwnRing * F::kStage;
+  const bool absent = n < 0;
   const int64_t room = (int64_t)a.width << a.page_log2;
   bool bad = n > room;
-  n = (int)min((int64_t)n, room);
+  n = (int)min((int64_t)max(n, 0), room);
   const int pad = (a.prefix + kPrefixAlign - 1) / kPrefixAlign * kPrefixAlign;
   // the list's visible range: from `begin` on, up to the prefix's end in its tiles and `end` in the others
   const int seen = a.window > 0 ? min(a.window, a.prefix + n) : a.prefix + n, low = a.prefix + n - seen;
   const int begin = a.shared_splits > 0 || low >= a.prefix ? pad + max(0, low - a.prefix) : low;
   const int end = n > 0 ? pad + n : a.prefix;
-  const int first_tile = begin / KT, n_tiles = begin < end ? (end - 1) / KT + 1 - first_tile : 0;
+  const int first_tile = begin / KT, n_tiles = begin < end && !spare && !absent ? (end - 1) / KT + 1 - first_tile : 0;
   const int per = (n_tiles + a.own_splits - 1) / a.own_splits;
-  const int end_tile = first_tile + min((split + 1) * per, n_tiles), first = first_tile + split * per + wave;
-  const int col = min(lane % 32, g - 1), head = kvh * g + col;
+  const int end_tile = first_tile + min((split + 1) * per, n_tiles), first = first_tile + split * per + rank;
+  const lds_u8 ring = lds + wave * kRing * F::kStage;
+  const int head = kvh * g + min(lane % 32, g - 1);
   F f;
   f.init(ring, a.d);
-  const float c2 = a.c2 * load_query<F, kF16>(f.q[0], a.q + b * a.q_stride + (int64_t)head * a.d, a.d);
+  load_query<F>(f.q[0], a.q + b * a.q_stride + (int64_t)head * a.d, a.d);
   const int64_t kv_stride = (int64_t)a.n_kv * a.d;
   const int32_t* own_table = a.tables + (int64_t)b * a.width;
   auto load = [&](int j, int slot) {
@@ -240,11 +259,13 @@ __device__ __forceinline__ void own_part(const BatchArgs& a, int wg, lds_u8 lds,
       load_to_lds(a.v_pages + at, stage + F::kMatBytes + i * 1024);
     }
   };
-  if (first < end_tile) load(first, 0);
-  if (first + kWaves < end_tile) load(first + kWaves, 1);
+#pragma unroll
+  for (int i = 0; i < kRing; ++i)
+    if (first + i * team < end_tile) load(first + i * team, i);
+  const float c2 = a.c2 * convert_query<F, kF16>(f.q[0]);
   int slot = 0;
-  for (int j = first; j < end_tile; j += kWaves) {
-    if (j + kWaves < end_tile)
+  for (int j = first; j < end_tile; j += team) {
+    if (kRing == 2 && j + team < end_tile)
       tile_wait<kLoads, false>();
     else
       tile_wait<0, false>();
@@ -252,10 +273,10 @@ __device__ __forceinline__ void own_part(const BatchArgs& a, int wg, lds_u8 lds,
     const int from = max(0, begin - j * KT), to = min(KT, (j * KT >= pad ? end : a.prefix) - j * KT);
     const bool part = from > 0 || to < KT;
     if (part) {
-      clear_values<F, KT>(ring + stage, from, to, lane, kWave);
+      clear_values<F, KT>(ring + stage + F::kMatBytes, from, to, lane, kWave);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    f32x16_t sc[1][KT / 32];
+    f32x16_t sc[1][1];
     f.scores(stage, sc);
     if (part) {
 #pragma unroll
@@ -264,73 +285,75 @@ __device__ __forceinline__ void own_part(const BatchArgs& a, int wg, lds_u8 lds,
         if (key < from || key >= to) sc[0][0][e] = -INFINITY;
       }
     }
-    u32x4_t p[1][KT / 16];
+    u32x4_t p[1][2];
     f.softmax(0, sc[0], c2, p[0]);
-    f.values(stage, p);
-    if (j + 2 * kWaves < end_tile) {
+    f.values(stage + F::kMatBytes, p);
+    if (j + kRing * team < end_tile) {
       tile_wait<63, false>();  // the slot's reads are done
-      load(j + 2 * kWaves, slot);
+      load(j + kRing * team, slot);
     }
-    slot ^= 1;
+    slot = (slot + 1) % kRing;
   }
 
-  // the waves' sums: [wave][head of the group][d], rows 16 bytes apart from a multiple of the banks
-  __syncthreads();
-  const int stride = a.d + 4;
-  typedef __attribute__((address_space(3))) float* lds_f32;
+  // the team's sums, lane by lane: [wave][quad][lane]
   typedef __attribute__((address_space(3))) f32x4_t* lds_f32x4;
-  const lds_f32 sums = (lds_f32)lds;
+  const lds_f32x4 sums = (lds_f32x4)lds;
   const float sum = add_halves(f.l[0]);
-  if (lane % 32 < g) {
-    if (lane < 32) wave_ml[wave][lane] = make_float2(f.m[0], bad ? __uint_as_float(0x7fc00000u) : sum);
-    const lds_f32 dst = sums + (wave * g + lane % 32) * stride + 4 * (lane / 32);
+  const bool live = lane % 32 < g;
+  if (team > 1) {
+    __syncthreads();
+    if (live) {
+      if (lane < 32) wave_ml[wave][lane] = make_float2(f.m[0], bad ? __uint_as_float(0x7fc00000u) : sum);
 #pragma unroll
-    for (int db = 0; db < F::kDimBlocks; ++db)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int dim = 32 * db + 2 * e;
-        if (!kFull && dim + 4 * (lane / 32) >= a.d) continue;
-        *(lds_f32x4)(dst + dim) = f32x4_t{f.o[0][db][e], f.o[0][db][e + 1], f.o[0][db][e + 2], f.o[0][db][e + 3]};
-      }
+      for (int i = 0; i < kQuads; ++i) sums[(wave * kQuads + i) * kWave + lane] = quad(f, i);
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  const int quads = a.d / 4;
-  for (int i = threadIdx.x; i < g * quads; i += kWaves * kWave) {
-    const int h = i / quads, dim = 4 * (i - h * quads);
-    float2 ml[kWaves];
-    float top = -INFINITY, sink = -INFINITY;
+  if (!live || spare) return;
+  const int64_t row = (int64_t)b * a.n_heads + head, at = row * splits + a.shared_splits + split;
+  float2 ml[kWaves];
+  float sink = -INFINITY;
+  if (splits == 1 && a.sinks != nullptr) sink = sink_log2(a.sinks[head]);
+  float top = sink;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      ml[w] = wave_ml[w][h];
-      top = fmaxf(top, ml[w].x);
-    }
-    if (splits == 1 && a.sinks != nullptr) top = fmaxf(top, sink = sink_log2(a.sinks[kvh * g + h]));
-    const float base = top == -INFINITY ? 0.f : top;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
+  for (int w = 0; w < kWaves; ++w) {
+    ml[w] = make_float2(-INFINITY, 0.f);
+    if (w < team) ml[w] = team > 1 ? wave_ml[wave - rank + w][lane % 32] : make_float2(f.m[0], bad ? __uint_as_float(0x7fc00000u) : sum);
+    top = fmaxf(top, ml[w].x);
+  }
+  const float base = top == -INFINITY ? 0.f : top;
+  float x[kWaves], l = sink != -INFINITY ? __builtin_amdgcn_exp2f(sink - base) : 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float x = __builtin_amdgcn_exp2f(ml[w].x - base);
-      const f32x4_t y = *(lds_f32x4)(sums + (w * g + h) * stride + dim);
-      l = fmaf(x, ml[w].y, l);
-      o.x = fmaf(x, y.x, o.x), o.y = fmaf(x, y.y, o.y), o.z = fmaf(x, y.z, o.z), o.w = fmaf(x, y.w, o.w);
-    }
-    const int64_t row = (int64_t)b * a.n_heads + kvh * g + h;
-    if (splits == 1) {
-      if (sink != -INFINITY) l += __builtin_amdgcn_exp2f(sink - base);
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      *reinterpret_cast<u32x2_t*>(a.out + row * a.d + dim) = u32x2_t{pack2<false>(o.x * inv, o.y * inv), pack2<false>(o.z * inv, o.w * inv)};
-    } else {
-      const int64_t at = row * splits + a.shared_splits + split;
-      *reinterpret_cast<float4*>(a.part_o + at * a.d + dim) = o;
-      if (dim == 0) a.part_ml[at] = make_float2(top, l);
+  for (int w = 0; w < kWaves; ++w) {
+    x[w] = __builtin_amdgcn_exp2f(ml[w].x - base);
+    l = fmaf(x[w], ml[w].y, l);
+  }
+  const float inv = l == 0.f || absent ? 0.f : 1.f / l;
+  auto put = [&](int i, f32x4_t o) {
+    if (!kFull && quad_dim(i) >= a.d) return;
+    if (splits == 1)
+      *reinterpret_cast<u32x2_t*>(a.out + row * a.d + quad_dim(i)) = u32x2_t{pack2<false>(o.x * inv, o.y * inv), pack2<false>(o.z * inv, o.w * inv)};
+    else
+      *reinterpret_cast<f32x4_t*>(a.part_o + at * a.d + quad_dim(i)) = o;
+  };
+  if (team == 1) {
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) put(i, x[0] * quad(f, i));
+  } else {
+    for (int i = rank; i < kQuads; i += team) {
+      f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w)
+        if (w < team) o += x[w] * sums[((wave - rank + w) * kQuads + i) * kWave + lane];
+      put(i, o);
     }
   }
+  if (splits > 1 && rank == 0 && lane < 32) a.part_ml[at] = make_float2(top, l);
 }
 
 template <int DP, bool kF16, bool kFull>
-__global__ __launch_bounds__(kWave * kWaves, DP == 64 ? 2 : 1) void batch_attention_kernel(BatchArgs a) {
-  __shared__ __align__(1024) uint8_t lds[kBatchLds<DP>];
+__global__ __launch_bounds__(kWave * kWaves, 2) void batch_attention_kernel(BatchArgs a) {
+  __shared__ __align__(1024) uint8_t lds[kBatchLds];
   __shared__ float2 wave_ml[kWaves][kBatchGroup];
   if ((int)blockIdx.x < a.shared_wgs)
     shared_part<DP, kF16, kFull>(a, blockIdx.x, (lds_u8)lds);
@@ -405,26 +428,26 @@ __global__ __launch_bounds__(256) void batch_join_kernel(BatchArgs a) {
 }
 
 struct BatchPlan {
-  int64_t shared_splits, shared_tiles, row_tiles, own_splits;
+  int64_t shared_splits, shared_tiles, row_tiles, own_splits, own_waves;
   int64_t splits() const { return shared_splits + own_splits; }
 };
-BatchPlan batch_plan(int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t d, int64_t prefix, int64_t max_own, int64_t window) {
+BatchPlan batch_plan(int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t prefix, int64_t max_own, int64_t window) {
   BatchPlan p{};
-  const int64_t rows = n_seq * (n_heads / n_kv);
-  p.row_tiles = (rows + 32 * kWaves - 1) / (32 * kWaves);
+  const int64_t rows = n_seq * (n_heads / n_kv), items = n_seq * n_kv;
+  p.row_tiles = (rows + 32 * kRowBlocks - 1) / (32 * kRowBlocks);
   const bool shared = prefix > 0 && window == 0 && n_seq > 1;
   int64_t keys = max_own + (shared ? 0 : prefix);
   if (window > 0 && window < keys) keys = window;
   if (shared) {
-    const int64_t tile = d <= 64 ? kSharedTile<64> : kSharedTile<128>;
-    const int64_t tiles = (prefix + tile - 1) / tile;
-    const int64_t want = (256 + n_kv * p.row_tiles - 1) / (n_kv * p.row_tiles);
+    const int64_t tile = kWaveTile * kKeyParts, tiles = (prefix + tile - 1) / tile;
+    const int64_t want = (512 + n_kv * p.row_tiles - 1) / (n_kv * p.row_tiles);
     p.shared_tiles = (tiles + want - 1) / want;
     p.shared_splits = (tiles + p.shared_tiles - 1) / p.shared_tiles;
   }
-  const int64_t own_tiles = keys / kOwnTile + 2;
-  const int64_t want = (512 + n_seq * n_kv - 1) / (n_seq * n_kv), most = (own_tiles + 2 * kWaves - 1) / (2 * kWaves);
-  p.own_splits = want < most ? want : most;
+  const int64_t tiles = keys / kWaveTile + 2;
+  p.own_waves = items >= 1536 ? 1 : items >= 768 ? 2 : 4;
+  const int64_t want = (512 + items - 1) / items, most = (tiles + 2 * kWaves - 1) / (2 * kWaves);
+  p.own_splits = p.own_waves < 4 ? 1 : want < most ? want : most;
   return p;
 }
 
@@ -435,7 +458,8 @@ int64_t batch_bytes(const BatchPlan& p, int64_t n_seq, int64_t n_heads, int64_t 
 
 template <int DP, bool kF16, bool kFull>
 int launch_batch(const BatchArgs& a, const BatchPlan& p, hipStream_t st) {
-  const int64_t wgs = a.shared_wgs + (int64_t)a.n_seq * a.n_kv * p.own_splits;
+  const int64_t items = (int64_t)a.n_seq * a.n_kv * p.own_splits, teams = kWaves / p.own_waves;
+  const int64_t wgs = a.shared_wgs + (items + teams - 1) / teams;
   batch_attention_kernel<DP, kF16, kFull><<<(unsigned)wgs, kWave * kWaves, 0, st>>>(a);
   const int rc = check_launch("batch_attention_kernel");
   if (rc || p.splits() == 1) return rc;
@@ -469,7 +493,7 @@ extern "C" int64_t klc_attn_batch_workspace_bytes(int64_t n_seq, int64_t n_heads
                                                   int64_t prefix_len, int64_t max_own, int64_t window) {
   const int rc = check_sizes("klc_attn_batch_workspace_bytes", n_seq, n_heads, n_kv, head_dim, prefix_len, max_own, window);
   if (rc) return rc;
-  return batch_bytes(batch_plan(n_seq, n_heads, n_kv, head_dim, prefix_len, max_own, window), n_seq, n_heads, head_dim);
+  return batch_bytes(batch_plan(n_seq, n_heads, n_kv, prefix_len, max_own, window), n_seq, n_heads, head_dim);
 }
 
 extern "C" int klc_attn_batch(const klc_attn_batch_args* args, void* stream) {
@@ -494,7 +518,7 @@ extern "C" int klc_attn_batch(const klc_attn_batch_args* args, void* stream) {
               "klc_attn_batch: scale %g", x.scale);
   KLC_REQUIRE(x.kv_dtype == KLC_DTYPE_BF16 || x.kv_dtype == KLC_DTYPE_F16, KLC_ERR_UNSUPPORTED,
               "klc_attn_batch: kv_dtype %lld (bfloat16 or float16)", (long long)x.kv_dtype);
-  const BatchPlan p = batch_plan(x.n_seq, x.n_heads, x.n_kv, d, x.prefix_len, max_own, x.window);
+  const BatchPlan p = batch_plan(x.n_seq, x.n_heads, x.n_kv, x.prefix_len, max_own, x.window);
   const int64_t need = batch_bytes(p, x.n_seq, x.n_heads, d);
   KLC_REQUIRE(need == 0 || (x.workspace && x.workspace_bytes >= need), KLC_ERR_ARGUMENT,
               "klc_attn_batch: workspace of %lld bytes, need %lld", (long long)x.workspace_bytes, (long long)need);
@@ -507,8 +531,8 @@ extern "C" int klc_attn_batch(const klc_attn_batch_args* args, void* stream) {
   const BatchArgs a{in(x.q), in(x.k_pages), in(x.v_pages), index(x.tables), index(x.lengths), index(x.prefix_table),
                     in(x.sinks), static_cast<uint16_t*>(x.out), part_o, part_ml, x.q_stride, (int)x.n_seq,
                     (int)x.n_heads, (int)x.n_kv, (int)d, (int)x.n_pages, page_log2, (int)x.table_width,
-                    (int)x.prefix_len, (int)x.window, (int)p.shared_splits, (int)p.own_splits, (int)p.shared_tiles,
-                    (int)(p.shared_splits * p.row_tiles * x.n_kv), (float)(x.scale * kLog2e)};
+                    (int)x.prefix_len, (int)x.window, (int)p.shared_splits, (int)p.shared_tiles,
+                    (int)(p.shared_splits * p.row_tiles * x.n_kv), (int)p.own_splits, (int)p.own_waves, (float)(x.scale * kLog2e)};
   const hipStream_t st = as_stream(stream);
   const bool f16 = x.kv_dtype == KLC_DTYPE_F16;
   if (d == 64) return f16 ? launch_batch<64, true, true>(a, p, st) : launch_batch<64, false, true>(a, p, st);

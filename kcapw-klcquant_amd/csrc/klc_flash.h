@@ -72,6 +72,14 @@ __device__ __forceinline__ void load_to_lds(const uint16_t* src, lds_u8 dst) {
                : "memory");
 }
 
+// the same from base + offset bytes, base uniform and offset below 2^31
+__device__ __forceinline__ void load_to_lds(const uint16_t* base, uint32_t offset, lds_u8 dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"((uint32_t)(uintptr_t)dst), "v"(offset), "s"(base)
+               : "memory");
+}
+
 // the other half's value beside the lane's own: both halves get the same pair
 __device__ __forceinline__ float max_halves(float v) {
   const uint32_t u = __float_as_uint(v);
@@ -90,26 +98,6 @@ __device__ __forceinline__ float sink_log2(uint16_t bits) {
   return fabsf(sink) < INFINITY ? fminf(fmaxf(sink * kLog2e, -3e38f), 3e38f) : sink;
 }
 
-// 1.0 for each half of `x` that is NaN or an infinity of the sign, else 0;
-// and x with those halves cleared.
-template <bool kF16>
-__device__ __forceinline__ uint32_t nonfinite_ones(uint32_t x, bool negative) {
-  constexpr uint32_t kExp = kF16 ? 0x7c00u : 0x7f80u, kOne = kF16 ? 0x3c00u : 0x3f80u;
-  uint32_t out = 0;
-#pragma unroll
-  for (int s = 0; s < 32; s += 16) {
-    const uint32_t h = (x >> s) & 0xffffu, mag = h & 0x7fffu;
-    const bool hit = mag > kExp || (mag == kExp && (h >> 15 != 0) == negative);
-    out |= hit ? kOne << s : 0u;
-  }
-  return out;
-}
-template <bool kF16>
-__device__ __forceinline__ uint32_t finite_only(uint32_t x) {
-  constexpr uint32_t kExp = kF16 ? 0x7c00u : 0x7f80u;
-  return ((x & kExp) == kExp ? 0u : x & 0xffffu) | (((x >> 16) & kExp) == kExp ? 0u : x & 0xffff0000u);
-}
-
 // One wave's state and one tile's work.
 //   DP     head size the tiles are laid out for (64 or 128)
 //   kFull  the head size is DP; else it is d < DP, a multiple of 8
@@ -117,6 +105,7 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t x) {
 //   KT     keys of a tile (32 or 64)
 template <int DP, bool kF16, bool kFull, int RB, int KT>
 struct Flash {
+  static constexpr bool kWhole = kFull;
   static constexpr int kRowBytes = 2 * DP;
   static constexpr int kChunks = DP / 8;                // 16-byte chunks of a row
   static constexpr int kSteps = DP / 16;                // MFMAs of a score block
@@ -157,7 +146,7 @@ struct Flash {
 #pragma unroll
       for (int db = 0; db < kDimBlocks; ++db) {
         const int row = 8 * u + 4 * h + i / 4, chunk = 4 * db + 2 * grp + (i % 4) / 2;
-        v_at[u][db] = ring + kMatBytes + row * kRowBytes + ((chunk ^ swizzle(row)) << 4) + (i & 1) * 8;
+        v_at[u][db] = ring + row * kRowBytes + ((chunk ^ swizzle(row)) << 4) + (i & 1) * 8;
         asm volatile("" : "+v"(v_at[u][db]));
       }
 #pragma unroll
@@ -178,7 +167,7 @@ struct Flash {
     return kFull ? c : min(c, head_dim / 8 - 1);  // chunks past the head repeat its last: their K is cleared, their V unused
   }
 
-  // Scores of the tile in `stage`: s[rb][kb][i] is q . k of key 32 kb + 8 (i / 4) + 4 (lane / 32) + i % 4.
+  // Scores of the K tile at `stage`: s[rb][kb][i] is q . k of key 32 kb + 8 (i / 4) + 4 (lane / 32) + i % 4.
   __device__ __forceinline__ void scores(int stage, f32x16_t (&s)[RB][KT / 32]) const {
     const bool upper = threadIdx.x % kWave >= 32;
 #pragma unroll
@@ -200,8 +189,8 @@ struct Flash {
     }
   }
 
-  // p = exp2(c2 s - m) of row block rb in place of the scores, packed; m and l brought up to date, o rescaled.
-  __device__ __forceinline__ void softmax(int rb, f32x16_t (&s)[KT / 32], float c2, u32x4_t (&p)[KT / 16]) {
+  // Brings row block rb's maximum up to the scores s, and what was summed below the old one to the new.
+  __device__ __forceinline__ void raise(int rb, const f32x16_t (&s)[KT / 32], float c2) {
     float t = s[0][0];
 #pragma unroll
     for (int kb = 0; kb < KT / 32; ++kb)
@@ -220,6 +209,10 @@ struct Flash {
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[rb][db][e] *= alpha;
     }
+  }
+
+  // p = exp2(c2 s - m) of row block rb, packed, and its part of the sum
+  __device__ __forceinline__ void weigh(int rb, const f32x16_t (&s)[KT / 32], float c2, u32x4_t (&p)[KT / 16]) {
     const float base = m[rb] == -INFINITY ? 0.f : m[rb];
     float sum = l[rb];
 #pragma unroll
@@ -232,6 +225,11 @@ struct Flash {
         sum = add2<kF16>(w, sum);  // the sum of what the values are multiplied by
       }
     l[rb] = sum;
+  }
+
+  __device__ __forceinline__ void softmax(int rb, const f32x16_t (&s)[KT / 32], float c2, u32x4_t (&p)[KT / 16]) {
+    raise(rb, s, c2);
+    weigh(rb, s, c2, p);
   }
 
   __device__ __forceinline__ u32x4_t v_operand(int stage, int t, int db) const {
@@ -253,45 +251,17 @@ struct Flash {
         for (int rb = 0; rb < RB; ++rb) o[rb][db] = mfma32<kF16>(v, p[rb][t], o[rb][db]);
       }
   }
-
-  // values() of a tile that some rows see in part, whose V holds NaN or infinities: finite values are multiplied
-  // as ever (0 in the others' place), and a row that sees an infinity or a NaN gets it added.  `seen` has 1.0
-  // where the key is visible.
-  __device__ __forceinline__ void values_careful(int stage, const u32x4_t (&p)[RB][KT / 16],
-                                                 const u32x4_t (&seen)[RB][KT / 16]) {
-    for (int db = 0; db < kDimBlocks; ++db) {
-      if (!kFull && 32 * db >= d) break;
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        f32x16_t up = {}, down = {};
-#pragma unroll
-        for (int t = 0; t < KT / 16; ++t) {
-          u32x4_t v;
-#pragma unroll
-          for (int b = 0; b < kDimBlocks; ++b)
-            if (b == db) v = v_operand(stage, t, b);
-          u32x4_t fin, hi, lo;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            fin[e] = finite_only<kF16>(v[e]);
-            hi[e] = nonfinite_ones<kF16>(v[e], false);
-            lo[e] = nonfinite_ones<kF16>(v[e], true);
-          }
-#pragma unroll
-          for (int b = 0; b < kDimBlocks; ++b)
-            if (b == db) o[rb][b] = mfma32<kF16>(fin, p[rb][t], o[rb][b]);
-          up = mfma32<kF16>(hi, seen[rb][t], up);
-          down = mfma32<kF16>(lo, seen[rb][t], down);
-        }
-#pragma unroll
-        for (int b = 0; b < kDimBlocks; ++b)
-          if (b == db)
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              o[rb][b][e] += (up[e] > 0.f ? INFINITY : 0.f) + (down[e] > 0.f ? -INFINITY : 0.f);
-      }
-    }
-  }
 };
+
+// Clears the V rows of a tile outside [from, to), whose values no query sees
+// (0 * inf would make NaN of them); the caller orders it.
+template <class F, int KT>
+__device__ __forceinline__ void clear_values(lds_u8 values, int from, int to, int thread, int threads) {
+  for (int i = thread; i < KT * F::kChunks; i += threads) {
+    const int r = i / F::kChunks;
+    if (r < from || r >= to)
+      *reinterpret_cast<__attribute__((address_space(3))) u32x4_t*>(values + i * 16) = u32x4_t{0, 0, 0, 0};
+  }
+}
 
 }  // namespace klc

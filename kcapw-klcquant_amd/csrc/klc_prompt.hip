@@ -17,17 +17,6 @@ struct PromptArgs {
   float c2;                     // scale * log2(e)
 };
 
-// One step of the ring: tile j has landed for every wave of the workgroup and
-// every wave is done with tile j - 1.
-template <int kOutstanding>
-__device__ __forceinline__ void tile_barrier() {
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm(kOutstanding));
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-}
-
-constexpr int kPromptRing = 3;
-
 // What a workgroup works on, the same for all its threads.
 struct PromptTile {
   int begin, len;   // the sequence
@@ -35,144 +24,269 @@ struct PromptTile {
   int kvh, g;
 };
 
-// The rows of one wave from w_row on, 32 RB of them, over every tile of keys
-// that a row of the workgroup sees.  Without kCareful it stores nothing and
-// returns true if a result has a NaN or infinity that may come from a value
-// the row must not see (0 * inf in the matrix instruction); kCareful keeps
-// those out.
-template <int DP, bool kF16, bool kFull, int RB, int W, int KT, bool kCareful>
-__device__ __forceinline__ bool prompt_rows(const PromptArgs& a, const PromptTile& t, int w_row, lds_u8 ring) {
-  using F = Flash<DP, kF16, kFull, RB, KT>;
-  constexpr int kLoads = 2 * F::kDmas / W;  // load instructions of a wave and tile
-  static_assert(F::kDmas % W == 0, "the tile's loads split evenly over the waves");
-  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int tok_lo = t.row0 / t.g, tok_hi = t.last / t.g;  // tokens of the workgroup's rows, and of the wave's
-  const int w_lo = min(w_row, t.last) / t.g, w_hi = min(w_row + 32 * RB - 1, t.last) / t.g;
-  const bool w_live = w_row <= t.last;
+// 64 keys a tile in LDS, of which a wave takes 32 at a time.
+constexpr int kKeys = 32;
+constexpr int kTileKeys = 64;
+
+template <int DP, bool kF16, bool kFull, int RB>
+struct Rows {
+  using F = Flash<DP, kF16, kFull, RB, kKeys>;
+  static constexpr int kStage = 2 * F::kStage;  // K of the tile, then V
+  static constexpr int kV = 2 * F::kMatBytes;
 
   F f;
-  f.init(ring, a.d);
-  int tok[RB], head[RB];
+  int tok[RB];
+
+  // the wave's rows from w_row on, with their sinks
+  __device__ __forceinline__ void begin(const PromptArgs& a, const PromptTile& t, int w_row, lds_u8 ring) {
+    const int lane = threadIdx.x % kWave;
+    f.init(ring, a.d);
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int row = min(w_row + 32 * rb + lane % 32, t.last);
-    tok[rb] = row / t.g;
-    head[rb] = t.kvh * t.g + row - tok[rb] * t.g;
-    const uint16_t* src = a.q + (t.begin + tok[rb]) * a.q_stride + (int64_t)head[rb] * a.d;
+    for (int rb = 0; rb < RB; ++rb) {
+      const int row = min(w_row + 32 * rb + lane % 32, t.last);
+      tok[rb] = row / t.g;
+      const int head = t.kvh * t.g + row - tok[rb] * t.g;
+      const uint16_t* src = a.q + (t.begin + tok[rb]) * a.q_stride + (int64_t)head * a.d;
 #pragma unroll
-    for (int st = 0; st < F::kSteps; ++st) {
-      const int c = 2 * st + lane / 32;
-      f.q[rb][st] = u32x4_t{0, 0, 0, 0};
-      if (kFull || 8 * c < a.d) f.q[rb][st] = *reinterpret_cast<const u32x4_t*>(src + 8 * c);
-    }
-    if (a.sinks != nullptr) {
-      const float sink = sink_log2(a.sinks[head[rb]]);
-      f.m[rb] = sink;
-      f.l[rb] = sink == -INFINITY || lane >= 32 ? 0.f : 1.f + (sink - sink);
+      for (int st = 0; st < F::kSteps; ++st) {
+        const int c = 2 * st + lane / 32;
+        f.q[rb][st] = u32x4_t{0, 0, 0, 0};
+        if (kFull || 8 * c < a.d) f.q[rb][st] = *reinterpret_cast<const u32x4_t*>(src + 8 * c);
+      }
+      if (a.sinks != nullptr) {
+        const float sink = sink_log2(a.sinks[head]);
+        f.m[rb] = sink;
+        f.l[rb] = sink == -INFINITY || lane >= 32 ? 0.f : 1.f + (sink - sink);
+      }
     }
   }
 
-  const int first = a.window > 0 ? max(0, tok_lo - a.window + 1) / KT * KT : 0;
-  const int n_tiles = (tok_hi - first) / KT + 1;
-  const uint16_t* kb = a.k + t.begin * a.k_stride + (int64_t)t.kvh * a.d;
-  const uint16_t* vb = a.v + t.begin * a.v_stride + (int64_t)t.kvh * a.d;
-  auto load = [&](int j) {
-    const int base = first + j * KT, stage = (j % kPromptRing) * F::kStage;
-#pragma unroll
-    for (int i = 0; i < F::kDmas / W; ++i) {
-      const int n = wave + i * W, r = F::dma_row(n);
-      const int64_t key = min(base + r, t.len - 1);
-      const int c = 8 * F::dma_chunk(r, a.d);
-      const lds_u8 dst = ring + stage + n * 1024;
-      load_to_lds(kb + key * a.k_stride + c, dst);
-      load_to_lds(vb + key * a.v_stride + c, dst + F::kMatBytes);
-    }
-  };
-#pragma unroll
-  for (int j = 0; j < kPromptRing - 1; ++j)
-    if (j < n_tiles) load(j);
-  for (int j = 0; j < n_tiles; ++j) {
-    if (j + 1 < n_tiles)
-      tile_barrier<kLoads*(kPromptRing - 2)>();
-    else
-      tile_barrier<0>();
-    if (j + kPromptRing - 1 < n_tiles) load(j + kPromptRing - 1);
-    const int k0 = first + j * KT, stage = (j % kPromptRing) * F::kStage;
-    if (!w_live || k0 > w_hi || (a.window > 0 && k0 + KT - 1 <= w_lo - a.window)) continue;
-    const bool masked = k0 + KT - 1 > w_lo || (a.window > 0 && k0 <= w_hi - a.window);
-    f32x16_t sc[RB][KT / 32];
-    f.scores(stage, sc);
-    u32x4_t p[RB][KT / 16];
-    // key k0 + 4 (lane / 32) + off is visible for low < off <= rel
-    auto rel = [&](int rb) { return tok[rb] - k0 - 4 * (lane / 32); };
-    auto low = [&](int rb) { return a.window > 0 ? rel(rb) - a.window : -0x40000000; };
-    if (masked) {
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-        for (int b = 0; b < KT / 32; ++b)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int off = 32 * b + 8 * (e / 4) + e % 4;
-            sc[rb][b][e] = off <= rel(rb) && off > low(rb) ? sc[rb][b][e] : -INFINITY;
-          }
-    }
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) f.softmax(rb, sc[rb], a.c2, p[rb]);
-    if (!kCareful || !masked) {
-      f.values(stage, p);
-    } else {
-      u32x4_t seen[RB][KT / 16];
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-        for (int x = 0; x < KT / 16; ++x)
-#pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const int off = 16 * x + 8 * (e / 4) + e % 4;
-            auto one = [&](int o) { return o <= rel(rb) && o > low(rb) ? 1.f : 0.f; };
-            seen[rb][x][e / 2] = pack2<kF16>(one(off), one(off + 1));
-          }
-      f.values_careful(stage, p, seen);
-    }
+  // key k0 + 4 (lane / 32) + off is visible for low < off <= rel
+  __device__ __forceinline__ int rel(int rb, int k0) const { return tok[rb] - k0 - 4 * ((int)(threadIdx.x % kWave) / 32); }
+  __device__ __forceinline__ int low(const PromptArgs& a, int rb, int k0) const {
+    return a.window > 0 ? rel(rb, k0) - a.window : -0x40000000;
   }
-  if constexpr (!kCareful) {
-    bool odd = false;
+  __device__ __forceinline__ void mask(const PromptArgs& a, int k0, f32x16_t (&s)[RB][1]) const {
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int off = 8 * (e / 4) + e % 4;
+        s[rb][0][e] = off <= rel(rb, k0) && off > low(a, rb, k0) ? s[rb][0][e] : -INFINITY;
+      }
+  }
+
+  // all rows, or those of token `only`
+  __device__ __forceinline__ void store(const PromptArgs& a, const PromptTile& t, int w_row, int only = -1) const {
+    const int lane = threadIdx.x % kWave;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const float sum = add_halves(f.l[rb]);
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key and no sink: zeros
+      const int row = w_row + 32 * rb + lane % 32, head = t.kvh * t.g + row - tok[rb] * t.g;
+      const bool live = row <= t.last && (only < 0 || tok[rb] == only);
+      uint16_t* dst = a.out + ((int64_t)(t.begin + tok[rb]) * a.n_heads + head) * a.d + 8 * (lane / 32);
+#pragma unroll
       for (int db = 0; db < F::kDimBlocks; ++db)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) odd |= !(fabsf(f.o[rb][db][e]) < INFINITY);
-    if (__syncthreads_or(odd)) return true;
-  }
+        for (int e = 0; e < 16; e += 8) {
+          // the lane has dims 4 (lane / 32) + 0..3 and 8 more of 16; the halves trade, so that each has 8 in a row
+          uint32_t w[2][2];
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const float sum = add_halves(f.l[rb]);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key and no sink: zeros
-    if (w_row + 32 * rb + lane % 32 > t.last) continue;
-    uint16_t* dst = a.out + ((int64_t)(t.begin + tok[rb]) * a.n_heads + head[rb]) * a.d + 4 * (lane / 32);
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              w[i][x] = pack2<kF16>(f.o[rb][db][e + 4 * i + 2 * x] * inv, f.o[rb][db][e + 4 * i + 2 * x + 1] * inv);
+          const auto lo = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+          const auto hi = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+          const int at = 32 * db + 2 * e;
+          if (!live || (!kFull && at + 8 * (lane / 32) >= a.d)) continue;
+          *reinterpret_cast<u32x4_t*>(dst + at) = u32x4_t{lo[0], hi[0], lo[1], hi[1]};
+        }
+    }
+  }
+};
+
+// The tiles of keys that a row of the workgroup sees, through a ring of
+// kRing of them in LDS that its W waves fill together.
+template <class R, int W, int kRing>
+struct Tiles {
+  using F = typename R::F;
+  static constexpr int kDmas = 2 * F::kDmas / W;  // load instructions of K, and of V, a wave and tile
+  static_assert(2 * F::kDmas % W == 0, "the tile's loads split evenly over the waves");
+  const PromptArgs& a;
+  const PromptTile& t;
+  lds_u8 ring;
+  const uint16_t *k, *v;  // of the first key
+  int wave, first, count, whole;
+  uint32_t k_off[kDmas], v_off[kDmas];
+
+  __device__ __forceinline__ Tiles(const PromptArgs& args, const PromptTile& tile, lds_u8 lds) : a(args), t(tile), ring(lds) {
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    first = a.window > 0 ? max(0, t.row0 / t.g - a.window + 1) : 0;
+    count = (t.last / t.g - first) / kTileKeys + 1;
+    k = a.k + (t.begin + first) * a.k_stride + (int64_t)t.kvh * a.d;
+    v = a.v + (t.begin + first) * a.v_stride + (int64_t)t.kvh * a.d;
+    // tiles whose rows all exist, and whose offsets fit a load's 32 bits: no address arithmetic in vector registers
+    whole = max(a.k_stride, a.v_stride) <= 0x7fffffff / (2 * kTileKeys) ? (t.len - first) / kTileKeys : 0;
+#pragma unroll
+    for (int i = 0; i < kDmas; ++i) {
+      const int r = F::dma_row(wave + i * W), c = 8 * F::dma_chunk(r, a.d);
+      k_off[i] = 2 * (uint32_t)(r * a.k_stride + c);
+      v_off[i] = 2 * (uint32_t)(r * a.v_stride + c);
+    }
+  }
+  __device__ __forceinline__ int stage(int j) const { return j % kRing * R::kStage; }
+  __device__ __forceinline__ void load(int j) const {
+    if (j >= count) return;
+    const lds_u8 dst = ring + stage(j) + wave * 1024;
+    const uint16_t *kj = k + (int64_t)j * kTileKeys * a.k_stride, *vj = v + (int64_t)j * kTileKeys * a.v_stride;
+    if (j < whole) {
+#pragma unroll
+      for (int i = 0; i < kDmas; ++i) {
+        load_to_lds(kj, k_off[i], dst + i * W * 1024);
+        load_to_lds(vj, v_off[i], dst + i * W * 1024 + R::kV);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kDmas; ++i) {
+        const int r = F::dma_row(wave + i * W), c = 8 * F::dma_chunk(r, a.d);
+        const int64_t key = min(first + j * kTileKeys + r, t.len - 1) - (first + j * kTileKeys);
+        load_to_lds(kj + key * a.k_stride + c, dst + i * W * 1024);
+        load_to_lds(vj + key * a.v_stride + c, dst + i * W * 1024 + R::kV);
+      }
+    }
+  }
+  // Tile j has landed for every wave, and every wave is done with the tiles before j - 1; kAhead later tiles may
+  // be in flight.
+  template <int kAhead>
+  __device__ __forceinline__ void arrive(int j) const {
+    if (j + kAhead < count)
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * kDmas * kAhead));
+    else
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  }
+};
+
+// The rows of one wave from w_row on, 32 RB of them.  Stores them, or returns
+// true and stores nothing if a row of the workgroup has a NaN or infinity
+// that may come from a value it must not see (0 * inf in the matrix
+// instruction).
+//
+// The scores of the next 32 keys are multiplied while the exponentials of
+// these are taken: the matrix instructions of a wave run beside its own
+// vector instructions, and not only beside another wave's.
+template <int DP, bool kF16, bool kFull, int RB, int W, int kRing>
+__device__ __forceinline__ bool prompt_rows(const PromptArgs& a, const PromptTile& t, int w_row, lds_u8 ring) {
+  using R = Rows<DP, kF16, kFull, RB>;
+  using F = typename R::F;
+  R r;
+  r.begin(a, t, w_row, ring);
+  const Tiles<R, W, kRing> tiles(a, t, ring);
+  // the wave's tokens, and the first and last tile that one of them sees
+  const int w_lo = min(w_row, t.last) / t.g, w_hi = min(w_row + 32 * RB - 1, t.last) / t.g;
+  const int from = a.window > 0 ? max(0, w_lo - a.window + 1 - tiles.first) / kTileKeys : 0;
+  const int to = w_row <= t.last ? (w_hi - tiles.first) / kTileKeys : from - 1;
+#pragma unroll
+  for (int j = 0; j < kRing - 1; ++j) tiles.load(j);
+
+  // what follows the scores of keys i: the mask and the maximum
+  auto settle = [&](int i, f32x16_t (&s)[RB][1]) {
+    const int k0 = tiles.first + i * kKeys;
+    if (k0 + kKeys - 1 > w_lo || (a.window > 0 && k0 <= w_hi - a.window)) r.mask(a, k0, s);
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) r.f.raise(rb, s[rb], a.c2);
+  };
+  f32x16_t sa[RB][1], sb[RB][1];
+  // the values of the keys at `here`, whose settled scores are s, and the scores of those at `there`
+  auto step = [&](int here, f32x16_t (&s)[RB][1], int there, f32x16_t (&next)[RB][1]) {
+    u32x4_t p[RB][2];
+    r.f.scores(there, next);
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) r.f.weigh(rb, s[rb], a.c2, p[rb]);
+    r.f.values(here + R::kV, p);
+  };
+  // tile j + 1 is there from here on, every wave is done with tile j - 1
+  auto advance = [&](int j) {
+    tiles.template arrive<kRing - 3>(j + 1);
+    tiles.load(j + kRing - 1);
+  };
+  tiles.template arrive<kRing - 2>(0);
+  int j = 0;
+  for (; j < min(from, tiles.count); ++j) advance(j);
+  if (from <= to) {
+    r.f.scores(tiles.stage(j), sa);
+    settle(2 * j, sa);
+    for (; j <= to; ++j) {
+      const int here = tiles.stage(j);
+      step(here, sa, here + F::kMatBytes, sb);
+      settle(2 * j + 1, sb);
+      advance(j);
+      step(here + F::kMatBytes, sb, tiles.stage(j + 1), sa);  // past the last tile: scores of nothing, not used
+      if (j < to) settle(2 * j + 2, sa);
+    }
+  }
+  for (; j < tiles.count; ++j) advance(j);
+
+  bool odd = false;
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
     for (int db = 0; db < F::kDimBlocks; ++db)
 #pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int at = 32 * db + 2 * e;
-        if (!kFull && at + 4 * (lane / 32) >= a.d) continue;
-        const u32x2_t w = {pack2<kF16>(f.o[rb][db][e] * inv, f.o[rb][db][e + 1] * inv),
-                           pack2<kF16>(f.o[rb][db][e + 2] * inv, f.o[rb][db][e + 3] * inv)};
-        *reinterpret_cast<u32x2_t*>(dst + at) = w;
-      }
-  }
+      for (int e = 0; e < 16; ++e) odd |= !(fabsf(r.f.o[rb][db][e]) < INFINITY);
+  if (__syncthreads_or(odd)) return true;
+  r.store(a, t, w_row);
   return false;
+}
+
+// The same for 32 rows, with NaN and infinities kept out of the rows that do
+// not see them: one token's rows at a time, all of which see the same keys,
+// with V cleared behind them.  The wave works alone, in `tile`.
+template <int DP, bool kF16, bool kFull>
+__device__ __forceinline__ void prompt_rows_careful(const PromptArgs& a, const PromptTile& t, int w_row, lds_u8 tile) {
+  using R = Rows<DP, kF16, kFull, 1>;
+  using F = typename R::F;
+  const int last_tok = min(w_row + 31, t.last) / t.g;
+  const uint16_t* k = a.k + t.begin * a.k_stride + (int64_t)t.kvh * a.d;
+  const uint16_t* v = a.v + t.begin * a.v_stride + (int64_t)t.kvh * a.d;
+  for (int tok = w_row / t.g; tok <= last_tok && w_row <= t.last; ++tok) {
+    R r;
+    r.begin(a, t, w_row, tile);
+    for (int k0 = a.window > 0 ? max(0, tok - a.window + 1) : 0; k0 <= tok; k0 += kKeys) {
+#pragma unroll
+      for (int n = 0; n < F::kDmas; ++n) {
+        const int row = F::dma_row(n), c = 8 * F::dma_chunk(row, a.d);
+        const int64_t key = min(k0 + row, tok);
+        load_to_lds(k + key * a.k_stride + c, tile + n * 1024);
+        load_to_lds(v + key * a.v_stride + c, tile + F::kMatBytes + n * 1024);
+      }
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+      clear_values<F, kKeys>(tile + F::kMatBytes, 0, tok - k0 + 1, threadIdx.x % kWave, kWave);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      f32x16_t s[1][1];
+      r.f.scores(0, s);
+      r.mask(a, k0, s);
+      u32x4_t p[1][2];
+      r.f.softmax(0, s[0], a.c2, p[0]);
+      r.f.values(F::kMatBytes, p);
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(63));  // the tile's reads are done
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+    }
+    r.store(a, t, w_row, tok);
+  }
 }
 
 // Workgroup: W waves x 32 RB rows of one KV head, a row being (token, query
 // head of the group), so that a group's heads share every K and V tile and a
 // tile of rows covers few tokens (little of the diagonal is wasted).
-template <int DP, bool kF16, bool kFull, int RB, int W, int KT>
-__global__ __launch_bounds__(64 * W, DP == 64 ? 2 : 1) void prompt_attention_kernel(PromptArgs a) {
+template <int DP, bool kF16, bool kFull, int RB, int W, int kRing, int kPerSimd>
+__global__ __launch_bounds__(64 * W, kPerSimd) void prompt_attention_kernel(PromptArgs a) {
   constexpr int kRows = 32 * RB * W;
-  __shared__ __align__(1024) uint8_t ring[kPromptRing * Flash<DP, kF16, kFull, RB, KT>::kStage];
+  __shared__ __align__(1024) uint8_t ring[kRing * Rows<DP, kF16, kFull, RB>::kStage];
   PromptTile t;
   t.g = a.n_heads / a.n_kv;
   t.kvh = blockIdx.x % a.n_kv;
@@ -182,10 +296,15 @@ __global__ __launch_bounds__(64 * W, DP == 64 ? 2 : 1) void prompt_attention_ker
   const int i = (int)(gridDim.x / a.n_kv) - 1 - (int)(blockIdx.x / a.n_kv);
   auto start_of = [&](int s) { return min(max(a.starts[s], 0), a.tokens); };
   auto tile_of = [&](int s) { return (int)((int64_t)start_of(s) * t.g / kRows) + s; };
-  int s = 0, step = 1;
-  while (step < a.n_seq) step <<= 1;
-  for (; step > 0; step >>= 1)
-    if (s + step < a.n_seq && tile_of(s + step) <= i) s += step;
+  // 64 sequences a look: the last one that starts at or before i (the first is taken to)
+  int s = 0, span = a.n_seq;  // it is among s .. s + span - 1
+  while (span > 1) {
+    const int stride = (span + kWave - 1) / kWave, at = s + stride * (int)(threadIdx.x % kWave);
+    const bool before = at == s || (at < s + span && tile_of(at) <= i);
+    const int found = __popcll(__ballot(before)) - 1;
+    span = min(stride, span - found * stride);
+    s += found * stride;
+  }
   s = __builtin_amdgcn_readfirstlane(s);
   t.begin = __builtin_amdgcn_readfirstlane(start_of(s));
   t.len = __builtin_amdgcn_readfirstlane(start_of(s + 1)) - t.begin;
@@ -194,20 +313,19 @@ __global__ __launch_bounds__(64 * W, DP == 64 ? 2 : 1) void prompt_attention_ker
   t.row0 = (int)row0;
   t.last = (int)(min(row0 + kRows, seq_rows) - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), w_row = t.row0 + wave * 32 * RB;
-  if (prompt_rows<DP, kF16, kFull, RB, W, KT, false>(a, t, w_row, (lds_u8)ring))
+  if (prompt_rows<DP, kF16, kFull, RB, W, kRing>(a, t, w_row, (lds_u8)ring))
 #pragma unroll 1
-    for (int rb = 0; rb < RB; ++rb) {
-      prompt_rows<DP, kF16, kFull, 1, W, KT, true>(a, t, w_row + 32 * rb, (lds_u8)ring);
-      __syncthreads();
-    }
+    for (int rb = 0; rb < RB; ++rb)
+      prompt_rows_careful<DP, kF16, kFull>(a, t, w_row + 32 * rb, (lds_u8)ring + wave * 2 * 2 * kKeys * DP);
 }
 
 template <int DP, bool kF16, bool kFull>
 int launch_prompt(const PromptArgs& a, hipStream_t st) {
   const int64_t g = a.n_heads / a.n_kv;
-  constexpr int RB = DP == 64 ? 2 : 1, W = 4, KT = 64;
+  // two waves a SIMD either way, by registers; the rows of a workgroup share its tiles
+  constexpr int RB = DP == 64 ? 2 : 1, W = DP == 64 ? 4 : 8;
   const int64_t tiles = a.tokens * g / (32 * RB * W) + a.n_seq;
-  prompt_attention_kernel<DP, kF16, kFull, RB, W, KT><<<(unsigned)(tiles * a.n_kv), 64 * W, 0, st>>>(a);
+  prompt_attention_kernel<DP, kF16, kFull, RB, W, 4, 2><<<(unsigned)(tiles * a.n_kv), 64 * W, 0, st>>>(a);
   return check_launch("prompt_attention_kernel");
 }
 

@@ -29,7 +29,7 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, first: torch.Tenso
     total = w.sum(dim=1, keepdim=True)
     if sink is not None:
         total = total + torch.exp(sink - base)
-    w = torch.where(total > 0, w / total, torch.zeros_like(w))
+    w = torch.where(total == 0, torch.zeros_like(w), w / total)
     finite = torch.isfinite(v)
     out = w @ torch.where(finite, v, torch.zeros_like(v))
     size = w @ torch.where(finite, v.abs(), torch.zeros_like(v))
