@@ -486,7 +486,7 @@ int klc_attn_step_wait(const void* host_record, int64_t tag, int64_t limit_us);
  * (streamed_attention.py:101-152); the mathematics, sinks and window are that
  * call's.  The cache's pools are [n_pages][page_size][n_kv][head_dim] of
  * kv_dtype (KLC_DTYPE_F16 or KLC_DTYPE_BF16), page_size a power of two from
- * 16 to 4096; slot i is token i % page_size of page i / page_size.  head_dim
+ * 16 to 4096, a page below 2 GiB; slot i is token i % page_size of page i / page_size.  head_dim
  * is a multiple of 8 up to 128; query head h reads KV head h / (n_heads / n_kv). */
 
 /* Causal attention of whole prompts, packed one behind the other: sequence s

@@ -3,9 +3,8 @@
 //
 // One launch with two kinds of workgroups, so that the compute-bound prefix
 // and the sequences' own keys, a stream from HBM, share the chip:
-//   shared  a KV head, 64 query rows (sequence, head of the group) and a range
-//           of the prefix: its 4 waves are 2 blocks of 32 rows x 2 halves of
-//           each tile of keys, over one ring of tiles
+//   shared  a KV head, 128 query rows (sequence, head of the group) and a
+//           range of the prefix: 4 waves x 32 rows over one ring of tiles
 //   own     a KV head of one sequence and a range of its own keys (with a
 //           window, or a prefix not worth the pass above, of all its keys):
 //           1, 2 or 4 waves take its tiles in turn, each through a ring of its
@@ -15,15 +14,18 @@
 // part, the own workgroup writes the result itself.
 #include <math.h>
 
+#include <algorithm>
+
 #include "klc_flash.h"
 
 namespace klc {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int kWaveTile = 32;     // keys that a wave takes at once
-constexpr int kRowBlocks = 2;     // of 32 rows, in a shared workgroup
-constexpr int kKeyParts = kWaves / kRowBlocks;
+constexpr int kKeys = 32;         // that a wave takes at once
+// keys of a shared workgroup's tiles: 16 KB of K and V
+template <int DP>
+constexpr int kSharedTile = DP == 64 ? 64 : 32;
 constexpr int kBatchGroup = 32;   // most query heads of a KV head: the columns of a wave's matrix instruction
 constexpr int kPrefixAlign = 64;  // own keys start at a multiple of this in a sequence's list of keys
 constexpr int kBatchLds = 64 * 1024;
@@ -61,6 +63,14 @@ __device__ __forceinline__ void load_query(u32x4_t (&q)[F::kSteps], const uint16
   }
 }
 
+// Has the row waited for here: past the page numbers' wait it costs nothing,
+// and later it would wait for the tiles in flight too.
+template <class F>
+__device__ __forceinline__ void settle_query(u32x4_t (&q)[F::kSteps]) {
+#pragma unroll
+  for (int st = 0; st < F::kSteps; ++st) asm volatile("" : "+v"(q[st]));
+}
+
 // The row in the cache's type.  A float16 cache takes it times a power of two
 // that brings its largest value to [1, 2): float16 then represents every value
 // as bfloat16 does, but for what lies 2^-24 below that one.  The returned
@@ -68,11 +78,15 @@ __device__ __forceinline__ void load_query(u32x4_t (&q)[F::kSteps], const uint16
 template <class F, bool kF16>
 __device__ __forceinline__ float convert_query(u32x4_t (&q)[F::kSteps]) {
   if constexpr (!kF16) return 1.f;
-  uint32_t most = 0;  // bit patterns of positive floats are in their order; NaN and infinity above 0x7f7f
+  // bit patterns of positive values are in their order, NaN and infinity above the others
+  typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+  u16x2_t pair = {0, 0};
 #pragma unroll
   for (int st = 0; st < F::kSteps; ++st)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) most = max(most, max(q[st][e] << 16 & 0x7fffffffu, q[st][e] & 0x7fff0000u));
+    for (int e = 0; e < 4; ++e)
+      pair = __builtin_elementwise_max(pair, __builtin_bit_cast(u16x2_t, q[st][e] & 0x7fff7fffu));
+  uint32_t most = (uint32_t)max(pair.x, pair.y) << 16;
   const auto both = __builtin_amdgcn_permlane32_swap(most, most, false, false);
   most = max(both[0], both[1]);
   int ex = (int)(most >> 23) - 127;
@@ -86,19 +100,52 @@ __device__ __forceinline__ float convert_query(u32x4_t (&q)[F::kSteps]) {
   return __builtin_amdgcn_ldexpf(1.f, ex);
 }
 
-// A lane's source row of a load instruction: `key` is the instruction's first
-// key (its rows lie in one page).  Keys outside the visible first..last take
-// the nearest visible one's row, so that only its pages are asked for.
-struct PageRow {
-  int64_t row;  // of [n_pages * page]
+// What a wave loads of a tile of KT keys: kCount instructions, the first of
+// rows n0 and the others kStep instructions on, each of rows of one page.  The
+// lanes hold 64 page numbers of the table, so that a tile costs no memory
+// access but its loads (a scalar one would hold up the LDS reads, which wait
+// by the same counter).
+template <class F, int KT, int kCount, int kStep>
+struct PageLoads {
+  const BatchArgs& a;
+  int n0;
+  uint32_t row_bytes, page_bytes;  // of a token, of a page (below 2^31)
+  const uint16_t *k0, *v0;         // the KV head's in the pools
+  const int32_t* table;            // held: page numbers from + lane of its `size`
+  int held, from, size;
   bool bad;
+
+  __device__ __forceinline__ PageLoads(const BatchArgs& args, int first, int kvh) : a(args), n0(first), table(nullptr), bad(false) {
+    row_bytes = 2u * (uint32_t)(a.n_kv * a.d);
+    page_bytes = row_bytes << a.page_log2;
+    k0 = a.k_pages + (int64_t)kvh * a.d;
+    v0 = a.v_pages + (int64_t)kvh * a.d;
+  }
+  __device__ __forceinline__ void hold(const int32_t* t, int at, int count) {
+    table = t;
+    from = at;
+    size = count;
+    held = t[min(from + (int)(threadIdx.x % kWave), size - 1)];
+    asm volatile("" : "+v"(held));  // waited for here, not again (with the tiles in flight) at every use
+  }
+  // Loads the tile from key `base` of the held table on to K at `k` and V at `v` of LDS.  Keys outside first..last
+  // take the nearest visible one's row, so that only its pages are asked for.
+  __device__ __forceinline__ void load(int base, int first, int last, lds_u8 k, lds_u8 v) {
+    const int mask = (1 << a.page_log2) - 1;
+    if ((min(base + KT - 1, last) >> a.page_log2) - from >= kWave) hold(table, min(max(base, first), last) >> a.page_log2, size);
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      const int n = n0 + i * kStep, r = F::dma_row(n);
+      const int page = __builtin_amdgcn_readlane(held, (min(max(base + n * F::kRowsPerDma, first), last) >> a.page_log2) - from);
+      const bool wrong = (unsigned)page >= (unsigned)a.n_pages;
+      bad |= wrong;
+      const uint64_t start = (uint64_t)(wrong ? 0u : (uint32_t)page) * page_bytes;
+      const uint32_t off = (uint32_t)(min(max(base + r, first), last) & mask) * row_bytes + 16u * (uint32_t)F::dma_chunk(r, a.d);
+      load_to_lds(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(k0) + start), off, k + n * 1024);
+      load_to_lds(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(v0) + start), off, v + n * 1024);
+    }
+  }
 };
-__device__ __forceinline__ PageRow page_row(const int32_t* table, int key, int lane_key, int first, int last,
-                                            int page_log2, int n_pages) {
-  const int page = table_at(table, __builtin_amdgcn_readfirstlane(min(max(key, first), last) >> page_log2));
-  const bool bad = (unsigned)page >= (unsigned)n_pages;
-  return {((int64_t)(bad ? 0 : page) << page_log2) + (min(max(lane_key, first), last) & ((1 << page_log2) - 1)), bad};
-}
 
 // The tile's loads have landed: of the wave's own, or with kBarrier of every
 // wave of the workgroup, each of which is then done with the tile before.
@@ -108,6 +155,11 @@ __device__ __forceinline__ void tile_wait() {
   if constexpr (kBarrier) __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
 }
+
+template <int kValue>
+struct Count {
+  static constexpr int value = kValue;
+};
 
 // Four dims of a wave's sums, as its lane holds them: block e of 32 dims / 8.
 template <class F>
@@ -119,94 +171,99 @@ __device__ __forceinline__ f32x4_t quad(const F& f, int i) {
 // the first of them
 __device__ __forceinline__ int quad_dim(int i) { return 8 * i + 4 * ((int)(threadIdx.x % kWave) / 32); }
 
-// The prefix's part of 64 query rows: workgroup (KV head, split of the keys,
-// tile of rows).
+// The prefix's part of 128 query rows: workgroup (KV head, split of the keys,
+// tile of rows).  As in the prompt's kernel, the scores of the next 32 keys
+// are multiplied while the exponentials of these are taken.
 template <int DP, bool kF16, bool kFull>
 __device__ __forceinline__ void shared_part(const BatchArgs& a, int wg, lds_u8 ring) {
-  constexpr int KT = kWaveTile * kKeyParts;
-  using F = Flash<DP, kF16, kFull, 1, kWaveTile>;
-  constexpr int kMat = kKeyParts * F::kMatBytes, kStage = 2 * kMat, kRing = kBatchLds / kStage;
-  constexpr int kDmas = kKeyParts * F::kDmas / kWaves;  // of K, and of V, a wave and tile
+  constexpr int KT = kSharedTile<DP>, kSub = KT / kKeys;
+  using F = Flash<DP, kF16, kFull, 1, kKeys>;
+  constexpr int kMat = kSub * F::kMatBytes, kStage = 2 * kMat, kRing = kBatchLds / kStage;
+  constexpr int kDmas = kSub * F::kDmas / kWaves;  // of K, and of V, a wave and tile
   constexpr int kQuads = 4 * F::kDimBlocks;
+  static_assert(kRing >= 3 && kSub * F::kDmas % kWaves == 0, "");
   const int g = a.n_heads / a.n_kv, rows = a.n_seq * g;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int kvh = wg % a.n_kv, split = wg / a.n_kv % a.shared_splits, row_tile = wg / (a.n_kv * a.shared_splits);
-  const int first = split * a.shared_tiles, end_tile = min(first + a.shared_tiles, (a.prefix + KT - 1) / KT);
-  const int block = wave % kRowBlocks, part = wave / kRowBlocks;
-  const int w_row = (row_tile * kRowBlocks + block) * 32;
+  const int key0 = split * a.shared_tiles * KT, keys = min(a.shared_tiles * KT, a.prefix - key0);  // of this split
+  const int tiles = (keys + KT - 1) / KT, steps = (keys + kKeys - 1) / kKeys;
+  const int w_row = (row_tile * kWaves + wave) * 32;
   const bool w_live = w_row < rows;
   const int row = min(w_row + lane % 32, rows - 1), b = row / g, head = kvh * g + row - b * g;
   F f;
   f.init(ring, a.d);
   load_query<F>(f.q[0], a.q + b * a.q_stride + (int64_t)head * a.d, a.d);
-  const int64_t kv_stride = (int64_t)a.n_kv * a.d;
-  bool bad = false;
+  PageLoads<F, KT, kDmas, kWaves> pages(a, wave, kvh);
+  pages.hold(a.prefix_table, key0 >> a.page_log2, ((a.prefix - 1) >> a.page_log2) + 1);
+  settle_query<F>(f.q[0]);
+  auto stage = [&](int j) { return j % kRing * kStage; };
   auto load = [&](int j) {
-    const lds_u8 stage = ring + ((j - first) % kRing) * kStage;
-#pragma unroll
-    for (int i = 0; i < kDmas; ++i) {
-      const int n = wave + i * kWaves, r = F::dma_row(n);
-      const PageRow p = page_row(a.prefix_table, j * KT + n * F::kRowsPerDma, j * KT + r, 0, a.prefix - 1, a.page_log2, a.n_pages);
-      bad |= p.bad;
-      const int64_t at = p.row * kv_stride + (int64_t)kvh * a.d + 8 * F::dma_chunk(r, a.d);
-      load_to_lds(a.k_pages + at, stage + n * 1024);
-      load_to_lds(a.v_pages + at, stage + kMat + n * 1024);
-    }
+    if (j < tiles) pages.load(key0 + j * KT, 0, a.prefix - 1, ring + stage(j), ring + stage(j) + kMat);
   };
 #pragma unroll
-  for (int i = 0; i < kRing - 1; ++i)
-    if (first + i < end_tile) load(first + i);
+  for (int j = 0; j < kRing - 1; ++j) load(j);
   const float c2 = a.c2 * convert_query<F, kF16>(f.q[0]);
-  for (int j = first; j < end_tile; ++j) {
-    if (j + kRing - 2 < end_tile)
-      tile_wait<2 * kDmas * (kRing - 2), true>();
+  // tile j is there for all waves, kAhead later ones may be in flight; a last tile's V is cleared behind its keys
+  auto arrive = [&](int j, auto ahead) {
+    if (j + decltype(ahead)::value < tiles)
+      tile_wait<2 * kDmas * decltype(ahead)::value, true>();
     else
       tile_wait<0, true>();
-    if (j + kRing - 1 < end_tile) load(j + kRing - 1);
-    const int stage = ((j - first) % kRing) * kStage, mine = part * F::kMatBytes;
-    const int left = a.prefix - j * KT;
-    if (left < KT) {
-      clear_values<F, KT>(ring + stage + kMat, 0, left, threadIdx.x, kWave * kWaves);
+    if ((j + 1) * KT > keys && j * KT < keys) {
+      clear_values<F, KT>(ring + stage(j) + kMat, 0, keys - j * KT, threadIdx.x, kWave * kWaves);
       tile_wait<0, true>();
     }
-    if (!w_live || left <= part * kWaveTile) continue;
-    f32x16_t sc[1][1];
-    f.scores(stage + mine, sc);
-    if (left < KT) {
+  };
+  auto settle = [&](int i, f32x16_t (&s)[1][1]) {
+    if ((i + 1) * kKeys > keys) {
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        if (part * kWaveTile + 8 * (e / 4) + e % 4 + 4 * (lane / 32) >= left) sc[0][0][e] = -INFINITY;
+        if (i * kKeys + 8 * (e / 4) + e % 4 + 4 * (lane / 32) >= keys) s[0][0][e] = -INFINITY;
     }
+    f.raise(0, s[0], c2);
+  };
+  // the values of keys i, whose settled scores are s, and the scores of keys i + 1; `last`: of their tile
+  auto step = [&](int i, auto last, f32x16_t (&s)[1][1], f32x16_t (&next)[1][1]) {
+    const int j = i / kSub, here = stage(j) + i % kSub * F::kMatBytes;
+    if constexpr (decltype(last)::value) {
+      arrive(j + 1, Count<kRing - 3>{});  // every wave is done with tile j - 1
+      load(j + kRing - 1);
+    }
+    if (!w_live) return;
     u32x4_t p[1][2];
-    f.softmax(0, sc[0], c2, p[0]);
-    f.values(stage + kMat + mine, p);
+    f.scores(stage((i + 1) / kSub) + (i + 1) % kSub * F::kMatBytes, next);  // past the last: of nothing, not used
+    f.weigh(0, s[0], c2, p[0]);
+    f.values(here + kMat, p);
+    if (i + 1 < steps) settle(i + 1, next);
+  };
+  f32x16_t sa[1][1], sb[1][1];
+  arrive(0, Count<kRing - 2>{});
+  f.scores(0, sa);
+  settle(0, sa);
+  for (int i = 0; i < steps; i += 2) {
+    step(i, Count<kSub == 1>{}, sa, sb);
+    if (i + 1 < steps) step(i + 1, Count<1>{}, sb, sa);
   }
 
-  // the key parts' sums, lane by lane: [block][quad][lane], [block][lane]
-  static_assert(kKeyParts == 2, "one part hands its sums to the other");
-  bad = __syncthreads_or(bad);
+  const bool bad = __syncthreads_or(pages.bad);
+  const float sum = add_halves(f.l[0]);
+  const int splits = a.shared_splits + a.own_splits;
+  if (lane < 32 && w_row + lane < rows)
+    a.part_ml[((int64_t)b * a.n_heads + head) * splits + split] = make_float2(f.m[0], bad ? __uint_as_float(0x7fc00000u) : sum);
+  // the wave's sums through LDS, so that they leave as whole rows: 16 bytes at (row, chunk ^ row) of [32][DP]
   typedef __attribute__((address_space(3))) f32x4_t* lds_f32x4;
-  typedef __attribute__((address_space(3))) f32x2_t* lds_f32x2;
-  const lds_f32x4 sums = (lds_f32x4)ring + block * kQuads * kWave + lane;
-  const lds_f32x2 ml = (lds_f32x2)(ring + kRowBlocks * kQuads * kWave * 16) + block * kWave + lane;
-  float m = f.m[0], l = add_halves(f.l[0]);
-  if (part == 1) {
+  constexpr int kRowQuads = DP / 4;
+  const lds_f32x4 out = (lds_f32x4)(ring + wave * 32 * DP * 4);
 #pragma unroll
-    for (int i = 0; i < kQuads; ++i) sums[i * kWave] = quad(f, i);
-    *ml = f32x2_t{m, l};
-  }
-  __syncthreads();
-  if (part == 1 || w_row + lane % 32 >= rows) return;
-  const f32x2_t other = *ml;
-  const float top = fmaxf(m, other.x), base = top == -INFINITY ? 0.f : top;
-  const float x = __builtin_amdgcn_exp2f(m - base), y = __builtin_amdgcn_exp2f(other.x - base);
-  const int64_t at = ((int64_t)b * a.n_heads + head) * (a.shared_splits + a.own_splits) + split;
-  if (lane < 32) a.part_ml[at] = make_float2(top, bad ? __uint_as_float(0x7fc00000u) : x * l + y * other.y);
-  float* dst = a.part_o + at * a.d;
-#pragma unroll
-  for (int i = 0; i < kQuads; ++i) {
-    if (!kFull && quad_dim(i) >= a.d) continue;
-    *reinterpret_cast<f32x4_t*>(dst + quad_dim(i)) = x * quad(f, i) + y * sums[i * kWave];
+  for (int i = 0; i < kQuads; ++i) out[lane % 32 * kRowQuads + ((quad_dim(i) / 4) ^ (lane % 8))] = quad(f, i);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 4
+  for (int i = 0; i < 32 * kRowQuads / kWave; ++i) {
+    const int r = (i * kWave + lane) / kRowQuads, c = lane % kRowQuads, at_row = w_row + r;
+    const int rb = at_row / g;
+    if (at_row < rows && 4 * c < a.d)
+      *reinterpret_cast<f32x4_t*>(a.part_o + (((int64_t)rb * a.n_heads + kvh * g + at_row - rb * g) * splits + split) * a.d + 4 * c) =
+          out[r * kRowQuads + (c ^ (r % 8))];
   }
 }
 
@@ -215,8 +272,8 @@ __device__ __forceinline__ void shared_part(const BatchArgs& a, int wg, lds_u8 r
 // as [prefix, padded to kPrefixAlign][own].
 template <int DP, bool kF16, bool kFull>
 __device__ __forceinline__ void own_part(const BatchArgs& a, int wg, lds_u8 lds, float2 (&wave_ml)[kWaves][kBatchGroup]) {
-  using F = Flash<DP, kF16, kFull, 1, kWaveTile>;
-  constexpr int KT = kWaveTile, kLoads = 2 * F::kDmas, kRing = kBatchLds / kWaves / F::kStage, kQuads = 4 * F::kDimBlocks;
+  using F = Flash<DP, kF16, kFull, 1, kKeys>;
+  constexpr int KT = kKeys, kLoads = 2 * F::kDmas, kRing = kBatchLds / kWaves / F::kStage, kQuads = 4 * F::kDimBlocks;
   static_assert(kRing == 1 || kRing == 2, "");
   const int g = a.n_heads / a.n_kv, lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int team = a.own_waves, rank = wave % team;  // the item's waves, and which of them this is
@@ -224,10 +281,17 @@ __device__ __forceinline__ void own_part(const BatchArgs& a, int wg, lds_u8 lds,
   const bool spare = wg * (kWaves / team) + wave / team >= items;  // past the last item: nothing to do but the barriers
   const int kvh = item % a.n_kv, split = item / a.n_kv % a.own_splits, b = item / (a.n_kv * a.own_splits);
   const int splits = a.shared_splits + a.own_splits;
+  const int head = kvh * g + min(lane % 32, g - 1);
+  F f;
+  load_query<F>(f.q[0], a.q + b * a.q_stride + (int64_t)head * a.d, a.d);
+  const int32_t* own_table = a.tables + (int64_t)b * a.width;
+  PageLoads<F, KT, F::kDmas, 1> pages(a, 0, kvh);
+  int holds = a.width > 0 ? 1 : -1;  // 1 the own table, 0 the prefix's (which may be a row of `tables`)
+  if (holds == 1) pages.hold(own_table, 0, a.width);  // while the length is on its way
   int n = table_at(a.lengths, b);
   const bool absent = n < 0;
   const int64_t room = (int64_t)a.width << a.page_log2;
-  bool bad = n > room;
+  const int64_t n_asked = n;
   n = (int)min((int64_t)max(n, 0), room);
   const int pad = (a.prefix + kPrefixAlign - 1) / kPrefixAlign * kPrefixAlign;
   // the list's visible range: from `begin` on, up to the prefix's end in its tiles and `end` in the others
@@ -238,27 +302,18 @@ __device__ __forceinline__ void own_part(const BatchArgs& a, int wg, lds_u8 lds,
   const int per = (n_tiles + a.own_splits - 1) / a.own_splits;
   const int end_tile = first_tile + min((split + 1) * per, n_tiles), first = first_tile + split * per + rank;
   const lds_u8 ring = lds + wave * kRing * F::kStage;
-  const int head = kvh * g + min(lane % 32, g - 1);
-  F f;
   f.init(ring, a.d);
-  load_query<F>(f.q[0], a.q + b * a.q_stride + (int64_t)head * a.d, a.d);
-  const int64_t kv_stride = (int64_t)a.n_kv * a.d;
-  const int32_t* own_table = a.tables + (int64_t)b * a.width;
+  pages.bad = n_asked > room;
+  // tile j: of the prefix or of the sequence's own keys
   auto load = [&](int j, int slot) {
-    const lds_u8 stage = ring + slot * F::kStage;
     const bool own = j * KT >= pad;
-    const int base = own ? j * KT - pad : j * KT, last = own ? n - 1 : a.prefix - 1;
-    const int visible = own ? max(begin - pad, 0) : begin;
-#pragma unroll
-    for (int i = 0; i < F::kDmas; ++i) {
-      const int r = F::dma_row(i);
-      const PageRow p = page_row(own ? own_table : a.prefix_table, base + i * F::kRowsPerDma, base + r, visible, last, a.page_log2, a.n_pages);
-      bad |= p.bad;
-      const int64_t at = p.row * kv_stride + (int64_t)kvh * a.d + 8 * F::dma_chunk(r, a.d);
-      load_to_lds(a.k_pages + at, stage + i * 1024);
-      load_to_lds(a.v_pages + at, stage + F::kMatBytes + i * 1024);
-    }
+    const int base = own ? j * KT - pad : j * KT, from = own ? max(begin - pad, 0) : begin, last = own ? n - 1 : a.prefix - 1;
+    if (holds != (int)own)
+      pages.hold(own ? own_table : a.prefix_table, max(base, from) >> a.page_log2, (last >> a.page_log2) + 1);
+    holds = own;
+    pages.load(base, from, last, ring + slot * F::kStage, ring + slot * F::kStage + F::kMatBytes);
   };
+  settle_query<F>(f.q[0]);
 #pragma unroll
   for (int i = 0; i < kRing; ++i)
     if (first + i * team < end_tile) load(first + i * team, i);
@@ -303,7 +358,7 @@ __device__ __forceinline__ void own_part(const BatchArgs& a, int wg, lds_u8 lds,
   if (team > 1) {
     __syncthreads();
     if (live) {
-      if (lane < 32) wave_ml[wave][lane] = make_float2(f.m[0], bad ? __uint_as_float(0x7fc00000u) : sum);
+      if (lane < 32) wave_ml[wave][lane] = make_float2(f.m[0], pages.bad ? __uint_as_float(0x7fc00000u) : sum);
 #pragma unroll
       for (int i = 0; i < kQuads; ++i) sums[(wave * kQuads + i) * kWave + lane] = quad(f, i);
     }
@@ -318,7 +373,7 @@ __device__ __forceinline__ void own_part(const BatchArgs& a, int wg, lds_u8 lds,
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
     ml[w] = make_float2(-INFINITY, 0.f);
-    if (w < team) ml[w] = team > 1 ? wave_ml[wave - rank + w][lane % 32] : make_float2(f.m[0], bad ? __uint_as_float(0x7fc00000u) : sum);
+    if (w < team) ml[w] = team > 1 ? wave_ml[wave - rank + w][lane % 32] : make_float2(f.m[0], pages.bad ? __uint_as_float(0x7fc00000u) : sum);
     top = fmaxf(top, ml[w].x);
   }
   const float base = top == -INFINITY ? 0.f : top;
@@ -355,6 +410,7 @@ template <int DP, bool kF16, bool kFull>
 __global__ __launch_bounds__(kWave * kWaves, 2) void batch_attention_kernel(BatchArgs a) {
   __shared__ __align__(1024) uint8_t lds[kBatchLds];
   __shared__ float2 wave_ml[kWaves][kBatchGroup];
+  // the shared ones first, one a CU; the own ones take the CUs' other halves
   if ((int)blockIdx.x < a.shared_wgs)
     shared_part<DP, kF16, kFull>(a, blockIdx.x, (lds_u8)lds);
   else
@@ -431,23 +487,28 @@ struct BatchPlan {
   int64_t shared_splits, shared_tiles, row_tiles, own_splits, own_waves;
   int64_t splits() const { return shared_splits + own_splits; }
 };
-BatchPlan batch_plan(int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t prefix, int64_t max_own, int64_t window) {
+BatchPlan batch_plan(int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t d, int64_t prefix, int64_t max_own, int64_t window) {
   BatchPlan p{};
   const int64_t rows = n_seq * (n_heads / n_kv), items = n_seq * n_kv;
-  p.row_tiles = (rows + 32 * kRowBlocks - 1) / (32 * kRowBlocks);
-  const bool shared = prefix > 0 && window == 0 && n_seq > 1;
+  p.row_tiles = (rows + 32 * kWaves - 1) / (32 * kWaves);
+  // 256 own workgroups, one a CU: 64 sequences of 8 KV heads (512 items) take 31.6 us with 2 waves an item, 34.7 with
+  // 1 and 33.9 with 4; 128 sequences with 1,000 own tokens 49 us with 1 wave and 57 with 2 or 4.
+  p.own_waves = items >= 1024 ? 1 : items >= 512 ? 2 : 4;
+  // The prefix again for every sequence, mostly out of the caches, or one pass and a join: 64 x 500 of head_dim 64 take
+  // 16.8 us without the pass and 19.7 with it, 200 x 300 25.6 and 28.8, 64 x 1,000 23.2 and 20.3, 200 x 1,000 48.8 and 32.7.
+  const bool shared = window == 0 && n_seq > 1 && items * prefix * d >= (int64_t)1 << 25;
   int64_t keys = max_own + (shared ? 0 : prefix);
   if (window > 0 && window < keys) keys = window;
   if (shared) {
-    const int64_t tile = kWaveTile * kKeyParts, tiles = (prefix + tile - 1) / tile;
-    const int64_t want = (512 + n_kv * p.row_tiles - 1) / (n_kv * p.row_tiles);
+    const int64_t tile = d <= 64 ? kSharedTile<64> : kSharedTile<128>, tiles = (prefix + tile - 1) / tile;
+    const int64_t want = (256 + n_kv * p.row_tiles - 1) / (n_kv * p.row_tiles);
     p.shared_tiles = (tiles + want - 1) / want;
     p.shared_splits = (tiles + p.shared_tiles - 1) / p.shared_tiles;
   }
-  const int64_t tiles = keys / kWaveTile + 2;
-  p.own_waves = items >= 1536 ? 1 : items >= 768 ? 2 : 4;
-  const int64_t want = (512 + items - 1) / items, most = (tiles + 2 * kWaves - 1) / (2 * kWaves);
-  p.own_splits = p.own_waves < 4 ? 1 : want < most ? want : most;
+  // With few items also parts of their keys, if that is worth a join: of 20 tiles (8 sequences) one part takes 9.2 us,
+  // and three 7.1 and the join's launch of 3.6 more.
+  const int64_t tiles = keys / kKeys + 2, want = ((shared ? 256 : 512) + items - 1) / items;
+  p.own_splits = p.own_waves < 4 || (!shared && tiles <= 8 * kWaves) ? 1 : std::min(want, (tiles + 2 * kWaves - 1) / (2 * kWaves));
   return p;
 }
 
@@ -493,7 +554,7 @@ extern "C" int64_t klc_attn_batch_workspace_bytes(int64_t n_seq, int64_t n_heads
                                                   int64_t prefix_len, int64_t max_own, int64_t window) {
   const int rc = check_sizes("klc_attn_batch_workspace_bytes", n_seq, n_heads, n_kv, head_dim, prefix_len, max_own, window);
   if (rc) return rc;
-  return batch_bytes(batch_plan(n_seq, n_heads, n_kv, prefix_len, max_own, window), n_seq, n_heads, head_dim);
+  return batch_bytes(batch_plan(n_seq, n_heads, n_kv, head_dim, prefix_len, max_own, window), n_seq, n_heads, head_dim);
 }
 
 extern "C" int klc_attn_batch(const klc_attn_batch_args* args, void* stream) {
@@ -510,6 +571,9 @@ extern "C" int klc_attn_batch(const klc_attn_batch_args* args, void* stream) {
   const int64_t max_own = x.table_width * x.page_size, d = x.head_dim, rows = x.n_seq * x.n_heads;
   int rc = check_sizes("klc_attn_batch", x.n_seq, x.n_heads, x.n_kv, d, x.prefix_len, max_own, x.window);
   if (rc) return rc;
+  KLC_REQUIRE(x.page_size * x.n_kv * d < ((int64_t)1 << 30), KLC_ERR_SHAPE,
+              "klc_attn_batch: pages of %lld tokens of %lld x %lld (below 2 GiB)", (long long)x.page_size,
+              (long long)x.n_kv, (long long)d);
   KLC_REQUIRE(x.q_stride >= x.n_heads * d && x.q_stride % 8 == 0, KLC_ERR_SHAPE,
               "klc_attn_batch: q stride %lld (a multiple of 8, no overlap)", (long long)x.q_stride);
   KLC_REQUIRE(((uintptr_t)x.q | (uintptr_t)x.k_pages | (uintptr_t)x.v_pages | (uintptr_t)x.workspace | (uintptr_t)x.out) % 16 == 0,
@@ -518,7 +582,7 @@ extern "C" int klc_attn_batch(const klc_attn_batch_args* args, void* stream) {
               "klc_attn_batch: scale %g", x.scale);
   KLC_REQUIRE(x.kv_dtype == KLC_DTYPE_BF16 || x.kv_dtype == KLC_DTYPE_F16, KLC_ERR_UNSUPPORTED,
               "klc_attn_batch: kv_dtype %lld (bfloat16 or float16)", (long long)x.kv_dtype);
-  const BatchPlan p = batch_plan(x.n_seq, x.n_heads, x.n_kv, x.prefix_len, max_own, x.window);
+  const BatchPlan p = batch_plan(x.n_seq, x.n_heads, x.n_kv, d, x.prefix_len, max_own, x.window);
   const int64_t need = batch_bytes(p, x.n_seq, x.n_heads, d);
   KLC_REQUIRE(need == 0 || (x.workspace && x.workspace_bytes >= need), KLC_ERR_ARGUMENT,
               "klc_attn_batch: workspace of %lld bytes, need %lld", (long long)x.workspace_bytes, (long long)need);

@@ -215,6 +215,36 @@ def test_many_splits_and_many_sequences(gpu, count, prefix, own, window):
     check(got, q, kp, vp, tables, lengths, pt, prefix, sk, window)
 
 
+@pytest.mark.parametrize("count,prefix,heads,kv,dim,dtype,page", [
+    (70, 1000, 64, 8, 64, "fp16", 64), (33, 2050, 16, 8, 64, "bf16", 16), (24, 1400, 8, 8, 128, "fp16", 32),
+    (40, 1801, 20, 4, 120, "bf16", 16), (300, 1201, 32, 1, 96, "fp16", 128), (60, 8800, 4, 2, 32, "bf16", 32),
+    (2, 70000, 14, 2, 128, "fp16", 16)])
+def test_prefixes_read_once(gpu, count, prefix, heads, kv, dim, dtype, page):
+    """Prefixes long enough for a pass of their own."""
+    rng = np.random.RandomState(count)
+    lengths = rng.randint(0, 150, count).tolist()
+    lengths[1 % count] = -1
+    q, kp, vp, tables, pt = make(gpu, lengths, prefix, heads, kv, dim, dtype, page=page, seed=count, q_std=2.0)
+    q[0, 0] = 0
+    q[0, 1] = 3e5  # past float16
+    sk = torch.randn(heads, device=gpu).bfloat16()
+    got = call(gpu, q, kp, vp, tables, lengths, pt, prefix, sinks=sk)
+    check(got, q, kp, vp, tables, lengths, pt, prefix, sk)
+    got = call(gpu, q, kp, vp, tables, lengths, pt[:-2] + [-5] + pt[-1:], prefix, sinks=sk)
+    here = torch.tensor([n >= 0 for n in lengths], device=gpu)
+    assert got[here].isnan().all() and not got[~here].any()
+
+
+def test_prefix_table_within_the_tables(gpu):
+    """The prefix's table may be a row of the sequences' tables."""
+    q, kp, vp, tables, _ = make(gpu, [2000, 300], 0, 8, 2, 64, "fp16", seed=12)
+    t, n = int32(tables, gpu), int32([1999, 300], gpu)
+    for window in (None, 2500):
+        got = ops.batch_attention(q, kp, vp, t, n, t[0], 1990, window=window)
+        assert torch.equal(got, ops.batch_attention(q, kp, vp, t, n, t[0].clone(), 1990, window=window))
+        check(got, q, kp, vp, tables, [1999, 300], tables[0], 1990, None, window)
+
+
 def test_wide_tables_of_short_sequences(gpu):
     """Tables made for long sequences (many splits), sequences of a few tokens."""
     lengths = [1, 2, 40, 0]

@@ -82,17 +82,18 @@ def batch_args(**kw):
 
 
 @pytest.mark.parametrize("change,status,text", [
-    (dict(lengths=0), nat.KLC_ERR_ARGUMENT, "null pointer"), (dict(workspace=0), nat.KLC_ERR_ARGUMENT, "workspace"),
+    (dict(lengths=0), nat.KLC_ERR_ARGUMENT, "null pointer"), (dict(workspace=0, prefix_len=3000), nat.KLC_ERR_ARGUMENT, "workspace"),
     (dict(tables=0), nat.KLC_ERR_ARGUMENT, "null table"), (dict(prefix_table=0), nat.KLC_ERR_ARGUMENT, "null table"),
     (dict(page_size=8), nat.KLC_ERR_SHAPE, "power of two"), (dict(page_size=48), nat.KLC_ERR_SHAPE, "power of two"),
-    (dict(page_size=8192), nat.KLC_ERR_SHAPE, "power of two"), (dict(n_pages=1 << 26), nat.KLC_ERR_SHAPE, "pages"),
+    (dict(page_size=8192), nat.KLC_ERR_SHAPE, "power of two"),
+    (dict(page_size=4096, n_heads=4096, n_kv=4096, q_stride=4096 * 64), nat.KLC_ERR_SHAPE, "2 GiB"), (dict(n_pages=1 << 26), nat.KLC_ERR_SHAPE, "pages"),
     (dict(table_width=-1), nat.KLC_ERR_SHAPE, "tables"), (dict(n_heads=66, q_stride=66 * 64), nat.KLC_ERR_SHAPE, "group"),
     (dict(head_dim=68), nat.KLC_ERR_SHAPE, "head_dim"), (dict(n_seq=0), nat.KLC_ERR_ARGUMENT, "sequences"),
     (dict(n_seq=70000), nat.KLC_ERR_ARGUMENT, "sequences"), (dict(prefix_len=-1), nat.KLC_ERR_ARGUMENT, "prefix"),
     (dict(window=-3), nat.KLC_ERR_ARGUMENT, "window"), (dict(table_width=1 << 24), nat.KLC_ERR_ARGUMENT, "own tokens"),
     (dict(q_stride=500), nat.KLC_ERR_SHAPE, "stride"), (dict(out=0x1008), nat.KLC_ERR_ARGUMENT, "aligned"),
     (dict(scale=-1.0), nat.KLC_ERR_ARGUMENT, "scale"), (dict(kv_dtype=nat.DTYPE_F32), nat.KLC_ERR_UNSUPPORTED, "kv_dtype"),
-    (dict(workspace_bytes=64), nat.KLC_ERR_ARGUMENT, "workspace")])
+    (dict(workspace_bytes=64, prefix_len=3000), nat.KLC_ERR_ARGUMENT, "workspace")])
 def test_batch_refusals(change, status, text):
     refused("klc_attn_batch", batch_args(**change), status, text)
 
