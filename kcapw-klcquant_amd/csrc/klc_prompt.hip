@@ -37,7 +37,7 @@ struct Rows {
   F f;
   int tok[RB];
 
-  // the wave's rows from w_row on, with their sinks
+  // the wave's rows from w_row on
   __device__ __forceinline__ void begin(const PromptArgs& a, const PromptTile& t, int w_row, lds_u8 ring) {
     const int lane = threadIdx.x % kWave;
     f.init(ring, a.d);
@@ -53,11 +53,18 @@ struct Rows {
         f.q[rb][st] = u32x4_t{0, 0, 0, 0};
         if (kFull || 8 * c < a.d) f.q[rb][st] = *reinterpret_cast<const u32x4_t*>(src + 8 * c);
       }
-      if (a.sinks != nullptr) {
-        const float sink = sink_log2(a.sinks[head]);
-        f.m[rb] = sink;
-        f.l[rb] = sink == -INFINITY || lane >= 32 ? 0.f : 1.f + (sink - sink);
-      }
+    }
+  }
+  // their sinks; loaded behind the first tiles, so that the wait for them is one for everything in flight
+  __device__ __forceinline__ void begin_sinks(const PromptArgs& a, const PromptTile& t, int w_row) {
+    if (a.sinks == nullptr) return;
+    const int lane = threadIdx.x % kWave;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const int head = t.kvh * t.g + min(w_row + 32 * rb + lane % 32, t.last) - tok[rb] * t.g;
+      const float sink = sink_log2(a.sinks[head]);
+      f.m[rb] = sink;
+      f.l[rb] = sink == -INFINITY || lane >= 32 ? 0.f : 1.f + (sink - sink);
     }
   }
 
@@ -191,6 +198,7 @@ __device__ __forceinline__ bool prompt_rows(const PromptArgs& a, const PromptTil
   const int to = w_row <= t.last ? (w_hi - tiles.first) / kTileKeys : from - 1;
 #pragma unroll
   for (int j = 0; j < kRing - 1; ++j) tiles.load(j);
+  r.begin_sinks(a, t, w_row);
 
   // what follows the scores of keys i: the mask and the maximum
   auto settle = [&](int i, f32x16_t (&s)[RB][1]) {
@@ -255,6 +263,7 @@ __device__ __forceinline__ void prompt_rows_careful(const PromptArgs& a, const P
   for (int tok = w_row / t.g; tok <= last_tok && w_row <= t.last; ++tok) {
     R r;
     r.begin(a, t, w_row, tile);
+    r.begin_sinks(a, t, w_row);
     for (int k0 = a.window > 0 ? max(0, tok - a.window + 1) : 0; k0 <= tok; k0 += kKeys) {
 #pragma unroll
       for (int n = 0; n < F::kDmas; ++n) {
@@ -294,21 +303,23 @@ __global__ __launch_bounds__(64 * W, kPerSimd) void prompt_attention_kernel(Prom
   // tiles as its rows need, and the list needs no pass over the lengths.  Late tiles, the longest of a
   // sequence, go first.
   const int i = (int)(gridDim.x / a.n_kv) - 1 - (int)(blockIdx.x / a.n_kv);
-  auto start_of = [&](int s) { return min(max(a.starts[s], 0), a.tokens); };
-  auto tile_of = [&](int s) { return (int)((int64_t)start_of(s) * t.g / kRows) + s; };
+  auto tile_at = [&](int begin, int s) { return (int)((int64_t)begin * t.g / kRows) + s; };
   // 64 sequences a look: the last one that starts at or before i (the first is taken to)
-  int s = 0, span = a.n_seq;  // it is among s .. s + span - 1
-  while (span > 1) {
-    const int stride = (span + kWave - 1) / kWave, at = s + stride * (int)(threadIdx.x % kWave);
-    const bool before = at == s || (at < s + span && tile_of(at) <= i);
-    const int found = __popcll(__ballot(before)) - 1;
+  int s = 0, span = a.n_seq, stride, start, found;  // it is among s .. s + span - 1
+  do {
+    stride = (span + kWave - 1) / kWave;
+    const int at = min(s + stride * (int)(threadIdx.x % kWave), a.n_seq);
+    start = min(max(a.starts[at], 0), a.tokens);
+    found = __popcll(__ballot(at == s || (at < s + span && tile_at(start, at) <= i))) - 1;
     span = min(stride, span - found * stride);
     s += found * stride;
-  }
+  } while (stride > 1);
   s = __builtin_amdgcn_readfirstlane(s);
-  t.begin = __builtin_amdgcn_readfirstlane(start_of(s));
-  t.len = __builtin_amdgcn_readfirstlane(start_of(s + 1)) - t.begin;
-  const int64_t row0 = (int64_t)(i - tile_of(s)) * kRows, seq_rows = (int64_t)t.len * t.g;
+  found = __builtin_amdgcn_readfirstlane(found);
+  t.begin = __builtin_amdgcn_readlane(start, found);
+  const int end = found + 1 < kWave ? __builtin_amdgcn_readlane(start, found + 1) : min(max(a.starts[s + 1], 0), a.tokens);
+  t.len = __builtin_amdgcn_readfirstlane(end) - t.begin;
+  const int64_t row0 = (int64_t)(i - tile_at(t.begin, s)) * kRows, seq_rows = (int64_t)t.len * t.g;
   if (row0 < 0 || row0 >= seq_rows) return;  // no tile of an (empty) sequence
   t.row0 = (int)row0;
   t.last = (int)(min(row0 + kRows, seq_rows) - 1);
@@ -319,13 +330,31 @@ __global__ __launch_bounds__(64 * W, kPerSimd) void prompt_attention_kernel(Prom
       prompt_rows_careful<DP, kF16, kFull>(a, t, w_row + 32 * rb, (lds_u8)ring + wave * 2 * 2 * kKeys * DP);
 }
 
+template <int kValue>
+struct Count {
+  static constexpr int value = kValue;
+};
+
 template <int DP, bool kF16, bool kFull>
 int launch_prompt(const PromptArgs& a, hipStream_t st) {
   const int64_t g = a.n_heads / a.n_kv;
-  // two waves a SIMD either way, by registers; the rows of a workgroup share its tiles
-  constexpr int RB = DP == 64 ? 2 : 1, W = DP == 64 ? 4 : 8;
-  const int64_t tiles = a.tokens * g / (32 * RB * W) + a.n_seq;
-  prompt_attention_kernel<DP, kF16, kFull, RB, W, 4, 2><<<(unsigned)(tiles * a.n_kv), 64 * W, 0, st>>>(a);
+  // Head sizes up to 64: 64 rows a wave share the K and V reads of a long sequence, 32 a wave give three workgroups a
+  // CU, whose starts and ends hide each other, and fill the chip sooner.  64 heads over 8: one sequence of 512 tokens
+  // takes 13.4 us with 32 rows and 19.8 with 64, of 1,000 22 and 31, of 3,000 95 and 99, of 8,192 615 and 587; 400 of
+  // 125 tokens 299 and 320, 7 of 2,857 762 and 748.  Past 64 a wave's registers take 32 rows, and eight waves share them.
+  const bool short_rows = a.tokens * g * a.n_kv < 1024 * 256 || a.tokens / a.n_seq < 2048;
+  auto run = [&](auto rb, auto w, auto ring, auto per_simd) {
+    constexpr int RB = decltype(rb)::value, W = decltype(w)::value;
+    const int64_t tiles = a.tokens * g / (32 * RB * W) + a.n_seq;
+    prompt_attention_kernel<DP, kF16, kFull, RB, W, decltype(ring)::value, decltype(per_simd)::value>
+        <<<(unsigned)(tiles * a.n_kv), 64 * W, 0, st>>>(a);
+  };
+  if constexpr (DP == 128)
+    run(Count<1>{}, Count<8>{}, Count<4>{}, Count<2>{});
+  else if (short_rows)
+    run(Count<1>{}, Count<4>{}, Count<3>{}, Count<3>{});
+  else
+    run(Count<2>{}, Count<4>{}, Count<4>{}, Count<2>{});
   return check_launch("prompt_attention_kernel");
 }
 

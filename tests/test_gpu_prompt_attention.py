@@ -181,6 +181,24 @@ def test_long_prompt_rows(gpu):
             assert ((got[row].double() - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("lengths,dim,window,sinks", [((2101,), 64, None, True), ((2500, 0, 1900, 2200), 64, 100, False),
+                                                      ((2201,), 24, None, True), ((2048,), 48, 700, False)])
+def test_many_rows_of_long_prompts(gpu, dtype, lengths, dim, window, sinks):
+    """Enough long rows that a wave takes 64 of them."""
+    heads = 128
+    q, k, v, starts = make(gpu, lengths, heads, 4, dim, DTYPES[dtype], seed=dim, lead=3, tail=2)
+    sk = torch.randn(heads, device=gpu).bfloat16() if sinks else None
+    out = torch.full_like(q, 7.0)
+    ops.prompt_attention(q, k, v, device_starts(starts, gpu), sk, window, out=out)
+    assert (out[:3] == 7).all() and (out[-2:] == 7).all()
+    shown = slice(5, heads, 31)  # heads 5, 36, 67 and 98: one of each group
+    check(out[:, shown], q[:, shown], k, v, starts, None if sk is None else sk[shown], window)
+    k[400], v[1000, 2, 3], v[1500, 1, 0] = math.nan, math.inf, -math.inf
+    ops.prompt_attention(q, k, v, device_starts(starts, gpu), sk, window, out=out)
+    check(out[:, shown], q[:, shown], k, v, starts, None if sk is None else sk[shown], window)
+
+
 def test_streams_graphs_and_repeats(gpu):
     """The same bits on another stream, twice at once, and from a graph replayed with new inputs between eager calls."""
     q, k, v, starts = make(gpu, (150, 333), 8, 2, 64, torch.bfloat16, seed=12)
