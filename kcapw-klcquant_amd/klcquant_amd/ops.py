@@ -365,9 +365,11 @@ def _check_heads(sinks: torch.Tensor | None, n_heads: int, n_kv: int, window: in
             dim ** -0.5 if scale is None else float(scale))
 
 
-def _result(name: str, out: torch.Tensor | None, shape: tuple, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
+def _result(name: str, out: torch.Tensor | None, like: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """``out``, or a new contiguous tensor as ``like`` (a view of wider rows of contiguous heads, so empty_like is)."""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=dev)
+        return torch.empty_like(like)
+    shape, dtype = like.shape, like.dtype
     if not _plain(out, dtype, shape, dev.index):
         _check_gpu(name, out, dtype)
         raise ValueError(f"{name} must be {tuple(shape)} on {dev}, got {tuple(out.shape)} on {out.device}")
@@ -411,7 +413,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     if n_seq < 0:
         raise ValueError("starts must hold the sequences' starts and the end of the last one")
     sink_ptr, window, scale = _check_heads(sinks, n_heads, n_kv, window, scale, dim, dev)
-    out = _result("out", out, shape, dtype, dev)
+    out = _result("out", out, q, dev)
     if tokens and n_seq:
         _call("klc_attn_prompt",
               _PROMPT_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), starts.data_ptr(), sink_ptr, out.data_ptr(),
@@ -460,8 +462,8 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.T
             raise ValueError(f"{name} must be [positions, {dim // 2}] on {dev}, got {tuple(t.shape)} on {t.device}")
     _check_index("positions", positions, (tokens,), dev)
     _check_index("slots", slots, (tokens,), dev)
-    q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
-    k_out = torch.empty(k.shape, dtype=torch.bfloat16, device=dev) if want_keys else None
+    q_out = _result("q", None, q, dev)
+    k_out = _result("k", None, k, dev) if want_keys else None
     if tokens:
         _call("klc_kv_append",
               _APPEND_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), cos.data_ptr(), sin.data_ptr(),
@@ -535,7 +537,7 @@ def batch_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         if held * page < prefix_len:
             raise ValueError(f"prefix of {prefix_len} tokens in {held} pages of {page}")
     sink_ptr, window, scale = _check_heads(sinks, n_heads, n_kv, window, scale, dim, dev)
-    out = _result("out", out, shape, torch.bfloat16, dev)
+    out = _result("out", out, q, dev)
     if not count:
         return out
     sizes = (count, n_heads, n_kv, dim, prefix_len, width * page, window)
