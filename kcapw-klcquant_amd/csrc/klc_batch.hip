@@ -128,8 +128,9 @@ struct PageLoads {
     held = t[min(from + (int)(threadIdx.x % kWave), size - 1)];
     asm volatile("" : "+v"(held));  // waited for here, not again (with the tiles in flight) at every use
   }
-  // Loads the tile from key `base` of the held table on to K at `k` and V at `v` of LDS.  Keys outside first..last
-  // take the nearest visible one's row, so that only its pages are asked for.
+  // Loads the tile from key `base` of the held table on to K at `k` and V at `v` of LDS, or one of the two.  Keys
+  // outside first..last take the nearest visible one's row, so that only its pages are asked for.
+  template <bool kKey = true, bool kValue = true>
   __device__ __forceinline__ void load(int base, int first, int last, lds_u8 k, lds_u8 v) {
     const int mask = (1 << a.page_log2) - 1;
     if ((min(base + KT - 1, last) >> a.page_log2) - from >= kWave) hold(table, min(max(base, first), last) >> a.page_log2, size);
@@ -141,8 +142,8 @@ struct PageLoads {
       bad |= wrong;
       const uint64_t start = (uint64_t)(wrong ? 0u : (uint32_t)page) * page_bytes;
       const uint32_t off = (uint32_t)(min(max(base + r, first), last) & mask) * row_bytes + 16u * (uint32_t)F::dma_chunk(r, a.d);
-      load_to_lds(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(k0) + start), off, k + n * 1024);
-      load_to_lds(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(v0) + start), off, v + n * 1024);
+      if constexpr (kKey) load_to_lds(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(k0) + start), off, k + n * 1024);
+      if constexpr (kValue) load_to_lds(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(v0) + start), off, v + n * 1024);
     }
   }
 };
@@ -273,8 +274,12 @@ __device__ __forceinline__ void shared_part(const BatchArgs& a, int wg, lds_u8 r
 template <int DP, bool kF16, bool kFull>
 __device__ __forceinline__ void own_part(const BatchArgs& a, int wg, lds_u8 lds, float2 (&wave_ml)[kWaves][kBatchGroup]) {
   using F = Flash<DP, kF16, kFull, 1, kKeys>;
-  constexpr int KT = kKeys, kLoads = 2 * F::kDmas, kRing = kBatchLds / kWaves / F::kStage, kQuads = 4 * F::kDimBlocks;
+  constexpr int KT = kKeys, kRing = kBatchLds / kWaves / F::kStage, kQuads = 4 * F::kDimBlocks;
   static_assert(kRing == 1 || kRing == 2, "");
+  // With one tile a wave, K and V take turns: the next K comes while this V is multiplied, and the other way round
+  // (64 sequences of 2,000 tokens, head size 128: 77.8 us by whole tiles, 69.7 so; with two tiles a wave the second
+  // addressing costs more than it hides, 124 us against 128 for 256 sequences of head size 64).
+  constexpr bool kHalves = kRing == 1;
   const int g = a.n_heads / a.n_kv, lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int team = a.own_waves, rank = wave % team;  // the item's waves, and which of them this is
   const int items = a.n_kv * a.own_splits * a.n_seq, item = min(wg * (kWaves / team) + wave / team, items - 1);
@@ -305,34 +310,46 @@ __device__ __forceinline__ void own_part(const BatchArgs& a, int wg, lds_u8 lds,
   f.init(ring, a.d);
   pages.bad = n_asked > room;
   // tile j: of the prefix or of the sequence's own keys
-  auto load = [&](int j, int slot) {
+  auto load = [&](auto key, auto value, int j, int slot) {
     const bool own = j * KT >= pad;
     const int base = own ? j * KT - pad : j * KT, from = own ? max(begin - pad, 0) : begin, last = own ? n - 1 : a.prefix - 1;
     if (holds != (int)own)
       pages.hold(own ? own_table : a.prefix_table, max(base, from) >> a.page_log2, (last >> a.page_log2) + 1);
     holds = own;
-    pages.load(base, from, last, ring + slot * F::kStage, ring + slot * F::kStage + F::kMatBytes);
+    pages.template load<decltype(key)::value, decltype(value)::value>(base, from, last, ring + slot * F::kStage,
+                                                                      ring + slot * F::kStage + F::kMatBytes);
   };
   settle_query<F>(f.q[0]);
 #pragma unroll
   for (int i = 0; i < kRing; ++i)
-    if (first + i * team < end_tile) load(first + i * team, i);
+    if (first + i * team < end_tile) {
+      if constexpr (kHalves) {
+        load(Count<true>{}, Count<false>{}, first + i * team, i);
+        load(Count<false>{}, Count<true>{}, first + i * team, i);
+      } else {
+        load(Count<true>{}, Count<true>{}, first + i * team, i);
+      }
+    }
   const float c2 = a.c2 * convert_query<F, kF16>(f.q[0]);
   int slot = 0;
   for (int j = first; j < end_tile; j += team) {
-    if (kRing == 2 && j + team < end_tile)
-      tile_wait<kLoads, false>();
+    // K is there, and V unless it comes by itself; the ring's other tile may be in flight
+    const bool refill = j + kRing * team < end_tile;
+    if (kHalves)
+      tile_wait<F::kDmas, false>();
+    else if (j + team < end_tile)
+      tile_wait<2 * F::kDmas, false>();
     else
       tile_wait<0, false>();
     const int stage = slot * F::kStage;
     const int from = max(0, begin - j * KT), to = min(KT, (j * KT >= pad ? end : a.prefix) - j * KT);
     const bool part = from > 0 || to < KT;
-    if (part) {
-      clear_values<F, KT>(ring + stage + F::kMatBytes, from, to, lane, kWave);
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    }
     f32x16_t sc[1][1];
     f.scores(stage, sc);
+    if (kHalves && refill) {
+      tile_wait<63, false>();  // K has been read
+      load(Count<true>{}, Count<false>{}, j + kRing * team, slot);
+    }
     if (part) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -342,10 +359,18 @@ __device__ __forceinline__ void own_part(const BatchArgs& a, int wg, lds_u8 lds,
     }
     u32x4_t p[1][2];
     f.softmax(0, sc[0], c2, p[0]);
+    if (kHalves && refill)
+      tile_wait<F::kDmas, false>();
+    else if (kHalves)
+      tile_wait<0, false>();
+    if (part) {
+      clear_values<F, KT>(ring + stage + F::kMatBytes, from, to, lane, kWave);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
     f.values(stage + F::kMatBytes, p);
-    if (j + kRing * team < end_tile) {
-      tile_wait<63, false>();  // the slot's reads are done
-      load(j + kRing * team, slot);
+    if (refill) {
+      tile_wait<63, false>();  // the slot has been read
+      load(Count<!kHalves>{}, Count<true>{}, j + kRing * team, slot);
     }
     slot = (slot + 1) % kRing;
   }
