@@ -11,7 +11,18 @@
 //           own with no barrier
 // Two workgroups fit a CU by LDS and registers.  Parts are float32 (sum,
 // maximum, normaliser) and a second launch joins them; where a row has one
-// part, the own workgroup writes the result itself.
+// part, the own workgroup writes the result itself:
+//
+//   out = sum_i 2^(m_i - m) o_i / (sum_i 2^(m_i - m) l_i + 2^(s - m)),  m = max(m_i, s)
+//
+// What bounds it (64 heads over 8 of size 64, float16 pages): 64 sequences
+// with up to 700 own tokens behind a prefix of 8,192, 28 to 32 us of which the
+// join is 4.5; the prefix's pass is the longer side, with one wave a SIMD 465
+// ns for 32 rows by 32 keys where two waves would take 227 each, but twice the
+// workgroups would write twice the parts.  256 sequences of 2,000 tokens, 124
+// us: HBM at 4.8 TB/s.  200 on a window of 128, 13.7 us, and 8 behind 500
+// tokens, 9 us: the chain of length, page numbers, first tile.  32 of 900
+// behind 16,000, 32 heads of size 128, 35.5 us and a join of 5.5.
 #include <math.h>
 
 #include <algorithm>

