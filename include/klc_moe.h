@@ -486,8 +486,9 @@ int klc_attn_step_wait(const void* host_record, int64_t tag, int64_t limit_us);
  * (streamed_attention.py:101-152); the mathematics, sinks and window are that
  * call's.  The cache's pools are [n_pages][page_size][n_kv][head_dim] of
  * kv_dtype (KLC_DTYPE_F16 or KLC_DTYPE_BF16), page_size a power of two from
- * 16 to 4096, a page below 2 GiB; slot i is token i % page_size of page i / page_size.  head_dim
- * is a multiple of 8 up to 128; query head h reads KV head h / (n_heads / n_kv). */
+ * 16 to 4096, a page below 2 GiB; slot i is token i % page_size of page
+ * i / page_size.  head_dim is a multiple of 8 up to 128; query head h reads KV
+ * head h / (n_heads / n_kv). */
 
 /* Causal attention of whole prompts, packed one behind the other: sequence s
  * is tokens starts[s] up to starts[s + 1] (int32 [n_seq + 1], ascending, on the
@@ -500,8 +501,8 @@ int klc_attn_step_wait(const void* host_record, int64_t tag, int64_t limit_us);
  * are rounded to `dtype` before the value product, which the sum of the
  * rounded ones normalises.  Rows of out [tokens][n_heads][head_dim] outside
  * every sequence are not written.  What a row must not see does not reach it,
- * NaN and infinities included.  q, k, v and out 16-byte aligned; tokens *
- * n_heads / n_kv < 2^30. */
+ * NaN and infinities included.  q, k, v and out 16-byte aligned, out apart
+ * from the others; tokens * n_heads / n_kv < 2^30. */
 typedef struct klc_attn_prompt_args {
   const void *q, *k, *v;  /* [tokens][heads][head_dim] of dtype */
   const void* starts;     /* int32 [n_seq + 1] */
@@ -547,7 +548,8 @@ int klc_kv_copy_pages(void* pools, int64_t n_pools, int64_t n_pages, int64_t pag
  * probabilities rounded to kv_dtype; out [n_seq][n_heads][head_dim] bfloat16.
  * lengths[b] < 0: no sequence, zeros.  A page number outside [0, n_pages) or a
  * length past table_width * page_size makes the sequence's output NaN (of the
- * prefix: every sequence's); nothing outside the pools is read.  n_heads / n_kv <= 32, n_seq <= 65535.
+ * prefix: every sequence's); nothing outside the pools is read.  n_heads /
+ * n_kv <= 32, n_seq <= 65535.
  * workspace: klc_attn_batch_workspace_bytes with max_own = table_width *
  * page_size (0: none needed), 16-byte aligned, no initialisation; calls that
  * may overlap need one each. */

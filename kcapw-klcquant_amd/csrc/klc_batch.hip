@@ -532,7 +532,7 @@ BatchPlan batch_plan(int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t d, in
   p.own_waves = items >= 1024 ? 1 : items >= 512 ? 2 : 4;
   // The prefix again for every sequence, mostly out of the caches, or one pass and a join: 64 x 500 of head_dim 64 take
   // 16.8 us without the pass and 19.7 with it, 200 x 300 25.6 and 28.8, 64 x 1,000 23.2 and 20.3, 200 x 1,000 48.8 and 32.7.
-  const bool shared = window == 0 && n_seq > 1 && items * prefix * d >= (int64_t)1 << 25;
+  const bool shared = window == 0 && n_seq > 1 && (double)items * prefix * d >= 1 << 25;
   int64_t keys = max_own + (shared ? 0 : prefix);
   if (window > 0 && window < keys) keys = window;
   if (shared) {

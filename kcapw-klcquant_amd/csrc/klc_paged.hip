@@ -90,23 +90,19 @@ constexpr int kMovesPerLaunch = 384;
 struct Moves {
   int32_t src[kMovesPerLaunch], dst[kMovesPerLaunch];
 };
-// Bound by HBM: 64 bytes a thread in flight, 400 pages of 64 KB in 8 pools
-// (419 MB moved) in 72 to 87 us, 16 in 72 pools (151 MB) in 24 to 35.
-constexpr int kCopyUnroll = 4;
-constexpr int kCopyBytes = kPagedThreads * 16 * kCopyUnroll;  // of a workgroup
+// Bound by HBM.  16 bytes a thread, past the caches on both ways, as neither
+// page is soon read: 400 pages of 64 KB in 8 pools (419 MB moved) take 73 us
+// (5.7 TB/s), 16 in 72 pools (151 MB) 27; cached 78 and 30, with 32 bytes a
+// thread 81 and 28, with 64 82 and 32, with 64 cached 88 and 37.
+constexpr int kCopyBytes = kPagedThreads * 16;  // of a workgroup
 
 __global__ __launch_bounds__(kPagedThreads) void copy_pages_kernel(uint8_t* __restrict__ pool, int64_t pool_bytes,
                                                                    int64_t page_bytes, Moves moves) {
-  const int64_t from = blockIdx.z * pool_bytes + moves.src[blockIdx.y] * page_bytes;
-  const int64_t to = blockIdx.z * pool_bytes + moves.dst[blockIdx.y] * page_bytes;
+  uint8_t* base = pool + blockIdx.z * pool_bytes;
   const int64_t at = (int64_t)blockIdx.x * kCopyBytes + threadIdx.x * 16;
-  u32x4_t x[kCopyUnroll];
-#pragma unroll
-  for (int i = 0; i < kCopyUnroll; ++i)
-    if (at + i * kPagedThreads * 16 < page_bytes) x[i] = *reinterpret_cast<const u32x4_t*>(pool + from + at + i * kPagedThreads * 16);
-#pragma unroll
-  for (int i = 0; i < kCopyUnroll; ++i)
-    if (at + i * kPagedThreads * 16 < page_bytes) *reinterpret_cast<u32x4_t*>(pool + to + at + i * kPagedThreads * 16) = x[i];
+  if (at >= page_bytes) return;
+  const u32x4_t x = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(base + moves.src[blockIdx.y] * page_bytes + at));
+  __builtin_nontemporal_store(x, reinterpret_cast<u32x4_t*>(base + moves.dst[blockIdx.y] * page_bytes + at));
 }
 
 }  // namespace

@@ -11,6 +11,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
+import operator
 import struct
 from typing import NamedTuple
 
@@ -359,9 +360,9 @@ def _check_heads(sinks: torch.Tensor | None, n_heads: int, n_kv: int, window: in
             raise ValueError(f"sinks must be [{n_heads}] on {dev}, got {tuple(sinks.shape)} on {sinks.device}")
         if sinks.requires_grad and torch.is_grad_enabled():
             raise ValueError("sinks require grad: this operator has no backward pass")
-    if window is not None and window <= 0:
+    if window is not None and operator.index(window) <= 0:
         raise ValueError(f"window must be positive (None: no window), got {window}")
-    return (0 if sinks is None else sinks.data_ptr(), min(int(window), (1 << 30) - 1) if window else 0,
+    return (0 if sinks is None else sinks.data_ptr(), min(operator.index(window), (1 << 30) - 1) if window else 0,
             dim ** -0.5 if scale is None else float(scale))
 
 
@@ -373,6 +374,8 @@ def _result(name: str, out: torch.Tensor | None, like: torch.Tensor, dev: torch.
     if not _plain(out, dtype, shape, dev.index):
         _check_gpu(name, out, dtype)
         raise ValueError(f"{name} must be {tuple(shape)} on {dev}, got {tuple(out.shape)} on {out.device}")
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires grad: this operator has no backward pass")
     return out
 
 
@@ -396,7 +399,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     bfloat16 or all float16 (views with contiguous heads too, such as splits of one projection), sequence ``s`` =
     tokens ``starts[s]:starts[s + 1]`` (int32 ``[S + 1]`` on the device, ascending) -> ``[T, n_heads, D]``.  A token
     sees the last ``window`` tokens up to itself (None: all); ``sinks`` bf16 ``[n_heads]``; ``scale`` 1 / sqrt(D)
-    unless given.  Rows outside every sequence are left as ``out`` had them."""
+    unless given.  Rows outside every sequence are left as ``out`` had them; ``out`` shares no memory with the inputs."""
     if not isinstance(q, torch.Tensor):
         raise TypeError(f"q must be a torch.Tensor, got {type(q).__name__}")
     dev, dtype = q.device, q.dtype
@@ -432,6 +435,8 @@ def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, dev: torch.device
             raise ValueError(f"tensors on different devices: {dev} vs {k_pages.device}, {v_pages.device}")
         if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
             raise ValueError(f"page pools mismatch: {k_pages.dtype} {tuple(k_pages.shape)}, {v_pages.dtype} {tuple(v_pages.shape)}")
+    if (k_pages.requires_grad or v_pages.requires_grad) and torch.is_grad_enabled():
+        raise ValueError("pages require grad: this operator has no backward pass")
     n_pages, page, n_kv, dim = k_pages.shape
     if n_pages == 0 or page < 16 or page > 4096 or page & (page - 1):
         raise ValueError(f"pages must hold a power of two of tokens, 16 to 4096, got {n_pages} of {page}")
@@ -460,6 +465,8 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.T
         if not _plain(t, torch.bfloat16, (n_pos, dim // 2), dev.index) or not n_pos:
             _check_gpu(name, t, torch.bfloat16, 2)
             raise ValueError(f"{name} must be [positions, {dim // 2}] on {dev}, got {tuple(t.shape)} on {t.device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} requires grad: this operator has no backward pass")
     _check_index("positions", positions, (tokens,), dev)
     _check_index("slots", slots, (tokens,), dev)
     q_out = _result("q", None, q, dev)
@@ -489,6 +496,8 @@ def copy_pages(pools: torch.Tensor, src, dst) -> None:
     ...]`` and page numbers on the host (sequences or int32 arrays).  The moves run at once: a destination is no other
     move's source or destination."""
     _check_gpu("pools", pools)
+    if pools.requires_grad and torch.is_grad_enabled():
+        raise ValueError("pools require grad: this operator has no backward pass")
     if pools.dim() < 3 or pools.numel() == 0:
         raise ValueError(f"pools must be [pools, pages, ...], got shape {tuple(pools.shape)}")
     src, dst = _page_numbers(src), _page_numbers(dst)
@@ -526,7 +535,7 @@ def batch_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     width = tables.shape[1] if isinstance(tables, torch.Tensor) and tables.dim() == 2 else 0
     _check_index("tables", tables, (count, width), dev)
     _check_index("lengths", lengths, (count,), dev)
-    prefix_len = int(prefix_len)
+    prefix_len = operator.index(prefix_len)
     if prefix_len < 0:
         raise ValueError(f"prefix_len must not be negative, got {prefix_len}")
     if prefix_len:

@@ -26,6 +26,9 @@ from . import ops
 from .attention import _KV_DTYPES, AttentionConfig, yarn_attention_scaling, yarn_inv_freq
 
 
+_MAX_ROWS = 65535  # of a batch_attention call
+
+
 class PageTable:
     """Pages of ``page_size`` tokens among sequences, numbered as they were added (numbers are used again)."""
 
@@ -264,6 +267,7 @@ class PagedAttention:
     def __init__(self, config: AttentionConfig) -> None:
         self.config = config
         self._tables: dict = {}  # device -> (cos, sin) of the positions so far
+        self._kept: list = []    # smaller ones, which captured graphs may still read
 
     def rope_tables(self, n_positions: int, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
         """bfloat16 ``[n, head_dim / 2]`` cosines and sines, row p as rope_cos_sin's of position p, n >= n_positions."""
@@ -274,6 +278,7 @@ class PagedAttention:
             s = yarn_attention_scaling(self.config)
             held = ((torch.cos(angle) * s).to(torch.bfloat16), (torch.sin(angle) * s).to(torch.bfloat16))
             torch.cuda.current_stream(device).synchronize()  # any stream may read them from here on
+            self._kept.append(self._tables.get(device))
             self._tables[device] = held
         return held
 
@@ -302,7 +307,10 @@ class PagedAttention:
         if batch.fresh:
             context = ops.prompt_attention(q, k, v, batch.starts, sinks, window)
         else:
-            context = ops.batch_attention(q, k_pages, v_pages, batch.tables, batch.lengths, batch.prefix_table,
-                                          batch.prefix_len, sinks, window)
+            context = torch.empty_like(q)
+            for i in range(0, batch.tokens, _MAX_ROWS):
+                rows = slice(i, i + _MAX_ROWS)
+                ops.batch_attention(q[rows], k_pages, v_pages, batch.tables[rows], batch.lengths[rows],
+                                    batch.prefix_table, batch.prefix_len, sinks, window, out=context[rows])
         o_weight = tensors[f"{prefix}.o_proj.weight"]
         return lin(context.view(batch.tokens, -1).to(o_weight.dtype), o_weight, tensors[f"{prefix}.o_proj.bias"])

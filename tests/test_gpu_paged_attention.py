@@ -8,7 +8,7 @@ import math
 import pytest
 import torch
 
-from klcquant_amd import ops
+from klcquant_amd import ops, paged_kv
 from klcquant_amd.attention import AttentionConfig
 from klcquant_amd.paged_kv import PagedAttention, PagedKVCache
 from oracle import prompt
@@ -125,6 +125,14 @@ def test_many_forks_of_a_long_prompt(gpu):
     assert batch.prefix_len == 960 and batch.tokens == 132
     for _ in range(2):
         run.extend(children, [1] * 66, checked=(0, 40))
+
+
+def test_more_rows_than_a_call_takes(gpu, monkeypatch):
+    monkeypatch.setattr(paged_kv, "_MAX_ROWS", 7)
+    run = Run(gpu, "fp16", 16, 20)
+    a, b = run.add(), run.add()
+    run.extend([a, b], [40, 3])
+    run.extend([a, b], [18, 5])
 
 
 def test_gradients_are_refused(gpu):

@@ -103,3 +103,22 @@ def test_copy_refusals(gpu):
         ops.copy_pages(pool.transpose(0, 1), [0], [1])
     with pytest.raises(ValueError, match="multiple of 16"):
         ops.copy_pages(torch.zeros((2, 6, 12), dtype=torch.int8, device=gpu), [0], [1])
+
+
+def test_grad_and_fractions_are_refused(gpu):
+    a = tensors(gpu)
+    g = {n: grad(a[n]) for n in ("cos", "sin", "k_pages", "v_pages")}
+    for name, t in g.items():
+        with pytest.raises(ValueError, match="no backward"):
+            ops.paged_append(*({**a, name: t}[n] for n in APPEND))
+    for name in ("k_pages", "v_pages"):
+        with pytest.raises(ValueError, match="no backward"):
+            ops.batch_attention(*({**a, name: g[name]}[n] for n in BATCH), prefix_len=20)
+    with pytest.raises(ValueError, match="no backward"):
+        ops.copy_pages(grad(torch.zeros((2, 6, 16, 8), dtype=torch.float16, device=gpu)), [0], [1])
+    with pytest.raises(ValueError, match="no backward"):
+        ops.prompt_attention(*(a[n] for n in PROMPT), out=grad(a["q"]))
+    with pytest.raises(TypeError):
+        ops.prompt_attention(*(a[n] for n in PROMPT), window=0.5)
+    with pytest.raises(TypeError):
+        ops.batch_attention(*(a[n] for n in BATCH), prefix_len=2.5)
