@@ -246,8 +246,10 @@ __device__ __forceinline__ bool prompt_rows(const PromptArgs& a, const PromptTil
     for (; j <= to; ++j) {
       const int here = tiles.stage(j);
       step(here, sa, here + F::kMatBytes, sb);
-      settle(2 * j + 1, sb);
+      const bool both = j < to || tiles.first + (2 * j + 1) * kKeys <= w_hi;  // else no row sees the second half
+      if (both) settle(2 * j + 1, sb);
       advance(j);
+      if (!both) continue;
       step(here + F::kMatBytes, sb, tiles.stage(j + 1), sa);  // past the last tile: scores of nothing, not used
       if (j < to) settle(2 * j + 2, sa);
     }
