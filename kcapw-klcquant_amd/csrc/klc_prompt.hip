@@ -10,12 +10,12 @@
 //
 // What bounds it: long prompts by the matrix instructions and the
 // exponentials beside them.  8,192 tokens of 64 heads over 8 of size 64 take
-// 574 to 594 us, 550 GFLOP at 0.93 to 0.96 PFLOP/s; a loop of the same
+// 577 to 592 us, 550 GFLOP at 0.93 to 0.95 PFLOP/s; a loop of the same
 // instructions on registers alone takes 466 us whatever its order and wave
-// count.  6,778 tokens of 32 heads of size 128 take 211 to 217 us (189 GFLOP,
-// 0.87 to 0.9 PFLOP/s).  Short prompts and windows by the start and end of a
-// workgroup (6,001 tokens in twelve with a window of 128: 42 to 51 us for 22 us
-// of bytes; without its compute 40 us remain, without its stores too 32).
+// count.  6,778 tokens of 32 heads of size 128 take 212 us (189 GFLOP, 0.89
+// PFLOP/s).  Short prompts and windows by the start and end of a workgroup:
+// 6,001 tokens in twelve with a window of 128 take 40 to 47 us for 22 us of
+// bytes, and two thirds of that without any compute.
 #include <math.h>
 
 #include "klc_flash.h"

@@ -132,6 +132,35 @@ def test_copy_past_32_bits(gpu):
     assert torch.equal(pool[:, 2098], pool[:, 2099]) and not pool[:, 2097].any()
 
 
+def test_append_and_copy_in_a_graph(gpu):
+    """Captured together: replays take the new queries and slots, and copy what the append just stored."""
+    q, k, v, cos, sin = rope_inputs(gpu, 20, 4, 2, 64, seed=3)
+    pool, want = (torch.zeros((2, 400, 16, 2, 64), dtype=torch.float16, device=gpu) for _ in range(2))
+    positions, slots = int32(list(range(20)), gpu), int32(list(range(20)), gpu)
+    src, dst = [i % 2 for i in range(390)], list(range(10, 400))  # more moves than a launch takes
+
+    def both(pages):
+        rotated_q, _ = ops.paged_append(q, k, v, cos, sin, positions, slots, pages[0], pages[1])
+        ops.copy_pages(pages, src, dst)
+        return rotated_q
+
+    both(pool)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both(pool)
+    for i in range(3):
+        for t in (q, k, v):
+            t.copy_(torch.randn_like(t))
+        positions.add_(7)
+        slots.copy_(torch.randperm(32, device=gpu)[:20])
+        pool.zero_()
+        want.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(both(want), out) and torch.equal(pool, want) and bool(pool[:, 399].any())
+
+
 # ---- batch attention --------------------------------------------------------------------
 
 

@@ -127,6 +127,31 @@ def test_many_forks_of_a_long_prompt(gpu):
         run.extend(children, [1] * 66, checked=(0, 40))
 
 
+def test_captured_step(gpu):
+    """A decode step captured once and replayed with the next tokens' arrays copied in, against eager steps."""
+    run = Run(gpu, "fp16", 64, 12)
+    seqs = [run.add(), run.add()]
+    run.extend(seqs, [70, 66])
+    batch = run.cache.extend(seqs)
+    hidden = torch.randn((2, run.config.hidden_size), device=gpu).bfloat16()
+    run.layer.forward(0, hidden, run.tensors, batch, run.cache)  # the tables of RoPE, before the capture
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run.layer.forward(0, hidden, run.tensors, batch, run.cache)
+    for _ in range(4):
+        new = run.cache.extend(seqs)
+        assert new.tables.shape == batch.tables.shape and new.prefix_len == batch.prefix_len == 0
+        for name in ("positions", "slots", "lengths", "tables"):
+            getattr(batch, name).copy_(getattr(new, name))
+        hidden.copy_(torch.randn_like(hidden))
+        out.fill_(math.nan)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.isfinite(out).all()
+        assert torch.equal(out, run.layer.forward(0, hidden, run.tensors, new, run.cache))
+
+
 def test_more_rows_than_a_call_takes(gpu, monkeypatch):
     monkeypatch.setattr(paged_kv, "_MAX_ROWS", 7)
     run = Run(gpu, "fp16", 16, 20)
