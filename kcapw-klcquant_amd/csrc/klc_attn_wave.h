@@ -104,7 +104,7 @@ __device__ __forceinline__ float sink_log2(uint16_t bits) {
 //   RB     blocks of 32 query rows
 //   KT     keys of a tile (32 or 64)
 template <int DP, bool kF16, bool kFull, int RB, int KT>
-struct Flash {
+struct AttnWave {
   static constexpr bool kWhole = kFull;
   static constexpr int kRowBytes = 2 * DP;
   static constexpr int kChunks = DP / 8;                // 16-byte chunks of a row

@@ -27,7 +27,7 @@
 
 #include <algorithm>
 
-#include "klc_flash.h"
+#include "klc_attn_wave.h"
 
 namespace klc {
 namespace {
@@ -189,7 +189,7 @@ __device__ __forceinline__ int quad_dim(int i) { return 8 * i + 4 * ((int)(threa
 template <int DP, bool kF16, bool kFull>
 __device__ __forceinline__ void shared_part(const BatchArgs& a, int wg, lds_u8 ring) {
   constexpr int KT = kSharedTile<DP>, kSub = KT / kKeys;
-  using F = Flash<DP, kF16, kFull, 1, kKeys>;
+  using F = AttnWave<DP, kF16, kFull, 1, kKeys>;
   constexpr int kMat = kSub * F::kMatBytes, kStage = 2 * kMat, kRing = kBatchLds / kStage;
   constexpr int kDmas = kSub * F::kDmas / kWaves;  // of K, and of V, a wave and tile
   constexpr int kQuads = 4 * F::kDimBlocks;
@@ -284,7 +284,7 @@ __device__ __forceinline__ void shared_part(const BatchArgs& a, int wg, lds_u8 r
 // as [prefix, padded to kPrefixAlign][own].
 template <int DP, bool kF16, bool kFull>
 __device__ __forceinline__ void own_part(const BatchArgs& a, int wg, lds_u8 lds, float2 (&wave_ml)[kWaves][kBatchGroup]) {
-  using F = Flash<DP, kF16, kFull, 1, kKeys>;
+  using F = AttnWave<DP, kF16, kFull, 1, kKeys>;
   constexpr int KT = kKeys, kRing = kBatchLds / kWaves / F::kStage, kQuads = 4 * F::kDimBlocks;
   static_assert(kRing == 1 || kRing == 2, "");
   // With one tile a wave, K and V take turns: the next K comes while this V is multiplied, and the other way round

@@ -4,7 +4,7 @@
 //   out_i = sum_j p_j v_j / (sum_j p_j + 2^(s - m)),  p_j = 2^(c2 q_i . k_j - m)
 //
 // over the visible j <= i in one pass over the keys, with the running maximum
-// m and sum of klc_flash.h.  A row is (token, head of the group), so that the
+// m and sum of klc_attn_wave.h.  A row is (token, head of the group), so that the
 // heads of a group share every K and V tile and 128 or 256 rows span few
 // tokens: little of the diagonal is multiplied in vain.
 //
@@ -18,7 +18,7 @@
 // bytes, and two thirds of that without any compute.
 #include <math.h>
 
-#include "klc_flash.h"
+#include "klc_attn_wave.h"
 
 namespace klc {
 namespace {
@@ -46,7 +46,7 @@ constexpr int kTileKeys = 64;
 
 template <int DP, bool kF16, bool kFull, int RB>
 struct Rows {
-  using F = Flash<DP, kF16, kFull, RB, kKeys>;
+  using F = AttnWave<DP, kF16, kFull, RB, kKeys>;
   static constexpr int kStage = 2 * F::kStage;  // K of the tile, then V
   static constexpr int kV = 2 * F::kMatBytes;
 

@@ -1,14 +1,15 @@
 """A KV cache of many sequences in pages, and the attention layer over it.
 
-``PageTable``       which sequence holds which pages: host bookkeeping alone.
-``PagedKVCache``    a PageTable with its pages in HBM, one slab for all layers'
-                    keys and values, so that a fork or a compaction is one
-                    launch (ops.copy_pages) whatever the number of layers.
-``PagedAttention``  StreamedAttention's layer (projections, RoPE, sinks,
-                    window) for a batch of tokens of several sequences:
-                    whole prompts by ops.prompt_attention, tokens behind
-                    cached ones by ops.batch_attention, which reads the pages
-                    that all of the batch's sequences share once.
+``PageTable``         which sequence holds which pages: host bookkeeping alone.
+``PagedKVCache``      a PageTable with its pages in HBM, one slab for all
+                      layers' keys and values, so that a fork or a compaction
+                      is one launch (ops.copy_pages) whatever the number of
+                      layers.
+``BatchedAttention``  StreamedAttention's layer (projections, RoPE, sinks,
+                      window) for a batch of tokens of several sequences:
+                      whole prompts by ops.prompt_attention, tokens behind
+                      cached ones by ops.batch_attention, which reads the pages
+                      that all of the batch's sequences share once.
 
 Pages are shared while they are full and never written then: a fork takes its
 parent's full pages as they are and a copy of the last one.  Work on the cache
@@ -261,7 +262,7 @@ class PagedKVCache:
                 "device": str(self.device), "precision": self.precision}
 
 
-class PagedAttention:
+class BatchedAttention:
     """StreamedAttention's layer for a PagedBatch (inference: no gradients)."""
 
     def __init__(self, config: AttentionConfig) -> None:

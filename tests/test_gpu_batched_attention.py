@@ -1,4 +1,4 @@
-"""The operators of many sequences as they are used together: PagedAttention over a PagedKVCache, from prompts through
+"""The operators of many sequences as they are used together: BatchedAttention over a PagedKVCache, from prompts through
 forks, suffixes, steps and a compaction, every row against attention's definition over its whole sequence."""
 
 from __future__ import annotations
@@ -10,7 +10,7 @@ import torch
 
 from klcquant_amd import ops, paged_kv
 from klcquant_amd.attention import AttentionConfig
-from klcquant_amd.paged_kv import PagedAttention, PagedKVCache
+from klcquant_amd.paged_kv import BatchedAttention, PagedKVCache
 from oracle import prompt
 
 pytestmark = pytest.mark.gpu
@@ -26,7 +26,7 @@ class Run:
         self.gpu = gpu
         width = (HEADS + 2 * KV) * DIM
         self.config = AttentionConfig(width, HEADS, KV, DIM, rope_factor=8.0)
-        self.layer = PagedAttention(self.config)
+        self.layer = BatchedAttention(self.config)
         self.cache = PagedKVCache(gpu, LAYERS, KV, DIM, n_pages, page, precision)
         self.cache.pool.fill_(math.nan)  # what is read before it is written shows
         pick = torch.eye(width, device=gpu).bfloat16()

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from klcquant_amd.paged_kv import PagedAttention, PagedKVCache, PageTable
+from klcquant_amd.paged_kv import BatchedAttention, PagedKVCache, PageTable
 from klcquant_amd.attention import AttentionConfig, rope_cos_sin
 
 
@@ -164,7 +164,7 @@ def test_cache_on_the_host():
     with pytest.raises(IndexError):
         cache.layer(2)
     with pytest.raises(ValueError, match="batch of 1 tokens"):
-        PagedAttention(AttentionConfig(128, 4, 2, 64)).forward(0, torch.zeros((3, 128)), {}, batch, cache)
+        BatchedAttention(AttentionConfig(128, 4, 2, 64)).forward(0, torch.zeros((3, 128)), {}, batch, cache)
 
 
 def test_rope_tables_are_rope_cos_sin(monkeypatch):
@@ -174,7 +174,7 @@ def test_rope_tables_are_rope_cos_sin(monkeypatch):
 
     monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream())
     cfg = AttentionConfig(128, 4, 2, 64, rope_factor=32.0)
-    att = PagedAttention(cfg)
+    att = BatchedAttention(cfg)
     cpu = torch.device("cpu")
     cos, sin = att.rope_tables(10, cpu)
     assert cos.shape == (1024, 32) and att.rope_tables(1024, cpu)[0] is cos
