@@ -10,9 +10,9 @@
 //
 // What bounds it: long prompts by the matrix instructions and the
 // exponentials beside them.  8,192 tokens of 64 heads over 8 of size 64 take
-// 577 to 592 us, 550 GFLOP at 0.93 to 0.95 PFLOP/s; a loop of the same
+// 577 to 598 us, 550 GFLOP at 0.92 to 0.95 PFLOP/s; a loop of the same
 // instructions on registers alone takes 466 us whatever its order and wave
-// count.  6,778 tokens of 32 heads of size 128 take 212 us (189 GFLOP, 0.89
+// count.  6,778 tokens of 32 heads of size 128 take 212 to 218 us (0.89
 // PFLOP/s).  Short prompts and windows by the start and end of a workgroup:
 // 6,001 tokens in twelve with a window of 128 take 40 to 47 us for 22 us of
 // bytes, and two thirds of that without any compute.
@@ -201,7 +201,10 @@ struct Tiles {
 // The scores of the next 32 keys are multiplied while the exponentials of
 // these are taken: the matrix instructions of a wave run beside its own
 // vector instructions, and not only beside another wave's.
-template <int DP, bool kF16, bool kFull, int RB, int W, int kRing>
+//
+// With kSplit 2 two waves take the same rows, each every other 32 keys, and
+// join at the end; the first of them stores.
+template <int DP, bool kF16, bool kFull, int RB, int W, int kSplit, int kRing>
 __device__ __forceinline__ bool prompt_rows(const PromptArgs& a, const PromptTile& t, int w_row, lds_u8 ring) {
   using R = Rows<DP, kF16, kFull, RB>;
   using F = typename R::F;
@@ -214,7 +217,8 @@ __device__ __forceinline__ bool prompt_rows(const PromptArgs& a, const PromptTil
   const int to = w_row <= t.last ? (w_hi - tiles.first) / kTileKeys : from - 1;
 #pragma unroll
   for (int j = 0; j < kRing - 1; ++j) tiles.load(j);
-  r.begin_sinks(a, t, w_row);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), part = wave % kSplit;
+  if (part == 0) r.begin_sinks(a, t, w_row);
 
   // what follows the scores of keys i: the mask and the maximum
   auto settle = [&](int i, f32x16_t (&s)[RB][1]) {
@@ -240,7 +244,22 @@ __device__ __forceinline__ bool prompt_rows(const PromptArgs& a, const PromptTil
   tiles.template arrive<kRing - 2>(0);
   int j = 0;
   for (; j < min(from, tiles.count); ++j) advance(j);
-  if (from <= to) {
+  if constexpr (kSplit == 2) {
+    if (from <= to) {
+      const int mine = part * F::kMatBytes;
+      r.f.scores(tiles.stage(j) + mine, sa);
+      settle(2 * j + part, sa);
+      for (; j <= to; ++j) {
+        advance(j);
+        step(tiles.stage(j) + mine, sa, tiles.stage(j + 1) + mine, sb);  // past the last tile: scores of nothing, not used
+        if (++j > to) break;
+        settle(2 * j + part, sb);
+        advance(j);
+        step(tiles.stage(j) + mine, sb, tiles.stage(j + 1) + mine, sa);
+        if (j < to) settle(2 * j + 2 + part, sa);
+      }
+    }
+  } else if (from <= to) {
     r.f.scores(tiles.stage(j), sa);
     settle(2 * j, sa);
     for (; j <= to; ++j) {
@@ -264,6 +283,33 @@ __device__ __forceinline__ bool prompt_rows(const PromptArgs& a, const PromptTil
 #pragma unroll
       for (int e = 0; e < 16; ++e) odd |= !(fabsf(r.f.o[rb][db][e]) < INFINITY);
   if (__syncthreads_or(odd)) return true;
+  if constexpr (kSplit == 2) {
+    // the second wave's sums to the first, lane by lane: [pair][4 dims or (maximum, sum)][lane]
+    constexpr int kQuads = 4 * F::kDimBlocks;
+    static_assert(RB == 1 && W / 2 * (kQuads + 1) * kWave * 16 <= kRing * R::kStage, "");
+    typedef __attribute__((address_space(3))) f32x4_t* lds_f32x4;
+    const lds_f32x4 sums = (lds_f32x4)ring + wave / 2 * (kQuads + 1) * kWave + threadIdx.x % kWave;
+    if (part == 1) {
+#pragma unroll
+      for (int i = 0; i < kQuads; ++i) {
+        const f32x16_t& o = r.f.o[0][i / 4];
+        sums[i * kWave] = f32x4_t{o[i % 4 * 4], o[i % 4 * 4 + 1], o[i % 4 * 4 + 2], o[i % 4 * 4 + 3]};
+      }
+      sums[kQuads * kWave] = f32x4_t{r.f.m[0], r.f.l[0], 0.f, 0.f};
+    }
+    __syncthreads();
+    if (part == 1) return false;
+    const f32x4_t other = sums[kQuads * kWave];
+    const float top = fmaxf(r.f.m[0], other.x), base = top == -INFINITY ? 0.f : top;
+    const float x = __builtin_amdgcn_exp2f(r.f.m[0] - base), y = __builtin_amdgcn_exp2f(other.x - base);
+    r.f.l[0] = fmaf(r.f.l[0], x, other.y * y);
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) {
+      const f32x4_t o = sums[i * kWave];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r.f.o[0][i / 4][i % 4 * 4 + e] = fmaf(r.f.o[0][i / 4][i % 4 * 4 + e], x, o[e] * y);
+    }
+  }
   r.store(a, t, w_row);
   return false;
 }
@@ -307,12 +353,12 @@ __device__ __forceinline__ void prompt_rows_careful(const PromptArgs& a, const P
   }
 }
 
-// Workgroup: W waves x 32 RB rows of one KV head, a row being (token, query
+// Workgroup: W / kSplit times 32 RB rows of one KV head, a row being (token, query
 // head of the group), so that a group's heads share every K and V tile and a
 // tile of rows covers few tokens (little of the diagonal is wasted).
-template <int DP, bool kF16, bool kFull, int RB, int W, int kRing, int kPerSimd>
+template <int DP, bool kF16, bool kFull, int RB, int W, int kSplit, int kRing, int kPerSimd>
 __global__ __launch_bounds__(64 * W, kPerSimd) void prompt_attention_kernel(PromptArgs a) {
-  constexpr int kRows = 32 * RB * W;
+  constexpr int kRows = 32 * RB * W / kSplit;
   __shared__ __align__(1024) uint8_t ring[kRing * Rows<DP, kF16, kFull, RB>::kStage];
   PromptTile t;
   t.g = a.n_heads / a.n_kv;
@@ -341,8 +387,8 @@ __global__ __launch_bounds__(64 * W, kPerSimd) void prompt_attention_kernel(Prom
   if (row0 < 0 || row0 >= seq_rows) return;  // no tile of an (empty) sequence
   t.row0 = (int)row0;
   t.last = (int)(min(row0 + kRows, seq_rows) - 1);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), w_row = t.row0 + wave * 32 * RB;
-  if (prompt_rows<DP, kF16, kFull, RB, W, kRing>(a, t, w_row, (lds_u8)ring))
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), w_row = t.row0 + wave / kSplit * 32 * RB;
+  if (prompt_rows<DP, kF16, kFull, RB, W, kSplit, kRing>(a, t, w_row, (lds_u8)ring) && wave % kSplit == 0)
 #pragma unroll 1
     for (int rb = 0; rb < RB; ++rb)
       prompt_rows_careful<DP, kF16, kFull>(a, t, w_row + 32 * rb, (lds_u8)ring + wave * 2 * 2 * kKeys * DP);
@@ -361,18 +407,33 @@ int launch_prompt(const PromptArgs& a, hipStream_t st) {
   // takes 13.4 us with 32 rows and 19.8 with 64, of 1,000 22 and 31, of 3,000 95 and 99, of 8,192 615 and 587; 400 of
   // 125 tokens 299 and 320, 7 of 2,857 762 and 748.  Past 64 a wave's registers take 32 rows, and eight waves share them.
   const bool short_rows = a.tokens * g * a.n_kv < 1024 * 256 || a.tokens / a.n_seq < 2048;
-  auto run = [&](auto rb, auto w, auto ring, auto per_simd) {
-    constexpr int RB = decltype(rb)::value, W = decltype(w)::value;
-    const int64_t tiles = a.tokens * g / (32 * RB * W) + a.n_seq;
-    prompt_attention_kernel<DP, kF16, kFull, RB, W, decltype(ring)::value, decltype(per_simd)::value>
+  // Where all rows are there at once, the longest set the time: a pair of waves a row, of half the keys each.  Size 64
+  // (three workgroups of 64 rows a CU): 513 tokens 13.9 -> 12.2 us, 750 18.7 -> 15.6, but 1,000 23.4 -> 24.2, 20 of 22
+  // tokens 7.2 -> 8.6, a window of 128 over 500 9.2 -> 10.1; other sizes below it would spill.  Size 128, 32 heads (one
+  // of 128 rows): 600 tokens 22.6 -> 17.8, 1,500 in two rounds 46.8 -> 36.2, but five of 360 21.5 -> 27.8, a window of
+  // 256 over 1,200 18.0 -> 25.4.
+  const int64_t mean = a.tokens / a.n_seq, seen = a.window > 0 && a.window < mean ? a.window : mean;
+  const int64_t split_wgs = (a.tokens * g / (DP == 64 ? 64 : 128) + a.n_seq) * a.n_kv;
+  const bool few_rows = DP == 64 ? kFull && split_wgs <= 768 && seen >= 256
+                                 : seen >= 256 && split_wgs <= (seen >= 768 ? 512 : 256);
+  auto run = [&](auto rb, auto w, auto split, auto ring, auto per_simd) {
+    constexpr int RB = decltype(rb)::value, W = decltype(w)::value, kSplit = decltype(split)::value;
+    const int64_t tiles = a.tokens * g / (32 * RB * W / kSplit) + a.n_seq;
+    prompt_attention_kernel<DP, kF16, kFull, RB, W, kSplit, decltype(ring)::value, decltype(per_simd)::value>
         <<<(unsigned)(tiles * a.n_kv), 64 * W, 0, st>>>(a);
   };
-  if constexpr (DP == 128)
-    run(Count<1>{}, Count<8>{}, Count<4>{}, Count<2>{});
-  else if (short_rows)
-    run(Count<1>{}, Count<4>{}, Count<3>{}, Count<3>{});
-  else
-    run(Count<2>{}, Count<4>{}, Count<4>{}, Count<2>{});
+  if constexpr (DP == 128) {
+    if (few_rows)
+      run(Count<1>{}, Count<8>{}, Count<2>{}, Count<4>{}, Count<2>{});
+    else
+      run(Count<1>{}, Count<8>{}, Count<1>{}, Count<4>{}, Count<2>{});
+  } else if (few_rows) {
+    if constexpr (kFull) run(Count<1>{}, Count<4>{}, Count<2>{}, Count<3>{}, Count<3>{});
+  } else if (short_rows) {
+    run(Count<1>{}, Count<4>{}, Count<1>{}, Count<3>{}, Count<3>{});
+  } else {
+    run(Count<2>{}, Count<4>{}, Count<1>{}, Count<4>{}, Count<2>{});
+  }
   return check_launch("prompt_attention_kernel");
 }
 

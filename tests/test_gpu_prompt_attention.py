@@ -182,8 +182,29 @@ def test_long_prompt_rows(gpu):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("lengths,heads,kv,dim,window,sinks", [((257,), 8, 2, 64, None, True), ((700,), 8, 1, 64, 256, False),
+                                                               ((300, 290, 0, 530), 6, 3, 64, 270, True),
+                                                               ((512,), 16, 2, 24, None, True), ((333,), 3, 1, 48, 300, False),
+                                                               ((601,), 8, 2, 128, None, True), ((400, 0, 333), 3, 3, 128, 300, False),
+                                                               ((450,), 6, 1, 80, None, True), ((777,), 2, 2, 104, 270, False)])
+def test_few_rows_of_long_prompts(gpu, dtype, lengths, heads, kv, dim, window, sinks):
+    """Few enough rows that two waves share them, and keys enough to share."""
+    q, k, v, starts = make(gpu, lengths, heads, kv, dim, DTYPES[dtype], seed=dim + heads, q_std=2.0, lead=3, tail=2)
+    sk = torch.randn(heads, device=gpu).bfloat16() if sinks else None
+    at, out = device_starts(starts, gpu), torch.full_like(q, 7.0)
+    ops.prompt_attention(q, k, v, at, sk, window, out=out)
+    assert (out[:3] == 7).all() and (out[-2:] == 7).all()
+    check(out, q, k, v, starts, sk, window)
+    assert torch.equal(out, ops.prompt_attention(q, k, v, at, sk, window, out=torch.full_like(q, 7.0)))
+    k[150], v[200, 0, 3], v[90, 0, 0] = math.nan, math.inf, -math.inf
+    ops.prompt_attention(q, k, v, at, sk, window, out=out)
+    check(out, q, k, v, starts, sk, window)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("lengths,dim,window,sinks", [((2101,), 64, None, True), ((2500, 0, 1900, 2200), 64, 100, False),
-                                                      ((2201,), 24, None, True), ((2048,), 48, 700, False)])
+                                                      ((2201,), 24, None, True), ((2048,), 48, 700, False),
+                                                      ((2101,), 128, None, True), ((1500, 700), 72, 500, False)])
 def test_many_rows_of_long_prompts(gpu, dtype, lengths, dim, window, sinks):
     """Enough long rows that a wave takes 64 of them."""
     heads = 128
