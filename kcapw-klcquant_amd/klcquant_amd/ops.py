@@ -331,16 +331,21 @@ def _row_strides(rows: tuple, dtype: torch.dtype, dev: torch.device) -> list[int
     index, grad = dev.index, torch.is_grad_enabled()
     strides = []
     for name, t in rows:
-        if (type(t) in _TENSORS and t.dtype is dtype and t.get_device() == index and t.dim() == 3 and t.numel()
-                and t.is_contiguous() and not (grad and t.requires_grad)):
-            strides.append(t.shape[1] * t.shape[2])
-        else:
-            strides.append(_row_stride(name, t, dtype, dev))
+        if (type(t) in _TENSORS and t.dtype is dtype and t.get_device() == index and t.is_contiguous()
+                and not (grad and t.requires_grad)):
+            shape = t.shape
+            if len(shape) == 3:
+                _, heads, dim = shape
+                if heads and dim:
+                    strides.append(heads * dim)
+                    continue
+        strides.append(_row_stride(name, t, dtype, dev))
     return strides
 
 
 def _check_index(name: str, t: torch.Tensor, shape: tuple, dev: torch.device) -> None:
-    if _plain(t, torch.int32, shape, dev.index):
+    if (type(t) in _TENSORS and t.dtype is torch.int32 and t.shape == shape and t.get_device() == dev.index
+            and t.is_contiguous()):
         return
     _check_gpu(name, t, torch.int32, len(shape))
     if t.device != dev:
