@@ -4,7 +4,10 @@
 //   out_i = sum_j p_j v_j / (sum_j p_j + 2^(s - m)),  p_j = 2^(c2 q_i . k_j - m)
 //
 // over the visible j <= i in one pass over the keys, with the running maximum
-// m and sum of klc_attn_wave.h.  A row is (token, head of the group), so that the
+// m and sum of klc_attn_wave.h.  The sink s joins at the end: m is the keys'
+// own, as p_j is rounded to 16 bits and float16 holds nothing 2^-24 below 1
+// (a sink 18 above 2,000 ordinary scores, taken into m, cost a quarter of the
+// result).  A row is (token, head of the group), so that the
 // heads of a group share every K and V tile and 128 or 256 rows span few
 // tokens: little of the diagonal is multiplied in vain.
 //
@@ -52,6 +55,7 @@ struct Rows {
 
   F f;
   int tok[RB];
+  uint32_t sink[RB];  // bfloat16, of the row's head
 
   // the wave's rows from w_row on
   __device__ __forceinline__ void begin(const PromptArgs& a, const PromptTile& t, int w_row, lds_u8 ring) {
@@ -69,18 +73,19 @@ struct Rows {
         f.q[rb][st] = u32x4_t{0, 0, 0, 0};
         if (kFull || 8 * c < a.d) f.q[rb][st] = *reinterpret_cast<const u32x4_t*>(src + 8 * c);
       }
+      asm volatile("" : "+v"(f.m[rb]), "+v"(f.l[rb]));  // not the constants they are: what follows from them spills
     }
   }
-  // their sinks; loaded behind the first tiles, so that the wait for them is one for everything in flight
-  __device__ __forceinline__ void begin_sinks(const PromptArgs& a, const PromptTile& t, int w_row) {
-    if (a.sinks == nullptr) return;
-    const int lane = threadIdx.x % kWave;
+  // their sinks (-inf: none), asked for behind the keys: held from the start they would spill, and so would the
+  // lane's rows and heads, which are worked out again from here on
+  __device__ __forceinline__ void load_sinks(const PromptArgs& a, const PromptTile& t, int w_row) {
+    int lane = threadIdx.x % kWave;
+    asm volatile("" : "+v"(lane));
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       const int head = t.kvh * t.g + min(w_row + 32 * rb + lane % 32, t.last) - tok[rb] * t.g;
-      const float sink = sink_log2(a.sinks[head]);
-      f.m[rb] = sink;
-      f.l[rb] = sink == -INFINITY || lane >= 32 ? 0.f : 1.f + (sink - sink);
+      sink[rb] = 0xff80u;
+      if (a.sinks != nullptr) sink[rb] = a.sinks[head];
     }
   }
 
@@ -101,11 +106,13 @@ struct Rows {
 
   // all rows, or those of token `only`
   __device__ __forceinline__ void store(const PromptArgs& a, const PromptTile& t, int w_row, int only = -1) const {
-    const int lane = threadIdx.x % kWave;
+    int lane = threadIdx.x % kWave;
+    asm volatile("" : "+v"(lane));
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      const float sum = add_halves(f.l[rb]);
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key and no sink: zeros
+      const float s = sink_log2((uint16_t)sink[rb]), top = fmaxf(f.m[rb], s), base = top == -INFINITY ? 0.f : top;
+      const float x = __builtin_amdgcn_exp2f(f.m[rb] - base), sum = fmaf(add_halves(f.l[rb]), x, __builtin_amdgcn_exp2f(s - base));
+      const float inv = sum == 0.f ? 0.f : x / sum;  // no key and no sink: zeros
       const int row = w_row + 32 * rb + lane % 32, head = t.kvh * t.g + row - tok[rb] * t.g;
       const bool live = row <= t.last && (only < 0 || tok[rb] == only);
       uint16_t* dst = a.out + ((int64_t)(t.begin + tok[rb]) * a.n_heads + head) * a.d + 8 * (lane / 32);
@@ -218,7 +225,6 @@ __device__ __forceinline__ bool prompt_rows(const PromptArgs& a, const PromptTil
 #pragma unroll
   for (int j = 0; j < kRing - 1; ++j) tiles.load(j);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), part = wave % kSplit;
-  if (part == 0) r.begin_sinks(a, t, w_row);
 
   // what follows the scores of keys i: the mask and the maximum
   auto settle = [&](int i, f32x16_t (&s)[RB][1]) {
@@ -275,6 +281,7 @@ __device__ __forceinline__ bool prompt_rows(const PromptArgs& a, const PromptTil
   }
   for (; j < tiles.count; ++j) advance(j);
 
+  r.load_sinks(a, t, w_row);
   bool odd = false;
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb)
@@ -302,6 +309,7 @@ __device__ __forceinline__ bool prompt_rows(const PromptArgs& a, const PromptTil
     const f32x4_t other = sums[kQuads * kWave];
     const float top = fmaxf(r.f.m[0], other.x), base = top == -INFINITY ? 0.f : top;
     const float x = __builtin_amdgcn_exp2f(r.f.m[0] - base), y = __builtin_amdgcn_exp2f(other.x - base);
+    r.f.m[0] = top;
     r.f.l[0] = fmaf(r.f.l[0], x, other.y * y);
 #pragma unroll
     for (int i = 0; i < kQuads; ++i) {
@@ -327,7 +335,6 @@ __device__ __forceinline__ void prompt_rows_careful(const PromptArgs& a, const P
   for (int tok = w_row / t.g; tok <= last_tok && w_row <= t.last; ++tok) {
     R r;
     r.begin(a, t, w_row, tile);
-    r.begin_sinks(a, t, w_row);
     for (int k0 = a.window > 0 ? max(0, tok - a.window + 1) : 0; k0 <= tok; k0 += kKeys) {
 #pragma unroll
       for (int n = 0; n < F::kDmas; ++n) {
@@ -349,6 +356,7 @@ __device__ __forceinline__ void prompt_rows_careful(const PromptArgs& a, const P
       __builtin_amdgcn_s_waitcnt(vmcnt_imm(63));  // the tile's reads are done
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
     }
+    r.load_sinks(a, t, w_row);
     r.store(a, t, w_row, tok);
   }
 }
