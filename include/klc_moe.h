@@ -501,8 +501,9 @@ int klc_attn_step_wait(const void* host_record, int64_t tag, int64_t limit_us);
  * are rounded to `dtype` before the value product, which the sum of the
  * rounded ones normalises.  Rows of out [tokens][n_heads][head_dim] outside
  * every sequence are not written.  What a row must not see does not reach it,
- * NaN and infinities included.  q, k, v and out 16-byte aligned, out apart
- * from the others; tokens * n_heads / n_kv < 2^30. */
+ * NaN and infinities included; scores that are all -inf without a sink give
+ * NaN, as their softmax.  q, k, v and out 16-byte aligned, out apart from the
+ * others; tokens * n_heads / n_kv < 2^30. */
 typedef struct klc_attn_prompt_args {
   const void *q, *k, *v;  /* [tokens][heads][head_dim] of dtype */
   const void* starts;     /* int32 [n_seq + 1] */
@@ -546,10 +547,11 @@ int klc_kv_copy_pages(void* pools, int64_t n_pools, int64_t n_pages, int64_t pag
  * It sees the last `window` of them (0: all).  q rows are bfloat16
  * [n_heads][head_dim], q_stride elements apart; softmax as klc_attn_prompt,
  * probabilities rounded to kv_dtype; out [n_seq][n_heads][head_dim] bfloat16.
- * lengths[b] < 0: no sequence, zeros.  A page number outside [0, n_pages) or a
- * length past table_width * page_size makes the sequence's output NaN (of the
- * prefix: every sequence's); nothing outside the pools is read.  n_heads /
- * n_kv <= 32, n_seq <= 65535.
+ * lengths[b] < 0: no sequence, zeros; a row without a key and a sink is zero
+ * too.  A page number outside [0, n_pages) or a length past table_width *
+ * page_size makes the sequence's output NaN (of the prefix: every
+ * sequence's); nothing outside the pools is read.  n_heads / n_kv <= 32,
+ * n_seq <= 65535.
  * workspace: klc_attn_batch_workspace_bytes with max_own = table_width *
  * page_size (0: none needed), 16-byte aligned, no initialisation; calls that
  * may overlap need one each. */

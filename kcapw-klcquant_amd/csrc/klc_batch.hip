@@ -419,7 +419,8 @@ __device__ __forceinline__ void own_part(const BatchArgs& a, int wg, lds_u8 lds,
     x[w] = __builtin_amdgcn_exp2f(ml[w].x - base);
     l = fmaf(x[w], ml[w].y, l);
   }
-  const float inv = l == 0.f || absent ? 0.f : 1.f / l;
+  // without a key zeros, else 1 / 0 and 0 times it for scores that are all -inf: NaN, as their softmax
+  const float inv = absent || (l == 0.f && a.prefix + n == 0) ? 0.f : 1.f / l;
   auto put = [&](int i, f32x4_t o) {
     if (!kFull && quad_dim(i) >= a.d) return;
     if (splits == 1)
@@ -466,7 +467,8 @@ __global__ __launch_bounds__(256) void batch_join_kernel(BatchArgs a) {
   const int splits = a.shared_splits + a.own_splits;
   const int lanes = a.d <= 32 ? 8 : a.d <= 64 ? 16 : 32, groups = kWave / lanes, grp = lane / lanes;
   const int dim = min(4 * (lane % lanes), a.d - 4);
-  const bool absent = a.lengths[r / a.n_heads] < 0;
+  const int n = a.lengths[r / a.n_heads];
+  const bool absent = n < 0;
   const float2* ml = a.part_ml + r * splits;
   const float sink = a.sinks != nullptr ? sink_log2(a.sinks[r % a.n_heads]) : -INFINITY;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -514,7 +516,7 @@ __global__ __launch_bounds__(256) void batch_join_kernel(BatchArgs a) {
       o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = absent || (l == 0.f && a.prefix + n == 0) ? 0.f : 1.f / l;
   if (live && lane < a.d / 4)
     *reinterpret_cast<u32x2_t*>(a.out + row * a.d + dim) = u32x2_t{pack2<false>(o.x * inv, o.y * inv), pack2<false>(o.z * inv, o.w * inv)};
 }

@@ -112,7 +112,7 @@ struct Rows {
     for (int rb = 0; rb < RB; ++rb) {
       const float s = sink_log2((uint16_t)sink[rb]), top = fmaxf(f.m[rb], s), base = top == -INFINITY ? 0.f : top;
       const float x = __builtin_amdgcn_exp2f(f.m[rb] - base), sum = fmaf(add_halves(f.l[rb]), x, __builtin_amdgcn_exp2f(s - base));
-      const float inv = sum == 0.f ? 0.f : x / sum;  // no key and no sink: zeros
+      const float inv = x / sum;  // 0 / 0 where a row's scores and its sink are all -inf: NaN, as their softmax
       const int row = w_row + 32 * rb + lane % 32, head = t.kvh * t.g + row - tok[rb] * t.g;
       const bool live = row <= t.last && (only < 0 || tok[rb] == only);
       uint16_t* dst = a.out + ((int64_t)(t.begin + tok[rb]) * a.n_heads + head) * a.d + 8 * (lane / 32);

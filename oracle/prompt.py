@@ -2,7 +2,8 @@
 
 ``attend`` is the definition, one head of one sequence at a time: softmax of
 ``scale * q . k`` over the keys that a row sees, and the sink logit, which has
-no value; a row that sees nothing and has no sink is zero.  Values that a row
+no value; a row that sees no key is zero (with a sink of -inf too, which is
+none), one that sees keys whose scores are all -inf is NaN.  Values that a row
 does not see do not enter its sum, whatever they hold.
 """
 
@@ -29,7 +30,7 @@ def weights(q: torch.Tensor, k: torch.Tensor, first: torch.Tensor, last: torch.T
     total = w.sum(dim=1, keepdim=True)
     if sink is not None:
         total = total + torch.exp(sink - base)
-    return torch.where(total == 0, torch.zeros_like(w), w / total), seen
+    return torch.where((total == 0) & ~seen.any(dim=1, keepdim=True), torch.zeros_like(w), w / total), seen
 
 
 def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, first: torch.Tensor, last: torch.Tensor,
