@@ -286,7 +286,8 @@ class BatchedAttention:
     def forward(self, layer_idx: int, hidden: torch.Tensor, tensors: dict, batch: PagedBatch, kv_cache: PagedKVCache,
                 sliding_window: int | None = None) -> torch.Tensor:
         """bfloat16 ``hidden [tokens, hidden_size]`` of the batch's tokens -> the layer's output for them; their keys
-        and values are stored to the cache.  ``tensors`` and ``sliding_window`` as StreamedAttention.forward's."""
+        and values are stored to the cache.  ``tensors`` and ``sliding_window`` (0: no window) as
+        StreamedAttention.forward's."""
         cfg = self.config
         prefix = f"model.layers.{layer_idx}.self_attn"
         if hidden.dim() != 2 or hidden.shape[0] != batch.tokens:
@@ -301,7 +302,7 @@ class BatchedAttention:
         k_pages, v_pages = kv_cache.layer(layer_idx)
         cos, sin = self.rope_tables(batch.end, q.device)
         q, k = ops.paged_append(q, k, v, cos, sin, batch.positions, batch.slots, k_pages, v_pages, want_keys=batch.fresh)
-        window = sliding_window if sliding_window is not None else cfg.sliding_window
+        window = (sliding_window if sliding_window is not None else cfg.sliding_window) or None  # 0: none
         sinks = tensors.get(f"{prefix}.sinks")
         if sinks is not None:
             sinks = sinks.to(torch.bfloat16).contiguous()
