@@ -63,15 +63,16 @@ class PageTable:
         if need > len(self._free):
             raise RuntimeError(f"the cache's {self.n_pages} pages are taken: {need} needed, {len(self._free)} free")
 
-    def _take(self, seq: int, count: int) -> None:
-        """`count` more pages behind those that the sequence's length fills."""
-        if count == 0:
-            return
-        at = int(self._held(self._lengths[seq]))
-        if at + count > self._pages.shape[1]:
-            wider = np.zeros((self._pages.shape[0], max(at + count, 2 * self._pages.shape[1])), np.int32)
+    def _widen(self, width: int) -> None:
+        """Space for sequences of ``width`` pages."""
+        if width > self._pages.shape[1]:
+            wider = np.zeros((self._pages.shape[0], max(width, 2 * self._pages.shape[1])), np.int32)
             wider[:, :self._pages.shape[1]] = self._pages
             self._pages = wider
+
+    def _take(self, seq: int, count: int) -> None:
+        """`count` more pages behind those that the sequence's length fills; there is space for them."""
+        at = int(self._held(self._lengths[seq]))
         new = self._free[-count:][::-1]
         del self._free[-count:]
         self._pages[seq, at:at + count] = new
@@ -134,15 +135,33 @@ class PageTable:
         if counts.dtype.kind not in "iu" or (counts <= 0).any():
             raise ValueError(f"token counts must be positive, got {counts.tolist()}")
         counts = counts.astype(np.int64)
-        before = self._lengths[at]
+        before = self._lengths[at]  # a copy
         after = before + counts
         if after.max() >= 1 << 29:
             raise ValueError(f"sequences must stay below 2^29 tokens, got {int(after.max())}")
         need = self._held(after) - self._held(before)
         self._room(int(need.sum()))
+        self._widen(int(self._held(after.max())))
         for s in np.flatnonzero(need):
             self._take(int(at[s]), int(need[s]))
         self._lengths[at] = after
+        try:
+            return self._batch(at, before, after, counts)
+        except BaseException:  # no memory for the arrays
+            self.undo_extend(at, counts)
+            raise
+
+    def undo_extend(self, seqs, counts) -> None:
+        """Takes back the extension of ``seqs`` by ``counts`` that was made last."""
+        for s, n in zip(np.asarray(seqs)[::-1], np.asarray(counts)[::-1]):
+            before, after = int(self._lengths[s]) - int(n), int(self._lengths[s])
+            pages = self._pages[s, self._held(before):self._held(after)]
+            self._holders[pages] = 0
+            self._free.extend(pages[::-1].tolist())
+            self._lengths[s] = before
+
+    def _batch(self, at, before, after, counts) -> dict:
+        """extend's arrays, of the tokens from ``before`` up to ``after`` of the sequences."""
         starts = np.concatenate(([0], np.cumsum(counts)))
         row = np.repeat(np.arange(at.size), counts)
         positions = np.arange(starts[-1]) - starts[row] + before[row]
@@ -161,19 +180,23 @@ class PageTable:
                    lengths=positions + 1 - shared * self.page_size)
         return {**{k: v.astype(np.int32) for k, v in out.items()}, "fresh": False}
 
-    def compact(self) -> tuple[list[int], list[int]]:
-        """Moves pages to the front, so that those held are the first: the moves (sources, destinations)."""
+    def moves(self) -> tuple[list[int], list[int]]:
+        """The page moves (sources, destinations) of a compaction: pages that are held go to the front."""
         held = np.flatnonzero(self._holders)
         dst = np.flatnonzero(self._holders[:held.size] == 0)
-        src = held[held >= held.size]
-        if src.size:
+        return held[held >= held.size].tolist(), dst.tolist()
+
+    def compact(self) -> tuple[list[int], list[int]]:
+        """Moves pages to the front, so that those held are the first: the moves (sources, destinations)."""
+        src, dst = self.moves()
+        if src:
             to = np.arange(self.n_pages, dtype=np.int32)
             to[src] = dst
             self._pages = to[self._pages]
             self._holders[dst] = self._holders[src]
             self._holders[src] = 0
-        self._free = list(range(self.n_pages - 1, held.size - 1, -1))
-        return src.tolist(), dst.tolist()
+        self._free = list(range(self.n_pages - 1, np.count_nonzero(self._holders) - 1, -1))
+        return src, dst
 
     def stats(self) -> dict:
         live = self._lengths >= 0
@@ -230,8 +253,13 @@ class PagedKVCache:
     def fork(self, seq: int, count: int = 1) -> list[int]:
         """New sequences with ``seq``'s tokens, which share its full pages."""
         children, src, dst = self.table.fork(seq, count)
-        if src:
-            ops.copy_pages(self.pool, src, dst)
+        try:
+            if src:
+                ops.copy_pages(self.pool, src, dst)
+        except BaseException:  # sequences without their last page must not stay
+            for child in reversed(children):
+                self.table.free(child)
+            raise
         return children
 
     def free(self, seq: int) -> None:
@@ -239,15 +267,23 @@ class PagedKVCache:
 
     def compact(self) -> int:
         """Moves the held pages to the pool's front and returns how many they are.  Batches made before are void."""
-        src, dst = self.table.compact()
+        src, dst = self.table.moves()
         if src:
             ops.copy_pages(self.pool, src, dst)
+        self.table.compact()  # once the copies are under way: the pages they came from are as they were
         return self.table.n_pages - self.table.stats()["free_pages"]
 
     def extend(self, seqs, counts=1) -> PagedBatch:
         """Room for ``counts`` (a number or one a sequence) more tokens of each sequence, and their batch.  Every layer
         has to run it before the sequences are extended, forked or compacted again."""
         x = self.table.extend(seqs, counts)
+        try:
+            return self._to_device(x)
+        except BaseException:  # no memory for the arrays
+            self.table.undo_extend(seqs, np.diff(x["starts"]))
+            raise
+
+    def _to_device(self, x: dict) -> PagedBatch:
         names = ("positions", "slots", "starts", "lengths", "prefix", "tables")
         host = torch.empty(sum(x[n].size for n in names), dtype=torch.int32, pin_memory=self.device.type == "cuda")
         np.concatenate([x[n].ravel() for n in names], out=host.numpy())
