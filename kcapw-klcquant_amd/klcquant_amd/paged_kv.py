@@ -299,9 +299,15 @@ class PagedKVCache:
 
 
 class BatchedAttention:
-    """StreamedAttention's layer for a PagedBatch (inference: no gradients)."""
+    """StreamedAttention's layer for a PagedBatch (inference: no gradients).  Refuses models whose steps batch_attention
+    does not take, though it could run their prompts: groups of more than 32 query heads."""
 
     def __init__(self, config: AttentionConfig) -> None:
+        heads, kv, dim = config.num_heads, config.num_kv_heads, config.head_dim
+        if kv <= 0 or heads <= 0 or heads % kv or heads // kv > 32 or heads > 4096:
+            raise ValueError(f"{heads} query heads over {kv} KV heads (groups of 1 to 32, up to 4096 heads)")
+        if dim < 8 or dim % 8 or dim > 128:
+            raise ValueError(f"head size {dim} (8 to 128, a multiple of 8)")
         self.config = config
         self._tables: dict = {}  # device -> (cos, sin) of the positions so far
         self._kept: list = []    # smaller ones, which captured graphs may still read
