@@ -63,8 +63,10 @@ __device__ __forceinline__ float add2(uint32_t p, float acc) {
 // 16 bytes a lane from memory to dst + 16 lane of LDS (dst uniform), counted
 // by vmcnt.  In assembly because the compiler, told of the load, waits for
 // every load in flight before any LDS read that might meet it; the kernels'
-// own waits order them by tile.  It has no output register, nothing reads its
-// LDS before those waits, and nothing else in these kernels uses m0.
+// own waits order them by tile.  It has no output register, and nothing reads
+// its LDS before those waits.  m0 is reserved, so that the compiler keeps
+// nothing in it and naming it as clobbered has no defined meaning; no other
+// instruction of these kernels uses it, which a test of the compiled code checks.
 __device__ __forceinline__ void load_to_lds(const uint16_t* src, lds_u8 dst) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                :
