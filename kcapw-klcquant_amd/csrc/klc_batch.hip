@@ -616,7 +616,7 @@ extern "C" int klc_attn_batch(const klc_attn_batch_args* args, void* stream) {
               "klc_attn_batch: q stride %lld (a multiple of 8, no overlap)", (long long)x.q_stride);
   KLC_REQUIRE(((uintptr_t)x.q | (uintptr_t)x.k_pages | (uintptr_t)x.v_pages | (uintptr_t)x.workspace | (uintptr_t)x.out) % 16 == 0,
               KLC_ERR_ARGUMENT, "klc_attn_batch: q, pages, workspace and out must be 16-byte aligned");
-  KLC_REQUIRE(x.scale > 0 && (float)x.scale > 0.f && (float)x.scale < INFINITY, KLC_ERR_ARGUMENT,
+  KLC_REQUIRE(x.scale > 0 && (float)x.scale > 0.f && (float)(x.scale * kLog2e) < INFINITY, KLC_ERR_ARGUMENT,
               "klc_attn_batch: scale %g", x.scale);
   KLC_REQUIRE(x.kv_dtype == KLC_DTYPE_BF16 || x.kv_dtype == KLC_DTYPE_F16, KLC_ERR_UNSUPPORTED,
               "klc_attn_batch: kv_dtype %lld (bfloat16 or float16)", (long long)x.kv_dtype);

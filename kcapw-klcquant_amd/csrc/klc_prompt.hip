@@ -470,7 +470,7 @@ extern "C" int klc_attn_prompt(const klc_attn_prompt_args* args, void* stream) {
   KLC_REQUIRE(((uintptr_t)x.q | (uintptr_t)x.k | (uintptr_t)x.v | (uintptr_t)x.out) % 16 == 0, KLC_ERR_ARGUMENT,
               "klc_attn_prompt: q, k, v and out must be 16-byte aligned");
   KLC_REQUIRE(x.window >= 0 && x.window < ((int64_t)1 << 30) && x.scale > 0 && (float)x.scale > 0.f &&
-                  (float)x.scale < INFINITY,
+                  (float)(x.scale * kLog2e) < INFINITY,
               KLC_ERR_ARGUMENT, "klc_attn_prompt: window %lld, scale %g", (long long)x.window, x.scale);
   KLC_REQUIRE(x.dtype == KLC_DTYPE_BF16 || x.dtype == KLC_DTYPE_F16, KLC_ERR_UNSUPPORTED,
               "klc_attn_prompt: dtype %lld (bfloat16 or float16)", (long long)x.dtype);

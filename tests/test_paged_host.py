@@ -126,3 +126,12 @@ def test_cpu_tensors_are_refused():
                  lambda: ops.paged_append(np.zeros(3), kv, kv, x, x, index, index, pages, pages)):
         with pytest.raises(TypeError, match="torch.Tensor"):
             call()
+
+
+@pytest.mark.parametrize("scale,fine", [(2.3e38, True), (2.4e38, False), (3.3e38, False), (1e39, False)])
+def test_scales_are_finite_as_the_kernels_hold_them(scale, fine):
+    """In powers of two a scale is log2(e) times itself: past 2.36e38 that is infinite, and every score of 0 NaN."""
+    for name, args in (("klc_attn_prompt", prompt_args(scale=scale, dtype=nat.DTYPE_F32)),
+                       ("klc_attn_batch", batch_args(scale=scale, kv_dtype=nat.DTYPE_F32))):
+        # the type is refused behind the scale
+        refused(name, args, nat.KLC_ERR_UNSUPPORTED if fine else nat.KLC_ERR_ARGUMENT, "dtype" if fine else "scale")
