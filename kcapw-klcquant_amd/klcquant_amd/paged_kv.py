@@ -234,8 +234,8 @@ class PagedKVCache:
         self.table = PageTable(n_pages, page_size)
         self.precision = precision
         self.dtype = _KV_DTYPES[precision][0]
-        self.device = torch.device(device)
-        self.pool = torch.empty((2 * n_layers, n_pages, page_size, n_kv, head_dim), dtype=self.dtype, device=self.device)
+        self.pool = torch.empty((2 * n_layers, n_pages, page_size, n_kv, head_dim), dtype=self.dtype, device=device)
+        self.device = self.pool.device  # "cuda" is the current device now, not the one of a later call
 
     def layer(self, layer_idx: int) -> tuple[torch.Tensor, torch.Tensor]:
         """The layer's key and value pages ``[n_pages, page_size, n_kv, head_dim]``."""
