@@ -541,17 +541,19 @@ int klc_kv_copy_pages(void* pools, int64_t n_pools, int64_t n_pages, int64_t pag
 
 /* Attention of one token of each of n_seq sequences over pages.  Sequence b's
  * keys are the first prefix_len tokens of the pages in prefix_table (int32
- * [ceil(prefix_len / page_size)]; the same for every sequence, read once for
- * all of them) and then lengths[b] (int32) tokens of its own, in the pages of
- * row b of tables (int32 [n_seq][table_width]); the token itself is the last.
+ * [ceil(prefix_len / page_size)]; the same for every sequence) and then
+ * lengths[b] (int32) tokens of its own, in the pages of row b of tables (int32
+ * [n_seq][table_width]); the token itself is the last.
  * It sees the last `window` of them (0: all).  q rows are bfloat16
  * [n_heads][head_dim], q_stride elements apart; softmax as klc_attn_prompt,
  * probabilities rounded to kv_dtype; out [n_seq][n_heads][head_dim] bfloat16.
  * lengths[b] < 0: no sequence, zeros; a row without a key and a sink is zero
- * too.  A page number outside [0, n_pages) or a length past table_width *
- * page_size makes the sequence's output NaN (of the prefix: every
- * sequence's); nothing outside the pools is read.  n_heads / n_kv <= 32,
- * n_seq <= 65535.
+ * too.  A page number outside [0, n_pages) that the sequence sees, or a length
+ * past table_width * page_size, makes its output NaN; nothing outside the
+ * pools is read.  The prefix is read once for all sequences if there is no
+ * window, more than one sequence and n_seq * n_kv * prefix_len * head_dim
+ * >= 2^25 (below that a second pass costs more than the caches do), else by
+ * every sequence.  n_heads / n_kv <= 32, n_seq <= 65535.
  * workspace: klc_attn_batch_workspace_bytes with max_own = table_width *
  * page_size (0: none needed), 16-byte aligned, no initialisation; calls that
  * may overlap need one each. */

@@ -16,13 +16,16 @@
 //   out = sum_i 2^(m_i - m) o_i / (sum_i 2^(m_i - m) l_i + 2^(s - m)),  m = max(m_i, s)
 //
 // What bounds it (64 heads over 8 of size 64, float16 pages): 64 sequences
-// with up to 700 own tokens behind a prefix of 8,192, 28 to 32 us of which the
+// with up to 700 own tokens behind a prefix of 8,192, 27 to 32 us of which the
 // join is 4.5; the prefix's pass is the longer side, with one wave a SIMD 465
-// ns for 32 rows by 32 keys where two waves would take 227 each, but twice the
-// workgroups would write twice the parts.  256 sequences of 2,000 tokens, 124
-// us: HBM at 4.8 TB/s.  200 on a window of 128, 13.7 us, and 8 behind 500
-// tokens, 9 us: the chain of length, page numbers, first tile.  32 of 900
-// behind 16,000, 32 heads of size 128, 35.5 us and a join of 5.5.
+// ns for 32 rows by 32 keys where two waves would take 227 each.  More
+// workgroups would write more parts; two waves that join theirs in LDS are not
+// tried.  256 sequences of 2,000 tokens, 124 us: HBM at 4.8 TB/s.  200 on a
+// window of 128, 13.6 us, and 8 behind 500 tokens, 9 us: the chain of length,
+// page numbers, first tile.  32 of 900 behind 16,000, 32 heads of size 128,
+// 29 to 37 us and a join of 5.5.  The plan goes by counts and the tables'
+// width, not by the lengths: 127 sequences of 200 to 1,000 tokens take 44 us,
+// and with one of 32,000 beside them 765, its keys being one wave's.
 #include <math.h>
 
 #include <algorithm>
@@ -83,9 +86,10 @@ __device__ __forceinline__ void settle_query(u32x4_t (&q)[F::kSteps]) {
 }
 
 // The row in the cache's type.  A float16 cache takes it times a power of two
-// that brings its largest value to [1, 2): float16 then represents every value
-// as bfloat16 does, but for what lies 2^-24 below that one.  The returned
-// factor puts it back.
+// that brings its largest value to [1, 2): float16 then holds every value down
+// to 2^-17 as it is, and smaller ones to the nearest multiple of 2^-24, so
+// that a score is off by at most 2^-25 of the largest |q| times sum |k|.  The
+// returned factor puts the power back.
 template <class F, bool kF16>
 __device__ __forceinline__ float convert_query(u32x4_t (&q)[F::kSteps]) {
   if constexpr (!kF16) return 1.f;
@@ -532,7 +536,8 @@ BatchPlan batch_plan(int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t d, in
   // 256 own workgroups, one a CU: 64 sequences of 8 KV heads (512 items) take 31.6 us with 2 waves an item, 34.7 with
   // 1 and 33.9 with 4; 128 sequences with 1,000 own tokens 49 us with 1 wave and 57 with 2 or 4.
   p.own_waves = items >= 1024 ? 1 : items >= 512 ? 2 : 4;
-  // The prefix again for every sequence, mostly out of the caches, or one pass and a join: 64 x 500 of head_dim 64 take
+  // The prefix again for every sequence, mostly out of the caches, or one pass and a join (without a window only, also
+  // where a window hides nothing: 200 x 1,000 with 500 own tokens 60 us, and 74 with a window of 4,096): 64 x 500 of head_dim 64 take
   // 16.8 us without the pass and 19.7 with it, 200 x 300 25.6 and 28.8, 64 x 1,000 23.2 and 20.3, 200 x 1,000 48.8 and 32.7.
   const bool shared = window == 0 && n_seq > 1 && (double)items * prefix * d >= 1 << 25;
   int64_t keys = max_own + (shared ? 0 : prefix);

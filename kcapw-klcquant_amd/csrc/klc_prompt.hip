@@ -13,10 +13,11 @@
 //
 // What bounds it: long prompts by the matrix instructions and the
 // exponentials beside them.  8,192 tokens of 64 heads over 8 of size 64 take
-// 577 to 598 us, 550 GFLOP at 0.92 to 0.95 PFLOP/s; a loop of the same
-// instructions on registers alone takes 466 us whatever its order and wave
-// count.  6,778 tokens of 32 heads of size 128 take 212 to 218 us (0.89
-// PFLOP/s).  Short prompts and windows by the start and end of a workgroup:
+// 550 to 588 us, 550 GFLOP at 0.94 to 1.0 PFLOP/s; a loop of the same
+// instructions on registers alone takes 466 to 490 us whatever its order and
+// wave count.  6,778 tokens of 32 heads of size 128 take 205 to 218 us (0.89
+// PFLOP/s), of which that size's loop on registers is 138 (388 ns for 32 rows
+// by 32 keys).  Short prompts and windows by the start and end of a workgroup:
 // 6,001 tokens in twelve with a window of 128 take 40 to 47 us for 22 us of
 // bytes, and two thirds of that without any compute.
 #include <math.h>

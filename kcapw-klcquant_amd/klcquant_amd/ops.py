@@ -525,8 +525,8 @@ def batch_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                     sinks: torch.Tensor | None = None, window: int | None = None, scale: float | None = None,
                     out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of one token of each of B sequences over pages (klc_attn_batch): bf16 ``q [B, n_heads, D]``; sequence
-    b's keys are the first ``prefix_len`` tokens of the pages ``prefix_table`` (int32, shared by all sequences and read
-    once) and then ``lengths[b]`` of the pages ``tables[b]`` (int32 ``[B, width]``), the token's own last.  ``lengths[b]
+    b's keys are the first ``prefix_len`` tokens of the pages ``prefix_table`` (int32, shared by all sequences; without a
+    window a long one is read once for all of them) and then ``lengths[b]`` of the pages ``tables[b]`` (int32 ``[B, width]``), the token's own last.  ``lengths[b]
     < 0``: no sequence, zeros.  Other arguments as :func:`prompt_attention`; returns bf16 ``[B, n_heads, D]``."""
     if not isinstance(q, torch.Tensor):
         raise TypeError(f"q must be a torch.Tensor, got {type(q).__name__}")

@@ -8,8 +8,10 @@
 ``BatchedAttention``  StreamedAttention's layer (projections, RoPE, sinks,
                       window) for a batch of tokens of several sequences:
                       whole prompts by ops.prompt_attention, tokens behind
-                      cached ones by ops.batch_attention, which reads the pages
-                      that all of the batch's sequences share once.
+                      cached ones by ops.batch_attention, each token a row
+                      of it.  Pages that all of the batch's sequences share
+                      are read once on layers without a window, if they are
+                      many.
 
 Pages are shared while they are full and never written then: a fork takes its
 parent's full pages as they are and a copy of the last one.  Work on the cache
@@ -275,7 +277,8 @@ class PagedKVCache:
 
     def extend(self, seqs, counts=1) -> PagedBatch:
         """Room for ``counts`` (a number or one a sequence) more tokens of each sequence, and their batch.  Every layer
-        has to run it before the sequences are extended, forked or compacted again."""
+        has to run it before the sequences are extended, forked, freed or compacted again.  A batch in which any
+        sequence has tokens goes row by row: prompts do better in a batch of their own."""
         x = self.table.extend(seqs, counts)
         try:
             return self._to_device(x)
