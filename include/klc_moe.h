@@ -570,6 +570,42 @@ typedef struct klc_attn_batch_args {
 } klc_attn_batch_args;
 int klc_attn_batch(const klc_attn_batch_args* args, void* stream);
 
+/* Attention of n_seq sequences' new tokens over pages: counts[s] of them (one
+ * or many), the last of the lengths[s] keys that the sequence has in the pages
+ * of row s of tables (int32 [n_seq][table_width]); their rows of q follow one
+ * another, sequence by sequence.  The token at key i sees the keys j <= i, and
+ * with a window those with j > i - window or j < first.  q, softmax and
+ * rounding as klc_attn_batch; out [tokens][n_heads][head_dim] bfloat16.  lse
+ * (float32 [tokens][n_heads], or NULL) receives the logs of the normalisers,
+ * the sink's part in them, of the probabilities before they are rounded: -inf
+ * for a row without a key or sink.  A row without a key is zero; a length past
+ * table_width * page_size or a page number outside [0, n_pages) that a row
+ * sees makes rows of that sequence NaN.  What a row must not see does not
+ * reach it, NaN and infinities included.
+ *
+ * klc_attn_plan, on the host, divides the work by HOST arrays counts and
+ * lengths (int32 [n_seq]): sizes [8] receives {int32 values of the plan,
+ * tokens, at_items, items, at_joins, joins, part_rows, workspace bytes}, and
+ * plan its values if capacity holds them (NULL and 0 to ask).  It begins with
+ * the int32 [n_seq + 1] starts of the sequences' rows.  The call takes a copy
+ * of it on the device, the sizes and the heads, window and first that it was
+ * made for.  counts are the plan's; `lengths` is read on the device, and
+ * others than the plan's (of at least 0) are as right, only divided less
+ * evenly: a captured step may be replayed as its sequences grow.  workspace:
+ * 16-byte aligned, no initialisation, one for calls that may overlap. */
+int klc_attn_plan(const int32_t* counts, const int32_t* lengths, int64_t n_seq, int64_t n_heads, int64_t n_kv,
+                  int64_t head_dim, int64_t window, int64_t first, int32_t* plan, int64_t capacity, int64_t* sizes);
+typedef struct klc_attn_chunk_args {
+  const void *q, *k_pages, *v_pages;
+  const void *tables, *lengths, *plan;  /* int32 on the device; tables may be NULL if table_width is 0 */
+  const void* sinks;
+  void *workspace, *out, *lse;
+  int64_t at_items, items, at_joins, joins, part_rows, n_heads, n_kv, head_dim, q_stride, n_pages, page_size, table_width,
+      window, first, kv_dtype, workspace_bytes;
+  double scale;
+} klc_attn_chunk_args;
+int klc_attn_chunk(const klc_attn_chunk_args* args, void* stream);
+
 /* ---- Synthetic inputs -------------------------------------------------------
  * Counter-based SplitMix64 stream, identical to klcquant_amd/synth.py:
  * mode 0: n random bytes; mode 1: n bytes uniform in [lo, hi]. */

@@ -213,16 +213,19 @@ struct AttnWave {
     }
   }
 
-  // p = exp2(c2 s - m) of row block rb, packed, and its part of the sum
-  __device__ __forceinline__ void weigh(int rb, const f32x16_t (&s)[KT / 32], float c2, u32x4_t (&p)[KT / 16]) {
+  // p = exp2(c2 s - m) of row block rb, packed, and its part of the sum; with kPlain also of the sum of p before packing
+  template <bool kPlain = false>
+  __device__ __forceinline__ void weigh(int rb, const f32x16_t (&s)[KT / 32], float c2, u32x4_t (&p)[KT / 16],
+                                        float* plain = nullptr) {
     const float base = m[rb] == -INFINITY ? 0.f : m[rb];
     float sum = l[rb];
 #pragma unroll
     for (int kb = 0; kb < KT / 32; ++kb)
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
-        const uint32_t w = pack2<kF16>(__builtin_amdgcn_exp2f(fmaf(s[kb][e], c2, -base)),
-                                       __builtin_amdgcn_exp2f(fmaf(s[kb][e + 1], c2, -base)));
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[kb][e], c2, -base)), y = __builtin_amdgcn_exp2f(fmaf(s[kb][e + 1], c2, -base));
+        if constexpr (kPlain) *plain += x + y;
+        const uint32_t w = pack2<kF16>(x, y);
         p[2 * kb + e / 8][(e % 8) / 2] = w;
         sum = add2<kF16>(w, sum);  // the sum of what the values are multiplied by
       }

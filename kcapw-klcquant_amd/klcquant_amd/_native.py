@@ -94,6 +94,8 @@ SIGNATURES: dict[str, tuple] = {
     "klc_kv_copy_pages": (_I32, [_P, _I64, _I64, _I64, _P, _P, _I64, _P]),
     "klc_attn_batch_workspace_bytes": (_I64, [_I64] * 7),
     "klc_attn_batch": (_I32, [ctypes.c_char_p, _P]),
+    "klc_attn_plan": (_I32, [_P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P]),
+    "klc_attn_chunk": (_I32, [ctypes.c_char_p, _P]),
     "klc_synth_fill": (_I32, [_P, _I64, _U64, _I32, _I32, _I32, _P]),
 }
 

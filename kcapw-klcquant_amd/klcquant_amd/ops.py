@@ -292,10 +292,11 @@ def workspace_bytes(n_tokens: int, hidden: int, inter: int, n_experts: int, k: i
 
 _KV_CODES = {torch.bfloat16: nat.DTYPE_BF16, torch.float16: nat.DTYPE_F16}
 _TENSORS = (torch.Tensor, torch.nn.Parameter)
-# klc_attn_prompt_args, klc_kv_append_args and klc_attn_batch_args: pointers, sizes, scale
+# klc_attn_prompt_args, klc_kv_append_args, klc_attn_batch_args, klc_attn_chunk_args: pointers, sizes, scale
 _PROMPT_ARGS = struct.Struct("=6Q10qd")
 _APPEND_ARGS = struct.Struct("=11Q10q")
 _BATCH_ARGS = struct.Struct("=9Q12qd")
+_CHUNK_ARGS = struct.Struct("=10Q16qd")
 _batch_bytes: dict = {}  # sizes -> klc_attn_batch's workspace bytes
 
 
@@ -568,6 +569,113 @@ def batch_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                            workspace.data_ptr() if nbytes else 0, out.data_ptr(), count, n_heads, n_kv, dim, stride,
                            n_pages, page, width, prefix_len, window, _KV_CODES[k_pages.dtype], nbytes, scale), dev)
     return out
+
+
+class AttentionPlan:
+    """How the machine divides the attention of a batch's new tokens, from :func:`attention_plan`: for any number of
+    layers of this shape, window and ``first`` tokens, on ``device``."""
+
+    def __init__(self, data: torch.Tensor, sizes, shape: tuple, window: int, first: int) -> None:
+        self.data = data  # int32: the sequences' starts among the rows, items, joins
+        self.device = data.device
+        (_, self.tokens, self.at_items, self.items, self.at_joins, self.joins, self.part_rows,
+         self.workspace_bytes) = (int(x) for x in sizes)
+        self.n_seq, self.n_heads, self.n_kv, self.head_dim = shape
+        self.window, self.first = window, first
+
+    @property
+    def starts(self) -> torch.Tensor:
+        """int32 ``[S + 1]``: sequence s's new tokens are rows ``starts[s]:starts[s + 1]``."""
+        return self.data[:self.n_seq + 1]
+
+
+def attention_plan(counts, lengths, n_heads: int, n_kv: int, head_dim: int, window: int | None = None, first: int = 0,
+                   device: torch.device | str = "cuda") -> AttentionPlan:
+    """The plan of a batch (klc_attn_plan) for :func:`chunk_attention` and :func:`add_key_weights`, on the host from the
+    sequences' ``counts`` of new tokens and ``lengths``, the keys up to and with them (sequences of whole numbers; one
+    copy to ``device``).  Made once for all layers of a kind: ``window`` and ``first`` (tokens at the start that stay
+    visible beside it) are the layers'."""
+    counts, lengths = (np.asarray(x) for x in (counts, lengths))
+    if counts.ndim != 1 or counts.shape != lengths.shape or counts.size == 0:
+        raise ValueError(f"counts and lengths must be one number a sequence, got shapes {counts.shape} and {lengths.shape}")
+    if counts.dtype.kind not in "iu" or lengths.dtype.kind not in "iu":
+        raise TypeError(f"counts and lengths must be whole numbers, got {counts.dtype} and {lengths.dtype}")
+    if counts.min() <= 0 or (lengths < counts).any() or lengths.max() >= 1 << 29:
+        raise ValueError("every sequence needs at least one new token, which its length counts in, and fewer than 2^29 keys")
+    if window is not None and operator.index(window) <= 0:
+        raise ValueError(f"window must be positive (None: no window), got {window}")
+    first = operator.index(first)
+    if first < 0 or (first and window is None):
+        raise ValueError(f"{first} first tokens beside {'no' if window is None else 'a'} window")
+    window = min(operator.index(window), (1 << 30) - 1) if window else 0
+    shape = (int(counts.size), operator.index(n_heads), operator.index(n_kv), operator.index(head_dim))
+    device = torch.device(device)
+    if device.type != "cuda":
+        raise ValueError(f"a plan must be on a GPU device (there is no CPU implementation), got {device}")
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a plan cannot be made while a graph is captured: make it before")
+    counts, lengths = (np.ascontiguousarray(x, dtype=np.int32) for x in (counts, lengths))
+    sizes = np.zeros(8, np.int64)
+    room = 64 * (counts.size + 64)
+    while True:
+        host = torch.empty(room, dtype=torch.int32, pin_memory=True)
+        rc = nat.load().klc_attn_plan(counts.ctypes.data, lengths.ctypes.data, *shape, window, min(first, (1 << 29) - 1),
+                                      host.data_ptr(), room, sizes.ctypes.data)
+        if rc in (nat.KLC_ERR_ARGUMENT, nat.KLC_ERR_SHAPE):
+            raise ValueError(nat.last_error())
+        if rc < 0:
+            raise nat.KlcError("klc_attn_plan", int(rc), nat.last_error())
+        if sizes[0] <= room:
+            break
+        room = int(sizes[0])
+    data = host[:int(sizes[0])].to(device, non_blocking=True)
+    return AttentionPlan(data, sizes, shape, window, min(first, (1 << 29) - 1))
+
+
+def _check_plan(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor,
+                lengths: torch.Tensor, plan: AttentionPlan) -> tuple:
+    """The checks of a call over a plan: device, q's stride, (pages, page size), the tables' width."""
+    if not isinstance(q, torch.Tensor):
+        raise TypeError(f"q must be a torch.Tensor, got {type(q).__name__}")
+    if not isinstance(plan, AttentionPlan):
+        raise TypeError(f"plan must be an AttentionPlan, got {type(plan).__name__}")
+    dev = q.device
+    stride, = _row_strides((("q", q),), torch.bfloat16, dev)
+    n_pages, page, n_kv, dim = _check_pages(k_pages, v_pages, dev)
+    if q.shape != (plan.tokens, plan.n_heads, plan.head_dim) or (n_kv, dim) != (plan.n_kv, plan.head_dim):
+        raise ValueError(f"shapes mismatch: q {tuple(q.shape)}, pages {tuple(k_pages.shape)}, a plan of {plan.tokens} tokens "
+                         f"of {plan.n_heads} heads over {plan.n_kv} of {plan.head_dim}")
+    if plan.device != dev:
+        raise ValueError(f"tensors on different devices: {dev} vs the plan's {plan.device}")
+    width = tables.shape[1] if isinstance(tables, torch.Tensor) and tables.dim() == 2 else 0
+    _check_index("tables", tables, (plan.n_seq, width), dev)
+    _check_index("lengths", lengths, (plan.n_seq,), dev)
+    return dev, stride, n_pages, page, width
+
+
+def chunk_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor,
+                    lengths: torch.Tensor, plan: AttentionPlan, sinks: torch.Tensor | None = None,
+                    scale: float | None = None, out: torch.Tensor | None = None, want_lse: bool = False):
+    """Attention of new tokens over pages (klc_attn_chunk): bf16 ``q [T, n_heads, D]``, the plan's sequences' new tokens
+    one behind the other; they are the last of the ``lengths[s]`` keys (int32 ``[S]``) of the pages ``tables[s]`` (int32
+    ``[S, width]``).  A token sees the keys up to itself, or with the plan's window the last ones and the first; other
+    arguments as :func:`batch_attention`.  Returns bf16 ``[T, n_heads, D]``, with ``want_lse`` also float32 ``[T,
+    n_heads]``, the logs of the softmax normalisers.  ``lengths`` may have grown since the plan was made, as in a
+    captured step that is replayed; the counts are the plan's."""
+    dev, stride, n_pages, page, width = _check_plan(q, k_pages, v_pages, tables, lengths, plan)
+    sink_ptr, _, scale = _check_heads(sinks, plan.n_heads, plan.n_kv, None, scale, plan.head_dim, dev)
+    out = _result("out", out, q, dev)
+    lse = torch.empty((plan.tokens, plan.n_heads), dtype=torch.float32, device=dev) if want_lse else None
+    nbytes = plan.workspace_bytes
+    # of this call alone: calls on other streams and captured graphs have theirs
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _call("klc_attn_chunk",
+          _CHUNK_ARGS.pack(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr() if width else 0,
+                           lengths.data_ptr(), plan.data.data_ptr(), sink_ptr, workspace.data_ptr() if nbytes else 0,
+                           out.data_ptr(), lse.data_ptr() if want_lse else 0, plan.at_items, plan.items, plan.at_joins,
+                           plan.joins, plan.part_rows, plan.n_heads, plan.n_kv, plan.head_dim, stride, n_pages, page,
+                           width, plan.window, plan.first, _KV_CODES[k_pages.dtype], nbytes, scale), dev)
+    return (out, lse) if want_lse else out
 
 
 def synth_fill(dst: torch.Tensor, seed: int, mode: int = 0, lo: int = 0, hi: int = 255) -> torch.Tensor:
