@@ -531,6 +531,17 @@ typedef struct klc_kv_append_args {
 } klc_kv_append_args;
 int klc_kv_append(const klc_kv_append_args* args, void* stream);
 
+/* The same with the heads of q and k normalised before the rotation: x' = x *
+ * w / sqrt(mean(x^2) + eps) over head_dim, w bfloat16 [head_dim] q_norm for
+ * queries and k_norm for keys (NULL: these are not normalised), rounded once
+ * with the rotation; the squares are summed in float64. */
+typedef struct klc_kv_norm_append_args {
+  klc_kv_append_args append;
+  const void *q_norm, *k_norm;
+  double eps;
+} klc_kv_norm_append_args;
+int klc_kv_norm_append(const klc_kv_norm_append_args* args, void* stream);
+
 /* Copies page src[i] to page dst[i] in each of n_pools pools (consecutive,
  * each n_pages pages of page_bytes, a multiple of 16) for i < n: the forks and
  * the compaction of a paged cache.  src and dst are HOST arrays, read before
@@ -605,6 +616,52 @@ typedef struct klc_attn_chunk_args {
   double scale;
 } klc_attn_chunk_args;
 int klc_attn_chunk(const klc_attn_chunk_args* args, void* stream);
+
+/* The weights that such tokens' queries give the keys: row rows[s] (int32
+ * [n_seq], distinct) of weights (float32 [n_rows][n_kv][capacity]) receives, for
+ * key j of sequence s, the sum over its new tokens that see the key and the
+ * query heads of the KV head of exp(scale * q . k - lse), lse as klc_attn_chunk
+ * wrote it for the same q: added for the keys that were there before the new
+ * tokens, set for the new ones.  Sums over a call's rows are float64, in the
+ * same order every time.  Of the plan the starts are read; plan, window,
+ * first, lengths and tables as klc_attn_chunk's, n_heads and n_kv the plan's.  A
+ * key in a page outside [0, n_pages), and all of a sequence whose length passes
+ * table_width * page_size, gets NaN; keys from capacity on, and sequences whose
+ * row is outside [0, n_rows), are left out. */
+typedef struct klc_attn_key_weights_args {
+  const void *q, *lse, *k_pages;
+  const void *tables, *lengths, *plan, *rows;
+  void* weights;
+  int64_t tokens, n_seq, n_rows, capacity, n_heads, n_kv, head_dim, q_stride, n_pages, page_size, table_width, window,
+      first, kv_dtype;
+  double scale;
+} klc_attn_key_weights_args;
+int klc_attn_key_weights(const klc_attn_key_weights_args* args, void* stream);
+
+/* Eviction of the keys of least weight, in place, in every layer and KV head by
+ * itself: a sequence with lengths[s] > keep keys keeps its first `first`, its
+ * last `recent` and, of those between, the keep - first - recent of the largest
+ * weights (row rows[s] of the layer's; of equal ones the lowest places; NaN
+ * counts as the largest).  A key whose place is below keep - recent stays
+ * there; the places that become free there take, in order, the other kept keys
+ * but the recent ones, which follow in order.  kept (int32
+ * [n_layers][n_seq][n_kv][keep]) receives each place's old one.  Keys, values
+ * (16-bit, pools [2 * n_layers][n_pages][page_size][n_kv][head_dim], a layer's
+ * keys before its values) and weights from place keep on are left as they were,
+ * and so are sequences of up to keep keys, whose kept is 0, 1, .. and -1 past
+ * the length.  A length past table_width * page_size or capacity, or a row
+ * outside [0, n_rows): nothing moves, kept is -1; moves from or to a page
+ * outside [0, n_pages) are left out.  The first ceil(keep / page_size) pages of
+ * a sequence that is cut must be in no other's table, and rows be distinct.
+ * workspace: 4 bytes for each of kept's values, no initialisation. */
+typedef struct klc_kv_evict_args {
+  void *pools, *weights;
+  const void *tables, *lengths, *rows;
+  void *kept, *workspace;
+  int64_t n_layers, n_seq, n_rows, capacity, n_kv, head_dim, n_pages, page_size, table_width, keep, recent, first,
+      workspace_bytes;
+} klc_kv_evict_args;
+int klc_kv_evict(const klc_kv_evict_args* args, void* stream);
 
 /* ---- Synthetic inputs -------------------------------------------------------
  * Counter-based SplitMix64 stream, identical to klcquant_amd/synth.py:

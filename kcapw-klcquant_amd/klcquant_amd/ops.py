@@ -292,11 +292,14 @@ def workspace_bytes(n_tokens: int, hidden: int, inter: int, n_experts: int, k: i
 
 _KV_CODES = {torch.bfloat16: nat.DTYPE_BF16, torch.float16: nat.DTYPE_F16}
 _TENSORS = (torch.Tensor, torch.nn.Parameter)
-# klc_attn_prompt_args, klc_kv_append_args, klc_attn_batch_args, klc_attn_chunk_args: pointers, sizes, scale
+# The entry points' argument structs: pointers, sizes, scale
 _PROMPT_ARGS = struct.Struct("=6Q10qd")
 _APPEND_ARGS = struct.Struct("=11Q10q")
 _BATCH_ARGS = struct.Struct("=9Q12qd")
 _CHUNK_ARGS = struct.Struct("=10Q16qd")
+_NORM_ARGS = struct.Struct("=2Qd")  # behind an append's
+_WEIGHT_ARGS = struct.Struct("=8Q14qd")
+_EVICT_ARGS = struct.Struct("=7Q13q")
 _batch_bytes: dict = {}  # sizes -> klc_attn_batch's workspace bytes
 
 
@@ -453,11 +456,14 @@ def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, dev: torch.device
 
 def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                  positions: torch.Tensor, slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
-                 want_keys: bool = True):
+                 want_keys: bool = True, q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None,
+                 eps: float = 1e-6):
     """Rotates bf16 ``q [T, n_heads, D]`` and ``k [T, n_kv, D]`` by rows ``positions`` of the bf16 tables ``cos`` and
     ``sin [n, D / 2]`` and stores the keys and ``v [T, n_kv, D]`` to ``slots`` (int32 ``[T]``, distinct; page * page
     size + offset, negative: stored nowhere) of the pools ``[n_pages, page, n_kv, D]`` (klc_kv_append).  Returns the
-    rotated bf16 ``(q, k)``, ``k`` None unless ``want_keys``."""
+    rotated bf16 ``(q, k)``, ``k`` None unless ``want_keys``.  With bf16 weights ``q_norm`` and ``k_norm [D]`` (either)
+    each head is first divided by its root mean square, ``sqrt(mean(x^2) + eps)``, and multiplied by them
+    (klc_kv_norm_append), with no rounding before the rotation's."""
     if not isinstance(q, torch.Tensor):
         raise TypeError(f"q must be a torch.Tensor, got {type(q).__name__}")
     dev = q.device
@@ -475,14 +481,30 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.T
             raise ValueError(f"{name} requires grad: this operator has no backward pass")
     _check_index("positions", positions, (tokens,), dev)
     _check_index("slots", slots, (tokens,), dev)
+    for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if t is None:
+            continue
+        if not _plain(t, torch.bfloat16, (dim,), dev.index):
+            _check_gpu(name, t, torch.bfloat16, 1)
+            raise ValueError(f"{name} must be [{dim}] on {dev}, got {tuple(t.shape)} on {t.device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} requires grad: this operator has no backward pass")
+    normed = q_norm is not None or k_norm is not None
+    if normed and not (math.isfinite(eps) and eps >= 0):
+        raise ValueError(f"eps must be a finite number of at least 0, got {eps}")
     q_out = _result("q", None, q, dev)
     k_out = _result("k", None, k, dev) if want_keys else None
     if tokens:
-        _call("klc_kv_append",
-              _APPEND_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-                                positions.data_ptr(), slots.data_ptr(), q_out.data_ptr(),
-                                k_out.data_ptr() if want_keys else 0, k_pages.data_ptr(), v_pages.data_ptr(), tokens,
-                                n_pos, n_pages * page, n_heads, n_kv, dim, *strides, _KV_CODES[k_pages.dtype]), dev)
+        args = _APPEND_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+                                 positions.data_ptr(), slots.data_ptr(), q_out.data_ptr(),
+                                 k_out.data_ptr() if want_keys else 0, k_pages.data_ptr(), v_pages.data_ptr(), tokens,
+                                 n_pos, n_pages * page, n_heads, n_kv, dim, *strides, _KV_CODES[k_pages.dtype])
+        if normed:
+            _call("klc_kv_norm_append",
+                  args + _NORM_ARGS.pack(0 if q_norm is None else q_norm.data_ptr(),
+                                         0 if k_norm is None else k_norm.data_ptr(), eps), dev)
+        else:
+            _call("klc_kv_append", args, dev)
     return q_out, k_out
 
 
@@ -676,6 +698,83 @@ def chunk_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                            plan.joins, plan.part_rows, plan.n_heads, plan.n_kv, plan.head_dim, stride, n_pages, page,
                            width, plan.window, plan.first, _KV_CODES[k_pages.dtype], nbytes, scale), dev)
     return (out, lse) if want_lse else out
+
+
+def _check_weights(weights: torch.Tensor, rows: torch.Tensor, count: int, ndim: int, dev: torch.device) -> None:
+    """Float32 weights on ``dev`` and the int32 rows of ``count`` sequences among them."""
+    _check_gpu("weights", weights, torch.float32, ndim)
+    if weights.device != dev:
+        raise ValueError(f"tensors on different devices: {dev} vs {weights.device}")
+    if weights.requires_grad and torch.is_grad_enabled():
+        raise ValueError("weights require grad: this operator has no backward pass")
+    if 0 in weights.shape:
+        raise ValueError(f"weights of no keys: {tuple(weights.shape)}")
+    _check_index("rows", rows, (count,), dev)
+
+
+def add_key_weights(q: torch.Tensor, lse: torch.Tensor, k_pages: torch.Tensor, tables: torch.Tensor,
+                    lengths: torch.Tensor, plan: AttentionPlan, weights: torch.Tensor, rows: torch.Tensor,
+                    scale: float | None = None) -> None:
+    """Adds to float32 ``weights [R, n_kv, capacity]`` what the new tokens' softmax gives every key of their sequence, summed
+    over the tokens and the query heads of each KV head (klc_attn_key_weights); the new tokens' own keys start at the
+    sum.  ``q``, ``lse`` (float32 ``[T, n_heads]``) and the other arguments are :func:`chunk_attention`'s; sequence s has
+    row ``rows[s]`` (int32 ``[S]``, distinct), and ``capacity`` at least its keys."""
+    dev, stride, n_pages, page, width = _check_plan(q, k_pages, k_pages, tables, lengths, plan)
+    if not _plain(lse, torch.float32, (plan.tokens, plan.n_heads), dev.index):
+        _check_gpu("lse", lse, torch.float32, 2)
+        raise ValueError(f"lse must be [{plan.tokens}, {plan.n_heads}] on {dev}, got {tuple(lse.shape)} on {lse.device}")
+    _check_weights(weights, rows, plan.n_seq, 3, dev)
+    n_rows, n_kv, capacity = weights.shape
+    if n_kv != plan.n_kv:
+        raise ValueError(f"weights of {n_kv} KV heads for {plan.n_kv}")
+    _, _, scale = _check_heads(None, plan.n_heads, n_kv, None, scale, plan.head_dim, dev)
+    _call("klc_attn_key_weights",
+          _WEIGHT_ARGS.pack(q.data_ptr(), lse.data_ptr(), k_pages.data_ptr(), tables.data_ptr() if width else 0,
+                            lengths.data_ptr(), plan.data.data_ptr(), rows.data_ptr(), weights.data_ptr(), plan.tokens,
+                            plan.n_seq, n_rows, capacity, plan.n_heads, n_kv, plan.head_dim, stride, n_pages, page,
+                            width, plan.window, plan.first, _KV_CODES[k_pages.dtype], scale), dev)
+
+
+def evict_keys(pools: torch.Tensor, weights: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor,
+               rows: torch.Tensor, keep: int, recent: int = 0, first: int = 0) -> torch.Tensor:
+    """Cuts sequences of more than ``keep`` keys down to as many, in place and in every layer and KV head by itself
+    (klc_kv_evict): the first ``first``, the last ``recent`` and those of the largest ``weights`` between them (equal
+    ones: the first; NaN: as the largest) stay.  ``pools [2 * layers, n_pages, page, n_kv, D]`` as PagedKVCache's,
+    float32 ``weights [layers, R, n_kv, capacity]``, of sequence s row ``rows[s]`` (int32 ``[S]``, distinct), ``tables``
+    and ``lengths`` as :func:`chunk_attention`'s.  Kept keys below place ``keep - recent`` stay where they are, the
+    others fill the free places there in order, and the recent ones follow in order; places from ``keep`` on are left
+    as they were.  Returns int32 ``[layers, S, n_kv, keep]``, each place's old one, -1 for none.  No other sequence may
+    hold the first ``keep`` keys' pages of one that is cut."""
+    _check_gpu("pools", pools, None, 5)
+    if pools.dtype not in _KV_CODES:
+        raise TypeError(f"pools must be bfloat16 or float16, got {pools.dtype}")
+    if pools.requires_grad and torch.is_grad_enabled():
+        raise ValueError("pools require grad: this operator has no backward pass")
+    dev = pools.device
+    n_pools, n_pages, page, n_kv, dim = pools.shape
+    if n_pools % 2 or 0 in pools.shape or page < 16 or page > 4096 or page & (page - 1):
+        raise ValueError(f"pools must be keys and values of layers, in pages of 16 to 4096 tokens (a power of two), got {tuple(pools.shape)}")
+    count, width = tables.shape if isinstance(tables, torch.Tensor) and tables.dim() == 2 else (0, 0)
+    _check_index("tables", tables, (count, width), dev)
+    _check_index("lengths", lengths, (count,), dev)
+    _check_weights(weights, rows, count, 4, dev)
+    layers, n_rows, heads, capacity = weights.shape
+    if layers != n_pools // 2 or heads != n_kv:
+        raise ValueError(f"weights {tuple(weights.shape)} for pools {tuple(pools.shape)}")
+    keep, recent, first = operator.index(keep), operator.index(recent), operator.index(first)
+    if keep <= 0 or recent < 0 or first < 0 or recent + first > keep or keep >= 1 << 29:
+        raise ValueError(f"{keep} keys kept, of them the first {first} and the last {recent}")
+    kept = torch.empty((layers, count, n_kv, keep), dtype=torch.int32, device=dev)
+    if not count:
+        return kept
+    if not width:
+        return kept.fill_(-1)
+    workspace = torch.empty_like(kept)  # of this call alone
+    _call("klc_kv_evict",
+          _EVICT_ARGS.pack(pools.data_ptr(), weights.data_ptr(), tables.data_ptr(), lengths.data_ptr(), rows.data_ptr(),
+                           kept.data_ptr(), workspace.data_ptr(), layers, count, n_rows, capacity, n_kv, dim, n_pages,
+                           page, width, keep, recent, first, 4 * workspace.numel()), dev)
+    return kept
 
 
 def synth_fill(dst: torch.Tensor, seed: int, mode: int = 0, lo: int = 0, hi: int = 255) -> torch.Tensor:
