@@ -136,9 +136,9 @@ __global__ __launch_bounds__(kPagedThreads) void norm_append_kernel(AppendArgs a
     for (int e = 0; e < V; ++e) sum += (double)xf[e] * xf[e] + (double)yf[e] * yf[e];
     if (!live) sum = 0.;
     for (int off = 1; off < 1 << lanes_log2; off <<= 1) sum += __shfl_xor(sum, off);
-    const float scale = (float)(1. / sqrt(sum / a.d + norms.eps));
+    const double scale = 1. / sqrt(sum / a.d + norms.eps);  // past float32's range for heads of subnormals
 #pragma unroll
-    for (int e = 0; e < V; ++e) xf[e] = xf[e] * scale * bf16_to_f32(wx[e]), yf[e] = yf[e] * scale * bf16_to_f32(wy[e]);
+    for (int e = 0; e < V; ++e) xf[e] = (float)(xf[e] * scale) * bf16_to_f32(wx[e]), yf[e] = (float)(yf[e] * scale) * bf16_to_f32(wy[e]);
   }
   if (!live) return;
   float first[V], second[V];
