@@ -627,13 +627,17 @@ int klc_attn_chunk(const klc_attn_chunk_args* args, void* stream);
  * first, lengths and tables as klc_attn_chunk's, n_heads and n_kv the plan's.  A
  * key in a page outside [0, n_pages), and all of a sequence whose length passes
  * table_width * page_size, gets NaN; keys from capacity on, and sequences whose
- * row is outside [0, n_rows), are left out. */
+ * row is outside [0, n_rows), are left out.  workspace:
+ * klc_attn_key_weights_workspace_bytes with max_keys = table_width * page_size
+ * (0: none needed), 8-byte aligned, no initialisation, one for calls that may
+ * overlap. */
+int64_t klc_attn_key_weights_workspace_bytes(int64_t tokens, int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t max_keys);
 typedef struct klc_attn_key_weights_args {
   const void *q, *lse, *k_pages;
   const void *tables, *lengths, *plan, *rows;
-  void* weights;
+  void *weights, *workspace;
   int64_t tokens, n_seq, n_rows, capacity, n_heads, n_kv, head_dim, q_stride, n_pages, page_size, table_width, window,
-      first, kv_dtype;
+      first, kv_dtype, workspace_bytes;
   double scale;
 } klc_attn_key_weights_args;
 int klc_attn_key_weights(const klc_attn_key_weights_args* args, void* stream);

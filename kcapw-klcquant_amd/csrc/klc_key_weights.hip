@@ -7,10 +7,13 @@
 // tokens' own keys start at the sum, the others have it added.
 //
 // A wave keeps 64 keys in registers as the matrix instruction's columns, and
-// rows come past in tiles of 32 through LDS: a lane has 16 rows of its one
-// key, so that the sums over rows never leave it but at the end.  KW waves
-// take other keys of the same rows, 4 / KW others rows of the same keys.
+// rows come past in tiles of 32 through LDS, for the four waves of a
+// workgroup: a lane has 16 rows of its one key, so that the sums over rows
+// never leave it but at the end.  Long chunks' rows go to several workgroups,
+// whose float64 sums a second launch adds in their order.
 #include <math.h>
+
+#include <algorithm>
 
 #include "klc_paged_tiles.h"
 
@@ -18,7 +21,8 @@ namespace klc {
 namespace {
 
 constexpr int kWaveKeys = 64;
-constexpr int kTileRows32 = 32;
+constexpr int kBlockKeys = kWaves * kWaveKeys;
+constexpr int kRows = 32;  // of a tile
 
 struct KeyWeightArgs {
   const uint16_t* q;                // bfloat16 [tokens] rows
@@ -27,58 +31,83 @@ struct KeyWeightArgs {
   const int32_t *tables, *lengths;  // [n_seq][width], [n_seq]
   const int32_t *starts, *rows;     // [n_seq + 1], [n_seq]
   float* weights;                   // [n_rows][n_kv][capacity]
+  double* part;                     // [parts][n_seq][n_kv][width * page], parts > 1
   int64_t q_stride, capacity;
-  int n_seq, n_rows, n_heads, n_kv, d, n_pages, page_log2, width, window, first, blocks;
+  int n_seq, n_rows, n_heads, n_kv, d, n_pages, page_log2, width, window, first, blocks, parts;
   float c2;
 };
 
-template <int DP, bool kF16, bool kFull, int KW>
-__global__ __launch_bounds__(kWave * kWaves, 2) void key_weights_kernel(KeyWeightArgs a) {
-  using F = AttnWave<DP, kF16, kFull, 1, kTileRows32>;
-  constexpr int RW = kWaves / KW, kStepRows = RW * kTileRows32, kBlock = KW * kWaveKeys;
-  constexpr int kThreads = kWave * kWaves, kPasses = kStepRows * F::kChunks / kThreads, kPassRows = kThreads / F::kChunks;
-  static_assert(kPasses * kPassRows == kStepRows, "");
-  __shared__ __align__(1024) uint8_t tile[2][kStepRows * F::kRowBytes];
-  __shared__ __align__(16) float factor[2][kStepRows], log_norm[2][kStepRows];
-  __shared__ __align__(16) int place[2][kStepRows];
-  __shared__ double joined[kWaves][kWave];
+// The keys of a block that some new token sees, and the rows that see one of them.
+struct BlockRows {
+  int base, last;     // the first new token's key, the block's last key
+  int row0, row_end;  // none: row0 >= row_end
+  __device__ __forceinline__ BlockRows(const KeyWeightArgs& a, int count, int n, int b0) {
+    const int g = a.n_heads / a.n_kv;
+    base = n - count;
+    last = min(b0 + kBlockKeys, n) - 1;
+    const int t_lo = max(0, b0 - base);
+    const int t_hi = a.window > 0 && b0 >= a.first ? (int)min((int64_t)count - 1, (int64_t)last + a.window - 1 - base) : count - 1;
+    row0 = t_lo * g;
+    row_end = b0 < n ? (t_hi + 1) * g : 0;
+  }
+};
+
+__device__ __forceinline__ void write_weight(const KeyWeightArgs& a, int out_row, int kvh, int key, int base, double sum) {
+  if (key >= a.capacity) return;
+  float* dst = a.weights + ((int64_t)out_row * a.n_kv + kvh) * a.capacity + key;
+  *dst = (float)(key >= base ? sum : (double)*dst + sum);
+}
+
+template <int DP, bool kF16, bool kFull>
+__global__ __launch_bounds__(kWave * kWaves, DP == 64 ? 4 : 2) void key_weights_kernel(KeyWeightArgs a) {
+  using F = AttnWave<DP, kF16, kFull, 1, kRows>;
+  constexpr int kThreads = kWave * kWaves, kPassRows = kThreads / F::kChunks, kPasses = kRows / kPassRows;
+  static_assert(kPasses * kPassRows == kRows, "");
+  __shared__ __align__(1024) uint8_t tile[2][kRows * F::kRowBytes];
+  __shared__ __align__(16) float factor[2][kRows], log_norm[2][kRows];
+  __shared__ __align__(16) int place[2][kRows];
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), half = lane / 32;
-  const int kw = wave % KW, rw = wave / KW;
-  const int kvh = blockIdx.x % a.n_kv, block = blockIdx.x / a.n_kv % a.blocks, seq = blockIdx.x / (a.n_kv * a.blocks);
-  const int g = a.n_heads / a.n_kv;
+  int i = blockIdx.x;
+  const int kvh = i % a.n_kv, block = i / a.n_kv % a.blocks;
+  i /= a.n_kv * a.blocks;
+  const int part = i % a.parts, seq = i / a.parts;
   const int begin = table_at(a.starts, seq), count = table_at(a.starts, seq + 1) - begin;
   const int64_t room = (int64_t)a.width << a.page_log2;
   const int asked = table_at(a.lengths, seq), n = (int)min((int64_t)max(asked, 0), room), out_row = table_at(a.rows, seq);
-  const int base = n - count;
-  const int b0 = block * kBlock, b1 = min(b0 + kBlock, n) - 1;  // the block's keys
-  if (b0 >= n) return;
-  // the tokens that see one of them
-  const int t_lo = max(0, b0 - base), t_hi = a.window > 0 && b0 >= a.first ? min(count - 1, b1 + a.window - 1 - base) : count - 1;
-  if (t_lo > t_hi || (unsigned)out_row >= (unsigned)a.n_rows) return;
-  const int r_lo = t_lo * g, r_end = (t_hi + 1) * g;
+  const int b0 = block * kBlockKeys;
+  const BlockRows rows(a, count, n, b0);
+  if (rows.row0 >= rows.row_end || (unsigned)out_row >= (unsigned)a.n_rows) return;
+  const int g = a.n_heads / a.n_kv, base = rows.base, b1 = rows.last;
+  // this part of the rows, in whole tiles
+  const int per = (rows.row_end - rows.row0 + kRows * a.parts - 1) / (kRows * a.parts) * kRows;
+  const int r_lo = rows.row0 + part * per, r_end = min(r_lo + per, rows.row_end);
 
-  // rows of a step to LDS, by all threads: chunk threadIdx % kChunks of every kPassRows-th row
-  const int chunk = threadIdx.x % F::kChunks;
+  // rows of a tile to LDS, by all threads: chunk threadIdx % kChunks of every kPassRows-th row
+  const int chunk = threadIdx.x % F::kChunks, tile_row = threadIdx.x / F::kChunks;
+  const int step_tok = kRows / g, step_head = kRows - step_tok * g;
   u32x4_t held[kPasses];
   float held_lse[kPasses];
-  int held_place[kPasses];
-  auto fetch = [&](int row0) {
+  int tok[kPasses], head[kPasses];  // of the rows that are fetched next
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int row = row0 + i * kPassRows + (int)threadIdx.x / F::kChunks;
-      const bool live = row < r_end;
-      const int tok = min(row, r_end - 1) / g, head = kvh * g + min(row, r_end - 1) - tok * g;
-      held[i] = u32x4_t{0, 0, 0, 0};
+  for (int p = 0; p < kPasses; ++p) {
+    tok[p] = (r_lo + p * kPassRows + tile_row) / g;
+    head[p] = r_lo + p * kPassRows + tile_row - tok[p] * g;
+  }
+  auto fetch = [&]() {
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int t = min(tok[p], count - 1);  // past the last row: something, masked
+      const int64_t at = begin + t;
+      held[p] = u32x4_t{0, 0, 0, 0};
       if (kFull || 8 * chunk < a.d)
-        held[i] = *reinterpret_cast<const u32x4_t*>(a.q + (begin + tok) * a.q_stride + (int64_t)head * a.d + 8 * chunk);
-      held_lse[i] = a.lse[(int64_t)(begin + tok) * a.n_heads + head];
-      held_place[i] = live ? base + tok : -1;
+        held[p] = *reinterpret_cast<const u32x4_t*>(a.q + at * a.q_stride + (kvh * g + head[p]) * a.d + 8 * chunk);
+      held_lse[p] = a.lse[at * a.n_heads + kvh * g + head[p]];
     }
   };
-  auto put = [&](int slot) {
+  auto put = [&](int slot, int row0) {
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int row = i * kPassRows + (int)threadIdx.x / F::kChunks;
+    for (int p = 0; p < kPasses; ++p) {
+      const int row = p * kPassRows + tile_row;
       float c2 = a.c2;
       if constexpr (kF16) {
         // times a power of two that brings the row's largest value to [1, 2), as the attention kernels' queries
@@ -86,7 +115,7 @@ __global__ __launch_bounds__(kWave * kWaves, 2) void key_weights_kernel(KeyWeigh
         u16x2_t pair = {0, 0};
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          pair = __builtin_elementwise_max(pair, __builtin_bit_cast(u16x2_t, held[i][e] & 0x7fff7fffu));
+          pair = __builtin_elementwise_max(pair, __builtin_bit_cast(u16x2_t, held[p][e] & 0x7fff7fffu));
         uint32_t most = (uint32_t)max(pair.x, pair.y) << 16;
 #pragma unroll
         for (int off = 1; off < F::kChunks; off <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, off));
@@ -94,132 +123,149 @@ __global__ __launch_bounds__(kWave * kWaves, 2) void key_weights_kernel(KeyWeigh
         if (most >= 0x7f800000u || most == 0) ex = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          held[i][e] = pack2<true>(__builtin_amdgcn_ldexpf(__uint_as_float(held[i][e] << 16), -ex),
-                                   __builtin_amdgcn_ldexpf(__uint_as_float(held[i][e] & 0xffff0000u), -ex));
+          held[p][e] = pack2<true>(__builtin_amdgcn_ldexpf(__uint_as_float(held[p][e] << 16), -ex),
+                                   __builtin_amdgcn_ldexpf(__uint_as_float(held[p][e] & 0xffff0000u), -ex));
         c2 *= __builtin_amdgcn_ldexpf(1.f, ex);
       }
-      *reinterpret_cast<u32x4_t*>(tile[slot] + row * F::kRowBytes + ((chunk ^ F::swizzle(row % 32)) << 4)) = held[i];
+      *reinterpret_cast<u32x4_t*>(tile[slot] + row * F::kRowBytes + ((chunk ^ F::swizzle(row)) << 4)) = held[p];
       if (chunk == 0) {
         factor[slot][row] = c2;
-        log_norm[slot][row] = held_lse[i] * kLog2e;
-        place[slot][row] = held_place[i];
+        log_norm[slot][row] = held_lse[p] * kLog2e;
+        place[slot][row] = row0 + row < r_end ? base + tok[p] : -1;
       }
+      tok[p] += step_tok;
+      head[p] += step_head;
+      if (head[p] >= g) head[p] -= g, ++tok[p];
     }
   };
-  fetch(r_lo);
 
-  // the wave's keys
   u32x4_t k[2][F::kSteps];
-  int key[2];
   bool bad[2];
-  const int32_t* table = a.tables + (int64_t)seq * a.width;
-#pragma unroll
-  for (int kb = 0; kb < 2; ++kb) {
-    key[kb] = b0 + kw * kWaveKeys + 32 * kb + lane % 32;
-    const int at = min(key[kb], b1), page = table[at >> a.page_log2];
-    bad[kb] = (unsigned)page >= (unsigned)a.n_pages || asked > room;
-    const uint16_t* src = a.k_pages + ((((int64_t)(bad[kb] ? 0 : page) << a.page_log2) + (at & ((1 << a.page_log2) - 1))) * a.n_kv + kvh) * a.d;
-    load_query<F>(k[kb], src, a.d);
-  }
-  put(0);
-  __syncthreads();
   double total[2] = {0., 0.};
+  const int k_lo = b0 + wave * kWaveKeys, key0 = k_lo + lane % 32;
+  if (r_lo < r_end) {
+    fetch();
+    // the wave's keys
+    const int32_t* table = a.tables + (int64_t)seq * a.width;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const int at = min(key0 + 32 * kb, b1), page = table[at >> a.page_log2];
+      bad[kb] = (unsigned)page >= (unsigned)a.n_pages || asked > room;
+      const uint16_t* src =
+          a.k_pages + ((((int64_t)(bad[kb] ? 0 : page) << a.page_log2) + (at & ((1 << a.page_log2) - 1))) * a.n_kv + kvh) * a.d;
+      load_query<F>(k[kb], src, a.d);
+    }
+    put(0, r_lo);
+    __syncthreads();
+  }
   int slot = 0;
-  for (int row0 = r_lo; row0 < r_end; row0 += kStepRows, slot ^= 1) {
-    const bool more = row0 + kStepRows < r_end;
-    if (more) fetch(row0 + kStepRows);
-    const int mine = row0 + rw * kTileRows32;
-    if (mine < r_end) {
-      f32x16_t s[2];
+  for (int row0 = r_lo; row0 < r_end; row0 += kRows, slot ^= 1) {
+    const bool more = row0 + kRows < r_end;
+    if (more) fetch();
+    f32x16_t s[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+#pragma unroll
+    for (int st = 0; st < F::kSteps; ++st) {
+      if (!kFull && 16 * st >= a.d) break;
+      const u32x4_t q = *reinterpret_cast<const u32x4_t*>(tile[slot] + lane % 32 * F::kRowBytes +
+                                                          (((2 * st + half) ^ F::swizzle(lane % 32)) << 4));
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) s[kb] = mfma32<kF16>(q, k[kb][st], s[kb]);
+    }
+    // whole: its rows see all keys of the wave
+    const int first_pos = place[slot][0], last_pos = place[slot][kRows - 1];
+    const bool whole = row0 + kRows <= r_end && k_lo + kWaveKeys - 1 <= first_pos && (a.window == 0 || k_lo > last_pos - a.window);
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      if (row0 + 8 * q4 >= r_end) break;
+      const int at = 8 * q4 + 4 * half;
+      const f32x4_t norm = *reinterpret_cast<const f32x4_t*>(&log_norm[slot][at]);
+      f32x4_t c2 = {a.c2, a.c2, a.c2, a.c2};
+      if constexpr (kF16) c2 = *reinterpret_cast<const f32x4_t*>(&factor[slot][at]);
+      f32x4_t p[2];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+        for (int e = 0; e < 4; ++e) p[kb][e] = __builtin_amdgcn_exp2f(fmaf(s[kb][4 * q4 + e], c2[e], -norm[e]));
+      if (!whole) {
 #pragma unroll
-      for (int st = 0; st < F::kSteps; ++st) {
-        if (!kFull && 16 * st >= a.d) break;
-        const u32x4_t q = *reinterpret_cast<const u32x4_t*>(tile[slot] + (rw * 32 + lane % 32) * F::kRowBytes +
-                                                            (((2 * st + half) ^ F::swizzle(lane % 32)) << 4));
+        for (int e = 0; e < 4; ++e) {
+          const int pos = place[slot][at + e];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) s[kb] = mfma32<kF16>(q, k[kb][st], s[kb]);
-      }
-      // all of its rows see all keys of the wave
-      const int first_pos = base + mine / g, last_pos = base + (mine + 31) / g;
-      const int k_lo = b0 + kw * kWaveKeys, k_hi = k_lo + kWaveKeys - 1;
-      const bool whole = mine + 32 <= r_end && k_hi <= first_pos && (a.window == 0 || k_lo > last_pos - a.window);
-#pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const int at = rw * 32 + 8 * q4 + 4 * half;
-        if (mine + 8 * q4 >= r_end) break;
-        const f32x4_t norm = *reinterpret_cast<const f32x4_t*>(&log_norm[slot][at]);
-        f32x4_t c2 = {a.c2, a.c2, a.c2, a.c2};
-        if constexpr (kF16) c2 = *reinterpret_cast<const f32x4_t*>(&factor[slot][at]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb) s[kb][4 * q4 + e] = __builtin_amdgcn_exp2f(fmaf(s[kb][4 * q4 + e], c2[e], -norm[e]));
-        if (!whole) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int pos = place[slot][at + e];
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-              if (key[kb] > pos || (a.window > 0 && key[kb] <= pos - a.window && key[kb] >= a.first)) s[kb][4 * q4 + e] = 0.f;
+          for (int kb = 0; kb < 2; ++kb) {
+            const int key = key0 + 32 * kb;
+            if (key > pos || (a.window > 0 && key <= pos - a.window && key >= a.first)) p[kb][e] = 0.f;
           }
         }
       }
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        float sum = 0.f;
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4)
-          if (mine + 8 * q4 < r_end) sum += (s[kb][4 * q4] + s[kb][4 * q4 + 1]) + (s[kb][4 * q4 + 2] + s[kb][4 * q4 + 3]);
-        total[kb] += (double)sum;  // as many sums as the chunk has tiles of rows
-      }
+      for (int kb = 0; kb < 2; ++kb) sum[kb] += (p[kb][0] + p[kb][1]) + (p[kb][2] + p[kb][3]);
     }
-    if (more) put(slot ^ 1);
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) total[kb] += (double)sum[kb];  // as many sums as the chunk has tiles of rows
+    if (more) put(slot ^ 1, row0 + kRows);
     __syncthreads();
   }
 #pragma unroll
   for (int kb = 0; kb < 2; ++kb) total[kb] += __shfl_xor(total[kb], 32);
   // lane l has key l of the wave's 64
   double sum = half == 0 ? total[0] : total[1];
-  const int own = b0 + kw * kWaveKeys + lane;
-  const bool wrong = half == 0 ? bad[0] : bad[1];
-  if constexpr (RW > 1) {
-    joined[wave][lane] = sum;
-    __syncthreads();
-    if (rw != 0) return;
-#pragma unroll
-    for (int i = 1; i < RW; ++i) sum += joined[i * KW + kw][lane];
-  }
-  if (own > b1 || own >= a.capacity) return;
-  float* dst = a.weights + ((int64_t)out_row * a.n_kv + kvh) * a.capacity + own;
-  if (wrong) sum = (double)__uint_as_float(0x7fc00000u);
-  *dst = (float)(own >= base ? sum : (double)*dst + sum);
+  const int own = k_lo + lane;
+  if (own > b1) return;
+  if (r_lo < r_end && (half == 0 ? bad[0] : bad[1])) sum = (double)__uint_as_float(0x7fc00000u);
+  if (a.parts > 1)
+    a.part[(((int64_t)part * a.n_seq + seq) * a.n_kv + kvh) * room + own] = sum;
+  else
+    write_weight(a, out_row, kvh, own, base, sum);
 }
 
-template <int DP, bool kF16, bool kFull, int KW>
-void run_key_weights(KeyWeightArgs a, hipStream_t st) {
-  a.blocks = (int)((((int64_t)a.width << a.page_log2) + KW * kWaveKeys - 1) / (KW * kWaveKeys));
-  key_weights_kernel<DP, kF16, kFull, KW><<<(unsigned)((int64_t)a.n_seq * a.blocks * a.n_kv), kWave * kWaves, 0, st>>>(a);
+// The parts' sums of one key a thread, in their order.
+__global__ __launch_bounds__(kBlockKeys) void key_weights_join_kernel(KeyWeightArgs a) {
+  int i = blockIdx.x;
+  const int kvh = i % a.n_kv, block = i / a.n_kv % a.blocks, seq = i / (a.n_kv * a.blocks);
+  const int count = table_at(a.starts, seq + 1) - table_at(a.starts, seq), out_row = table_at(a.rows, seq);
+  const int64_t room = (int64_t)a.width << a.page_log2;
+  const int n = (int)min((int64_t)max(table_at(a.lengths, seq), 0), room), key = block * kBlockKeys + (int)threadIdx.x;
+  const BlockRows rows(a, count, n, block * kBlockKeys);
+  if (rows.row0 >= rows.row_end || (unsigned)out_row >= (unsigned)a.n_rows || key > rows.last) return;
+  double sum = 0.;
+  for (int p = 0; p < a.parts; ++p) sum += a.part[(((int64_t)p * a.n_seq + seq) * a.n_kv + kvh) * room + key];
+  write_weight(a, out_row, kvh, key, rows.base, sum);
+}
+
+// Parts of the rows: enough workgroups for two rounds of the chip, of at least eight tiles each.
+int64_t key_weight_parts(int64_t tokens, int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t keys) {
+  const int64_t tiles = tokens / n_seq * (n_heads / n_kv) / kRows, wgs = n_seq * n_kv * ((keys + kBlockKeys - 1) / kBlockKeys);
+  return std::max<int64_t>(1, std::min(tiles / 8, (2048 + wgs - 1) / std::max<int64_t>(wgs, 1)));
 }
 
 template <int DP, bool kF16, bool kFull>
-int launch_key_weights(const KeyWeightArgs& a, int64_t tokens, hipStream_t st) {
-  const int64_t keys = (int64_t)a.width << a.page_log2, rows = tokens / a.n_seq * (a.n_heads / a.n_kv);
-  const int64_t wgs = a.n_seq * a.n_kv * ((keys + 4 * kWaveKeys - 1) / (4 * kWaveKeys));
-  if (rows <= 32 || wgs >= 768)
-    run_key_weights<DP, kF16, kFull, 4>(a, st);
-  else
-    run_key_weights<DP, kF16, kFull, 1>(a, st);
-  return check_launch("key_weights_kernel");
+int launch_key_weights(const KeyWeightArgs& a, hipStream_t st) {
+  const int64_t joins = (int64_t)a.n_seq * a.blocks * a.n_kv;
+  key_weights_kernel<DP, kF16, kFull><<<(unsigned)(joins * a.parts), kWave * kWaves, 0, st>>>(a);
+  const int rc = check_launch("key_weights_kernel");
+  if (rc || a.parts == 1) return rc;
+  key_weights_join_kernel<<<(unsigned)joins, kBlockKeys, 0, st>>>(a);
+  return check_launch("key_weights_join_kernel");
 }
 
 }  // namespace
 }  // namespace klc
 
 using namespace klc;
+
+extern "C" int64_t klc_attn_key_weights_workspace_bytes(int64_t tokens, int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t max_keys) {
+  KLC_REQUIRE(n_seq > 0 && tokens >= n_seq && n_kv > 0 && n_heads > 0 && n_heads % n_kv == 0 && max_keys >= 0 &&
+                  max_keys < ((int64_t)1 << 29) && n_seq < ((int64_t)1 << 20) && tokens < ((int64_t)1 << 30) && n_heads <= 4096,
+              KLC_ERR_ARGUMENT, "klc_attn_key_weights_workspace_bytes: %lld tokens of %lld sequences, heads %lld / %lld, %lld keys",
+              (long long)tokens, (long long)n_seq, (long long)n_heads, (long long)n_kv, (long long)max_keys);
+  const int64_t parts = key_weight_parts(tokens, n_seq, n_heads, n_kv, max_keys);
+  return parts == 1 ? 0 : 8 * parts * n_seq * n_kv * max_keys;
+}
 
 extern "C" int klc_attn_key_weights(const klc_attn_key_weights_args* args, void* stream) {
   KLC_REQUIRE(args != nullptr, KLC_ERR_ARGUMENT, "klc_attn_key_weights: null pointer");
@@ -237,7 +283,7 @@ extern "C" int klc_attn_key_weights(const klc_attn_key_weights_args* args, void*
               (long long)x.n_pages, (long long)x.page_size, (long long)x.table_width);
   KLC_REQUIRE(x.n_seq > 0 && x.n_seq < ((int64_t)1 << 20) && x.tokens >= x.n_seq && x.tokens * (x.n_heads / x.n_kv) < ((int64_t)1 << 30) &&
                   x.n_rows > 0 && x.n_rows < ((int64_t)1 << 31) && x.capacity > 0 && x.capacity < ((int64_t)1 << 31) &&
-                  x.n_seq * x.n_kv * (x.table_width * x.page_size / kWaveKeys + 1) < ((int64_t)1 << 31),
+                  x.n_seq * x.n_kv * (x.table_width * x.page_size / kBlockKeys + 1) < ((int64_t)1 << 28),
               KLC_ERR_ARGUMENT, "klc_attn_key_weights: %lld tokens of %lld sequences, %lld rows of %lld weights", (long long)x.tokens,
               (long long)x.n_seq, (long long)x.n_rows, (long long)x.capacity);
   KLC_REQUIRE(x.q_stride >= x.n_heads * d && x.q_stride % 8 == 0, KLC_ERR_SHAPE,
@@ -251,19 +297,22 @@ extern "C" int klc_attn_key_weights(const klc_attn_key_weights_args* args, void*
   KLC_REQUIRE(x.kv_dtype == KLC_DTYPE_BF16 || x.kv_dtype == KLC_DTYPE_F16, KLC_ERR_UNSUPPORTED,
               "klc_attn_key_weights: kv_dtype %lld (bfloat16 or float16)", (long long)x.kv_dtype);
   if (x.table_width == 0) return KLC_OK;  // no key
+  const int64_t keys = x.table_width * x.page_size, parts = key_weight_parts(x.tokens, x.n_seq, x.n_heads, x.n_kv, keys);
+  const int64_t need = parts == 1 ? 0 : 8 * parts * x.n_seq * x.n_kv * keys;
+  KLC_REQUIRE(need == 0 || (x.workspace && (uintptr_t)x.workspace % 8 == 0 && x.workspace_bytes >= need), KLC_ERR_ARGUMENT,
+              "klc_attn_key_weights: workspace of %lld bytes, need %lld, 8-byte aligned", (long long)x.workspace_bytes, (long long)need);
   auto in = [](const void* v) { return static_cast<const uint16_t*>(v); };
   auto index = [](const void* v) { return static_cast<const int32_t*>(v); };
   int page_log2 = 0;
   while ((1 << page_log2) < x.page_size) ++page_log2;
   const KeyWeightArgs a{in(x.q), static_cast<const float*>(x.lse), in(x.k_pages), index(x.tables), index(x.lengths),
-                        index(x.plan), index(x.rows), static_cast<float*>(x.weights), x.q_stride, x.capacity, (int)x.n_seq,
+                        index(x.plan), index(x.rows), static_cast<float*>(x.weights), static_cast<double*>(x.workspace), x.q_stride, x.capacity, (int)x.n_seq,
                         (int)x.n_rows, (int)x.n_heads, (int)x.n_kv, (int)d, (int)x.n_pages, page_log2, (int)x.table_width,
-                        (int)x.window, (int)x.first, 0, (float)(x.scale * kLog2e)};
+                        (int)x.window, (int)x.first, (int)((keys + kBlockKeys - 1) / kBlockKeys), (int)parts, (float)(x.scale * kLog2e)};
   const hipStream_t st = as_stream(stream);
   const bool f16 = x.kv_dtype == KLC_DTYPE_F16;
-  const int64_t t = x.tokens;
-  if (d == 64) return f16 ? launch_key_weights<64, true, true>(a, t, st) : launch_key_weights<64, false, true>(a, t, st);
-  if (d == 128) return f16 ? launch_key_weights<128, true, true>(a, t, st) : launch_key_weights<128, false, true>(a, t, st);
-  if (d < 64) return f16 ? launch_key_weights<64, true, false>(a, t, st) : launch_key_weights<64, false, false>(a, t, st);
-  return f16 ? launch_key_weights<128, true, false>(a, t, st) : launch_key_weights<128, false, false>(a, t, st);
+  if (d == 64) return f16 ? launch_key_weights<64, true, true>(a, st) : launch_key_weights<64, false, true>(a, st);
+  if (d == 128) return f16 ? launch_key_weights<128, true, true>(a, st) : launch_key_weights<128, false, true>(a, st);
+  if (d < 64) return f16 ? launch_key_weights<64, true, false>(a, st) : launch_key_weights<64, false, false>(a, st);
+  return f16 ? launch_key_weights<128, true, false>(a, st) : launch_key_weights<128, false, false>(a, st);
 }

@@ -298,7 +298,7 @@ _APPEND_ARGS = struct.Struct("=11Q10q")
 _BATCH_ARGS = struct.Struct("=9Q12qd")
 _CHUNK_ARGS = struct.Struct("=10Q16qd")
 _NORM_ARGS = struct.Struct("=2Qd")  # behind an append's
-_WEIGHT_ARGS = struct.Struct("=8Q14qd")
+_WEIGHT_ARGS = struct.Struct("=9Q15qd")
 _EVICT_ARGS = struct.Struct("=7Q13q")
 _batch_bytes: dict = {}  # sizes -> klc_attn_batch's workspace bytes
 
@@ -728,11 +728,14 @@ def add_key_weights(q: torch.Tensor, lse: torch.Tensor, k_pages: torch.Tensor, t
     if n_kv != plan.n_kv:
         raise ValueError(f"weights of {n_kv} KV heads for {plan.n_kv}")
     _, _, scale = _check_heads(None, plan.n_heads, n_kv, None, scale, plan.head_dim, dev)
+    nbytes = nat.call("klc_attn_key_weights_workspace_bytes", plan.tokens, plan.n_seq, plan.n_heads, n_kv, width * page)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None  # of this call alone
     _call("klc_attn_key_weights",
           _WEIGHT_ARGS.pack(q.data_ptr(), lse.data_ptr(), k_pages.data_ptr(), tables.data_ptr() if width else 0,
-                            lengths.data_ptr(), plan.data.data_ptr(), rows.data_ptr(), weights.data_ptr(), plan.tokens,
-                            plan.n_seq, n_rows, capacity, plan.n_heads, n_kv, plan.head_dim, stride, n_pages, page,
-                            width, plan.window, plan.first, _KV_CODES[k_pages.dtype], scale), dev)
+                            lengths.data_ptr(), plan.data.data_ptr(), rows.data_ptr(), weights.data_ptr(),
+                            workspace.data_ptr() if nbytes else 0, plan.tokens, plan.n_seq, n_rows, capacity,
+                            plan.n_heads, n_kv, plan.head_dim, stride, n_pages, page, width, plan.window,
+                            plan.first, _KV_CODES[k_pages.dtype], nbytes, scale), dev)
 
 
 def evict_keys(pools: torch.Tensor, weights: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor,
