@@ -7,20 +7,28 @@
                       layers.
 ``BatchedAttention``  StreamedAttention's layer (projections, RoPE, sinks,
                       window) for a batch of tokens of several sequences:
-                      whole prompts by ops.prompt_attention, tokens behind
-                      cached ones by ops.batch_attention, each token a row
-                      of it.  Pages that all of the batch's sequences share
-                      are read once on layers without a window, if they are
-                      many.
+                      whole prompts by ops.prompt_attention, steps of one
+                      token a sequence by ops.batch_attention, where pages
+                      that all of them share are read once on layers without
+                      a window, if they are many, and suffixes of several
+                      tokens, alone or beside steps, by ops.chunk_attention.
+                      So are all tokens that see some first ones beside their
+                      window, and all of a cache that keeps weights.
+
+A cache may keep the weights that its keys were given, layer by layer and head
+by head, and evict the keys of the least (ops.add_key_weights, ops.evict_keys):
+sequences of any number of tokens then stay within a number of keys.
 
 Pages are shared while they are full and never written then: a fork takes its
-parent's full pages as they are and a copy of the last one.  Work on the cache
-is ordered by the stream it runs on; a caller with several streams orders them.
+parent's full pages as they are and a copy of the last one, and an eviction
+writes to copies.  Work on the cache is ordered by the stream it runs on; a
+caller with several streams orders them.
 """
 
 from __future__ import annotations
 
-from dataclasses import dataclass
+import operator
+from dataclasses import dataclass, field
 
 import numpy as np
 import torch
@@ -41,10 +49,12 @@ class PageTable:
         if n_pages * page_size >= 1 << 31:
             raise ValueError(f"{n_pages} pages of {page_size} tokens: their slots pass 32 bits")
         self.n_pages, self.page_size = int(n_pages), int(page_size)
+        self.max_keys: int | None = None  # that a sequence may hold
         self._free = list(range(self.n_pages - 1, -1, -1))  # taken from the end: low pages first
         self._holders = np.zeros(self.n_pages, np.int32)    # sequences that hold the page
         self._pages = np.zeros((8, 8), np.int32)            # [sequence][page of it]
         self._lengths = np.full(8, -1, np.int64)            # tokens; -1: no sequence
+        self._evicted = np.zeros(8, np.int64)               # tokens before them whose keys have left
 
     def _held(self, n_tokens):
         return -(-n_tokens // self.page_size)
@@ -87,7 +97,8 @@ class PageTable:
             free = np.array([len(self._lengths)])
             self._lengths = np.concatenate((self._lengths, np.full(len(self._lengths), -1, np.int64)))
             self._pages = np.concatenate((self._pages, np.zeros_like(self._pages)))
-        self._lengths[free[0]] = 0
+            self._evicted = np.concatenate((self._evicted, np.zeros_like(self._evicted)))
+        self._lengths[free[0]] = self._evicted[free[0]] = 0
         return int(free[0])
 
     def length(self, seq: int) -> int:
@@ -115,7 +126,7 @@ class PageTable:
                 self._take(child, 1)
                 src.append(int(self._pages[parent, full]))
                 dst.append(int(self._pages[child, full]))
-            self._lengths[child] = n
+            self._lengths[child], self._evicted[child] = n, self._evicted[parent]
             children.append(child)
         return children, src, dst
 
@@ -131,7 +142,7 @@ class PageTable:
         batch of these tokens, sequence by sequence: ``positions`` and ``slots`` of the tokens, ``starts`` of the
         sequences' runs, ``prefix`` (full pages that all share, in front), and for every token the pages behind them
         (``tables``) and the tokens in those up to itself (``lengths``).  ``fresh``: no sequence had tokens, and what
-        tells of earlier ones is empty."""
+        tells of earlier ones is empty.  Of the sequences: ``seqs``, ``counts``, ``keys`` with the new ones and ``pages``."""
         at = self._check(seqs)
         counts = np.broadcast_to(np.asarray(counts), at.shape)
         if counts.dtype.kind not in "iu" or (counts <= 0).any():
@@ -139,8 +150,10 @@ class PageTable:
         counts = counts.astype(np.int64)
         before = self._lengths[at]  # a copy
         after = before + counts
-        if after.max() >= 1 << 29:
-            raise ValueError(f"sequences must stay below 2^29 tokens, got {int(after.max())}")
+        if (after + self._evicted[at]).max() >= 1 << 29:
+            raise ValueError(f"sequences must stay below 2^29 tokens, got {int((after + self._evicted[at]).max())}")
+        if self.max_keys is not None and after.max() > self.max_keys:
+            raise RuntimeError(f"the cache keeps the weights of {self.max_keys} keys a sequence, {int(after.max())} needed")
         need = self._held(after) - self._held(before)
         self._room(int(need.sum()))
         self._widen(int(self._held(after.max())))
@@ -168,19 +181,59 @@ class PageTable:
         row = np.repeat(np.arange(at.size), counts)
         positions = np.arange(starts[-1]) - starts[row] + before[row]
         slots = self._pages[at[row], positions // self.page_size].astype(np.int64) * self.page_size + positions % self.page_size
+        pages = self._pages[at, :self._held(int(after.max()))]
+        pages = np.where(np.arange(pages.shape[1]) < self._held(after)[:, None], pages, -1)
+        of = dict(seqs=at, counts=counts, keys=after, pages=pages)
         if not before.any():  # prompts, which attend to themselves
             none = np.zeros(0, np.int32)
-            out = dict(positions=positions, slots=slots, starts=starts, prefix=none, tables=none.reshape(0, 0), lengths=none)
+            out = dict(positions=positions, slots=slots, starts=starts, prefix=none, tables=none.reshape(0, 0), lengths=none, **of)
             return {**{k: v.astype(np.int32) for k, v in out.items()}, "fresh": True}
         full = int(before.min()) // self.page_size
         rows = self._pages[at, :full]
         same = (rows == rows[:1]).all(axis=0)
         shared = full if same.all() else int(np.argmin(same))
-        tables = self._pages[at, shared:self._held(int(after.max()))]
-        tables = np.where(np.arange(tables.shape[1]) < (self._held(after) - shared)[:, None], tables, -1)
-        out = dict(positions=positions, slots=slots, starts=starts, prefix=self._pages[at[0], :shared], tables=tables[row],
-                   lengths=positions + 1 - shared * self.page_size)
+        out = dict(positions=positions + self._evicted[at][row], slots=slots, starts=starts, prefix=self._pages[at[0], :shared],
+                   tables=pages[row, shared:], lengths=positions + 1 - shared * self.page_size, **of)
         return {**{k: v.astype(np.int32) for k, v in out.items()}, "fresh": False}
+
+    def eviction(self, seqs, keep: int) -> dict:
+        """What cutting those of ``seqs`` with more than ``keep`` keys to as many needs, for ``evict`` afterwards: the cut
+        ones (``seqs``), their ``keys`` and ``pages``, and the moves (``src``, ``dst``) to free pages of those to be written
+        that others hold too, which ``pages`` has already."""
+        at = self._check(seqs)
+        if keep <= 0:
+            raise ValueError(f"a cut to {keep} keys")
+        at = at[self._lengths[at] > keep]
+        holders, free = self._holders.copy(), list(self._free)
+        width = self._held(int(self._lengths[at].max())) if at.size else 0
+        pages = self._pages[at, :width].copy()
+        src, dst = [], []
+        for row in range(at.size):
+            for i in range(self._held(keep)):
+                page = int(pages[row, i])
+                if holders[page] > 1:
+                    if not free:
+                        raise RuntimeError(f"the cache's {self.n_pages} pages are taken: no page for a shared one to be cut")
+                    holders[page] -= 1
+                    src.append(page)
+                    dst.append(free.pop())
+                    pages[row, i] = dst[-1]
+        pages = np.where(np.arange(width) < self._held(self._lengths[at])[:, None], pages, -1).astype(np.int32)
+        return dict(seqs=at, keys=self._lengths[at].astype(np.int32), pages=pages, src=src, dst=dst)
+
+    def evict(self, plan: dict, keep: int) -> None:
+        """Books the ``eviction`` that was asked for last."""
+        del self._free[len(self._free) - len(plan["dst"]):]
+        self._holders[plan["dst"]] = 1
+        np.subtract.at(self._holders, plan["src"], 1)
+        for s, n, pages in zip(plan["seqs"], plan["keys"], plan["pages"]):
+            held = self._held(int(n))
+            self._pages[s, :held] = pages[:held]
+            left = pages[self._held(keep):held]
+            self._holders[left] -= 1
+            self._free.extend(left[self._holders[left] == 0][::-1].tolist())
+            self._lengths[s] = keep
+            self._evicted[s] += int(n) - keep
 
     def moves(self) -> tuple[list[int], list[int]]:
         """The page moves (sources, destinations) of a compaction: pages that are held go to the front."""
@@ -221,14 +274,42 @@ class PagedBatch:
     fresh: bool                  # whole prompts: no sequence had tokens
     tokens: int
     end: int                     # past the largest position
+    host: dict = field(default_factory=dict, repr=False)  # of the sequences: see PageTable.extend
+    _made: dict = field(default_factory=dict, repr=False)
+
+    def sequences(self) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Of each sequence its pages (int32 ``[sequences, pages]``), its keys and its number, on the device."""
+        if "sequences" not in self._made:
+            if self.positions.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a batch's arrays cannot be copied while a graph is captured: run a layer before")
+            parts = [self.host[n] for n in ("pages", "keys", "seqs")]
+            self._made["sequences"] = _to_device(parts, self.positions.device)
+        return self._made["sequences"]
+
+    def plan(self, config: AttentionConfig, window: int | None, first: int) -> ops.AttentionPlan:
+        """The division of its tokens' attention over the cache, for all layers with this window."""
+        key = (config.num_heads, config.num_kv_heads, config.head_dim, window, first)
+        if key not in self._made:
+            self._made[key] = ops.attention_plan(self.host["counts"], self.host["keys"], *key[:3], window, first,
+                                                 self.positions.device)
+        return self._made[key]
+
+
+def _to_device(parts: list, device: torch.device) -> tuple:
+    """int32 arrays in one copy."""
+    host = torch.empty(sum(x.size for x in parts), dtype=torch.int32, pin_memory=device.type == "cuda")
+    np.concatenate([x.ravel() for x in parts], out=host.numpy())
+    return tuple(t.view(x.shape) for t, x in zip(host.to(device, non_blocking=True).split([x.size for x in parts]), parts))
 
 
 class PagedKVCache:
     """Keys and values of ``n_layers`` layers for many sequences: ``pool [2 * n_layers, n_pages, page_size, n_kv,
-    head_dim]`` of the ``precision`` ("fp16" or "bf16", as DeviceKVCache's), a layer's keys, then its values."""
+    head_dim]`` of the ``precision`` ("fp16" or "bf16", as DeviceKVCache's), a layer's keys, then its values.  With
+    ``weighted`` = (sequences, keys) also the float32 ``weights [n_layers, sequences, n_kv, keys]`` that each key was given
+    so far by the tokens behind it, for ``evict``; it then holds at most as many sequences, each of at most as many keys."""
 
     def __init__(self, device: torch.device | str, n_layers: int, n_kv: int, head_dim: int, n_pages: int,
-                 page_size: int = 64, precision: str = "fp16") -> None:
+                 page_size: int = 64, precision: str = "fp16", weighted: tuple[int, int] | None = None) -> None:
         if precision not in _KV_DTYPES:
             raise ValueError(f"unsupported KV cache precision for the device cache: {precision}")
         if n_layers <= 0 or n_kv <= 0 or head_dim <= 0:
@@ -238,6 +319,12 @@ class PagedKVCache:
         self.dtype = _KV_DTYPES[precision][0]
         self.pool = torch.empty((2 * n_layers, n_pages, page_size, n_kv, head_dim), dtype=self.dtype, device=device)
         self.device = self.pool.device  # "cuda" is the current device now, not the one of a later call
+        self.weights = None
+        if weighted is not None:
+            if len(weighted) != 2 or min(weighted) <= 0:
+                raise ValueError(f"weights of (sequences, keys), got {weighted}")
+            self.table.max_keys = int(weighted[1])
+            self.weights = torch.zeros((n_layers, weighted[0], n_kv, weighted[1]), dtype=torch.float32, device=self.device)
 
     def layer(self, layer_idx: int) -> tuple[torch.Tensor, torch.Tensor]:
         """The layer's key and value pages ``[n_pages, page_size, n_kv, head_dim]``."""
@@ -247,15 +334,26 @@ class PagedKVCache:
 
     def add(self) -> int:
         """A new sequence without tokens."""
-        return self.table.add()
+        seq = self.table.add()
+        if self.weights is not None and seq >= self.weights.shape[1]:
+            self.table.free(seq)
+            raise RuntimeError(f"the cache keeps the weights of {self.weights.shape[1]} sequences, which are taken")
+        return seq
 
     def length(self, seq: int) -> int:
+        """The tokens whose keys it holds."""
         return self.table.length(seq)
 
     def fork(self, seq: int, count: int = 1) -> list[int]:
         """New sequences with ``seq``'s tokens, which share its full pages."""
         children, src, dst = self.table.fork(seq, count)
         try:
+            if self.weights is not None:
+                if max(children, default=0) >= self.weights.shape[1]:
+                    raise RuntimeError(f"the cache keeps the weights of {self.weights.shape[1]} sequences, which are taken")
+                n = self.table.length(seq)
+                for child in children:
+                    self.weights[:, child, :, :n].copy_(self.weights[:, seq, :, :n])
             if src:
                 ops.copy_pages(self.pool, src, dst)
         except BaseException:  # sequences without their last page must not stay
@@ -267,6 +365,25 @@ class PagedKVCache:
     def free(self, seq: int) -> None:
         self.table.free(seq)
 
+    def evict(self, seqs, keep: int, recent: int = 0, first: int = 0) -> list[int]:
+        """Cuts those of ``seqs`` with more than ``keep`` keys to as many, in every layer and KV head by itself: the
+        ``first`` and the last ``recent`` ones stay, and of the others those of the largest weights (ops.evict_keys).
+        Returns the sequences that were cut.  New tokens go on at their positions in the whole text.  A window counts
+        keys that are held: layers with one need ``recent`` of at least it.  Batches made before are void."""
+        if self.weights is None:
+            raise ValueError("a cache without weights: give `weighted` when it is made")
+        keep, recent, first = operator.index(keep), operator.index(recent), operator.index(first)
+        if recent < 0 or first < 0 or recent + first > keep:
+            raise ValueError(f"{keep} keys kept, of them the first {first} and the last {recent}")
+        plan = self.table.eviction(seqs, keep)
+        if plan["seqs"].size:
+            tables, lengths, rows = _to_device([plan["pages"], plan["keys"], plan["seqs"].astype(np.int32)], self.device)
+            if plan["src"]:
+                ops.copy_pages(self.pool, plan["src"], plan["dst"])
+            ops.evict_keys(self.pool, self.weights, tables, lengths, rows, keep, recent=recent, first=first)
+            self.table.evict(plan, keep)  # once the work is under way
+        return plan["seqs"].tolist()
+
     def compact(self) -> int:
         """Moves the held pages to the pool's front and returns how many they are.  Batches made before are void."""
         src, dst = self.table.moves()
@@ -277,8 +394,8 @@ class PagedKVCache:
 
     def extend(self, seqs, counts=1) -> PagedBatch:
         """Room for ``counts`` (a number or one a sequence) more tokens of each sequence, and their batch.  Every layer
-        has to run it before the sequences are extended, forked, freed or compacted again.  A batch in which any
-        sequence has tokens goes row by row: prompts do better in a batch of their own."""
+        has to run it before the sequences are extended, forked, freed, evicted from or compacted again.  Prompts do
+        better in a batch of their own."""
         x = self.table.extend(seqs, counts)
         try:
             return self._to_device(x)
@@ -288,13 +405,10 @@ class PagedKVCache:
 
     def _to_device(self, x: dict) -> PagedBatch:
         names = ("positions", "slots", "starts", "lengths", "prefix", "tables")
-        host = torch.empty(sum(x[n].size for n in names), dtype=torch.int32, pin_memory=self.device.type == "cuda")
-        np.concatenate([x[n].ravel() for n in names], out=host.numpy())
-        parts = host.to(self.device, non_blocking=True).split([x[n].size for n in names])
-        d = {n: p.view(x[n].shape) for n, p in zip(names, parts)}
+        d = dict(zip(names, _to_device([x[n] for n in names], self.device)))
         return PagedBatch(d["positions"], d["slots"], d["starts"], d["tables"], d["lengths"], d["prefix"],
                           x["prefix"].size * self.table.page_size, x["fresh"], x["positions"].size,
-                          int(x["positions"].max()) + 1)
+                          int(x["positions"].max()) + 1, {n: x[n] for n in ("seqs", "counts", "keys", "pages")})
 
     def stats(self) -> dict:
         return {**self.table.stats(), "resident_bytes": self.pool.numel() * self.pool.element_size(),
@@ -303,15 +417,21 @@ class PagedKVCache:
 
 class BatchedAttention:
     """StreamedAttention's layer for a PagedBatch (inference: no gradients).  Refuses models whose steps batch_attention
-    does not take, though it could run their prompts: groups of more than 32 query heads."""
+    does not take, though it could run their prompts: groups of more than 32 query heads.  ``first_tokens`` at the start
+    of a sequence stay visible beside the windows of layers that have one.  Where a layer's tensors hold
+    ``q_norm.weight`` or ``k_norm.weight [head_dim]``, its queries' or keys' heads are normalised before they are rotated
+    (``config.rms_norm_eps``)."""
 
-    def __init__(self, config: AttentionConfig) -> None:
+    def __init__(self, config: AttentionConfig, first_tokens: int = 0) -> None:
         heads, kv, dim = config.num_heads, config.num_kv_heads, config.head_dim
         if kv <= 0 or heads <= 0 or heads % kv or heads // kv > 32 or heads > 4096:
             raise ValueError(f"{heads} query heads over {kv} KV heads (groups of 1 to 32, up to 4096 heads)")
         if dim < 8 or dim % 8 or dim > 128:
             raise ValueError(f"head size {dim} (8 to 128, a multiple of 8)")
+        if first_tokens < 0:
+            raise ValueError(f"{first_tokens} first tokens")
         self.config = config
+        self.first_tokens = int(first_tokens)
         self._tables: dict = {}  # device -> (cos, sin) of the positions so far
         self._kept: list = []    # smaller ones, which captured graphs may still read
 
@@ -327,6 +447,17 @@ class BatchedAttention:
             self._kept.append(self._tables.get(device))
             self._tables[device] = held
         return held
+
+    @staticmethod
+    def _suffixes(batch: PagedBatch, window: int | None) -> bool:
+        """Whether a batch with tokens behind cached ones goes by sequences rather than row by row: if any has several.
+        Short suffixes behind a long prefix that all share do better by rows, for which it is read once (64 heads over
+        8 of size 64, us by rows and by sequences: 64 behind 8,192 tokens 2 each 49 and 87, 8 each 158 and 193, 20 each
+        326 and 277; 200 behind 1,000 2 each 37 and 49; 66 behind 960 20 each 92 and 58)."""
+        count = batch.starts.shape[0] - 1
+        if window is None and batch.tokens <= 16 * count and 8 * batch.prefix_len >= 7 * batch.host["keys"].max():
+            return False
+        return batch.tokens > count
 
     def forward(self, layer_idx: int, hidden: torch.Tensor, tensors: dict, batch: PagedBatch, kv_cache: PagedKVCache,
                 sliding_window: int | None = None) -> torch.Tensor:
@@ -346,12 +477,26 @@ class BatchedAttention:
         q, k, v = project("q_proj", cfg.num_heads), project("k_proj", cfg.num_kv_heads), project("v_proj", cfg.num_kv_heads)
         k_pages, v_pages = kv_cache.layer(layer_idx)
         cos, sin = self.rope_tables(batch.end, q.device)
-        q, k = ops.paged_append(q, k, v, cos, sin, batch.positions, batch.slots, k_pages, v_pages, want_keys=batch.fresh)
         window = (sliding_window if sliding_window is not None else cfg.sliding_window) or None  # 0: none
+        first = self.first_tokens if window else 0
+        weights = kv_cache.weights
+        chunks = weights is not None or first > 0 or (not batch.fresh and self._suffixes(batch, window))
+        norms = [tensors.get(f"{prefix}.{name}.weight") for name in ("q_norm", "k_norm")]
+        norms = [t if t is None else t.to(torch.bfloat16).contiguous() for t in norms]
+        q, k = ops.paged_append(q, k, v, cos, sin, batch.positions, batch.slots, k_pages, v_pages,
+                                want_keys=batch.fresh and not chunks, q_norm=norms[0], k_norm=norms[1], eps=cfg.rms_norm_eps)
         sinks = tensors.get(f"{prefix}.sinks")
         if sinks is not None:
             sinks = sinks.to(torch.bfloat16).contiguous()
-        if batch.fresh:
+        if chunks:
+            tables, lengths, rows = batch.sequences()
+            plan = batch.plan(cfg, window, first)
+            if weights is None:
+                context = ops.chunk_attention(q, k_pages, v_pages, tables, lengths, plan, sinks)
+            else:
+                context, lse = ops.chunk_attention(q, k_pages, v_pages, tables, lengths, plan, sinks, want_lse=True)
+                ops.add_key_weights(q, lse, k_pages, tables, lengths, plan, weights[layer_idx], rows)
+        elif batch.fresh:
             context = ops.prompt_attention(q, k, v, batch.starts, sinks, window)
         else:
             context = torch.empty_like(q)
