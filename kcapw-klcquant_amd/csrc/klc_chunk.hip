@@ -27,6 +27,9 @@ constexpr int kWideRows = 32 * kWaves;
 constexpr int kNarrowRows = 32;
 constexpr int kJoinRows = 16;    // of one workgroup
 constexpr int kRecord = 8;       // int32 of an item and of a join
+// LDS of a workgroup: three fit a CU, past head size 64 two
+template <int DP>
+constexpr int kChunkLds = (DP == 64 ? 48 : 64) * 1024;
 
 struct ChunkArgs {
   const uint16_t* q;                  // bfloat16 [tokens] rows
@@ -76,6 +79,10 @@ struct Span {
   __device__ __forceinline__ int tile_of(int key) const {
     const int t = key / KT;
     return t >= low_tile ? t - low_tile + head_tiles : t;
+  }
+  // all keys of the tile that starts at `tile` are in the ranges
+  __device__ __forceinline__ bool whole(int tile) const {
+    return tile < head_tiles * KT ? tile + KT <= head_end : tile >= low && tile + KT - 1 <= high;
   }
   // the key whose row stands for `key` of the tile that starts at `tile`
   __device__ __forceinline__ auto at(int tile) const {
@@ -196,7 +203,7 @@ __device__ __forceinline__ void wide_part(const ChunkArgs& a, const ChunkItem& i
   constexpr int KT = kSharedTile<DP>, kSub = KT / kKeys;
   using R = ChunkRows<DP, kF16, kFull, kLse>;
   using F = typename R::F;
-  constexpr int kMat = kSub * F::kMatBytes, kStage = 2 * kMat, kRing = kTileLds / kStage;
+  constexpr int kMat = kSub * F::kMatBytes, kStage = 2 * kMat, kRing = kChunkLds<DP> / kStage;
   constexpr int kDmas = kSub * F::kDmas / kWaves;  // of K, and of V, a wave and tile
   static_assert(kRing >= 3 && kSub * F::kDmas % kWaves == 0, "");
   const int g = a.n_heads / a.n_kv, lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -212,11 +219,17 @@ __device__ __forceinline__ void wide_part(const ChunkArgs& a, const ChunkItem& i
   R r;
   r.begin(a, it, kvh, base, w_row, ring);
   PageLoads<ChunkArgs, F, KT, kDmas, kWaves> pages(a, wave, kvh);
+  pages.prepare_whole();
   if (tiles > 0) pages.hold(table, span.at(span.base(t0))(span.base(t0)) >> a.page_log2, a.width);
   settle_query<F>(r.f.q[0]);
   auto stage = [&](int j) { return j % kRing * kStage; };
   auto load = [&](int j) {
-    if (j < tiles) pages.load(span.base(t0 + j), span.at(span.base(t0 + j)), ring + stage(j), ring + stage(j) + kMat);
+    if (j >= tiles) return;
+    const int at = span.base(t0 + j);
+    if (span.whole(at))
+      pages.load_whole(at, ring + stage(j), ring + stage(j) + kMat);
+    else
+      pages.load(at, span.at(at), ring + stage(j), ring + stage(j) + kMat);
   };
 #pragma unroll
   for (int j = 0; j < kRing - 1; ++j) load(j);
@@ -260,7 +273,7 @@ __device__ __forceinline__ void wide_part(const ChunkArgs& a, const ChunkItem& i
   }
 
   const bool bad = __syncthreads_or(pages.bad) || wrong;
-  const lds_u8 mine = ring + wave * (kTileLds / kWaves);
+  const lds_u8 mine = ring + wave * (kChunkLds<DP> / kWaves);
   // all rows, or those of token `only`
   auto finish = [&](int only) {
     const ChunkRow row(a, it, kvh, w_row);
@@ -322,7 +335,7 @@ __device__ __forceinline__ void narrow_part(const ChunkArgs& a, const ChunkItem&
                                             float4 (&wave_ml)[kWaves][kNarrowRows]) {
   using R = ChunkRows<DP, kF16, kFull, kLse>;
   using F = typename R::F;
-  constexpr int KT = kKeys, kRing = kTileLds / kWaves / F::kStage, kQuads = R::kQuads;
+  constexpr int KT = kKeys, kRing = kChunkLds<DP> / kWaves / F::kStage, kQuads = R::kQuads;
   static_assert(kRing == 1 || kRing == 2, "");
   constexpr bool kHalves = kRing == 1;  // with one tile a wave, K and V take turns
   const int g = a.n_heads / a.n_kv, lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -333,14 +346,19 @@ __device__ __forceinline__ void narrow_part(const ChunkArgs& a, const ChunkItem&
   R r;
   r.begin(a, it, kvh, base, it.row0, ring);
   PageLoads<ChunkArgs, F, KT, F::kDmas, 1> pages(a, 0, kvh);
+  pages.prepare_whole();
   const Span<KT> span(a, p_lo, p_hi);
   const int per = (span.tiles + it.splits - 1) / it.splits, t0 = min(it.split * per, span.tiles), end = min(t0 + per, span.tiles);
   const int first = t0 + wave;
   if (first < end) pages.hold(table, span.at(span.base(first))(span.base(first)) >> a.page_log2, a.width);
   settle_query<F>(r.f.q[0]);
   auto load = [&](auto key, auto value, int j, int slot) {
-    pages.template load<decltype(key)::value, decltype(value)::value>(
-        span.base(j), span.at(span.base(j)), ring + slot * F::kStage, ring + slot * F::kStage + F::kMatBytes);
+    const int at = span.base(j);
+    const lds_u8 k = ring + slot * F::kStage, v = k + F::kMatBytes;
+    if (span.whole(at))
+      pages.template load_whole<decltype(key)::value, decltype(value)::value>(at, k, v);
+    else
+      pages.template load<decltype(key)::value, decltype(value)::value>(at, span.at(at), k, v);
   };
 #pragma unroll
   for (int i = 0; i < kRing; ++i)
@@ -442,15 +460,15 @@ __device__ __forceinline__ void narrow_part(const ChunkArgs& a, const ChunkItem&
 #pragma unroll 1
   for (int tok = careful ? it.row0 / g : -1; tok <= (careful ? last / g : -1); ++tok) {
     if (careful) careful_token<DP, kF16, kFull, kLse, KT>(a, it, r, span, kvh, base, it.row0, tok, first, end, kWaves,
-                                                          lds + wave * (kTileLds / kWaves));
+                                                          lds + wave * (kChunkLds<DP> / kWaves));
     finish(tok);
     __syncthreads();  // the sums have been read
   }
 }
 
 template <int DP, bool kF16, bool kFull, bool kLse>
-__global__ __launch_bounds__(kWave * kWaves, 2) void chunk_attention_kernel(ChunkArgs a) {
-  __shared__ __align__(1024) uint8_t lds[kTileLds];
+__global__ __launch_bounds__(kWave * kWaves, DP == 64 ? 3 : 2) void chunk_attention_kernel(ChunkArgs a) {
+  __shared__ __align__(1024) uint8_t lds[kChunkLds<DP>];
   __shared__ float4 wave_ml[kWaves][kNarrowRows];
   const int kvh = blockIdx.x % a.n_kv;
   const int32_t* rec = a.items + (int64_t)(blockIdx.x / a.n_kv) * kRecord;

@@ -82,6 +82,7 @@ struct PageLoads {
   const int32_t* table;            // held: page numbers from + lane of its `size`
   int held, from, size;
   bool bad;
+  uint32_t lane_off[kCount];       // bytes from an instruction's first key, for load_whole
 
   __device__ __forceinline__ PageLoads(const Args& args, int first, int kvh) : a(args), n0(first), table(nullptr), bad(false) {
     row_bytes = 2u * (uint32_t)(a.n_kv * a.d);
@@ -113,6 +114,29 @@ struct PageLoads {
       const uint32_t off = (uint32_t)(at(base + r) & mask) * row_bytes + 16u * (uint32_t)F::dma_chunk(r, a.d);
       if constexpr (kKey) load_to_lds(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(k0) + start), off, k + n * 1024);
       if constexpr (kValue) load_to_lds(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(v0) + start), off, v + n * 1024);
+    }
+  }
+  // The same for a tile whose keys are all visible: what differs among lanes is worked out once.
+  __device__ __forceinline__ void prepare_whole() {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      const int n = n0 + i * kStep, r = F::dma_row(n);
+      lane_off[i] = (uint32_t)(r - n * F::kRowsPerDma) * row_bytes + 16u * (uint32_t)F::dma_chunk(r, a.d);
+    }
+  }
+  template <bool kKey = true, bool kValue = true>
+  __device__ __forceinline__ void load_whole(int base, lds_u8 k, lds_u8 v) {
+    const int mask = (1 << a.page_log2) - 1;
+    if (((base + KT - 1) >> a.page_log2) - from >= kWave) hold(table, base >> a.page_log2, size);
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      const int n = n0 + i * kStep, key = base + n * F::kRowsPerDma;
+      const int page = __builtin_amdgcn_readlane(held, (key >> a.page_log2) - from);
+      const bool wrong = (unsigned)page >= (unsigned)a.n_pages;
+      bad |= wrong;
+      const uint64_t start = (uint64_t)(wrong ? 0u : (uint32_t)page) * page_bytes + (uint32_t)(key & mask) * row_bytes;
+      if constexpr (kKey) load_to_lds(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(k0) + start), lane_off[i], k + n * 1024);
+      if constexpr (kValue) load_to_lds(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(v0) + start), lane_off[i], v + n * 1024);
     }
   }
 };
