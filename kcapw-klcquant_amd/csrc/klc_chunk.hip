@@ -75,6 +75,8 @@ struct Span {
     tiles = p_hi < 0 ? 0 : head_tiles + p_hi / KT + 1 - low_tile;
   }
   __device__ __forceinline__ int base(int j) const { return (j < head_tiles ? j : j - head_tiles + low_tile) * KT; }
+  // of the tile behind the one at `tile`
+  __device__ __forceinline__ int next(int tile) const { return tile + KT == head_tiles * KT ? low_tile * KT : tile + KT; }
   // the tile with key `high` or a lower one of a row
   __device__ __forceinline__ int tile_of(int key) const {
     const int t = key / KT;
@@ -211,10 +213,12 @@ __device__ __forceinline__ void wide_part(const ChunkArgs& a, const ChunkItem& i
   const bool w_live = w_row <= last;
   const Span<KT> span(a, base + it.row0 / g, base + last / g);
   const int per = (span.tiles + it.splits - 1) / it.splits, t0 = min(it.split * per, span.tiles), tiles = min(per, span.tiles - t0);
-  // the wave's first and last position, and its pieces of kKeys keys
+  // the wave's first and last position, its last tile, and whether it sees that tile's second half
   const int w_lo = base + min(w_row, last) / g, w_hi = base + min(w_row + 31, last) / g;
-  const int w_steps =
-      w_live && w_hi >= 0 ? min(max((span.tile_of(w_hi) - t0) * kSub + w_hi % KT / kKeys + 1, 0), tiles * kSub) : 0;
+  const int w_last = w_live && w_hi >= 0 ? min(span.tile_of(w_hi) - t0, tiles - 1) : -1;
+  const bool w_both = t0 + w_last < span.tile_of(w_hi) || w_hi % KT >= kKeys;
+  // pieces of keys from `plain_from` to `plain_to` are seen by all of its rows
+  const int plain_from = a.window > 0 ? w_hi - a.window + 1 : 0, plain_to = w_lo - kKeys + 1;
   const int32_t* table = a.tables + (int64_t)it.seq * a.width;
   R r;
   r.begin(a, it, kvh, base, w_row, ring);
@@ -222,17 +226,17 @@ __device__ __forceinline__ void wide_part(const ChunkArgs& a, const ChunkItem& i
   pages.prepare_whole();
   if (tiles > 0) pages.hold(table, span.at(span.base(t0))(span.base(t0)) >> a.page_log2, a.width);
   settle_query<F>(r.f.q[0]);
-  auto stage = [&](int j) { return j % kRing * kStage; };
-  auto load = [&](int j) {
+  int load_key = span.base(t0);  // of the tile to be loaded next
+  auto load = [&](int j, int slot) {
     if (j >= tiles) return;
-    const int at = span.base(t0 + j);
-    if (span.whole(at))
-      pages.load_whole(at, ring + stage(j), ring + stage(j) + kMat);
+    if (span.whole(load_key))
+      pages.load_whole(load_key, ring + slot, ring + slot + kMat);
     else
-      pages.load(at, span.at(at), ring + stage(j), ring + stage(j) + kMat);
+      pages.load(load_key, span.at(load_key), ring + slot, ring + slot + kMat);
+    load_key = span.next(load_key);
   };
 #pragma unroll
-  for (int j = 0; j < kRing - 1; ++j) load(j);
+  for (int j = 0; j < kRing - 1; ++j) load(j, j * kStage);
   r.convert(a);
   // tile j is there for all waves, `ahead` later ones may be in flight
   auto arrive = [&](int j, auto ahead) {
@@ -241,35 +245,60 @@ __device__ __forceinline__ void wide_part(const ChunkArgs& a, const ChunkItem& i
     else
       tile_wait<0, true>();
   };
-  auto settle = [&](int i, f32x16_t (&s)[1][1]) {
-    const int k0 = span.base(t0 + i / kSub) + i % kSub * kKeys;
-    if (k0 + kKeys - 1 > w_lo || (a.window > 0 && k0 <= w_hi - a.window)) r.mask(a, k0, s);
+  auto settle = [&](int k0, f32x16_t (&s)[1][1]) {
+    if (k0 < plain_from || k0 > plain_to) r.mask(a, k0, s);
     r.raise(s[0]);
   };
-  // the values of keys i, whose settled scores are s, and the scores of keys i + 1; `end`: of their tile
-  auto step = [&](int i, auto end, f32x16_t (&s)[1][1], f32x16_t (&next)[1][1]) {
-    const int j = i / kSub, here = stage(j) + i % kSub * F::kMatBytes;
-    if constexpr (decltype(end)::value) {
-      arrive(j + 1, Count<kRing - 3>{});  // every wave is done with tile j - 1
-      load(j + kRing - 1);
-    }
-    if (i >= w_steps) return;
+  // the values of the keys at `here`, whose settled scores are s, and the scores of those at `there`
+  auto step = [&](int here, f32x16_t (&s)[1][1], int there, f32x16_t (&next)[1][1]) {
     u32x4_t p[1][2];
-    r.f.scores(stage((i + 1) / kSub) + (i + 1) % kSub * F::kMatBytes, next);  // past the last: of nothing, not used
+    r.f.scores(there, next);
     r.weigh(s[0], p[0]);
     r.f.values(here + kMat, p);
-    if (i + 1 < w_steps) settle(i + 1, next);
+  };
+  int j = 0, cur = 0, fill = (kRing - 1) * kStage, key = span.base(t0);
+  auto behind = [&](int slot) { return slot + kStage == kRing * kStage ? 0 : slot + kStage; };
+  // tile j + 1 is there from here on, every wave is done with tile j - 1
+  auto advance = [&]() {
+    arrive(j + 1, Count<kRing - 3>{});
+    load(j + kRing - 1, fill);
+    fill = cur;
   };
   f32x16_t sa[1][1], sb[1][1];
   arrive(0, Count<kRing - 2>{});
-  if (w_steps > 0) {
+  if (w_last >= 0) {
     r.f.scores(0, sa);
-    settle(0, sa);
+    settle(key, sa);
+    if constexpr (kSub == 2) {
+      for (; j <= w_last; ++j) {
+        const int here = cur, there = behind(cur), next_key = span.next(key);
+        step(here, sa, here + F::kMatBytes, sb);
+        const bool both = j < w_last || w_both;
+        if (both) settle(key + kKeys, sb);
+        advance();
+        if (both) step(here + F::kMatBytes, sb, there, sa);  // past the last tile: scores of nothing, not used
+        if (j < w_last) settle(next_key, sa);
+        cur = there, key = next_key;
+      }
+    } else {
+      auto tile = [&](f32x16_t (&s)[1][1], f32x16_t (&next)[1][1]) {
+        const int here = cur, there = behind(cur);
+        advance();
+        step(here, s, there, next);
+        key = span.next(key);
+        if (j < w_last) settle(key, next);
+        cur = there;
+        ++j;
+      };
+      while (j <= w_last) {
+        tile(sa, sb);
+        if (j <= w_last) tile(sb, sa);
+      }
+    }
   }
-  const int steps = tiles * kSub;
-  for (int i = 0; i < steps; i += 2) {
-    step(i, Count<kSub == 1>{}, sa, sb);
-    if (i + 1 < steps) step(i + 1, Count<1>{}, sb, sa);
+  for (; j < tiles; ++j) {
+    advance();
+    cur = behind(cur);
   }
 
   const bool bad = __syncthreads_or(pages.bad) || wrong;

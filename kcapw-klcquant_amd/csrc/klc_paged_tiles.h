@@ -128,15 +128,24 @@ struct PageLoads {
   __device__ __forceinline__ void load_whole(int base, lds_u8 k, lds_u8 v) {
     const int mask = (1 << a.page_log2) - 1;
     if (((base + KT - 1) >> a.page_log2) - from >= kWave) hold(table, base >> a.page_log2, size);
-#pragma unroll
-    for (int i = 0; i < kCount; ++i) {
-      const int n = n0 + i * kStep, key = base + n * F::kRowsPerDma;
+    auto start = [&](int key) {
       const int page = __builtin_amdgcn_readlane(held, (key >> a.page_log2) - from);
       const bool wrong = (unsigned)page >= (unsigned)a.n_pages;
       bad |= wrong;
-      const uint64_t start = (uint64_t)(wrong ? 0u : (uint32_t)page) * page_bytes + (uint32_t)(key & mask) * row_bytes;
-      if constexpr (kKey) load_to_lds(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(k0) + start), lane_off[i], k + n * 1024);
-      if constexpr (kValue) load_to_lds(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(v0) + start), lane_off[i], v + n * 1024);
+      return (uint64_t)(wrong ? 0u : (uint32_t)page) * page_bytes + (uint32_t)(key & mask) * row_bytes;
+    };
+    auto bring = [&](int i, uint64_t at) {
+      const int n = n0 + i * kStep;
+      if constexpr (kKey) load_to_lds(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(k0) + at), lane_off[i], k + n * 1024);
+      if constexpr (kValue) load_to_lds(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(v0) + at), lane_off[i], v + n * 1024);
+    };
+    if (mask + 1 >= KT) {  // one page
+      const uint64_t at = start(base);
+#pragma unroll
+      for (int i = 0; i < kCount; ++i) bring(i, at + (uint32_t)((n0 + i * kStep) * F::kRowsPerDma) * row_bytes);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kCount; ++i) bring(i, start(base + (n0 + i * kStep) * F::kRowsPerDma));
     }
   }
 };
