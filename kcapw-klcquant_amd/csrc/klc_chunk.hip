@@ -8,8 +8,10 @@
 // group).  A plan made on the host, where the sizes are known, lists the
 // workgroups' items, the longest first: up to 128 rows of one KV head of one
 // sequence and a part of the keys that they see.
-//   wide    more than 32 rows: 4 waves x 32 rows over one ring of tiles
-//   narrow  up to 32 rows: each wave takes every fourth tile through a ring of
+//   wide    more than 64 rows: 4 waves x 32 rows over one ring of tiles
+//   pairs   33 to 64 rows, head sizes up to 64: the same of 2 pairs of waves,
+//           of half the keys each, which join in LDS
+//   narrow  up to 32 rows (past head size 64 wide has the others): each wave takes every fourth tile through a ring of
 //           its own, with no barrier, and the waves join in LDS
 // Rows whose keys are in parts leave float32 sums, which a second launch joins.
 #include <math.h>
@@ -25,6 +27,8 @@ namespace {
 
 constexpr int kWideRows = 32 * kWaves;
 constexpr int kNarrowRows = 32;
+// most rows of an item whose waves work in pairs; head sizes past 64 have no tiles of 64 keys for them
+__host__ __device__ constexpr int pair_rows(int dim) { return dim <= 64 ? 64 : kNarrowRows; }
 constexpr int kJoinRows = 16;    // of one workgroup
 constexpr int kRecord = 8;       // int32 of an item and of a join
 // LDS of a workgroup: three fit a CU, past head size 64 two
@@ -168,11 +172,12 @@ __device__ __forceinline__ Norm normalise(const ChunkArgs& a, int head, float m,
 
 // Tile by tile for the rows of one token, with V cleared where that token does
 // not see it, so that no NaN or infinity comes from there (0 * inf).  The
-// wave works alone, in `lds`, on tiles from + i * step of the list.
+// wave works alone, in `lds`, on tiles from + i * step of the list, of each on
+// the keys from `piece` on, 32 of every piece_step.
 template <int DP, bool kF16, bool kFull, bool kLse, int KT>
 __device__ __forceinline__ void careful_token(const ChunkArgs& a, const ChunkItem& it, ChunkRows<DP, kF16, kFull, kLse>& r,
                                               const Span<KT>& span, int kvh, int base, int row0, int tok, int from, int to,
-                                              int step, lds_u8 lds) {
+                                              int step, int piece, int piece_step, lds_u8 lds) {
   using F = typename ChunkRows<DP, kF16, kFull, kLse>::F;
   typedef __attribute__((address_space(3))) u32x4_t* lds_u32x4;
   const int lane = threadIdx.x % kWave, pos = base + tok;
@@ -182,7 +187,7 @@ __device__ __forceinline__ void careful_token(const ChunkArgs& a, const ChunkIte
   PageLoads<ChunkArgs, F, kKeys, F::kDmas, 1> pages(a, 0, kvh);
   if (from < to) pages.hold(table, span.at(span.base(from))(span.base(from)) >> a.page_log2, a.width);
   for (int j = from; j < to; j += step)
-    for (int k0 = span.base(j); k0 < span.base(j) + KT; k0 += kKeys) {
+    for (int k0 = span.base(j) + piece; k0 < span.base(j) + KT; k0 += piece_step) {
       if (k0 > pos) break;
       pages.load(k0, span.at(span.base(j)), lds, lds + F::kMatBytes);
       tile_wait<0, false>();
@@ -200,16 +205,18 @@ __device__ __forceinline__ void careful_token(const ChunkArgs& a, const ChunkIte
     }
 }
 
-template <int DP, bool kF16, bool kFull, bool kLse>
+// Rows of an item in blocks of 32: a wave each, or with kSplit 2 a pair of
+// waves each, of which one takes the tiles' first 32 keys and one the others.
+template <int DP, bool kF16, bool kFull, bool kLse, int kSplit>
 __device__ __forceinline__ void wide_part(const ChunkArgs& a, const ChunkItem& it, int kvh, int n, bool wrong, lds_u8 ring) {
   constexpr int KT = kSharedTile<DP>, kSub = KT / kKeys;
   using R = ChunkRows<DP, kF16, kFull, kLse>;
   using F = typename R::F;
   constexpr int kMat = kSub * F::kMatBytes, kStage = 2 * kMat, kRing = kChunkLds<DP> / kStage;
   constexpr int kDmas = kSub * F::kDmas / kWaves;  // of K, and of V, a wave and tile
-  static_assert(kRing >= 3 && kSub * F::kDmas % kWaves == 0, "");
+  static_assert(kRing >= 3 && kSub * F::kDmas % kWaves == 0 && kSub >= kSplit, "");
   const int g = a.n_heads / a.n_kv, lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int base = n - it.count, last = it.row0 + it.rows - 1, w_row = it.row0 + 32 * wave;
+  const int base = n - it.count, last = it.row0 + it.rows - 1, w_row = it.row0 + 32 * (wave / kSplit), part = wave % kSplit;
   const bool w_live = w_row <= last;
   const Span<KT> span(a, base + it.row0 / g, base + last / g);
   const int per = (span.tiles + it.splits - 1) / it.splits, t0 = min(it.split * per, span.tiles), tiles = min(per, span.tiles - t0);
@@ -267,9 +274,10 @@ __device__ __forceinline__ void wide_part(const ChunkArgs& a, const ChunkItem& i
   f32x16_t sa[1][1], sb[1][1];
   arrive(0, Count<kRing - 2>{});
   if (w_last >= 0) {
-    r.f.scores(0, sa);
-    settle(key, sa);
-    if constexpr (kSub == 2) {
+    const int mine = part * F::kMatBytes, ahead = part * kKeys;  // of a pair's wave
+    r.f.scores(mine, sa);
+    settle(key + ahead, sa);
+    if constexpr (kSub == 2 && kSplit == 1) {
       for (; j <= w_last; ++j) {
         const int here = cur, there = behind(cur), next_key = span.next(key);
         step(here, sa, here + F::kMatBytes, sb);
@@ -284,9 +292,9 @@ __device__ __forceinline__ void wide_part(const ChunkArgs& a, const ChunkItem& i
       auto tile = [&](f32x16_t (&s)[1][1], f32x16_t (&next)[1][1]) {
         const int here = cur, there = behind(cur);
         advance();
-        step(here, s, there, next);
+        step(here + mine, s, there + mine, next);
         key = span.next(key);
-        if (j < w_last) settle(key, next);
+        if (j < w_last) settle(key + ahead, next);
         cur = there;
         ++j;
       };
@@ -303,8 +311,34 @@ __device__ __forceinline__ void wide_part(const ChunkArgs& a, const ChunkItem& i
 
   const bool bad = __syncthreads_or(pages.bad) || wrong;
   const lds_u8 mine = ring + wave * (kChunkLds<DP> / kWaves);
-  // all rows, or those of token `only`
+  // all rows, or those of token `only`; of a pair every wave comes here
   auto finish = [&](int only) {
+    if constexpr (kSplit == 2) {
+      // the second wave's sums to the first, lane by lane: [pair][quad or (maximum, sums)][lane]
+      typedef __attribute__((address_space(3))) f32x4_t* lds_f32x4;
+      static_assert(kWaves / 2 * (R::kQuads + 1) * kWave * 16 <= kChunkLds<DP>, "");
+      const lds_f32x4 sums = (lds_f32x4)ring + wave / 2 * (R::kQuads + 1) * kWave + lane;
+      __syncthreads();
+      if (part == 1) {
+#pragma unroll
+        for (int i = 0; i < R::kQuads; ++i) sums[i * kWave] = quad(r.f, i);
+        sums[R::kQuads * kWave] = f32x4_t{r.f.m[0], r.f.l[0], r.plain, 0.f};
+      }
+      __syncthreads();
+      if (part == 1) return;
+      const f32x4_t other = sums[R::kQuads * kWave];
+      const float top = fmaxf(r.f.m[0], other.x), ref = top == -INFINITY ? 0.f : top;
+      const float x = __builtin_amdgcn_exp2f(r.f.m[0] - ref), y = __builtin_amdgcn_exp2f(other.x - ref);
+      r.f.m[0] = top;
+      r.f.l[0] = fmaf(r.f.l[0], x, other.y * y);
+      r.plain = fmaf(r.plain, x, other.z * y);
+#pragma unroll
+      for (int i = 0; i < R::kQuads; ++i) {
+        const f32x4_t o = sums[i * kWave];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r.f.o[0][i / 4][i % 4 * 4 + e] = fmaf(r.f.o[0][i / 4][i % 4 * 4 + e], x, o[e] * y);
+      }
+    }
     const ChunkRow row(a, it, kvh, w_row);
     const float sum = bad ? __uint_as_float(0x7fc00000u) : add_halves(r.f.l[0]), plain = kLse ? add_halves(r.plain) : 0.f;
     const bool live = w_row + lane % 32 <= last && (only < 0 || row.tok == only);
@@ -351,11 +385,15 @@ __device__ __forceinline__ void wide_part(const ChunkArgs& a, const ChunkItem& i
   };
   // one `finish` for both: with two of them head size 128 spills
   const bool careful = __syncthreads_or(r.odd()) && !bad;
-  if (!w_live) return;
+  if (kSplit == 1 && !w_live) return;
+  const int tok0 = (kSplit == 2 ? it.row0 : w_row) / g, tok1 = (kSplit == 2 ? last : min(w_row + 31, last)) / g;
 #pragma unroll 1
-  for (int tok = careful ? w_row / g : -1; tok <= (careful ? min(w_row + 31, last) / g : -1); ++tok) {
-    if (careful) careful_token<DP, kF16, kFull, kLse, KT>(a, it, r, span, kvh, base, w_row, tok, t0, t0 + tiles, 1, mine);
+  for (int tok = careful ? tok0 : -1; tok <= (careful ? tok1 : -1); ++tok) {
+    if (careful)
+      careful_token<DP, kF16, kFull, kLse, KT>(a, it, r, span, kvh, base, w_row, tok, t0, t0 + tiles, 1, part * kKeys,
+                                               kSplit * kKeys, mine);
     finish(tok);
+    if (kSplit == 2 && careful) __syncthreads();  // the sums have been read
   }
 }
 
@@ -488,8 +526,8 @@ __device__ __forceinline__ void narrow_part(const ChunkArgs& a, const ChunkItem&
   const bool careful = __syncthreads_or(r.odd()) && !bad;
 #pragma unroll 1
   for (int tok = careful ? it.row0 / g : -1; tok <= (careful ? last / g : -1); ++tok) {
-    if (careful) careful_token<DP, kF16, kFull, kLse, KT>(a, it, r, span, kvh, base, it.row0, tok, first, end, kWaves,
-                                                          lds + wave * (kChunkLds<DP> / kWaves));
+    if (careful) careful_token<DP, kF16, kFull, kLse, KT>(a, it, r, span, kvh, base, it.row0, tok, first, end, kWaves, 0,
+                                                          kKeys, lds + wave * (kChunkLds<DP> / kWaves));
     finish(tok);
     __syncthreads();  // the sums have been read
   }
@@ -506,8 +544,10 @@ __global__ __launch_bounds__(kWave * kWaves, DP == 64 ? 3 : 2) void chunk_attent
   const int asked = table_at(a.lengths, it.seq);
   const int64_t room = (int64_t)a.width << a.page_log2;
   const int n = (int)min((int64_t)max(asked, 0), room);
-  if (it.rows > kNarrowRows)
-    wide_part<DP, kF16, kFull, kLse>(a, it, kvh, n, asked > room, (lds_u8)lds);
+  if (it.rows > pair_rows(DP))
+    wide_part<DP, kF16, kFull, kLse, 1>(a, it, kvh, n, asked > room, (lds_u8)lds);
+  else if (DP == 64 && it.rows > kNarrowRows)
+    wide_part<DP, kF16, kFull, kLse, DP == 64 ? 2 : 1>(a, it, kvh, n, asked > room, (lds_u8)lds);
   else
     narrow_part<DP, kF16, kFull, kLse>(a, it, kvh, n, asked > room, (lds_u8)lds, wave_ml);
 }
@@ -569,17 +609,23 @@ __global__ __launch_bounds__(kWave * kWaves) void chunk_join_kernel(ChunkArgs a)
 
 // ---- the plan -------------------------------------------------------------------------
 
-constexpr int kSlots = 512;  // workgroups that the chip holds at once
+constexpr int kCus = 256;
 
 // Rows of a sequence that share their tiles of keys, and the keys they see in
 // tiles of kKeys.
 struct RowTile {
   int seq, row0, rows, tiles, splits;
-  double cost() const { return kFixed + rate() * ((tiles + splits - 1) / splits); }
-  // In units of a wide tile, half a microsecond with two workgroups a CU; a narrow item's four waves take four tiles
-  // at once and wait for memory.  kFixed: a workgroup's start and end.
-  static constexpr double kFixed = 5.;
-  double rate() const { return rows > kNarrowRows ? 1. : .4; }
+  // Microseconds, measured: of a workgroup by itself, and of what it takes from a CU that has others to run.  A wide
+  // tile's throughput goes by its blocks of 32 rows, a narrow one's by its bytes from memory; a part's sums go out and
+  // in (128 rows of size 64: 64 KB, 3.3 us of a CU's share).
+  double alone(int64_t dim) const {
+    const double tile = rows <= kNarrowRows ? .25 : dim <= 64 ? .62 : .75;
+    return 4. + tile * ((tiles + splits - 1) / splits);
+  }
+  double shared(int64_t dim) const {
+    const double tile = rows <= kNarrowRows ? .4 * dim / 64 : (dim <= 64 ? .33 : .55) * ((rows + 31) / 32) / 4;
+    return 1.7 + tile * ((tiles + splits - 1) / splits) + (splits > 1 ? rows * dim / 2500. : 0.);
+  }
 };
 
 struct ChunkPlan {
@@ -595,37 +641,43 @@ int64_t span_tiles(int64_t p_lo, int64_t p_hi, int64_t window, int64_t first) {
   return p_hi < 0 ? 0 : head_tiles + p_hi / kKeys + 1 - std::max(low / kKeys, head_tiles);
 }
 
-// When the last of the items is done, if the longest go first.
-double makespan(const std::vector<RowTile>& tiles, int64_t n_kv) {
-  std::vector<double> costs;
-  for (const RowTile& t : tiles) costs.insert(costs.end(), (size_t)(t.splits * n_kv), t.cost());
+// When the last of `servers` is done, if the longest items go first.
+double makespan(std::vector<double>& costs, int64_t servers) {
   std::sort(costs.begin(), costs.end(), std::greater<double>());
   std::priority_queue<double, std::vector<double>, std::greater<double>> ends;
   double last = 0.;
   for (double c : costs) {
     double at = 0.;
-    if (ends.size() >= kSlots) at = ends.top(), ends.pop();
+    if ((int64_t)ends.size() >= servers) at = ends.top(), ends.pop();
     ends.push(at + c);
     last = std::max(last, at + c);
   }
   return last;
 }
 
-// Keys in parts where that ends sooner: tiles of more than `most` cost are cut into about equal ones.
-void split_tiles(std::vector<RowTile>& tiles, double most) {
-  for (RowTile& t : tiles) {
-    const int least = t.rows > kNarrowRows ? 4 : 2 * kWaves;  // tiles of a part
-    t.splits = 1;
-    if (most > 0.) t.splits = (int)std::max(1., std::min(std::ceil(t.rate() * t.tiles / most), (double)(t.tiles / least)));
+// How long a plan takes: two workgroups a CU, of one KV head's share of the chip.
+double duration(const std::vector<RowTile>& tiles, int64_t n_kv, int64_t dim) {
+  std::vector<double> alone, shared;
+  bool joins = false;
+  for (const RowTile& t : tiles) {
+    alone.insert(alone.end(), t.splits, t.alone(dim));
+    shared.insert(shared.end(), t.splits, t.shared(dim));
+    joins |= t.splits > 1;
   }
+  const int64_t cus = std::max<int64_t>(1, kCus / n_kv);
+  return std::max(makespan(alone, 2 * cus), makespan(shared, cus)) + (joins ? 5. : 0.);  // the join's launch
 }
 
-ChunkPlan chunk_plan(const int32_t* counts, const int32_t* lengths, int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t window,
-                     int64_t first) {
+// Tiles' keys in parts of about `most` tiles, or whole (0).
+void split_tiles(std::vector<RowTile>& tiles, int64_t most) {
+  for (RowTile& t : tiles) t.splits = most > 0 ? (int)std::max<int64_t>(1, (t.tiles + most / 2) / most) : 1;
+}
+
+ChunkPlan chunk_plan(const int32_t* counts, const int32_t* lengths, int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t dim,
+                     int64_t window, int64_t first) {
   ChunkPlan p;
   const int64_t g = n_heads / n_kv;
-  int64_t begin = 0;
-  double total = 0.;
+  int64_t begin = 0, longest = 0;
   for (int64_t s = 0; s < n_seq; ++s) {
     p.starts.push_back((int32_t)begin);
     const int64_t rows = counts[s] * g, past = (int64_t)lengths[s] - counts[s];
@@ -633,24 +685,29 @@ ChunkPlan chunk_plan(const int32_t* counts, const int32_t* lengths, int64_t n_se
       const int64_t n = std::min<int64_t>(kWideRows, rows - row0);
       const int64_t tiles = span_tiles(past + row0 / g, past + (row0 + n - 1) / g, window, first);
       p.tiles.push_back({(int)s, (int)row0, (int)n, (int)tiles, 1});
-      total += p.tiles.back().rate() * tiles * n_kv;
+      longest = std::max(longest, tiles);
     }
     begin += counts[s];
   }
   p.starts.push_back((int32_t)begin);
-  // A join is a launch and the parts' way through memory.  Past some rounds of workgroups nothing is left to gain.
-  constexpr double kJoin = 12.;
-  if ((int64_t)p.tiles.size() * n_kv <= 16 * kSlots) {
-    double best = makespan(p.tiles, n_kv), most = 0.;
-    for (int rounds = 1; rounds <= 4; ++rounds) {
-      const double limit = std::max(total / (kSlots * rounds), 4.);
-      split_tiles(p.tiles, limit);
-      const double t = makespan(p.tiles, n_kv) + kJoin;
-      if (t < best) best = t, most = limit;
+  // Keys in parts where that ends sooner.  Past four workgroups a CU there is nothing to gain.
+  auto count = [&] {
+    int64_t n = 0;
+    for (const RowTile& t : p.tiles) n += t.splits;
+    return n * n_kv;
+  };
+  if (count() <= 4 * kCus) {
+    double best = duration(p.tiles, n_kv, dim);
+    int64_t most = 0;
+    for (int64_t m = longest * 2 / 3; m >= 12; m = m * 3 / 4) {
+      split_tiles(p.tiles, m);
+      if (count() > 4 * kCus) break;
+      const double t = duration(p.tiles, n_kv, dim);
+      if (t < best) best = t, most = m;
     }
     split_tiles(p.tiles, most);
   }
-  std::stable_sort(p.tiles.begin(), p.tiles.end(), [](const RowTile& a, const RowTile& b) { return a.cost() > b.cost(); });
+  std::stable_sort(p.tiles.begin(), p.tiles.end(), [dim](const RowTile& a, const RowTile& b) { return a.alone(dim) > b.alone(dim); });
   for (const RowTile& t : p.tiles) {
     p.items += t.splits;
     if (t.splits > 1) {
@@ -700,7 +757,7 @@ extern "C" int klc_attn_plan(const int32_t* counts, const int32_t* lengths, int6
               "klc_attn_plan: %lld tokens of groups of %lld heads (below 2^30 rows)", (long long)tokens,
               (long long)(n_heads / n_kv));
   try {
-    const ChunkPlan p = chunk_plan(counts, lengths, n_seq, n_heads, n_kv, window, first);
+    const ChunkPlan p = chunk_plan(counts, lengths, n_seq, n_heads, n_kv, head_dim, window, first);
     const int64_t at_items = (n_seq + 1 + kRecord - 1) / kRecord * kRecord, at_joins = at_items + p.items * kRecord;
     KLC_REQUIRE(p.part_rows < ((int64_t)1 << 31) && p.items * n_kv < ((int64_t)1 << 31) && p.joins * n_kv < ((int64_t)1 << 31),
                 KLC_ERR_ARGUMENT, "klc_attn_plan: %lld tokens of %lld heads are too many", (long long)tokens, (long long)n_heads);
