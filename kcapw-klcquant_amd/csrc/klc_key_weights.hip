@@ -159,7 +159,13 @@ __global__ __launch_bounds__(kWave * kWaves, DP == 64 ? 4 : 2) void key_weights_
     __syncthreads();
   }
   int slot = 0;
-  for (int row0 = r_lo; row0 < r_end; row0 += kRows, slot ^= 1) {
+  // tokens of the tile's first and last row, and their heads
+  int first_tok = r_lo / g, first_head = r_lo - first_tok * g, last_tok = (r_lo + kRows - 1) / g, last_head = r_lo + kRows - 1 - last_tok * g;
+  auto move_on = [&](int& t, int& h) {
+    t += step_tok, h += step_head;
+    if (h >= g) h -= g, ++t;
+  };
+  for (int row0 = r_lo; row0 < r_end; row0 += kRows, slot ^= 1, move_on(first_tok, first_head), move_on(last_tok, last_head)) {
     const bool more = row0 + kRows < r_end;
     if (more) fetch();
     f32x16_t s[2];
@@ -176,34 +182,46 @@ __global__ __launch_bounds__(kWave * kWaves, DP == 64 ? 4 : 2) void key_weights_
       for (int kb = 0; kb < 2; ++kb) s[kb] = mfma32<kF16>(q, k[kb][st], s[kb]);
     }
     // whole: its rows see all keys of the wave
-    const int first_pos = place[slot][0], last_pos = place[slot][kRows - 1];
-    const bool whole = row0 + kRows <= r_end && k_lo + kWaveKeys - 1 <= first_pos && (a.window == 0 || k_lo > last_pos - a.window);
+    const bool whole = row0 + kRows <= r_end && k_lo + kWaveKeys - 1 <= base + first_tok &&
+                       (a.window == 0 || k_lo > base + last_tok - a.window);
     float sum[2] = {0.f, 0.f};
-#pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4) {
-      if (row0 + 8 * q4 >= r_end) break;
+    // the weights of the lane's rows 8 q4 on, four of each key
+    auto weigh = [&](int q4, f32x4_t (&p)[2]) {
       const int at = 8 * q4 + 4 * half;
       const f32x4_t norm = *reinterpret_cast<const f32x4_t*>(&log_norm[slot][at]);
       f32x4_t c2 = {a.c2, a.c2, a.c2, a.c2};
       if constexpr (kF16) c2 = *reinterpret_cast<const f32x4_t*>(&factor[slot][at]);
-      f32x4_t p[2];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int e = 0; e < 4; ++e) p[kb][e] = __builtin_amdgcn_exp2f(fmaf(s[kb][4 * q4 + e], c2[e], -norm[e]));
-      if (!whole) {
+    };
+    if (whole) {  // by itself, so that nothing divides its instructions
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        f32x4_t p[2];
+        weigh(q4, p);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) sum[kb] += (p[kb][0] + p[kb][1]) + (p[kb][2] + p[kb][3]);
+      }
+    } else {
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        if (row0 + 8 * q4 >= r_end) break;
+        f32x4_t p[2];
+        weigh(q4, p);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int pos = place[slot][at + e];
+          const int pos = place[slot][8 * q4 + 4 * half + e];
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb) {
             const int key = key0 + 32 * kb;
             if (key > pos || (a.window > 0 && key <= pos - a.window && key >= a.first)) p[kb][e] = 0.f;
           }
         }
-      }
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) sum[kb] += (p[kb][0] + p[kb][1]) + (p[kb][2] + p[kb][3]);
+        for (int kb = 0; kb < 2; ++kb) sum[kb] += (p[kb][0] + p[kb][1]) + (p[kb][2] + p[kb][3]);
+      }
     }
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) total[kb] += (double)sum[kb];  // as many sums as the chunk has tiles of rows
