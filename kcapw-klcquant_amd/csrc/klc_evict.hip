@@ -74,8 +74,20 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(EvictArgs a) {
     for (int i = t; i < kBins; i += kEvictThreads) bins[i] = 0;
     __syncthreads();
     for (int i = a.first + t; i < middle_end; i += kEvictThreads) {
-      const uint32_t u = order_bits(weights[i]);
-      if ((u & mask) == least) atomicAdd(&bins[(u >> shift) & ((1u << bits) - 1)], 1u);
+      const uint32_t u = order_bits(weights[i]), bin = (u >> shift) & ((1u << bits) - 1);
+      bool open = (u & mask) == least;
+      // lists have many equal weights, zeros above all: a wave's first two bins by one addition each
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint64_t all = __ballot(open);
+        if (all == 0) break;
+        const int leader = __ffsll((unsigned long long)all) - 1;
+        const bool same = open && bin == (uint32_t)__builtin_amdgcn_readlane((int)bin, leader);
+        const uint64_t alike = __ballot(same);
+        if (lane == leader) atomicAdd(&bins[bin], (uint32_t)__popcll(alike));
+        open = open && !same;
+      }
+      if (open) atomicAdd(&bins[bin], 1u);
     }
     __syncthreads();
     // the highest digit at which as many as needed are reached, from the top: thread t has digits 2047 - 2 t and the next
