@@ -604,6 +604,7 @@ class AttentionPlan:
          self.workspace_bytes) = (int(x) for x in sizes)
         self.n_seq, self.n_heads, self.n_kv, self.head_dim = shape
         self.window, self.first = window, first
+        self.weight_bytes: dict = {}  # keys of the tables -> klc_attn_key_weights' workspace bytes
 
     @property
     def starts(self) -> torch.Tensor:
@@ -728,7 +729,10 @@ def add_key_weights(q: torch.Tensor, lse: torch.Tensor, k_pages: torch.Tensor, t
     if n_kv != plan.n_kv:
         raise ValueError(f"weights of {n_kv} KV heads for {plan.n_kv}")
     _, _, scale = _check_heads(None, plan.n_heads, n_kv, None, scale, plan.head_dim, dev)
-    nbytes = nat.call("klc_attn_key_weights_workspace_bytes", plan.tokens, plan.n_seq, plan.n_heads, n_kv, width * page)
+    nbytes = plan.weight_bytes.get(width * page)
+    if nbytes is None:
+        nbytes = plan.weight_bytes[width * page] = nat.call("klc_attn_key_weights_workspace_bytes", plan.tokens, plan.n_seq,
+                                                            plan.n_heads, n_kv, width * page)
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None  # of this call alone
     _call("klc_attn_key_weights",
           _WEIGHT_ARGS.pack(q.data_ptr(), lse.data_ptr(), k_pages.data_ptr(), tables.data_ptr() if width else 0,
