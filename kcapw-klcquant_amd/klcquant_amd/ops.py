@@ -595,7 +595,8 @@ def batch_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
 class AttentionPlan:
     """How the machine divides the attention of a batch's new tokens, from :func:`attention_plan`: for any number of
-    layers of this shape, window and ``first`` tokens, on ``device``."""
+    layers of this shape, window and ``first`` tokens, on ``device``.  Calls only read it; it has to live as long as
+    graphs that captured them."""
 
     def __init__(self, data: torch.Tensor, sizes, shape: tuple, window: int, first: int) -> None:
         self.data = data  # int32: the sequences' starts among the rows, items, joins

@@ -452,12 +452,15 @@ class BatchedAttention:
     def _suffixes(batch: PagedBatch, window: int | None) -> bool:
         """Whether a batch with tokens behind cached ones goes by sequences rather than row by row: if any has several.
         Short suffixes behind a long prefix that all share do better by rows, for which it is read once (64 heads over
-        8 of size 64, us by rows and by sequences: 64 behind 8,192 tokens 2 each 49 and 87, 8 each 158 and 193, 20 each
-        326 and 277; 200 behind 1,000 2 each 37 and 49; 66 behind 960 20 each 92 and 58)."""
+        8 of size 64, us by rows and by sequences: 64 behind 8,192 tokens 2 each 49 and 85, 8 each 159 and 126; 8 behind
+        8,192 2 each 18 and 26; 200 behind 1,000 2 each 38 and 42; 66 behind 960 2 each 23 and 20), and a captured graph,
+        which may be replayed with other ``tables`` and ``lengths`` of the rows, keeps to them."""
         count = batch.starts.shape[0] - 1
-        if window is None and batch.tokens <= 16 * count and 8 * batch.prefix_len >= 7 * batch.host["keys"].max():
+        if batch.tokens == count or not batch.host or torch.cuda.is_current_stream_capturing():
             return False
-        return batch.tokens > count
+        if window is None and batch.tokens <= 4 * count and 8 * batch.prefix_len >= 7 * batch.host["keys"].max():
+            return False
+        return True
 
     def forward(self, layer_idx: int, hidden: torch.Tensor, tensors: dict, batch: PagedBatch, kv_cache: PagedKVCache,
                 sliding_window: int | None = None) -> torch.Tensor:
