@@ -27,7 +27,7 @@ constexpr int kRows = 32;  // of a tile
 struct KeyWeightArgs {
   const uint16_t* q;                // bfloat16 [tokens] rows
   const float* lse;                 // [tokens][n_heads]
-  const uint16_t* k_pages;          // [n_pages][page][n_kv][d]
+  const uint16_t *k_pages, *v_pages;  // [n_pages][page][n_kv][d]; values are not read
   const int32_t *tables, *lengths;  // [n_seq][width], [n_seq]
   const int32_t *starts, *rows;     // [n_seq + 1], [n_seq]
   float* weights;                   // [n_rows][n_kv][capacity]
@@ -63,7 +63,9 @@ __global__ __launch_bounds__(kWave * kWaves, DP == 64 ? 4 : 2) void key_weights_
   using F = AttnWave<DP, kF16, kFull, 1, kRows>;
   constexpr int kThreads = kWave * kWaves, kPassRows = kThreads / F::kChunks, kPasses = kRows / kPassRows;
   static_assert(kPasses * kPassRows == kRows, "");
-  __shared__ __align__(1024) uint8_t tile[2][kRows * F::kRowBytes];
+  // the block's keys on their way into registers, then two tiles of rows
+  constexpr int kTileBytes = kRows * F::kRowBytes, kWaveBytes = 8192, kStageKeys = kWaveBytes / F::kRowBytes;
+  __shared__ __align__(1024) uint8_t lds[kWaves * kWaveBytes];
   __shared__ __align__(16) float factor[2][kRows], log_norm[2][kRows];
   __shared__ __align__(16) int place[2][kRows];
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), half = lane / 32;
@@ -127,7 +129,7 @@ __global__ __launch_bounds__(kWave * kWaves, DP == 64 ? 4 : 2) void key_weights_
                                    __builtin_amdgcn_ldexpf(__uint_as_float(held[p][e] & 0xffff0000u), -ex));
         c2 *= __builtin_amdgcn_ldexpf(1.f, ex);
       }
-      *reinterpret_cast<u32x4_t*>(tile[slot] + row * F::kRowBytes + ((chunk ^ F::swizzle(row)) << 4)) = held[p];
+      *reinterpret_cast<u32x4_t*>(lds + slot * kTileBytes + row * F::kRowBytes + ((chunk ^ F::swizzle(row)) << 4)) = held[p];
       if (chunk == 0) {
         factor[slot][row] = c2;
         log_norm[slot][row] = held_lse[p] * kLog2e;
@@ -145,16 +147,29 @@ __global__ __launch_bounds__(kWave * kWaves, DP == 64 ? 4 : 2) void key_weights_
   const int k_lo = b0 + wave * kWaveKeys, key0 = k_lo + lane % 32;
   if (r_lo < r_end) {
     fetch();
-    // the wave's keys
+    // the wave's keys, whole rows at a time: read by the lanes that need them, 32 bytes of a row an instruction, 200
+    // steps of 1,500 keys take 70 us instead of 64
     const int32_t* table = a.tables + (int64_t)seq * a.width;
+    PageLoads<KeyWeightArgs, F, kStageKeys, kStageKeys / F::kRowsPerDma, 1> pages(a, 0, kvh);
+    pages.hold(table, min(k_lo, b1) >> a.page_log2, a.width);
+    const lds_u8 mine = (lds_u8)lds + wave * kWaveBytes;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      const int at = min(key0 + 32 * kb, b1), page = table[at >> a.page_log2];
-      bad[kb] = (unsigned)page >= (unsigned)a.n_pages || asked > room;
-      const uint16_t* src =
-          a.k_pages + ((((int64_t)(bad[kb] ? 0 : page) << a.page_log2) + (at & ((1 << a.page_log2) - 1))) * a.n_kv + kvh) * a.d;
-      load_query<F>(k[kb], src, a.d);
+      if (kb * 32 % kStageKeys == 0) {
+        tile_wait<63, false>();  // the keys before them have been read
+        pages.template load<true, false>(k_lo + 32 * kb, within(0, b1), mine, mine);
+        tile_wait<0, false>();
+      }
+#pragma unroll
+      for (int st = 0; st < F::kSteps; ++st) {
+        k[kb][st] = u32x4_t{0, 0, 0, 0};
+        if (kFull || 16 * st + 8 * half < a.d)
+          k[kb][st] = *reinterpret_cast<const u32x4_t*>(lds + wave * kWaveBytes + (32 * kb % kStageKeys + lane % 32) * F::kRowBytes +
+                                                        (((2 * st + half) ^ F::swizzle(lane % 32)) << 4));
+      }
+      bad[kb] = (unsigned)table[min(key0 + 32 * kb, b1) >> a.page_log2] >= (unsigned)a.n_pages || asked > room;
     }
+    __syncthreads();  // the keys have been read
     put(0, r_lo);
     __syncthreads();
   }
@@ -176,7 +191,7 @@ __global__ __launch_bounds__(kWave * kWaves, DP == 64 ? 4 : 2) void key_weights_
 #pragma unroll
     for (int st = 0; st < F::kSteps; ++st) {
       if (!kFull && 16 * st >= a.d) break;
-      const u32x4_t q = *reinterpret_cast<const u32x4_t*>(tile[slot] + lane % 32 * F::kRowBytes +
+      const u32x4_t q = *reinterpret_cast<const u32x4_t*>(lds + slot * kTileBytes + lane % 32 * F::kRowBytes +
                                                           (((2 * st + half) ^ F::swizzle(lane % 32)) << 4));
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) s[kb] = mfma32<kF16>(q, k[kb][st], s[kb]);
@@ -323,7 +338,7 @@ extern "C" int klc_attn_key_weights(const klc_attn_key_weights_args* args, void*
   auto index = [](const void* v) { return static_cast<const int32_t*>(v); };
   int page_log2 = 0;
   while ((1 << page_log2) < x.page_size) ++page_log2;
-  const KeyWeightArgs a{in(x.q), static_cast<const float*>(x.lse), in(x.k_pages), index(x.tables), index(x.lengths),
+  const KeyWeightArgs a{in(x.q), static_cast<const float*>(x.lse), in(x.k_pages), in(x.k_pages), index(x.tables), index(x.lengths),
                         index(x.plan), index(x.rows), static_cast<float*>(x.weights), static_cast<double*>(x.workspace), x.q_stride, x.capacity, (int)x.n_seq,
                         (int)x.n_rows, (int)x.n_heads, (int)x.n_kv, (int)d, (int)x.n_pages, page_log2, (int)x.table_width,
                         (int)x.window, (int)x.first, (int)((keys + kBlockKeys - 1) / kBlockKeys), (int)parts, (float)(x.scale * kLog2e)};
