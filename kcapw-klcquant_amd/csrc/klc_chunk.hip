@@ -10,10 +10,23 @@
 // sequence and a part of the keys that they see.
 //   wide    more than 64 rows: 4 waves x 32 rows over one ring of tiles
 //   pairs   33 to 64 rows, head sizes up to 64: the same of 2 pairs of waves,
-//           of half the keys each, which join in LDS
-//   narrow  up to 32 rows (past head size 64 wide has the others): each wave takes every fourth tile through a ring of
-//           its own, with no barrier, and the waves join in LDS
+//           of half the keys each, which join in LDS (past 64 wide has them)
+//   narrow  up to 32 rows: each wave takes every fourth tile through a ring
+//           of its own, with no barrier, and the waves join in LDS
 // Rows whose keys are in parts leave float32 sums, which a second launch joins.
+// As in the prompt's kernel a row with a NaN or infinity that may come from a
+// value it must not see is computed again, token by token.
+//
+// What bounds it (64 heads over 8 of size 64 unless said): wide items by LDS
+// reads, 96 bytes a clock of the 128 it has with three workgroups a CU, and
+// the exponentials.  6,000 tokens over 2,000 beside 64 steps, 584 us (0.84
+// PFLOP/s), 8,192 over none 638 (0.86; 64 rows a wave, half the reads at two
+// waves a SIMD: 673 and 677 on one box), 2,000 over 16,000 of 32 heads of size
+// 128 575 (0.97).  Twelve suffixes of 50 to 100 over 2,000 to 4,000 take 84,
+// 464 items on 256 CUs, each waiting for itself.  Steps by HBM: 200 of a
+// window of 1,024 and 4 first tokens 92 us (4.6 TB/s), 256 of 2,000 155 (5.1);
+// eight of 700 keys take 12, the chain of item, length, page numbers and six
+// tiles a wave.
 #include <math.h>
 
 #include <algorithm>
@@ -31,7 +44,8 @@ constexpr int kNarrowRows = 32;
 __host__ __device__ constexpr int pair_rows(int dim) { return dim <= 64 ? 64 : kNarrowRows; }
 constexpr int kJoinRows = 16;    // of one workgroup
 constexpr int kRecord = 8;       // int32 of an item and of a join
-// LDS of a workgroup: three fit a CU, past head size 64 two
+// LDS of a workgroup: three fit a CU, past head size 64 two (with two of size 64 6,000 tokens beside 64 steps take 700 us,
+// with three 647)
 template <int DP>
 constexpr int kChunkLds = (DP == 64 ? 48 : 64) * 1024;
 

@@ -11,6 +11,11 @@
 // workgroup: a lane has 16 rows of its one key, so that the sums over rows
 // never leave it but at the end.  Long chunks' rows go to several workgroups,
 // whose float64 sums a second launch adds in their order.
+//
+// What bounds it (64 heads over 8 of size 64): the exponentials and the two
+// instructions beside each, 46 us of the 67 that 1,000 tokens over 4,000 take,
+// 164 for a prompt of 4,096; steps by memory, 64 of 1,000 to 2,000 keys in 30
+// us (3.5 TB/s), and the start and end of a workgroup for 256 keys.
 #include <math.h>
 
 #include <algorithm>
