@@ -221,3 +221,11 @@ def test_workspace_sizes():
     for bad in ((0, 1, 8, 2, 10), (1, 0, 8, 2, 10), (5, 6, 8, 2, 10), (5, 1, 8, 3, 10), (5, 1, 8, 2, -1)):
         assert size(*bad) == nat.KLC_ERR_ARGUMENT
     assert ctypes.sizeof(ctypes.c_void_p) == 8
+
+
+def test_one_long_sequence_among_many_is_cut():
+    """Whatever the others are: the longest keys set the time of a plan that leaves them whole."""
+    lengths = [200 + 6 * i for i in range(127)] + [32000]
+    sizes, out = plan([1] * 128, lengths)
+    splits = {int(x[0]): int(x[6]) for x in out[sizes[2]:sizes[4]].reshape(-1, 8)}
+    assert splits[127] >= 8 and max(splits[s] for s in range(127)) == 1

@@ -148,6 +148,12 @@ def test_keys_in_parts(gpu, heads, kv, dim, dtype, counts, keys):
     c.check_weights(lse)
 
 
+def test_one_long_sequence_among_many(gpu):
+    c = Case(gpu, "fp16", 8, 8, 64, 64, [1] * 130, [100 + i for i in range(129)] + [20000])
+    assert 0 < c.plan.joins < 130
+    _, lse = c.check(only=(0, 64, 128, 129))
+
+
 def test_a_fused_projection_and_out(gpu):
     c = Case(gpu, "fp16", 16, 4, 64, 16, [5, 1, 90], [60, 200, 91], fused=True)
     assert not c.q.is_contiguous()
