@@ -595,9 +595,10 @@ int klc_attn_batch(const klc_attn_batch_args* args, void* stream);
  * reach it, NaN and infinities included.
  *
  * klc_attn_plan, on the host, divides the work by HOST arrays counts and
- * lengths (int32 [n_seq]): sizes [8] receives {int32 values of the plan,
- * tokens, at_items, items, at_joins, joins, part_rows, workspace bytes}, and
- * plan its values if capacity holds them (NULL and 0 to ask).  It begins with
+ * lengths (int32 [n_seq]): sizes [12] receives {int32 values of the plan,
+ * tokens, at_items, items, at_joins, joins, part_rows, workspace bytes} and, for
+ * klc_attn_key_weights, {at_items, items, joins, parts}, and plan its values if
+ * capacity holds them (NULL and 0 to ask).  It begins with
  * the int32 [n_seq + 1] starts of the sequences' rows.  The call takes a copy
  * of it on the device, the sizes and the heads, window and first that it was
  * made for.  counts are the plan's; `lengths` is read on the device, and
@@ -623,21 +624,18 @@ int klc_attn_chunk(const klc_attn_chunk_args* args, void* stream);
  * query heads of the KV head of exp(scale * q . k - lse), lse as klc_attn_chunk
  * wrote it for the same q: added for the keys that were there before the new
  * tokens, set for the new ones.  Sums over a call's rows are float64, in the
- * same order every time.  Of the plan the starts are read; plan, window,
- * first, lengths and tables as klc_attn_chunk's, n_heads and n_kv the plan's.  A
- * key in a page outside [0, n_pages), and all of a sequence whose length passes
- * table_width * page_size, gets NaN; keys from capacity on, and sequences whose
- * row is outside [0, n_rows), are left out.  workspace:
- * klc_attn_key_weights_workspace_bytes with max_keys = table_width * page_size
- * (0: none needed), 8-byte aligned, no initialisation, one for calls that may
- * overlap. */
-int64_t klc_attn_key_weights_workspace_bytes(int64_t tokens, int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t max_keys);
+ * same order every time.  plan, window, first, lengths and tables as
+ * klc_attn_chunk's, n_heads and n_kv the plan's.  A key in a page outside [0,
+ * n_pages), and all of a sequence whose length passes table_width * page_size,
+ * gets NaN; keys from capacity on, and sequences whose row is outside [0,
+ * n_rows), are left out.  workspace: 8 * parts * n_kv * table_width * page_size
+ * bytes, 8-byte aligned, no initialisation, one for calls that may overlap. */
 typedef struct klc_attn_key_weights_args {
   const void *q, *lse, *k_pages;
   const void *tables, *lengths, *plan, *rows;
   void *weights, *workspace;
-  int64_t tokens, n_seq, n_rows, capacity, n_heads, n_kv, head_dim, q_stride, n_pages, page_size, table_width, window,
-      first, kv_dtype, workspace_bytes;
+  int64_t at_items, items, joins, parts, n_rows, capacity, n_heads, n_kv, head_dim, q_stride, n_pages, page_size,
+      table_width, window, first, kv_dtype, workspace_bytes;
   double scale;
 } klc_attn_key_weights_args;
 int klc_attn_key_weights(const klc_attn_key_weights_args* args, void* stream);

@@ -145,10 +145,14 @@ struct ChunkRows {
   }
   __device__ __forceinline__ void convert(const ChunkArgs& a) { c2 = a.c2 * convert_query<F, kF16>(f.q[0]); }
   __device__ __forceinline__ void mask(const ChunkArgs& a, int k0, f32x16_t (&s)[1][1]) const {
-    const int first = k0 + 4 * ((int)(threadIdx.x % kWave) / 32);
+    // of the keys from the lane's first one on: up to its row in the window, or below the first tokens' end
+    const int from = k0 + 4 * ((int)(threadIdx.x % kWave) / 32), rel = pos - from, head = min(a.first, pos + 1) - from;
+    const uint32_t reach = a.window > 0 ? a.window : 0x7fffffffu;
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-      if (!sees(a, pos, first + 8 * (e / 4) + e % 4)) s[0][0][e] = -INFINITY;
+    for (int e = 0; e < 16; ++e) {
+      const int off = 8 * (e / 4) + e % 4;
+      if (!((uint32_t)(rel - off) < reach || off < head)) s[0][0][e] = -INFINITY;
+    }
   }
   __device__ __forceinline__ void raise(const f32x16_t (&s)[1]) {
     const float before = f.m[0];
@@ -642,10 +646,18 @@ struct RowTile {
   }
 };
 
+// Of a sequence's rows the part that one workgroup of the key weights' kernel
+// takes by every block of keys.
+struct WeightPart {
+  int seq, part, parts, offset;  // offset: of the first part among those that are joined
+};
+
 struct ChunkPlan {
   std::vector<int32_t> starts;
   std::vector<RowTile> tiles;
   int64_t items = 0, joins = 0, part_rows = 0;
+  std::vector<WeightPart> weights;
+  int64_t weight_joins = 0, weight_parts = 0;
 };
 
 int64_t span_tiles(int64_t p_lo, int64_t p_hi, int64_t window, int64_t first) {
@@ -731,6 +743,30 @@ ChunkPlan chunk_plan(const int32_t* counts, const int32_t* lengths, int64_t n_se
       p.part_rows += (int64_t)t.rows * t.splits;
     }
   }
+  // The key weights' rows: in all eight workgroups a CU, of at least eight tiles of rows.  Parts that are joined come
+  // first, the first of each sequence at the very front.
+  constexpr int64_t kBlock = 256, kTileRows = 32, kLeast = 8;
+  double work = 0.;
+  auto row_tiles = [&](int64_t s) { return (counts[s] * g + kTileRows - 1) / kTileRows; };
+  for (int64_t s = 0; s < n_seq; ++s) work += (double)n_kv * ((lengths[s] + kBlock - 1) / kBlock) * row_tiles(s);
+  const int64_t most = std::max<int64_t>(kLeast, (int64_t)std::ceil(work / (8 * kCus)));
+  std::vector<WeightPart> rest, single;
+  // First tokens beside a window are seen by all rows, their block of keys by far more than the others, which leave
+  // the parts that they have no rows for: 16 tiles a part there, in up to 64 (6,000 tokens over 2,000, a window of 128
+  // and 4 first tokens, 176 us instead of 736).
+  for (int64_t s = 0; s < n_seq; ++s) {
+    int parts = (int)((row_tiles(s) + most - 1) / most);
+    if (first > 0) parts = std::max(parts, (int)std::min<int64_t>((row_tiles(s) + 15) / 16, 64));
+    if (parts == 1) {
+      single.push_back({(int)s, 0, 1, 0});
+      continue;
+    }
+    for (int i = 0; i < parts; ++i) (i == 0 ? p.weights : rest).push_back({(int)s, i, parts, (int)p.weight_parts});
+    p.weight_parts += parts;
+  }
+  p.weight_joins = (int64_t)p.weights.size();
+  p.weights.insert(p.weights.end(), rest.begin(), rest.end());
+  p.weights.insert(p.weights.end(), single.begin(), single.end());
   return p;
 }
 
@@ -775,13 +811,15 @@ extern "C" int klc_attn_plan(const int32_t* counts, const int32_t* lengths, int6
   try {
     const ChunkPlan p = chunk_plan(counts, lengths, n_seq, n_heads, n_kv, head_dim, window, first);
     const int64_t at_items = (n_seq + 1 + kRecord - 1) / kRecord * kRecord, at_joins = at_items + p.items * kRecord;
-    KLC_REQUIRE(p.part_rows < ((int64_t)1 << 31) && p.items * n_kv < ((int64_t)1 << 31) && p.joins * n_kv < ((int64_t)1 << 31),
+    KLC_REQUIRE(p.part_rows < ((int64_t)1 << 31) && p.items * n_kv < kMostBlocks && p.joins * n_kv < kMostBlocks,
                 KLC_ERR_ARGUMENT, "klc_attn_plan: %lld tokens of %lld heads are too many", (long long)tokens, (long long)n_heads);
-    sizes[0] = at_joins + p.joins * kRecord;
+    const int64_t at_weights = at_joins + p.joins * kRecord;
+    sizes[0] = at_weights + (int64_t)p.weights.size() * 4;
     sizes[1] = tokens;
     sizes[2] = at_items, sizes[3] = p.items;
     sizes[4] = at_joins, sizes[5] = p.joins;
     sizes[6] = p.part_rows, sizes[7] = part_bytes(p.part_rows, n_kv, head_dim);
+    sizes[8] = at_weights, sizes[9] = (int64_t)p.weights.size(), sizes[10] = p.weight_joins, sizes[11] = p.weight_parts;
     if (sizes[0] > capacity) return KLC_OK;
     std::fill(plan, plan + at_items, 0);
     std::copy(p.starts.begin(), p.starts.end(), plan);
@@ -799,6 +837,11 @@ extern "C" int klc_attn_plan(const int32_t* counts, const int32_t* lengths, int6
         std::copy(rec, rec + kRecord, join);
       }
       part += (int64_t)t.rows * t.splits;
+    }
+    int32_t* weight = plan + at_weights;
+    for (const WeightPart& w : p.weights) {
+      const int32_t rec[4] = {w.seq, w.part, w.parts, w.offset};
+      weight = std::copy(rec, rec + 4, weight);
     }
   } catch (const std::exception& e) {
     return set_error(KLC_ERR_ARGUMENT, "klc_attn_plan: %s", e.what());
@@ -835,8 +878,8 @@ extern "C" int klc_attn_chunk(const klc_attn_chunk_args* args, void* stream) {
   KLC_REQUIRE(x.kv_dtype == KLC_DTYPE_BF16 || x.kv_dtype == KLC_DTYPE_F16, KLC_ERR_UNSUPPORTED,
               "klc_attn_chunk: kv_dtype %lld (bfloat16 or float16)", (long long)x.kv_dtype);
   const int64_t need = part_bytes(x.part_rows, x.n_kv, d);
-  KLC_REQUIRE(x.items > 0 && x.joins >= 0 && x.part_rows >= 0 && x.items * x.n_kv < ((int64_t)1 << 31) &&
-                  x.joins * x.n_kv < ((int64_t)1 << 31),
+  KLC_REQUIRE(x.items > 0 && x.joins >= 0 && x.part_rows >= 0 && x.items * x.n_kv < kMostBlocks &&
+                  x.joins * x.n_kv < kMostBlocks,
               KLC_ERR_ARGUMENT, "klc_attn_chunk: a plan of %lld items, %lld joins", (long long)x.items, (long long)x.joins);
   KLC_REQUIRE(need == 0 || (x.workspace && x.workspace_bytes >= need), KLC_ERR_ARGUMENT,
               "klc_attn_chunk: workspace of %lld bytes, need %lld", (long long)x.workspace_bytes, (long long)need);

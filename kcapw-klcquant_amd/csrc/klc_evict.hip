@@ -247,7 +247,7 @@ extern "C" int klc_kv_evict(const klc_kv_evict_args* args, void* stream) {
   KLC_REQUIRE(x.pools && x.weights && x.tables && x.lengths && x.rows && x.kept && x.workspace, KLC_ERR_ARGUMENT,
               "klc_kv_evict: null pointer");
   KLC_REQUIRE(x.n_layers > 0 && x.n_seq > 0 && x.n_kv > 0 && x.n_kv <= 4096 && x.head_dim >= 8 && x.head_dim % 8 == 0 &&
-                  x.head_dim <= 128 && x.n_layers * x.n_seq * x.n_kv < ((int64_t)1 << 31),
+                  x.head_dim <= 128 && x.n_layers * x.n_seq * x.n_kv < ((int64_t)1 << 32) / kEvictThreads,
               KLC_ERR_SHAPE, "klc_kv_evict: %lld layers, %lld sequences, %lld KV heads, head_dim %lld (8..128, multiple of 8)",
               (long long)x.n_layers, (long long)x.n_seq, (long long)x.n_kv, (long long)x.head_dim);
   KLC_REQUIRE(x.page_size >= 16 && x.page_size <= 4096 && (x.page_size & (x.page_size - 1)) == 0 && x.n_pages > 0 &&

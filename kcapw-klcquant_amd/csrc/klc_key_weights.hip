@@ -10,12 +10,13 @@
 // rows come past in tiles of 32 through LDS, for the four waves of a
 // workgroup: a lane has 16 rows of its one key, so that the sums over rows
 // never leave it but at the end.  Long chunks' rows go to several workgroups,
-// whose float64 sums a second launch adds in their order.
+// as many as the plan says, whose float64 sums a second launch adds in their
+// order.
 //
 // What bounds it (64 heads over 8 of size 64): the exponentials and the two
-// instructions beside each, 46 us of the 67 that 1,000 tokens over 4,000 take,
-// 164 for a prompt of 4,096; steps by memory, 64 of 1,000 to 2,000 keys in 30
-// us (3.5 TB/s), and the start and end of a workgroup for 256 keys.
+// instructions beside each, 46 us of the 66 that 1,000 tokens over 4,000 take,
+// 164 for a prompt of 4,096; steps by memory, 64 of 1,000 to 2,000 keys in 26
+// us (4.0 TB/s), and the start and end of a workgroup for 256 keys.
 #include <math.h>
 
 #include <algorithm>
@@ -28,6 +29,7 @@ namespace {
 constexpr int kWaveKeys = 64;
 constexpr int kBlockKeys = kWaves * kWaveKeys;
 constexpr int kRows = 32;  // of a tile
+constexpr int kPartTiles = 8;
 
 struct KeyWeightArgs {
   const uint16_t* q;                // bfloat16 [tokens] rows
@@ -35,10 +37,11 @@ struct KeyWeightArgs {
   const uint16_t *k_pages, *v_pages;  // [n_pages][page][n_kv][d]; values are not read
   const int32_t *tables, *lengths;  // [n_seq][width], [n_seq]
   const int32_t *starts, *rows;     // [n_seq + 1], [n_seq]
+  const int32_t* items;             // of the plan: sequence, part of its rows, parts, its first part among the joined
   float* weights;                   // [n_rows][n_kv][capacity]
-  double* part;                     // [parts][n_seq][n_kv][width * page], parts > 1
+  double* part;                     // [parts][n_kv][width * page]
   int64_t q_stride, capacity;
-  int n_seq, n_rows, n_heads, n_kv, d, n_pages, page_log2, width, window, first, blocks, parts;
+  int n_rows, n_heads, n_kv, d, n_pages, page_log2, width, window, first, blocks;
   float c2;
 };
 
@@ -54,6 +57,11 @@ struct BlockRows {
     const int t_hi = a.window > 0 && b0 >= a.first ? (int)min((int64_t)count - 1, (int64_t)last + a.window - 1 - base) : count - 1;
     row0 = t_lo * g;
     row_end = b0 < n ? (t_hi + 1) * g : 0;
+  }
+  // rows of a part, in whole tiles: one part is not cut, others have at least kPartTiles
+  __device__ __forceinline__ int per(int parts) const {
+    const int tiles = (row_end - row0 + kRows - 1) / kRows;
+    return (parts == 1 ? tiles : max((tiles + parts - 1) / parts, kPartTiles)) * kRows;
   }
 };
 
@@ -74,10 +82,12 @@ __global__ __launch_bounds__(kWave * kWaves, DP == 64 ? 4 : 2) void key_weights_
   __shared__ __align__(16) float factor[2][kRows], log_norm[2][kRows];
   __shared__ __align__(16) int place[2][kRows];
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), half = lane / 32;
-  int i = blockIdx.x;
-  const int kvh = i % a.n_kv, block = i / a.n_kv % a.blocks;
-  i /= a.n_kv * a.blocks;
-  const int part = i % a.parts, seq = i / a.parts;
+  // Each record's blocks begin one further on, or where blocks and CUs agree in number, one CU would have all parts of
+  // the block that has most rows (6,000 tokens over 2,000, a window of 128 and 4 first tokens, 176 us instead of 273).
+  const int list = blockIdx.x / a.n_kv, item = list / a.blocks;
+  const int kvh = blockIdx.x % a.n_kv, block = (list + item) % a.blocks;
+  const int32_t* rec = a.items + (int64_t)item * 4;
+  const int seq = table_at(rec, 0), part = table_at(rec, 1), parts = table_at(rec, 2), offset = table_at(rec, 3);
   const int begin = table_at(a.starts, seq), count = table_at(a.starts, seq + 1) - begin;
   const int64_t room = (int64_t)a.width << a.page_log2;
   const int asked = table_at(a.lengths, seq), n = (int)min((int64_t)max(asked, 0), room), out_row = table_at(a.rows, seq);
@@ -85,8 +95,8 @@ __global__ __launch_bounds__(kWave * kWaves, DP == 64 ? 4 : 2) void key_weights_
   const BlockRows rows(a, count, n, b0);
   if (rows.row0 >= rows.row_end || (unsigned)out_row >= (unsigned)a.n_rows) return;
   const int g = a.n_heads / a.n_kv, base = rows.base, b1 = rows.last;
-  // this part of the rows, in whole tiles
-  const int per = (rows.row_end - rows.row0 + kRows * a.parts - 1) / (kRows * a.parts) * kRows;
+  const int per = rows.per(parts);
+  if (part * (int64_t)per >= rows.row_end - rows.row0) return;  // the others have all its rows
   const int r_lo = rows.row0 + part * per, r_end = min(r_lo + per, rows.row_end);
 
   // rows of a tile to LDS, by all threads: chunk threadIdx % kChunks of every kPassRows-th row
@@ -150,35 +160,34 @@ __global__ __launch_bounds__(kWave * kWaves, DP == 64 ? 4 : 2) void key_weights_
   bool bad[2];
   double total[2] = {0., 0.};
   const int k_lo = b0 + wave * kWaveKeys, key0 = k_lo + lane % 32;
-  if (r_lo < r_end) {
-    fetch();
-    // the wave's keys, whole rows at a time: read by the lanes that need them, 32 bytes of a row an instruction, 200
-    // steps of 1,500 keys take 70 us instead of 64
-    const int32_t* table = a.tables + (int64_t)seq * a.width;
-    PageLoads<KeyWeightArgs, F, kStageKeys, kStageKeys / F::kRowsPerDma, 1> pages(a, 0, kvh);
-    pages.hold(table, min(k_lo, b1) >> a.page_log2, a.width);
-    const lds_u8 mine = (lds_u8)lds + wave * kWaveBytes;
+  fetch();
+  // the wave's keys, whole rows at a time: read by the lanes that need them, 32 bytes of a row an instruction, 200
+  // steps of 1,500 keys take 70 us instead of 64
+  const int32_t* table = a.tables + (int64_t)seq * a.width;
+  PageLoads<KeyWeightArgs, F, kStageKeys, kStageKeys / F::kRowsPerDma, 1> pages(a, 0, kvh);
+  pages.hold(table, min(k_lo, b1) >> a.page_log2, a.width);
+  const lds_u8 mine = (lds_u8)lds + wave * kWaveBytes;
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      if (kb * 32 % kStageKeys == 0) {
-        tile_wait<63, false>();  // the keys before them have been read
-        pages.template load<true, false>(k_lo + 32 * kb, within(0, b1), mine, mine);
-        tile_wait<0, false>();
-      }
-#pragma unroll
-      for (int st = 0; st < F::kSteps; ++st) {
-        k[kb][st] = u32x4_t{0, 0, 0, 0};
-        if (kFull || 16 * st + 8 * half < a.d)
-          k[kb][st] = *reinterpret_cast<const u32x4_t*>(lds + wave * kWaveBytes + (32 * kb % kStageKeys + lane % 32) * F::kRowBytes +
-                                                        (((2 * st + half) ^ F::swizzle(lane % 32)) << 4));
-      }
-      bad[kb] = (unsigned)table[min(key0 + 32 * kb, b1) >> a.page_log2] >= (unsigned)a.n_pages || asked > room;
+  for (int kb = 0; kb < 2; ++kb) {
+    if (kb * 32 % kStageKeys == 0) {
+      tile_wait<63, false>();  // the keys before them have been read
+      pages.template load<true, false>(k_lo + 32 * kb, within(0, b1), mine, mine);
+      tile_wait<0, false>();
     }
-    __syncthreads();  // the keys have been read
-    put(0, r_lo);
-    __syncthreads();
+#pragma unroll
+    for (int st = 0; st < F::kSteps; ++st) {
+      k[kb][st] = u32x4_t{0, 0, 0, 0};
+      if (kFull || 16 * st + 8 * half < a.d)
+        k[kb][st] = *reinterpret_cast<const u32x4_t*>(lds + wave * kWaveBytes + (32 * kb % kStageKeys + lane % 32) * F::kRowBytes +
+                                                      (((2 * st + half) ^ F::swizzle(lane % 32)) << 4));
+    }
+    bad[kb] = (unsigned)table[min(key0 + 32 * kb, b1) >> a.page_log2] >= (unsigned)a.n_pages || asked > room;
   }
+  __syncthreads();  // the keys have been read
+  put(0, r_lo);
+  __syncthreads();
   int slot = 0;
+  const uint32_t reach = a.window > 0 ? a.window : 0x7fffffffu;
   // tokens of the tile's first and last row, and their heads
   int first_tok = r_lo / g, first_head = r_lo - first_tok * g, last_tok = (r_lo + kRows - 1) / g, last_head = r_lo + kRows - 1 - last_tok * g;
   auto move_on = [&](int& t, int& h) {
@@ -204,6 +213,8 @@ __global__ __launch_bounds__(kWave * kWaves, DP == 64 ? 4 : 2) void key_weights_
     // whole: its rows see all keys of the wave
     const bool whole = row0 + kRows <= r_end && k_lo + kWaveKeys - 1 <= base + first_tok &&
                        (a.window == 0 || k_lo > base + last_tok - a.window);
+    // none: no row of it sees one
+    const bool none = k_lo > base + last_tok || (a.window > 0 && k_lo + kWaveKeys - 1 <= base + first_tok - a.window && k_lo >= a.first);
     float sum[2] = {0.f, 0.f};
     // the weights of the lane's rows 8 q4 on, four of each key
     auto weigh = [&](int q4, f32x4_t (&p)[2]) {
@@ -224,7 +235,7 @@ __global__ __launch_bounds__(kWave * kWaves, DP == 64 ? 4 : 2) void key_weights_
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) sum[kb] += (p[kb][0] + p[kb][1]) + (p[kb][2] + p[kb][3]);
       }
-    } else {
+    } else if (!none) {
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
         if (row0 + 8 * q4 >= r_end) break;
@@ -236,7 +247,9 @@ __global__ __launch_bounds__(kWave * kWaves, DP == 64 ? 4 : 2) void key_weights_
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb) {
             const int key = key0 + 32 * kb;
-            if (key > pos || (a.window > 0 && key <= pos - a.window && key >= a.first)) p[kb][e] = 0.f;
+            bool seen = (uint32_t)(pos - key) < reach;
+            if (k_lo < a.first) seen = seen || (key < a.first && key <= pos);
+            if (!seen) p[kb][e] = 0.f;
           }
         }
 #pragma unroll
@@ -254,40 +267,45 @@ __global__ __launch_bounds__(kWave * kWaves, DP == 64 ? 4 : 2) void key_weights_
   double sum = half == 0 ? total[0] : total[1];
   const int own = k_lo + lane;
   if (own > b1) return;
-  if (r_lo < r_end && (half == 0 ? bad[0] : bad[1])) sum = (double)__uint_as_float(0x7fc00000u);
-  if (a.parts > 1)
-    a.part[(((int64_t)part * a.n_seq + seq) * a.n_kv + kvh) * room + own] = sum;
+  if (half == 0 ? bad[0] : bad[1]) sum = (double)__uint_as_float(0x7fc00000u);
+  if (parts > 1)
+    a.part[((int64_t)(offset + part) * a.n_kv + kvh) * room + own] = sum;
   else
     write_weight(a, out_row, kvh, own, base, sum);
 }
 
 // The parts' sums of one key a thread, in their order.
 __global__ __launch_bounds__(kBlockKeys) void key_weights_join_kernel(KeyWeightArgs a) {
-  int i = blockIdx.x;
-  const int kvh = i % a.n_kv, block = i / a.n_kv % a.blocks, seq = i / (a.n_kv * a.blocks);
+  const int i = blockIdx.x, kvh = i % a.n_kv, block = i / a.n_kv % a.blocks;
+  const int32_t* rec = a.items + (int64_t)(i / (a.n_kv * a.blocks)) * 4;
+  const int seq = table_at(rec, 0), parts = table_at(rec, 2), offset = table_at(rec, 3);
   const int count = table_at(a.starts, seq + 1) - table_at(a.starts, seq), out_row = table_at(a.rows, seq);
   const int64_t room = (int64_t)a.width << a.page_log2;
   const int n = (int)min((int64_t)max(table_at(a.lengths, seq), 0), room), key = block * kBlockKeys + (int)threadIdx.x;
   const BlockRows rows(a, count, n, block * kBlockKeys);
   if (rows.row0 >= rows.row_end || (unsigned)out_row >= (unsigned)a.n_rows || key > rows.last) return;
+  const int per = rows.per(parts), held = min(parts, (rows.row_end - rows.row0 + per - 1) / per);
+  const double* part = a.part + ((int64_t)offset * a.n_kv + kvh) * room + key;
   double sum = 0.;
-  for (int p = 0; p < a.parts; ++p) sum += a.part[(((int64_t)p * a.n_seq + seq) * a.n_kv + kvh) * room + key];
+  constexpr int kAhead = 8;
+  for (int p = 0; p < held; p += kAhead) {
+    double x[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) x[i] = part[(int64_t)min(p + i, held - 1) * a.n_kv * room];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (p + i < held) sum += x[i];
+  }
   write_weight(a, out_row, kvh, key, rows.base, sum);
 }
 
-// Parts of the rows: enough workgroups for two rounds of the chip, of at least eight tiles each.
-int64_t key_weight_parts(int64_t tokens, int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t keys) {
-  const int64_t tiles = tokens / n_seq * (n_heads / n_kv) / kRows, wgs = n_seq * n_kv * ((keys + kBlockKeys - 1) / kBlockKeys);
-  return std::max<int64_t>(1, std::min(tiles / 8, (2048 + wgs - 1) / std::max<int64_t>(wgs, 1)));
-}
-
 template <int DP, bool kF16, bool kFull>
-int launch_key_weights(const KeyWeightArgs& a, hipStream_t st) {
-  const int64_t joins = (int64_t)a.n_seq * a.blocks * a.n_kv;
-  key_weights_kernel<DP, kF16, kFull><<<(unsigned)(joins * a.parts), kWave * kWaves, 0, st>>>(a);
+int launch_key_weights(const KeyWeightArgs& a, int64_t items, int64_t joins, hipStream_t st) {
+  const int64_t lists = (int64_t)a.blocks * a.n_kv;
+  key_weights_kernel<DP, kF16, kFull><<<(unsigned)(items * lists), kWave * kWaves, 0, st>>>(a);
   const int rc = check_launch("key_weights_kernel");
-  if (rc || a.parts == 1) return rc;
-  key_weights_join_kernel<<<(unsigned)joins, kBlockKeys, 0, st>>>(a);
+  if (rc || joins == 0) return rc;
+  key_weights_join_kernel<<<(unsigned)(joins * lists), kBlockKeys, 0, st>>>(a);
   return check_launch("key_weights_join_kernel");
 }
 
@@ -295,15 +313,6 @@ int launch_key_weights(const KeyWeightArgs& a, hipStream_t st) {
 }  // namespace klc
 
 using namespace klc;
-
-extern "C" int64_t klc_attn_key_weights_workspace_bytes(int64_t tokens, int64_t n_seq, int64_t n_heads, int64_t n_kv, int64_t max_keys) {
-  KLC_REQUIRE(n_seq > 0 && tokens >= n_seq && n_kv > 0 && n_heads > 0 && n_heads % n_kv == 0 && max_keys >= 0 &&
-                  max_keys < ((int64_t)1 << 29) && n_seq < ((int64_t)1 << 20) && tokens < ((int64_t)1 << 30) && n_heads <= 4096,
-              KLC_ERR_ARGUMENT, "klc_attn_key_weights_workspace_bytes: %lld tokens of %lld sequences, heads %lld / %lld, %lld keys",
-              (long long)tokens, (long long)n_seq, (long long)n_heads, (long long)n_kv, (long long)max_keys);
-  const int64_t parts = key_weight_parts(tokens, n_seq, n_heads, n_kv, max_keys);
-  return parts == 1 ? 0 : 8 * parts * n_seq * n_kv * max_keys;
-}
 
 extern "C" int klc_attn_key_weights(const klc_attn_key_weights_args* args, void* stream) {
   KLC_REQUIRE(args != nullptr, KLC_ERR_ARGUMENT, "klc_attn_key_weights: null pointer");
@@ -319,11 +328,14 @@ extern "C" int klc_attn_key_weights(const klc_attn_key_weights_args* args, void*
                   x.table_width < ((int64_t)1 << 25) && x.table_width * x.page_size < ((int64_t)1 << 29),
               KLC_ERR_SHAPE, "klc_attn_key_weights: %lld pages of %lld tokens (a power of two, 16..4096), tables of %lld",
               (long long)x.n_pages, (long long)x.page_size, (long long)x.table_width);
-  KLC_REQUIRE(x.n_seq > 0 && x.n_seq < ((int64_t)1 << 20) && x.tokens >= x.n_seq && x.tokens * (x.n_heads / x.n_kv) < ((int64_t)1 << 30) &&
-                  x.n_rows > 0 && x.n_rows < ((int64_t)1 << 31) && x.capacity > 0 && x.capacity < ((int64_t)1 << 31) &&
-                  x.n_seq * x.n_kv * (x.table_width * x.page_size / kBlockKeys + 1) < ((int64_t)1 << 28),
-              KLC_ERR_ARGUMENT, "klc_attn_key_weights: %lld tokens of %lld sequences, %lld rows of %lld weights", (long long)x.tokens,
-              (long long)x.n_seq, (long long)x.n_rows, (long long)x.capacity);
+  KLC_REQUIRE(x.page_size * x.n_kv * d < ((int64_t)1 << 30), KLC_ERR_SHAPE,
+              "klc_attn_key_weights: pages of %lld tokens of %lld x %lld (below 2 GiB)", (long long)x.page_size, (long long)x.n_kv,
+              (long long)d);
+  KLC_REQUIRE(x.n_rows > 0 && x.n_rows < ((int64_t)1 << 31) && x.capacity > 0 && x.capacity < ((int64_t)1 << 31) && x.items > 0 &&
+                  x.joins >= 0 && x.joins <= x.items && x.parts >= 0 && x.parts <= x.items &&
+                  x.items < kMostBlocks && x.items * x.n_kv * (x.table_width * x.page_size / kBlockKeys + 1) < kMostBlocks,
+              KLC_ERR_ARGUMENT, "klc_attn_key_weights: a plan of %lld items, %lld joins, %lld parts; %lld rows of %lld weights",
+              (long long)x.items, (long long)x.joins, (long long)x.parts, (long long)x.n_rows, (long long)x.capacity);
   KLC_REQUIRE(x.q_stride >= x.n_heads * d && x.q_stride % 8 == 0, KLC_ERR_SHAPE,
               "klc_attn_key_weights: q stride %lld (a multiple of 8, no overlap)", (long long)x.q_stride);
   KLC_REQUIRE(((uintptr_t)x.q | (uintptr_t)x.k_pages) % 16 == 0 && ((uintptr_t)x.lse | (uintptr_t)x.weights) % 4 == 0, KLC_ERR_ARGUMENT,
@@ -335,8 +347,7 @@ extern "C" int klc_attn_key_weights(const klc_attn_key_weights_args* args, void*
   KLC_REQUIRE(x.kv_dtype == KLC_DTYPE_BF16 || x.kv_dtype == KLC_DTYPE_F16, KLC_ERR_UNSUPPORTED,
               "klc_attn_key_weights: kv_dtype %lld (bfloat16 or float16)", (long long)x.kv_dtype);
   if (x.table_width == 0) return KLC_OK;  // no key
-  const int64_t keys = x.table_width * x.page_size, parts = key_weight_parts(x.tokens, x.n_seq, x.n_heads, x.n_kv, keys);
-  const int64_t need = parts == 1 ? 0 : 8 * parts * x.n_seq * x.n_kv * keys;
+  const int64_t keys = x.table_width * x.page_size, need = 8 * x.parts * x.n_kv * keys;
   KLC_REQUIRE(need == 0 || (x.workspace && (uintptr_t)x.workspace % 8 == 0 && x.workspace_bytes >= need), KLC_ERR_ARGUMENT,
               "klc_attn_key_weights: workspace of %lld bytes, need %lld, 8-byte aligned", (long long)x.workspace_bytes, (long long)need);
   auto in = [](const void* v) { return static_cast<const uint16_t*>(v); };
@@ -344,13 +355,13 @@ extern "C" int klc_attn_key_weights(const klc_attn_key_weights_args* args, void*
   int page_log2 = 0;
   while ((1 << page_log2) < x.page_size) ++page_log2;
   const KeyWeightArgs a{in(x.q), static_cast<const float*>(x.lse), in(x.k_pages), in(x.k_pages), index(x.tables), index(x.lengths),
-                        index(x.plan), index(x.rows), static_cast<float*>(x.weights), static_cast<double*>(x.workspace), x.q_stride, x.capacity, (int)x.n_seq,
-                        (int)x.n_rows, (int)x.n_heads, (int)x.n_kv, (int)d, (int)x.n_pages, page_log2, (int)x.table_width,
-                        (int)x.window, (int)x.first, (int)((keys + kBlockKeys - 1) / kBlockKeys), (int)parts, (float)(x.scale * kLog2e)};
+                        index(x.plan), index(x.rows), index(x.plan) + x.at_items, static_cast<float*>(x.weights),
+                        static_cast<double*>(x.workspace), x.q_stride, x.capacity, (int)x.n_rows, (int)x.n_heads, (int)x.n_kv, (int)d, (int)x.n_pages, page_log2, (int)x.table_width,
+                        (int)x.window, (int)x.first, (int)((keys + kBlockKeys - 1) / kBlockKeys), (float)(x.scale * kLog2e)};
   const hipStream_t st = as_stream(stream);
   const bool f16 = x.kv_dtype == KLC_DTYPE_F16;
-  if (d == 64) return f16 ? launch_key_weights<64, true, true>(a, st) : launch_key_weights<64, false, true>(a, st);
-  if (d == 128) return f16 ? launch_key_weights<128, true, true>(a, st) : launch_key_weights<128, false, true>(a, st);
-  if (d < 64) return f16 ? launch_key_weights<64, true, false>(a, st) : launch_key_weights<64, false, false>(a, st);
-  return f16 ? launch_key_weights<128, true, false>(a, st) : launch_key_weights<128, false, false>(a, st);
+  if (d == 64) return f16 ? launch_key_weights<64, true, true>(a, x.items, x.joins, st) : launch_key_weights<64, false, true>(a, x.items, x.joins, st);
+  if (d == 128) return f16 ? launch_key_weights<128, true, true>(a, x.items, x.joins, st) : launch_key_weights<128, false, true>(a, x.items, x.joins, st);
+  if (d < 64) return f16 ? launch_key_weights<64, true, false>(a, x.items, x.joins, st) : launch_key_weights<64, false, false>(a, x.items, x.joins, st);
+  return f16 ? launch_key_weights<128, true, false>(a, x.items, x.joins, st) : launch_key_weights<128, false, false>(a, x.items, x.joins, st);
 }

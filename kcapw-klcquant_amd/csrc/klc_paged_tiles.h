@@ -7,6 +7,7 @@
 namespace klc {
 
 constexpr int kWaves = 4;             // of a workgroup
+constexpr int64_t kMostBlocks = 1 << 24;  // of a launch: its threads are counted in 32 bits
 constexpr int kKeys = 32;             // that a wave takes at once
 constexpr int kTileLds = 64 * 1024;   // for a workgroup's tiles: two workgroups fit a CU
 // keys of the tiles that a workgroup's waves share: 16 KB of K and V

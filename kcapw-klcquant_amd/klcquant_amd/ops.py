@@ -298,7 +298,7 @@ _APPEND_ARGS = struct.Struct("=11Q10q")
 _BATCH_ARGS = struct.Struct("=9Q12qd")
 _CHUNK_ARGS = struct.Struct("=10Q16qd")
 _NORM_ARGS = struct.Struct("=2Qd")  # behind an append's
-_WEIGHT_ARGS = struct.Struct("=9Q15qd")
+_WEIGHT_ARGS = struct.Struct("=9Q17qd")
 _EVICT_ARGS = struct.Struct("=7Q13q")
 _batch_bytes: dict = {}  # sizes -> klc_attn_batch's workspace bytes
 
@@ -602,10 +602,10 @@ class AttentionPlan:
         self.data = data  # int32: the sequences' starts among the rows, items, joins
         self.device = data.device
         (_, self.tokens, self.at_items, self.items, self.at_joins, self.joins, self.part_rows,
-         self.workspace_bytes) = (int(x) for x in sizes)
+         self.workspace_bytes, self.at_weights, self.weight_items, self.weight_joins,
+         self.weight_parts) = (int(x) for x in sizes)
         self.n_seq, self.n_heads, self.n_kv, self.head_dim = shape
         self.window, self.first = window, first
-        self.weight_bytes: dict = {}  # keys of the tables -> klc_attn_key_weights' workspace bytes
 
     @property
     def starts(self) -> torch.Tensor:
@@ -617,7 +617,7 @@ def attention_plan(counts, lengths, n_heads: int, n_kv: int, head_dim: int, wind
                    device: torch.device | str = "cuda") -> AttentionPlan:
     """The plan of a batch (klc_attn_plan) for :func:`chunk_attention` and :func:`add_key_weights`, on the host from the
     sequences' ``counts`` of new tokens and ``lengths``, the keys up to and with them (sequences of whole numbers; one
-    copy to ``device``).  Made once for all layers of a kind: ``window`` and ``first`` (tokens at the start that stay
+    copy to ``device``, on its current stream: calls on other streams have to wait for it).  Made once for all layers of a kind: ``window`` and ``first`` (tokens at the start that stay
     visible beside it) are the layers'."""
     counts, lengths = (np.asarray(x) for x in (counts, lengths))
     if counts.ndim != 1 or counts.shape != lengths.shape or counts.size == 0:
@@ -639,7 +639,7 @@ def attention_plan(counts, lengths, n_heads: int, n_kv: int, head_dim: int, wind
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("a plan cannot be made while a graph is captured: make it before")
     counts, lengths = (np.ascontiguousarray(x, dtype=np.int32) for x in (counts, lengths))
-    sizes = np.zeros(8, np.int64)
+    sizes = np.zeros(12, np.int64)
     room = 64 * (counts.size + 64)
     while True:
         host = torch.empty(room, dtype=torch.int32, pin_memory=True)
@@ -730,17 +730,14 @@ def add_key_weights(q: torch.Tensor, lse: torch.Tensor, k_pages: torch.Tensor, t
     if n_kv != plan.n_kv:
         raise ValueError(f"weights of {n_kv} KV heads for {plan.n_kv}")
     _, _, scale = _check_heads(None, plan.n_heads, n_kv, None, scale, plan.head_dim, dev)
-    nbytes = plan.weight_bytes.get(width * page)
-    if nbytes is None:
-        nbytes = plan.weight_bytes[width * page] = nat.call("klc_attn_key_weights_workspace_bytes", plan.tokens, plan.n_seq,
-                                                            plan.n_heads, n_kv, width * page)
+    nbytes = 8 * plan.weight_parts * n_kv * width * page
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None  # of this call alone
     _call("klc_attn_key_weights",
           _WEIGHT_ARGS.pack(q.data_ptr(), lse.data_ptr(), k_pages.data_ptr(), tables.data_ptr() if width else 0,
                             lengths.data_ptr(), plan.data.data_ptr(), rows.data_ptr(), weights.data_ptr(),
-                            workspace.data_ptr() if nbytes else 0, plan.tokens, plan.n_seq, n_rows, capacity,
-                            plan.n_heads, n_kv, plan.head_dim, stride, n_pages, page, width, plan.window,
-                            plan.first, _KV_CODES[k_pages.dtype], nbytes, scale), dev)
+                            workspace.data_ptr() if nbytes else 0, plan.at_weights, plan.weight_items, plan.weight_joins,
+                            plan.weight_parts, n_rows, capacity, plan.n_heads, n_kv, plan.head_dim, stride, n_pages, page,
+                            width, plan.window, plan.first, _KV_CODES[k_pages.dtype], nbytes, scale), dev)
 
 
 def evict_keys(pools: torch.Tensor, weights: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor,

@@ -3,7 +3,6 @@ work (no GPU)."""
 
 from __future__ import annotations
 
-import ctypes
 import random
 import struct
 
@@ -16,7 +15,7 @@ from klcquant_amd import ops
 
 def plan(counts, lengths, heads=64, kv=8, dim=64, window=0, first=0, capacity=1 << 18):
     counts, lengths = np.array(counts, np.int32), np.array(lengths, np.int32)
-    sizes, out = np.zeros(8, np.int64), np.full(capacity, -7, np.int32)
+    sizes, out = np.zeros(12, np.int64), np.full(capacity, -7, np.int32)
     nat.call("klc_attn_plan", counts.ctypes.data, lengths.ctypes.data, len(counts), heads, kv, dim, window, first,
              out.ctypes.data if capacity else None, capacity, sizes.ctypes.data)
     return sizes.tolist(), out
@@ -36,11 +35,12 @@ def test_every_row_and_part_once(seed):
         lengths = [r.choice((r.randint(1, 200), r.randint(1, 20000))) for _ in range(n_seq)]
         counts = [r.choice((1, r.randint(1, min(n, 700)))) for n in lengths]
         window = r.choice((0, 0, r.randint(1, 3000)))
-        (size, tokens, at_items, items, at_joins, joins, part_rows, nbytes), out = plan(
+        (size, tokens, at_items, items, at_joins, joins, part_rows, nbytes, at_weights, w_items, w_joins, w_parts), out = plan(
             counts, lengths, heads, kv, dim, window, r.randint(0, 50) if window else 0)
         starts = np.concatenate(([0], np.cumsum(counts)))
         assert tokens == sum(counts) and out[:n_seq + 1].tolist() == starts.tolist()
-        assert at_items >= n_seq + 1 and at_joins == at_items + 8 * items and size == at_joins + 8 * joins
+        assert at_items >= n_seq + 1 and at_joins == at_items + 8 * items and at_weights == at_joins + 8 * joins
+        assert size == at_weights + 4 * w_items
         assert (out[size:] == -7).all() and nbytes == part_rows * kv * (4 * dim + 16)
         rows, parts, splits_of = set(), {}, {}
         for s, begin, count, row0, n, split, splits, part in out[at_items:at_joins].reshape(-1, 8).tolist():
@@ -58,13 +58,21 @@ def test_every_row_and_part_once(seed):
         assert set(splits_of) == {(s, x) for s in range(n_seq) for x in range(counts[s] * group)}
         assert len(rows) == sum(splits_of.values()) and len(parts) == part_rows
         seen = set()
-        for s, begin, count, row0, n, splits, part, stride in out[at_joins:size].reshape(-1, 8).tolist():
+        for s, begin, count, row0, n, splits, part, stride in out[at_joins:at_weights].reshape(-1, 8).tolist():
             assert begin == starts[s] and count == counts[s] and 0 < n <= 16
             for x in range(n):
                 for p in range(splits):
                     assert parts[part + x + p * stride] == (s, row0 + x, p)
                     seen.add(part + x + p * stride)
         assert seen == set(parts)
+        of, places = {}, []
+        for i, (s, part, n, offset) in enumerate(out[at_weights:size].reshape(-1, 4).tolist()):
+            assert 0 <= part < n <= -(-counts[s] * group // 256) and (i < w_joins) == (n > 1 and part == 0)
+            of.setdefault(s, []).append(part)
+            places += [offset + part] if n > 1 else []
+            assert n == 1 or out[at_weights:size].reshape(-1, 4)[i, 3] == offset
+        assert {s: sorted(x) for s, x in of.items()} == {s: list(range(len(x))) for s, x in of.items()} and len(of) == n_seq
+        assert sorted(places) == list(range(w_parts))
 
 
 def span(keys_a_tile, p_lo, p_hi, window, first):
@@ -170,18 +178,19 @@ def test_chunk_refusals(change):
     refused("klc_attn_chunk", CHUNK, "=10Q16qd", **change)
 
 
-WEIGHTS = dict(q=FAKE, lse=FAKE, k_pages=FAKE, tables=FAKE, lengths=FAKE, plan=FAKE, rows=FAKE, weights=FAKE, workspace=0, tokens=1, n_seq=1,
-               n_rows=1, capacity=64, n_heads=8, n_kv=2, head_dim=64, q_stride=512, n_pages=4, page_size=16, table_width=2, window=0,
-               first=0, kv_dtype=1, workspace_bytes=0, scale=0.125)
+WEIGHTS = dict(q=FAKE, lse=FAKE, k_pages=FAKE, tables=FAKE, lengths=FAKE, plan=FAKE, rows=FAKE, weights=FAKE, workspace=0, at_items=8, items=1,
+               joins=0, parts=0, n_rows=1, capacity=64, n_heads=8, n_kv=2, head_dim=64, q_stride=512, n_pages=4, page_size=16, table_width=2,
+               window=0, first=0, kv_dtype=1, workspace_bytes=0, scale=0.125)
 
 
 @pytest.mark.parametrize("change", [
     dict(q=0), dict(lse=0), dict(k_pages=0), dict(tables=0), dict(lengths=0), dict(plan=0), dict(rows=0), dict(weights=0),
-    dict(q=FAKE + 2), dict(weights=FAKE + 2), dict(tokens=0), dict(n_seq=0), dict(n_seq=2), dict(n_rows=0), dict(capacity=0), dict(n_heads=9),
-    dict(head_dim=12), dict(q_stride=100), dict(page_size=17), dict(n_pages=-1), dict(window=-1), dict(first=3), dict(kv_dtype=5),
-    dict(scale=0.0), dict(tokens=4000, table_width=300), dict(tokens=4000, table_width=300, workspace=FAKE + 4, workspace_bytes=1 << 40)])
+    dict(q=FAKE + 2), dict(weights=FAKE + 2), dict(items=0), dict(joins=-1), dict(joins=2), dict(parts=-1), dict(parts=2), dict(n_rows=0),
+    dict(capacity=0), dict(n_heads=9), dict(head_dim=12), dict(q_stride=100), dict(page_size=17), dict(n_pages=-1), dict(window=-1),
+    dict(first=3), dict(kv_dtype=5), dict(scale=0.0), dict(items=2, parts=2), dict(items=2, parts=2, workspace=FAKE, workspace_bytes=1023),
+    dict(items=2, parts=2, workspace=FAKE + 4, workspace_bytes=1 << 40), dict(items=1 << 31), dict(items=1 << 23), dict(items=1 << 62), dict(n_heads=4096, n_kv=4096, head_dim=128, q_stride=1 << 20, page_size=4096)])
 def test_key_weight_refusals(change):
-    refused("klc_attn_key_weights", WEIGHTS, "=9Q15qd", **change)
+    refused("klc_attn_key_weights", WEIGHTS, "=9Q17qd", **change)
 
 
 EVICT = dict(pools=FAKE, weights=FAKE, tables=FAKE, lengths=FAKE, rows=FAKE, kept=FAKE, workspace=FAKE, n_layers=1, n_seq=1, n_rows=1,
@@ -212,15 +221,6 @@ def test_null_arguments():
     for name in ("klc_attn_chunk", "klc_attn_key_weights", "klc_kv_evict", "klc_kv_norm_append"):
         with pytest.raises(nat.KlcError, match="null pointer"):
             nat.call(name, None, None)
-
-
-def test_workspace_sizes():
-    size = nat.load().klc_attn_key_weights_workspace_bytes
-    assert size(64, 64, 64, 8, 2048) == 0 and size(1000, 1, 64, 8, 5056) > 0
-    assert size(1000, 1, 64, 8, 0) >= 0
-    for bad in ((0, 1, 8, 2, 10), (1, 0, 8, 2, 10), (5, 6, 8, 2, 10), (5, 1, 8, 3, 10), (5, 1, 8, 2, -1)):
-        assert size(*bad) == nat.KLC_ERR_ARGUMENT
-    assert ctypes.sizeof(ctypes.c_void_p) == 8
 
 
 def test_one_long_sequence_among_many_is_cut():

@@ -148,6 +148,15 @@ def test_keys_in_parts(gpu, heads, kv, dim, dtype, counts, keys):
     c.check_weights(lse)
 
 
+@pytest.mark.parametrize("window,first", [(None, 0), (100, 0), (100, 4), (300, 270)])
+def test_weights_of_rows_in_parts(gpu, window, first):
+    """A long chunk beside steps: parts that some blocks of keys have no rows for."""
+    c = Case(gpu, "fp16", 16, 4, 64, 16, [1, 700, 5, 90], [800, 1500, 5, 1000], window, first)
+    assert c.plan.weight_joins > 0 and c.plan.weight_parts > 2 * c.plan.weight_joins
+    _, lse = c.check()
+    c.check_weights(lse)
+
+
 def test_one_long_sequence_among_many(gpu):
     c = Case(gpu, "fp16", 8, 8, 64, 64, [1] * 130, [100 + i for i in range(129)] + [20000])
     assert 0 < c.plan.joins < 130
