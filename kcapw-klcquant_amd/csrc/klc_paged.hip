@@ -229,7 +229,7 @@ int append_args(const char* name, const klc_kv_append_args& x, AppendArgs& a) {
 // Workgroups of `per_row` threads a head, negative: too many.
 int64_t append_blocks(const char* name, const klc_kv_append_args& x, int64_t per_row) {
   const int64_t blocks = (x.tokens * (x.n_heads + 2 * x.n_kv) * per_row + kPagedThreads - 1) / kPagedThreads;
-  KLC_REQUIRE(blocks < ((int64_t)1 << 31), KLC_ERR_SHAPE, "%s: %lld tokens of %lld heads", name, (long long)x.tokens,
+  KLC_REQUIRE(blocks < ((int64_t)1 << 32) / kPagedThreads, KLC_ERR_SHAPE, "%s: %lld tokens of %lld heads", name, (long long)x.tokens,
               (long long)x.n_heads);
   return blocks;
 }

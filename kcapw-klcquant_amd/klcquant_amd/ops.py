@@ -599,7 +599,7 @@ class AttentionPlan:
     graphs that captured them."""
 
     def __init__(self, data: torch.Tensor, sizes, shape: tuple, window: int, first: int) -> None:
-        self.data = data  # int32: the sequences' starts among the rows, items, joins
+        self.data = data  # int32: the sequences' starts among the rows, items, joins, parts of the rows
         self.device = data.device
         (_, self.tokens, self.at_items, self.items, self.at_joins, self.joins, self.part_rows,
          self.workspace_bytes, self.at_weights, self.weight_items, self.weight_joins,
@@ -617,8 +617,8 @@ def attention_plan(counts, lengths, n_heads: int, n_kv: int, head_dim: int, wind
                    device: torch.device | str = "cuda") -> AttentionPlan:
     """The plan of a batch (klc_attn_plan) for :func:`chunk_attention` and :func:`add_key_weights`, on the host from the
     sequences' ``counts`` of new tokens and ``lengths``, the keys up to and with them (sequences of whole numbers; one
-    copy to ``device``, on its current stream: calls on other streams have to wait for it).  Made once for all layers of a kind: ``window`` and ``first`` (tokens at the start that stay
-    visible beside it) are the layers'."""
+    copy to ``device``, on its current stream: calls on other streams have to wait for it).  Made once for all layers of
+    a kind: ``window`` and ``first`` (tokens at the start that stay visible beside it) are the layers'."""
     counts, lengths = (np.asarray(x) for x in (counts, lengths))
     if counts.ndim != 1 or counts.shape != lengths.shape or counts.size == 0:
         raise ValueError(f"counts and lengths must be one number a sequence, got shapes {counts.shape} and {lengths.shape}")

@@ -321,9 +321,10 @@ class PagedKVCache:
         self.device = self.pool.device  # "cuda" is the current device now, not the one of a later call
         self.weights = None
         if weighted is not None:
+            weighted = tuple(operator.index(x) for x in weighted)
             if len(weighted) != 2 or min(weighted) <= 0:
                 raise ValueError(f"weights of (sequences, keys), got {weighted}")
-            self.table.max_keys = int(weighted[1])
+            self.table.max_keys = weighted[1]
             self.weights = torch.zeros((n_layers, weighted[0], n_kv, weighted[1]), dtype=torch.float32, device=self.device)
 
     def layer(self, layer_idx: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -428,10 +429,11 @@ class BatchedAttention:
             raise ValueError(f"{heads} query heads over {kv} KV heads (groups of 1 to 32, up to 4096 heads)")
         if dim < 8 or dim % 8 or dim > 128:
             raise ValueError(f"head size {dim} (8 to 128, a multiple of 8)")
+        first_tokens = operator.index(first_tokens)
         if first_tokens < 0:
             raise ValueError(f"{first_tokens} first tokens")
         self.config = config
-        self.first_tokens = int(first_tokens)
+        self.first_tokens = first_tokens
         self._tables: dict = {}  # device -> (cos, sin) of the positions so far
         self._kept: list = []    # smaller ones, which captured graphs may still read
 
