@@ -150,8 +150,9 @@ class PageTable:
         counts = counts.astype(np.int64)
         before = self._lengths[at]  # a copy
         after = before + counts
-        if (after + self._evicted[at]).max() >= 1 << 29:
-            raise ValueError(f"sequences must stay below 2^29 tokens, got {int((after + self._evicted[at]).max())}")
+        longest = int((after + self._evicted[at]).max())
+        if longest >= 1 << 29:
+            raise ValueError(f"sequences must stay below 2^29 tokens, got {longest}")
         if self.max_keys is not None and after.max() > self.max_keys:
             raise RuntimeError(f"the cache keeps the weights of {self.max_keys} keys a sequence, {int(after.max())} needed")
         need = self._held(after) - self._held(before)
@@ -180,19 +181,20 @@ class PageTable:
         starts = np.concatenate(([0], np.cumsum(counts)))
         row = np.repeat(np.arange(at.size), counts)
         positions = np.arange(starts[-1]) - starts[row] + before[row]
-        slots = self._pages[at[row], positions // self.page_size].astype(np.int64) * self.page_size + positions % self.page_size
-        pages = self._pages[at, :self._held(int(after.max()))]
-        pages = np.where(np.arange(pages.shape[1]) < self._held(after)[:, None], pages, -1)
+        held = self._held(after)
+        pages = self._pages[at, :int(held.max())]  # a copy
+        if held.min() < pages.shape[1]:
+            pages[np.arange(pages.shape[1]) >= held[:, None]] = -1
+        slots = pages[row, positions // self.page_size].astype(np.int64) * self.page_size + positions % self.page_size
         of = dict(seqs=at, counts=counts, keys=after, pages=pages)
         if not before.any():  # prompts, which attend to themselves
             none = np.zeros(0, np.int32)
             out = dict(positions=positions, slots=slots, starts=starts, prefix=none, tables=none.reshape(0, 0), lengths=none, **of)
             return {**{k: v.astype(np.int32) for k, v in out.items()}, "fresh": True}
         full = int(before.min()) // self.page_size
-        rows = self._pages[at, :full]
-        same = (rows == rows[:1]).all(axis=0)
+        same = (pages[:, :full] == pages[:1, :full]).all(axis=0)
         shared = full if same.all() else int(np.argmin(same))
-        out = dict(positions=positions + self._evicted[at][row], slots=slots, starts=starts, prefix=self._pages[at[0], :shared],
+        out = dict(positions=positions + self._evicted[at][row], slots=slots, starts=starts, prefix=pages[0, :shared],
                    tables=pages[row, shared:], lengths=positions + 1 - shared * self.page_size, **of)
         return {**{k: v.astype(np.int32) for k, v in out.items()}, "fresh": False}
 
