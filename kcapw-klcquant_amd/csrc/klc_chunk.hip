@@ -19,7 +19,7 @@
 //
 // What bounds it (64 heads over 8 of size 64 unless said): wide items by LDS
 // reads, 96 bytes a clock of the 128 it has with three workgroups a CU, and
-// the exponentials.  6,000 tokens over 2,000 beside 64 steps, 584 us (0.84
+// the exponentials.  6,000 tokens over 2,000 beside 64 steps, 582 us (0.85
 // PFLOP/s), 8,192 over none 638 (0.86; 64 rows a wave, half the reads at two
 // waves a SIMD: 673 and 677 on one card), 2,000 over 16,000 of 32 heads of size
 // 128 575 (0.97).  Twelve suffixes of 50 to 100 over 2,000 to 4,000 take 84,
