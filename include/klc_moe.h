@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define KLC_ABI_VERSION 1
+#define KLC_ABI_VERSION 2
 
 #define KLC_OK 0
 #define KLC_ERR_ARGUMENT (-1)    /* null pointer or non-positive size */
@@ -596,9 +596,10 @@ int klc_attn_batch(const klc_attn_batch_args* args, void* stream);
  *
  * klc_attn_plan, on the host, divides the work by HOST arrays counts and
  * lengths (int32 [n_seq]): sizes [12] receives {int32 values of the plan,
- * tokens, at_items, items, at_joins, joins, part_rows, workspace bytes} and, for
- * klc_attn_key_weights, {at_items, items, joins, parts}, and plan its values if
- * capacity holds them (NULL and 0 to ask).  It begins with
+ * tokens, at_items, items, at_joins, joins, part_rows, workspace bytes} and, of
+ * the records from which klc_attn_weight_list makes its list, {where they
+ * begin, records, sequences of several parts, their parts}, and plan its values
+ * if capacity holds them (NULL and 0 to ask).  It begins with
  * the int32 [n_seq + 1] starts of the sequences' rows.  The call takes a copy
  * of it on the device, the sizes and the heads, window and first that it was
  * made for.  counts are the plan's; `lengths` is read on the device, and
@@ -624,12 +625,25 @@ int klc_attn_chunk(const klc_attn_chunk_args* args, void* stream);
  * query heads of the KV head of exp(scale * q . k - lse), lse as klc_attn_chunk
  * wrote it for the same q: added for the keys that were there before the new
  * tokens, set for the new ones.  Sums over a call's rows are float64, in the
- * same order every time.  plan, window, first, lengths and tables as
+ * same order every time.  Window, first, lengths and tables as
  * klc_attn_chunk's, n_heads and n_kv the plan's.  A key in a page outside [0,
  * n_pages), and all of a sequence whose length passes table_width * page_size,
  * gets NaN; keys from capacity on, and sequences whose row is outside [0,
- * n_rows), are left out.  workspace: 8 * parts * n_kv * table_width * page_size
- * bytes, 8-byte aligned, no initialisation, one for calls that may overlap. */
+ * n_rows), are left out.
+ *
+ * klc_attn_weight_list, on the host, lists the work from a plan and its sizes
+ * (HOST arrays, with the counts' sum and the lengths, heads, window and first of
+ * klc_attn_plan): list_sizes [4] receives {int32 values of the list, items,
+ * joins, parts}, and list its values if capacity holds them (NULL and 0 to
+ * ask).  `plan` of the call is a copy on the device that has the list's values
+ * from at_items on, four values behind a multiple of 8 (behind the plan's own,
+ * to need but one copy).  Its size goes by what each sequence's own new tokens see.  Sequences
+ * that have grown since need no other one: the workgroups of their last blocks
+ * go on, so that a list is best made for the longest lengths of its replays.
+ * workspace: 2048 * parts * n_kv bytes, 8-byte aligned, no initialisation, one
+ * for calls that may overlap. */
+int klc_attn_weight_list(const int32_t* plan, const int64_t* sizes, const int32_t* lengths, int64_t n_seq, int64_t n_heads,
+                         int64_t n_kv, int64_t window, int64_t first, int32_t* list, int64_t capacity, int64_t* list_sizes);
 typedef struct klc_attn_key_weights_args {
   const void *q, *lse, *k_pages;
   const void *tables, *lengths, *plan, *rows;

@@ -33,6 +33,7 @@
 #include <queue>
 #include <vector>
 
+#include "klc_key_blocks.h"
 #include "klc_paged_tiles.h"
 
 namespace klc {
@@ -647,7 +648,7 @@ struct RowTile {
 };
 
 // Of a sequence's rows the part that one workgroup of the key weights' kernel
-// takes by every block of keys.
+// takes by a block of keys.
 struct WeightPart {
   int seq, part, parts, offset;  // offset: of the first part among those that are joined
 };
@@ -743,20 +744,13 @@ ChunkPlan chunk_plan(const int32_t* counts, const int32_t* lengths, int64_t n_se
       p.part_rows += (int64_t)t.rows * t.splits;
     }
   }
-  // The key weights' rows: in all eight workgroups a CU, of at least eight tiles of rows.  Parts that are joined come
-  // first, the first of each sequence at the very front.
-  constexpr int64_t kBlock = 256, kTileRows = 32, kLeast = 8;
-  double work = 0.;
-  auto row_tiles = [&](int64_t s) { return (counts[s] * g + kTileRows - 1) / kTileRows; };
-  for (int64_t s = 0; s < n_seq; ++s) work += (double)n_kv * ((lengths[s] + kBlock - 1) / kBlock) * row_tiles(s);
-  const int64_t most = std::max<int64_t>(kLeast, (int64_t)std::ceil(work / (8 * kCus)));
+  // The key weights' rows in the parts of the block that most of them see.  Parts that are joined come first, the first of
+  // each sequence at the very front.
+  const int least = least_tiles(p.starts.data(), lengths, n_seq, g, n_kv, window, first);
   std::vector<WeightPart> rest, single;
-  // First tokens beside a window are seen by all rows, their block of keys by far more than the others, which leave
-  // the parts that they have no rows for: 16 tiles a part there, in up to 64 (6,000 tokens over 2,000, a window of 128
-  // and 4 first tokens, 176 us instead of 736).
   for (int64_t s = 0; s < n_seq; ++s) {
-    int parts = (int)((row_tiles(s) + most - 1) / most);
-    if (first > 0) parts = std::max(parts, (int)std::min<int64_t>((row_tiles(s) + 15) / 16, 64));
+    const KeyBlocks keys(lengths[s], counts[s], (int)g, (int)window, (int)first);
+    const int parts = keys.parts(keys.heads > 0, 1 << 30, least);
     if (parts == 1) {
       single.push_back({(int)s, 0, 1, 0});
       continue;

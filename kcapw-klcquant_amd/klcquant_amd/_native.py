@@ -97,6 +97,7 @@ SIGNATURES: dict[str, tuple] = {
     "klc_attn_batch": (_I32, [ctypes.c_char_p, _P]),
     "klc_attn_plan": (_I32, [_P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P]),
     "klc_attn_chunk": (_I32, [ctypes.c_char_p, _P]),
+    "klc_attn_weight_list": (_I32, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P]),
     "klc_attn_key_weights": (_I32, [ctypes.c_char_p, _P]),
     "klc_kv_evict": (_I32, [ctypes.c_char_p, _P]),
     "klc_synth_fill": (_I32, [_P, _I64, _U64, _I32, _I32, _I32, _P]),

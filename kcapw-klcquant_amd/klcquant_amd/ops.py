@@ -598,12 +598,15 @@ class AttentionPlan:
     layers of this shape, window and ``first`` tokens, on ``device``.  Calls only read it; it has to live as long as
     graphs that captured them."""
 
-    def __init__(self, data: torch.Tensor, sizes, shape: tuple, window: int, first: int) -> None:
-        self.data = data  # int32: the sequences' starts among the rows, items, joins, parts of the rows
+    def __init__(self, data: torch.Tensor, sizes, shape: tuple, window: int, first: int, at_list: int | None, list_sizes) -> None:
+        self.data = data  # int32: the sequences' starts among the rows, items, joins, parts of the rows; the list of the key weights
         self.device = data.device
         (_, self.tokens, self.at_items, self.items, self.at_joins, self.joins, self.part_rows,
          self.workspace_bytes, self.at_weights, self.weight_items, self.weight_joins,
          self.weight_parts) = (int(x) for x in sizes)
+        # the key weights' list, None: there is none
+        self.at_list = at_list
+        _, self.list_items, self.list_joins, self.list_parts = (int(x) for x in list_sizes)
         self.n_seq, self.n_heads, self.n_kv, self.head_dim = shape
         self.window, self.first = window, first
 
@@ -614,11 +617,13 @@ class AttentionPlan:
 
 
 def attention_plan(counts, lengths, n_heads: int, n_kv: int, head_dim: int, window: int | None = None, first: int = 0,
-                   device: torch.device | str = "cuda") -> AttentionPlan:
+                   device: torch.device | str = "cuda", key_weights: bool = True) -> AttentionPlan:
     """The plan of a batch (klc_attn_plan) for :func:`chunk_attention` and :func:`add_key_weights`, on the host from the
     sequences' ``counts`` of new tokens and ``lengths``, the keys up to and with them (sequences of whole numbers; one
     copy to ``device``, on its current stream: calls on other streams have to wait for it).  Made once for all layers of
-    a kind: ``window`` and ``first`` (tokens at the start that stay visible beside it) are the layers'."""
+    a kind: ``window`` and ``first`` (tokens at the start that stay visible beside it) are the layers'.  Without
+    ``key_weights`` it is for :func:`chunk_attention` alone.  For a captured step whose sequences grow between replays it
+    is best made with the longest ``lengths`` that they will have."""
     counts, lengths = (np.asarray(x) for x in (counts, lengths))
     if counts.ndim != 1 or counts.shape != lengths.shape or counts.size == 0:
         raise ValueError(f"counts and lengths must be one number a sequence, got shapes {counts.shape} and {lengths.shape}")
@@ -639,21 +644,34 @@ def attention_plan(counts, lengths, n_heads: int, n_kv: int, head_dim: int, wind
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("a plan cannot be made while a graph is captured: make it before")
     counts, lengths = (np.ascontiguousarray(x, dtype=np.int32) for x in (counts, lengths))
-    sizes = np.zeros(12, np.int64)
-    room = 64 * (counts.size + 64)
-    while True:
-        host = torch.empty(room, dtype=torch.int32, pin_memory=True)
-        rc = nat.load().klc_attn_plan(counts.ctypes.data, lengths.ctypes.data, *shape, window, min(first, (1 << 29) - 1),
-                                      host.data_ptr(), room, sizes.ctypes.data)
+    sizes, list_sizes = np.zeros(12, np.int64), np.zeros(4, np.int64)
+    first = min(first, (1 << 29) - 1)
+    lib = nat.load()
+
+    def checked(name: str, rc: int) -> None:
         if rc in (nat.KLC_ERR_ARGUMENT, nat.KLC_ERR_SHAPE):
             raise ValueError(nat.last_error())
         if rc < 0:
-            raise nat.KlcError("klc_attn_plan", int(rc), nat.last_error())
-        if sizes[0] <= room:
+            raise nat.KlcError(name, int(rc), nat.last_error())
+
+    room = 64 * (counts.size + 64)
+    while True:
+        host = torch.empty(room, dtype=torch.int32, pin_memory=True)
+        checked("klc_attn_plan", lib.klc_attn_plan(counts.ctypes.data, lengths.ctypes.data, *shape, window, first, host.data_ptr(),
+                                                   room, sizes.ctypes.data))
+        end = int(sizes[0])
+        at_list = end // 8 * 8 + (4 if end % 8 <= 4 else 12) if key_weights else None
+        if key_weights and at_list <= room:
+            checked("klc_attn_weight_list",
+                    lib.klc_attn_weight_list(host.data_ptr(), sizes.ctypes.data, lengths.ctypes.data, *shape[:3], window, first,
+                                             host.data_ptr() + 4 * at_list, room - at_list, list_sizes.ctypes.data))
+        if key_weights:
+            end = at_list + int(list_sizes[0])
+        if end <= room and (not key_weights or list_sizes[0]):
             break
-        room = int(sizes[0])
-    data = host[:int(sizes[0])].to(device, non_blocking=True)
-    return AttentionPlan(data, sizes, shape, window, min(first, (1 << 29) - 1))
+        room = 2 * end
+    data = host[:end].to(device, non_blocking=True)
+    return AttentionPlan(data, sizes, shape, window, first, at_list, list_sizes)
 
 
 def _check_plan(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor,
@@ -730,13 +748,15 @@ def add_key_weights(q: torch.Tensor, lse: torch.Tensor, k_pages: torch.Tensor, t
     if n_kv != plan.n_kv:
         raise ValueError(f"weights of {n_kv} KV heads for {plan.n_kv}")
     _, _, scale = _check_heads(None, plan.n_heads, n_kv, None, scale, plan.head_dim, dev)
-    nbytes = 8 * plan.weight_parts * n_kv * width * page
+    if plan.at_list is None:
+        raise ValueError("a plan without key weights: make it with key_weights=True")
+    nbytes = 2048 * plan.list_parts * n_kv
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None  # of this call alone
     _call("klc_attn_key_weights",
           _WEIGHT_ARGS.pack(q.data_ptr(), lse.data_ptr(), k_pages.data_ptr(), tables.data_ptr() if width else 0,
                             lengths.data_ptr(), plan.data.data_ptr(), rows.data_ptr(), weights.data_ptr(),
-                            workspace.data_ptr() if nbytes else 0, plan.at_weights, plan.weight_items, plan.weight_joins,
-                            plan.weight_parts, n_rows, capacity, plan.n_heads, n_kv, plan.head_dim, stride, n_pages, page,
+                            workspace.data_ptr() if nbytes else 0, plan.at_list, plan.list_items, plan.list_joins,
+                            plan.list_parts, n_rows, capacity, plan.n_heads, n_kv, plan.head_dim, stride, n_pages, page,
                             width, plan.window, plan.first, _KV_CODES[k_pages.dtype], nbytes, scale), dev)
 
 

@@ -288,12 +288,13 @@ class PagedBatch:
             self._made["sequences"] = _to_device(parts, self.positions.device)
         return self._made["sequences"]
 
-    def plan(self, config: AttentionConfig, window: int | None, first: int) -> ops.AttentionPlan:
-        """The division of its tokens' attention over the cache, for all layers with this window."""
-        key = (config.num_heads, config.num_kv_heads, config.head_dim, window, first)
+    def plan(self, config: AttentionConfig, window: int | None, first: int, key_weights: bool = True) -> ops.AttentionPlan:
+        """The division of its tokens' attention over the cache, for all layers with this window; without ``key_weights``
+        for those of a cache that keeps none."""
+        key = (config.num_heads, config.num_kv_heads, config.head_dim, window, first, key_weights)
         if key not in self._made:
-            self._made[key] = ops.attention_plan(self.host["counts"], self.host["keys"], *key[:3], window, first,
-                                                 self.positions.device)
+            self._made[key] = ops.attention_plan(self.host["counts"], self.host["keys"], *key[:5], self.positions.device,
+                                                 key_weights)
         return self._made[key]
 
 
@@ -497,7 +498,7 @@ class BatchedAttention:
             sinks = sinks.to(torch.bfloat16).contiguous()
         if chunks:
             tables, lengths, rows = batch.sequences()
-            plan = batch.plan(cfg, window, first)
+            plan = batch.plan(cfg, window, first, weights is not None)
             if weights is None:
                 context = ops.chunk_attention(q, k_pages, v_pages, tables, lengths, plan, sinks)
             else:

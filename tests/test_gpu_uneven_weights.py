@@ -1,0 +1,75 @@
+"""Key weights of batches whose sequences differ much, and of lengths that are far from those the plan was made for: right
+against their definition in float64, with scratch memory that goes by what each sequence's own new tokens see."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from klcquant_amd import ops
+from test_gpu_chunk_attention import Case, int32
+
+pytestmark = pytest.mark.gpu
+
+
+def scratch_bytes(call):
+    """What a call allocates beyond what is held before and after it."""
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    call()
+    torch.cuda.synchronize()
+    return torch.cuda.max_memory_allocated() - before
+
+
+@pytest.mark.parametrize("counts,keys,window,first", [
+    ([100] * 24 + [1], [600] * 24 + [60000], None, 0), ([500] * 12 + [1], [900] * 12 + [60000], 128, 4)])
+def test_suffixes_beside_one_long_sequence(gpu, counts, keys, window, first):
+    """Not a row of scratch over the longest sequence's keys for every part of the others' rows (24 x 60,000 x 8 x 8
+    bytes and more): blocks of 256 keys x 8 x 8 bytes, one for each that is seen and 512 more."""
+    c = Case(gpu, "fp16", 64, 8, 64, 64, counts, keys, window, first)
+    _, lse = c.run(want_lse=True)
+    weights = torch.zeros((len(counts), 8, 60032), device=gpu)
+    rows = torch.arange(len(counts), dtype=torch.int32, device=gpu)
+    used = scratch_bytes(lambda: ops.add_key_weights(c.q, lse, c.k, c.table, c.lengths, c.plan, weights, rows))
+    assert used <= 2048 * 8 * (sum(-(-n // 256) for n in keys) + 512 + 1)
+    del weights
+    c.check_weights(lse)
+
+
+@pytest.mark.parametrize("window,first", [(None, 0), (100, 0), (100, 4), (300, 270)])
+@pytest.mark.parametrize("heads,kv,dim,dtype", [(16, 4, 64, "fp16"), (8, 1, 128, "bf16"), (6, 2, 96, "fp16")])
+def test_far_from_the_planned_lengths(gpu, heads, kv, dim, dtype, window, first):
+    """Sequences that have grown by many blocks of keys, in parts of rows and whole, and shorter ones."""
+    counts, keys = [1, 600, 6, 300], [3000, 2600, 800, 300]
+    c = Case(gpu, dtype, heads, kv, dim, 64, counts, keys, window, first)
+    _, lse = c.check()
+    for planned in (counts, [n + 2000 for n in keys], [300, 5000, 6, 301], keys):
+        c.plan = ops.attention_plan(counts, planned, heads, kv, dim, window, first)
+        c.check_weights(lse)
+
+
+def test_two_streams_and_one_plan(gpu):
+    c = Case(gpu, "bf16", 8, 2, 64, 64, [2, 900], [6000, 2000])
+    assert c.plan.list_joins > 0
+    _, lse = c.run(want_lse=True)
+    rows = int32([1, 0], gpu)
+    weights = [torch.zeros((2, 2, 6016), device=gpu) for _ in range(7)]
+    streams = [torch.cuda.Stream(gpu) for _ in range(2)]
+    torch.cuda.synchronize()
+    for i, w in enumerate(weights):
+        with torch.cuda.stream(streams[i % 2]):
+            ops.add_key_weights(c.q, lse, c.k, c.table, c.lengths, c.plan, w, rows)
+    torch.cuda.synchronize()
+    assert weights[0].any() and all(torch.equal(w, weights[0]) for w in weights)
+
+
+def test_a_plan_without_key_weights(gpu):
+    c = Case(gpu, "bf16", 8, 2, 64, 64, [2], [100])
+    _, lse = c.run(want_lse=True)
+    plan = ops.attention_plan([2], [100], 8, 2, 64, key_weights=False)
+    assert plan.data.numel() < c.plan.data.numel()
+    assert torch.equal(ops.chunk_attention(c.q, c.k, c.v, c.table, c.lengths, plan), c.run())
+    with pytest.raises(ValueError, match="key_weights"):
+        ops.add_key_weights(c.q, lse, c.k, c.table, c.lengths, plan, torch.zeros((1, 2, 128), device=gpu), int32([0], gpu))
