@@ -626,10 +626,11 @@ int klc_attn_chunk(const klc_attn_chunk_args* args, void* stream);
  * wrote it for the same q: added for the keys that were there before the new
  * tokens, set for the new ones.  Sums over a call's rows are float64, in the
  * same order every time.  Window, first, lengths and tables as
- * klc_attn_chunk's, n_heads and n_kv the plan's.  A key in a page outside [0,
- * n_pages), and all of a sequence whose length passes table_width * page_size,
- * gets NaN; keys from capacity on, and sequences whose row is outside [0,
- * n_rows), are left out.
+ * klc_attn_chunk's, n_heads and n_kv the plan's.  A key that a new token sees
+ * gets NaN if it is in a page outside [0, n_pages), or if its sequence's length
+ * passes table_width * page_size, as which it then counts; what no new token
+ * sees keeps its weight.  Keys from capacity on, and sequences whose row is
+ * outside [0, n_rows), are left out.
  *
  * klc_attn_weight_list, on the host, lists the work from a plan and its sizes
  * (HOST arrays, with the counts' sum and the lengths, heads, window and first of

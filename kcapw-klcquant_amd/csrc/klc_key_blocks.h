@@ -57,6 +57,8 @@ struct KeyBlocks {
     }
     return (last + 1) * g;
   }
+  // a key that some row sees
+  __host__ __device__ bool sees(int key) const { return window == 0 || key > base - window || key < first; }
   // the parts of a block's rows, of up to `most` with at least `least` tiles each, whatever the lengths are
   __host__ __device__ int parts(bool head, int most, int least) const {
     const int64_t reach = (int64_t)window + kBlockKeys - 1;

@@ -291,7 +291,8 @@ __device__ __forceinline__ void block_weights(const KeyWeightArgs& a, const Weig
   double sum = half == 0 ? total[0] : total[1];
   const int own = k_lo + lane;
   if (own > b1) return;
-  if (it.wrong || (unsigned)table[own >> a.page_log2] >= (unsigned)a.n_pages) sum = (double)__uint_as_float(0x7fc00000u);
+  // what no row sees keeps its weight, whichever keys share its block
+  if (it.keys.sees(own) && (it.wrong || (unsigned)table[own >> a.page_log2] >= (unsigned)a.n_pages)) sum = (double)__uint_as_float(0x7fc00000u);
   if (part != nullptr)
     part[own - b0] = sum;
   else

@@ -50,6 +50,39 @@ def test_far_from_the_planned_lengths(gpu, heads, kv, dim, dtype, window, first)
         c.check_weights(lse)
 
 
+@pytest.mark.parametrize("window,first", [(None, 0), (40, 0), (40, 4), (40, 300)])
+def test_bad_pages_and_lengths_touch_what_is_seen(gpu, window, first):
+    """A page outside the pool makes the weights NaN of its keys that some new token sees, whichever others share their
+    block of 256, and so does a length past the table; the others keep theirs."""
+    keys, new, page = [900, 700], [1, 30], 16
+    c = Case(gpu, "fp16", 8, 2, 64, page, new, keys, window, first)
+    _, lse = c.run(want_lse=True)
+    rows = int32([0, 1], gpu)
+
+    def seen(n, count):
+        at = torch.arange(n, device=gpu)
+        return at >= 0 if window is None else (at > n - count - window) | (at < first)
+
+    bad = [0, 3, 17, 30, 41, 42, 43, 54, 55, 56]
+    for number in (-1, c.k.shape[0], 2 ** 31 - 1, -2 ** 31):
+        table = c.table.clone()
+        for p in bad:
+            table[:, p] = torch.where(table[:, p] >= 0, number, table[:, p])
+        weights = torch.full((2, 2, 1024), 7.0, device=gpu)
+        ops.add_key_weights(c.q, lse, c.k, table, c.lengths, c.plan, weights, rows)
+        for b, n in enumerate(keys):
+            at = torch.arange(n, device=gpu)
+            hit = seen(n, new[b]) & torch.isin(at // page, torch.tensor(bad, device=gpu))
+            assert hit.any() and torch.equal(weights[b, :, :n].isnan(), hit.expand(2, n))
+            assert (weights[b, :, :n][:, ~seen(n, new[b])] == 7).all() and (weights[b, :, n:] == 7).all()
+    room = c.width * page
+    c.lengths[0] = room + 1
+    weights = torch.full((2, 2, 1024), 7.0, device=gpu)
+    ops.add_key_weights(c.q, lse, c.k, c.table, c.lengths, c.plan, weights, rows)
+    assert torch.equal(weights[0, :, :room].isnan(), seen(room, 1).expand(2, room)) and torch.isfinite(weights[1]).all()
+    assert (weights[0, :, :room][:, ~seen(room, 1)] == 7).all() and (weights[0, :, room:] == 7).all()
+
+
 def test_two_streams_and_one_plan(gpu):
     c = Case(gpu, "bf16", 8, 2, 64, 64, [2, 900], [6000, 2000])
     assert c.plan.list_joins > 0
