@@ -38,6 +38,7 @@ from .attention import _KV_DTYPES, AttentionConfig, yarn_attention_scaling, yarn
 
 
 _MAX_ROWS = 65535  # of a batch_attention call
+_ALL = 1 << 30     # more than a sequence has
 
 
 class PageTable:
@@ -55,6 +56,7 @@ class PageTable:
         self._pages = np.zeros((8, 8), np.int32)            # [sequence][page of it]
         self._lengths = np.full(8, -1, np.int64)            # tokens; -1: no sequence
         self._evicted = np.zeros(8, np.int64)               # tokens before them whose keys have left
+        self._firsts = np.full(8, _ALL, np.int64)           # tokens at the start whose keys are still at their places
 
     def _held(self, n_tokens):
         return -(-n_tokens // self.page_size)
@@ -98,7 +100,9 @@ class PageTable:
             self._lengths = np.concatenate((self._lengths, np.full(len(self._lengths), -1, np.int64)))
             self._pages = np.concatenate((self._pages, np.zeros_like(self._pages)))
             self._evicted = np.concatenate((self._evicted, np.zeros_like(self._evicted)))
+            self._firsts = np.concatenate((self._firsts, np.full_like(self._firsts, _ALL)))
         self._lengths[free[0]] = self._evicted[free[0]] = 0
+        self._firsts[free[0]] = _ALL
         return int(free[0])
 
     def length(self, seq: int) -> int:
@@ -126,7 +130,7 @@ class PageTable:
                 self._take(child, 1)
                 src.append(int(self._pages[parent, full]))
                 dst.append(int(self._pages[child, full]))
-            self._lengths[child], self._evicted[child] = n, self._evicted[parent]
+            self._lengths[child], self._evicted[child], self._firsts[child] = n, self._evicted[parent], self._firsts[parent]
             children.append(child)
         return children, src, dst
 
@@ -142,7 +146,8 @@ class PageTable:
         batch of these tokens, sequence by sequence: ``positions`` and ``slots`` of the tokens, ``starts`` of the
         sequences' runs, ``prefix`` (full pages that all share, in front), and for every token the pages behind them
         (``tables``) and the tokens in those up to itself (``lengths``).  ``fresh``: no sequence had tokens, and what
-        tells of earlier ones is empty.  Of the sequences: ``seqs``, ``counts``, ``keys`` with the new ones and ``pages``."""
+        tells of earlier ones is empty.  Of the sequences: ``seqs``, ``counts``, ``keys`` with the new ones, ``pages`` and ``firsts``, the
+        tokens at their starts that evictions have left in place."""
         at = self._check(seqs)
         counts = np.broadcast_to(np.asarray(counts), at.shape)
         if counts.dtype.kind not in "iu" or (counts <= 0).any():
@@ -186,7 +191,7 @@ class PageTable:
         if held.min() < pages.shape[1]:
             pages[np.arange(pages.shape[1]) >= held[:, None]] = -1
         slots = pages[row, positions // self.page_size].astype(np.int64) * self.page_size + positions % self.page_size
-        of = dict(seqs=at, counts=counts, keys=after, pages=pages)
+        of = dict(seqs=at, counts=counts, keys=after, pages=pages, firsts=self._firsts[at])
         if not before.any():  # prompts, which attend to themselves
             none = np.zeros(0, np.int32)
             out = dict(positions=positions, slots=slots, starts=starts, prefix=none, tables=none.reshape(0, 0), lengths=none, **of)
@@ -223,8 +228,8 @@ class PageTable:
         pages = np.where(np.arange(width) < self._held(self._lengths[at])[:, None], pages, -1).astype(np.int32)
         return dict(seqs=at, keys=self._lengths[at].astype(np.int32), pages=pages, src=src, dst=dst)
 
-    def evict(self, plan: dict, keep: int) -> None:
-        """Books the ``eviction`` that was asked for last."""
+    def evict(self, plan: dict, keep: int, first: int = 0) -> None:
+        """Books the ``eviction`` that was asked for last, which leaves the ``first`` keys in place."""
         del self._free[len(self._free) - len(plan["dst"]):]
         self._holders[plan["dst"]] = 1
         np.subtract.at(self._holders, plan["src"], 1)
@@ -236,6 +241,7 @@ class PageTable:
             self._free.extend(left[self._holders[left] == 0][::-1].tolist())
             self._lengths[s] = keep
             self._evicted[s] += int(n) - keep
+            self._firsts[s] = min(self._firsts[s], first)
 
     def moves(self) -> tuple[list[int], list[int]]:
         """The page moves (sources, destinations) of a compaction: pages that are held go to the front."""
@@ -322,6 +328,7 @@ class PagedKVCache:
         self.dtype = _KV_DTYPES[precision][0]
         self.pool = torch.empty((2 * n_layers, n_pages, page_size, n_kv, head_dim), dtype=self.dtype, device=device)
         self.device = self.pool.device  # "cuda" is the current device now, not the one of a later call
+        self.first_tokens = 0  # that a layer saw beside its window, the most so far
         self.weights = None
         if weighted is not None:
             weighted = tuple(operator.index(x) for x in weighted)
@@ -373,19 +380,23 @@ class PagedKVCache:
         """Cuts those of ``seqs`` with more than ``keep`` keys to as many, in every layer and KV head by itself: the
         ``first`` and the last ``recent`` ones stay, and of the others those of the largest weights (ops.evict_keys).
         Returns the sequences that were cut.  New tokens go on at their positions in the whole text.  A window counts
-        keys that are held: layers with one need ``recent`` of at least it.  Batches made before are void."""
+        keys that are held: layers with one need ``recent`` of at least it.  What layers see beside one are the keys at the
+        start: a ``first`` below their ``first_tokens`` is refused, and so is such a layer on a sequence that was cut with
+        one before.  Batches made before are void."""
         if self.weights is None:
             raise ValueError("a cache without weights: give `weighted` when it is made")
         keep, recent, first = operator.index(keep), operator.index(recent), operator.index(first)
         if recent < 0 or first < 0 or recent + first > keep:
             raise ValueError(f"{keep} keys kept, of them the first {first} and the last {recent}")
+        if first < self.first_tokens:
+            raise ValueError(f"the first {first} keys kept, of {self.first_tokens} that layers see beside their windows")
         plan = self.table.eviction(seqs, keep)
         if plan["seqs"].size:
             tables, lengths, rows = _to_device([plan["pages"], plan["keys"], plan["seqs"].astype(np.int32)], self.device)
             if plan["src"]:
                 ops.copy_pages(self.pool, plan["src"], plan["dst"])
             ops.evict_keys(self.pool, self.weights, tables, lengths, rows, keep, recent=recent, first=first)
-            self.table.evict(plan, keep)  # once the work is under way
+            self.table.evict(plan, keep, first)  # once the work is under way
         return plan["seqs"].tolist()
 
     def compact(self) -> int:
@@ -412,7 +423,8 @@ class PagedKVCache:
         d = dict(zip(names, _to_device([x[n] for n in names], self.device)))
         return PagedBatch(d["positions"], d["slots"], d["starts"], d["tables"], d["lengths"], d["prefix"],
                           x["prefix"].size * self.table.page_size, x["fresh"], x["positions"].size,
-                          int(x["positions"].max()) + 1, {n: x[n] for n in ("seqs", "counts", "keys", "pages")})
+                          int(x["positions"].max()) + 1,
+                          {**{n: x[n] for n in ("seqs", "counts", "keys", "pages")}, "first": int(x["firsts"].min())})
 
     def stats(self) -> dict:
         return {**self.table.stats(), "resident_bytes": self.pool.numel() * self.pool.element_size(),
@@ -476,6 +488,12 @@ class BatchedAttention:
         prefix = f"model.layers.{layer_idx}.self_attn"
         if hidden.dim() != 2 or hidden.shape[0] != batch.tokens:
             raise ValueError(f"a batch of {batch.tokens} tokens, got hidden {tuple(hidden.shape)}")
+        window = (sliding_window if sliding_window is not None else cfg.sliding_window) or None  # 0: none
+        first = self.first_tokens if window else 0
+        if first:
+            if batch.host.get("first", first) < first:
+                raise ValueError(f"{first} first tokens beside a window, of sequences that were cut to the first {batch.host['first']} keys")
+            kv_cache.first_tokens = max(kv_cache.first_tokens, first)
         lin = torch.nn.functional.linear
 
         def project(name: str, heads: int) -> torch.Tensor:
@@ -485,8 +503,6 @@ class BatchedAttention:
         q, k, v = project("q_proj", cfg.num_heads), project("k_proj", cfg.num_kv_heads), project("v_proj", cfg.num_kv_heads)
         k_pages, v_pages = kv_cache.layer(layer_idx)
         cos, sin = self.rope_tables(batch.end, q.device)
-        window = (sliding_window if sliding_window is not None else cfg.sliding_window) or None  # 0: none
-        first = self.first_tokens if window else 0
         weights = kv_cache.weights
         chunks = weights is not None or first > 0 or (not batch.fresh and self._suffixes(batch, window))
         norms = [tensors.get(f"{prefix}.{name}.weight") for name in ("q_norm", "k_norm")]
