@@ -16,7 +16,7 @@ def test_first_tokens_stay_in_place(gpu, first, page):
     run.extend([a, b], [150, 47])
     run.extend([a, b], [9, 1])
     run.evict([a, b], 96, 30, first)
-    child, = run.fork(a)
+    child, = run.fork(a, 1)
     for _ in range(3):
         run.extend([a, b, child], [1, 20, 2])
     run.evict([a, b, child], 80, 24, first + 3)
