@@ -287,21 +287,44 @@ class PagedBatch:
 
     def sequences(self) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """Of each sequence its pages (int32 ``[sequences, pages]``), its keys and its number, on the device."""
-        if "sequences" not in self._made:
+        def make():
             if self.positions.is_cuda and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("a batch's arrays cannot be copied while a graph is captured: run a layer before")
-            parts = [self.host[n] for n in ("pages", "keys", "seqs")]
-            self._made["sequences"] = _to_device(parts, self.positions.device)
-        return self._made["sequences"]
+                raise RuntimeError("a batch's arrays cannot be copied while a graph is captured: call sequences() and plan() before")
+            made = _to_device([self.host[n] for n in ("pages", "keys", "seqs")], self.positions.device)
+            return made, made
+        return self._once("sequences", make)
 
     def plan(self, config: AttentionConfig, window: int | None, first: int, key_weights: bool = True) -> ops.AttentionPlan:
         """The division of its tokens' attention over the cache, for all layers with this window; without ``key_weights``
         for those of a cache that keeps none."""
         key = (config.num_heads, config.num_kv_heads, config.head_dim, window, first, key_weights)
-        if key not in self._made:
-            self._made[key] = ops.attention_plan(self.host["counts"], self.host["keys"], *key[:5], self.positions.device,
-                                                 key_weights)
-        return self._made[key]
+
+        def make():
+            made = ops.attention_plan(self.host["counts"], self.host["keys"], *key[:5], self.positions.device, key_weights)
+            return made, (made.data,)
+        return self._once(key, make)
+
+    def _once(self, key, make):
+        """``make()``'s first part, made at the first call; its second are the device tensors in it.  Calls on other streams
+        than the first one's wait there for the copies, but for captured ones: a graph's replays come behind them anyway,
+        since torch.cuda.graph waits for the device before it captures."""
+        device = self.positions.device
+        made = self._made.get(key)
+        if made is None:
+            what, tensors = make()
+            event = torch.cuda.current_stream(device).record_event() if device.type == "cuda" else None
+            self._made[key] = made = (what, tensors, _stream(device), event)
+        elif made[2] != _stream(device) and not torch.cuda.is_current_stream_capturing():
+            stream = torch.cuda.current_stream(device)
+            stream.wait_event(made[3])
+            for t in made[1]:
+                t.record_stream(stream)
+        return made[0]
+
+
+def _stream(device: torch.device) -> int | None:
+    """The current stream's number, None on the CPU."""
+    return torch._C._cuda_getCurrentRawStream(device.index) if device.type == "cuda" else None
 
 
 def _to_device(parts: list, device: torch.device) -> tuple:
