@@ -269,7 +269,8 @@ def _intercepted() -> bool:
 
 
 class StreamedAttention:
-    """StreamedAttention (streamed_attention.py:101-152)."""
+    """StreamedAttention (streamed_attention.py:101-152).  A projection without a bias
+    tensor has none."""
 
     def __init__(self, config: AttentionConfig) -> None:
         self.config = config
@@ -409,9 +410,12 @@ class StreamedAttention:
             return stepped
         prefix = f"model.layers.{layer_idx}.self_attn"
         lin = torch.nn.functional.linear
-        q = lin(hidden, tensors[f"{prefix}.q_proj.weight"], tensors[f"{prefix}.q_proj.bias"]).view(cfg.num_heads, cfg.head_dim)
-        k = lin(hidden, tensors[f"{prefix}.k_proj.weight"], tensors[f"{prefix}.k_proj.bias"]).view(cfg.num_kv_heads, cfg.head_dim)
-        v = lin(hidden, tensors[f"{prefix}.v_proj.weight"], tensors[f"{prefix}.v_proj.bias"]).view(cfg.num_kv_heads, cfg.head_dim)
+
+        def project(name: str, heads: int) -> torch.Tensor:
+            x = lin(hidden, tensors[f"{prefix}.{name}_proj.weight"], tensors.get(f"{prefix}.{name}_proj.bias")).view(heads, cfg.head_dim)
+            return x
+
+        q, k, v = project("q", cfg.num_heads), project("k", cfg.num_kv_heads), project("v", cfg.num_kv_heads)
         if not isinstance(kv_cache, DeviceKVCache) or q.dtype != torch.bfloat16 or q.device.type != "cuda":
             raise ValueError("StreamedAttention runs on a DeviceKVCache with bfloat16 activations on the GPU")
         window = sliding_window if sliding_window is not None else cfg.sliding_window
@@ -439,7 +443,7 @@ class StreamedAttention:
                      cfg.num_kv_heads, cfg.head_dim, kv_cache.kv_code, P(self._workspace.data_ptr()),
                      self._workspace.numel(), P(context.data_ptr()), stream)
         o_weight = tensors[f"{prefix}.o_proj.weight"]
-        out = lin(context.reshape(-1).to(o_weight.dtype), o_weight, tensors[f"{prefix}.o_proj.bias"])
+        out = lin(context.reshape(-1).to(o_weight.dtype), o_weight, tensors.get(f"{prefix}.o_proj.bias"))
         qf, kf, qp, kp = q_rot.float(), k_rot.float(), q.float(), k.float()
         diagnostics = {
             "rope_position": int(position),

@@ -459,7 +459,7 @@ class BatchedAttention:
     does not take, though it could run their prompts: groups of more than 32 query heads.  ``first_tokens`` at the start
     of a sequence stay visible beside the windows of layers that have one.  Where a layer's tensors hold
     ``q_norm.weight`` or ``k_norm.weight [head_dim]``, its queries' or keys' heads are normalised before they are rotated
-    (``config.rms_norm_eps``)."""
+    (``config.rms_norm_eps``); a projection without a bias tensor has none."""
 
     def __init__(self, config: AttentionConfig, first_tokens: int = 0) -> None:
         heads, kv, dim = config.num_heads, config.num_kv_heads, config.head_dim
@@ -520,7 +520,7 @@ class BatchedAttention:
         lin = torch.nn.functional.linear
 
         def project(name: str, heads: int) -> torch.Tensor:
-            x = lin(hidden, tensors[f"{prefix}.{name}.weight"], tensors[f"{prefix}.{name}.bias"])
+            x = lin(hidden, tensors[f"{prefix}.{name}.weight"], tensors.get(f"{prefix}.{name}.bias"))
             return x.view(batch.tokens, heads, cfg.head_dim)
 
         q, k, v = project("q_proj", cfg.num_heads), project("k_proj", cfg.num_kv_heads), project("v_proj", cfg.num_kv_heads)
@@ -552,4 +552,4 @@ class BatchedAttention:
                 ops.batch_attention(q[rows], k_pages, v_pages, batch.tables[rows], batch.lengths[rows],
                                     batch.prefix_table, batch.prefix_len, sinks, window, out=context[rows])
         o_weight = tensors[f"{prefix}.o_proj.weight"]
-        return lin(context.view(batch.tokens, -1).to(o_weight.dtype), o_weight, tensors[f"{prefix}.o_proj.bias"])
+        return lin(context.view(batch.tokens, -1).to(o_weight.dtype), o_weight, tensors.get(f"{prefix}.o_proj.bias"))
