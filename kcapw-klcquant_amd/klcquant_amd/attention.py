@@ -269,8 +269,9 @@ def _intercepted() -> bool:
 
 
 class StreamedAttention:
-    """StreamedAttention (streamed_attention.py:101-152).  A projection without a bias
-    tensor has none."""
+    """StreamedAttention (streamed_attention.py:101-152).  Where a layer's tensors hold ``q_norm.weight`` or ``k_norm.weight
+    [head_dim]``, its queries' or keys' heads go through rms_norm before they are rotated, as BatchedAttention's do; a
+    projection without a bias tensor has none."""
 
     def __init__(self, config: AttentionConfig) -> None:
         self.config = config
@@ -323,9 +324,12 @@ class StreamedAttention:
         if names is None:
             pre = f"model.layers.{layer_idx}.self_attn"
             names = self._names[layer_idx] = (*(f"{pre}.{n}_proj.{t}" for t in ("weight", "bias") for n in "qkvo"),
-                                              f"{pre}.sinks")
+                                              f"{pre}.sinks", f"{pre}.q_norm.weight", f"{pre}.k_norm.weight")
         get = tensors.get
         held = [get(n) for n in names]
+        if held[9] is not None or held[10] is not None:
+            return None
+        del held[9:]
         o_weight = held[3]
         if type(o_weight) not in _TENSORS or o_weight.dim() != 2:
             return None
@@ -413,7 +417,8 @@ class StreamedAttention:
 
         def project(name: str, heads: int) -> torch.Tensor:
             x = lin(hidden, tensors[f"{prefix}.{name}_proj.weight"], tensors.get(f"{prefix}.{name}_proj.bias")).view(heads, cfg.head_dim)
-            return x
+            norm = tensors.get(f"{prefix}.{name}_norm.weight") if name != "v" else None
+            return x if norm is None else rms_norm(x, norm.to(x.dtype), cfg.rms_norm_eps)
 
         q, k, v = project("q", cfg.num_heads), project("k", cfg.num_kv_heads), project("v", cfg.num_kv_heads)
         if not isinstance(kv_cache, DeviceKVCache) or q.dtype != torch.bfloat16 or q.device.type != "cuda":
