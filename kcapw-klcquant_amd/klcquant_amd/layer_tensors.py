@@ -44,6 +44,9 @@ LAYER_TENSOR_SUFFIXES = (
     "post_attention_layernorm.weight",
 )
 
+#: Beside them, where a checkpoint has them: the norms of queries and keys that the attention layers apply.
+NORM_TENSOR_SUFFIXES = ("self_attn.q_norm.weight", "self_attn.k_norm.weight")
+
 
 def layer_tensor_names(layer_idx: int) -> list[str]:
     prefix = f"model.layers.{layer_idx}"
@@ -94,7 +97,7 @@ class LayerTensorLoader:
             return dict(cached)
         self.layer_tensor_cache_misses += 1
         by_file: dict[str, list[str]] = {}
-        for name in layer_tensor_names(layer_idx):
+        for name in layer_tensor_names(layer_idx) + [f"model.layers.{layer_idx}.{s}" for s in NORM_TENSOR_SUFFIXES]:
             if self._skip(name):
                 continue
             file = self.index.weight_map.get(name)

@@ -1,13 +1,15 @@
-"""Models that normalise queries and keys, without biases: the same of both attention layers."""
+"""Models that normalise queries and keys, without biases: loaded from a checkpoint, and the same of both attention layers."""
 
 from __future__ import annotations
 
+import json
 import math
 
 import pytest
 import torch
 
 from klcquant_amd.attention import AttentionConfig, DeviceKVCache, StreamedAttention, rms_norm
+from klcquant_amd.layer_tensors import LayerTensorLoader
 from klcquant_amd.paged_kv import BatchedAttention, PagedKVCache
 
 pytestmark = pytest.mark.gpu
@@ -87,3 +89,18 @@ def test_biases_that_are_not_there(gpu):
         assert torch.equal(outs[0][0], outs[1][0])
         # one token's context is its value, rounded once, on every path
         assert torch.equal(outs[0][1], outs[1][1])
+
+
+def test_the_loader_brings_them(gpu, tmp_path):
+    from safetensors.torch import save_file
+
+    held = {n: t.cpu() for n, t in layer_tensors(gpu).items()}
+    other = {"model.layers.1.self_attn.q_norm.weight": torch.ones(DIM), "model.layers.1.input_layernorm.weight": torch.ones(WIDTH)}
+    save_file(held | other, str(tmp_path / "model.safetensors"))
+    index = {"weight_map": {n: "model.safetensors" for n in held | other}}
+    (tmp_path / "model.safetensors.index.json").write_text(json.dumps(index))
+    loader = LayerTensorLoader(tmp_path, gpu)
+    got = loader.load(0)
+    assert set(got) == set(held) and all(torch.equal(got[n].cpu(), t) for n, t in held.items())
+    assert set(loader.load(1)) == set(other)
+    assert set(LayerTensorLoader(tmp_path, gpu, skip=[f"{AT}.q_norm.weight"]).load(0)) == set(held) - {f"{AT}.q_norm.weight"}
