@@ -11,8 +11,8 @@
 //   wide    more than 64 rows: 4 waves x 32 rows over one ring of tiles
 //   pairs   33 to 64 rows, head sizes up to 64: the same of 2 pairs of waves,
 //           of half the keys each, which join in LDS (past 64 wide has them)
-//   narrow  up to 32 rows: each wave takes every fourth tile through a ring
-//           of its own, with no barrier, and the waves join in LDS
+//   narrow  up to 32 rows: each wave takes every fourth tile, K and V in turn
+//           through LDS of its own, with no barrier, and the waves join there
 // Rows whose keys are in parts leave float32 sums, which a second launch joins.
 // As in the prompt's kernel a row with a NaN or infinity that may come from a
 // value it must not see is computed again, token by token.
@@ -421,16 +421,15 @@ __device__ __forceinline__ void narrow_part(const ChunkArgs& a, const ChunkItem&
                                             float4 (&wave_ml)[kWaves][kNarrowRows]) {
   using R = ChunkRows<DP, kF16, kFull, kLse>;
   using F = typename R::F;
-  constexpr int KT = kKeys, kRing = kChunkLds<DP> / kWaves / F::kStage, kQuads = R::kQuads;
-  static_assert(kRing == 1 || kRing == 2, "");
-  constexpr bool kHalves = kRing == 1;  // with one tile a wave, K and V take turns
+  constexpr int KT = kKeys, kQuads = R::kQuads;
+  static_assert(kChunkLds<DP> / kWaves / F::kStage == 1, "one tile a wave: K and V take turns");
   const int g = a.n_heads / a.n_kv, lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int base = n - it.count, last = it.row0 + it.rows - 1;
   const int p_lo = base + it.row0 / g, p_hi = base + last / g;
   const int32_t* table = a.tables + (int64_t)it.seq * a.width;
-  const lds_u8 ring = lds + wave * kRing * F::kStage;
+  const lds_u8 tile = lds + wave * F::kStage;
   R r;
-  r.begin(a, it, kvh, base, it.row0, ring);
+  r.begin(a, it, kvh, base, it.row0, tile);
   PageLoads<ChunkArgs, F, KT, F::kDmas, 1> pages(a, 0, kvh);
   pages.prepare_whole();
   const Span<KT> span(a, p_lo, p_hi);
@@ -438,56 +437,42 @@ __device__ __forceinline__ void narrow_part(const ChunkArgs& a, const ChunkItem&
   const int first = t0 + wave;
   if (first < end) pages.hold(table, span.at(span.base(first))(span.base(first)) >> a.page_log2, a.width);
   settle_query<F>(r.f.q[0]);
-  auto load = [&](auto key, auto value, int j, int slot) {
+  auto load = [&](auto key, int j) {  // K of a tile, or V
+    constexpr bool kKey = decltype(key)::value;
     const int at = span.base(j);
-    const lds_u8 k = ring + slot * F::kStage, v = k + F::kMatBytes;
     if (span.whole(at))
-      pages.template load_whole<decltype(key)::value, decltype(value)::value>(at, k, v);
+      pages.template load_whole<kKey, !kKey>(at, tile, tile + F::kMatBytes);
     else
-      pages.template load<decltype(key)::value, decltype(value)::value>(at, span.at(at), k, v);
+      pages.template load<kKey, !kKey>(at, span.at(at), tile, tile + F::kMatBytes);
   };
-#pragma unroll
-  for (int i = 0; i < kRing; ++i)
-    if (first + i * kWaves < end) {
-      if constexpr (kHalves) {
-        load(Count<true>{}, Count<false>{}, first + i * kWaves, i);
-        load(Count<false>{}, Count<true>{}, first + i * kWaves, i);
-      } else {
-        load(Count<true>{}, Count<true>{}, first + i * kWaves, i);
-      }
-    }
+  if (first < end) {
+    load(Count<true>{}, first);
+    load(Count<false>{}, first);
+  }
   r.convert(a);
-  int slot = 0;
   for (int j = first; j < end; j += kWaves) {
-    // K is there, and V unless it comes by itself; the ring's other tile may be in flight
-    const bool refill = j + kRing * kWaves < end;
-    if (kHalves)
-      tile_wait<F::kDmas, false>();
-    else if (j + kWaves < end)
-      tile_wait<2 * F::kDmas, false>();
-    else
-      tile_wait<0, false>();
-    const int stage = slot * F::kStage, k0 = span.base(j);
+    const bool refill = j + kWaves < end;
+    tile_wait<F::kDmas, false>();  // K is there, V may be in flight
+    const int k0 = span.base(j);
     f32x16_t s[1][1];
-    r.f.scores(stage, s);
-    if (kHalves && refill) {
+    r.f.scores(0, s);
+    if (refill) {
       tile_wait<63, false>();  // K has been read
-      load(Count<true>{}, Count<false>{}, j + kRing * kWaves, slot);
+      load(Count<true>{}, j + kWaves);
     }
     if (k0 + kKeys - 1 > p_lo || (a.window > 0 && k0 <= p_hi - a.window)) r.mask(a, k0, s);
     r.raise(s[0]);
     u32x4_t p[1][2];
     r.weigh(s[0], p[0]);
-    if (kHalves && refill)
+    if (refill)
       tile_wait<F::kDmas, false>();
-    else if (kHalves)
+    else
       tile_wait<0, false>();
-    r.f.values(stage + F::kMatBytes, p);
+    r.f.values(F::kMatBytes, p);
     if (refill) {
-      tile_wait<63, false>();  // the slot has been read
-      load(Count<!kHalves>{}, Count<true>{}, j + kRing * kWaves, slot);
+      tile_wait<63, false>();  // V has been read
+      load(Count<false>{}, j + kWaves);
     }
-    slot = (slot + 1) % kRing;
   }
 
   const bool bad = __syncthreads_or(pages.bad) || wrong;
