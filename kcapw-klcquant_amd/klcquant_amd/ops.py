@@ -654,7 +654,9 @@ def attention_plan(counts, lengths, n_heads: int, n_kv: int, head_dim: int, wind
         if rc < 0:
             raise nat.KlcError(name, int(rc), nat.last_error())
 
-    room = 64 * (counts.size + 64)
+    room = 64 * (counts.size + 64)  # mostly enough: what does not fit is planned once more
+    if key_weights:
+        room += 8 * (int(lengths.sum(dtype=np.int64) >> 8) + counts.size + 1024)
     while True:
         host = torch.empty(room, dtype=torch.int32, pin_memory=True)
         checked("klc_attn_plan", lib.klc_attn_plan(counts.ctypes.data, lengths.ctypes.data, *shape, window, first, host.data_ptr(),
