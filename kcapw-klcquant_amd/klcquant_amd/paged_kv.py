@@ -524,10 +524,13 @@ class BatchedAttention:
             return x.view(batch.tokens, heads, cfg.head_dim)
 
         q, k, v = project("q_proj", cfg.num_heads), project("k_proj", cfg.num_kv_heads), project("v_proj", cfg.num_kv_heads)
-        k_pages, v_pages = kv_cache.layer(layer_idx)
-        cos, sin = self.rope_tables(batch.end, q.device)
         weights = kv_cache.weights
         chunks = weights is not None or first > 0 or (not batch.fresh and self._suffixes(batch, window))
+        if chunks:  # before the keys are stored: what cannot be planned leaves the cache as it was
+            tables, lengths, rows = batch.sequences()
+            plan = batch.plan(cfg, window, first, weights is not None)
+        k_pages, v_pages = kv_cache.layer(layer_idx)
+        cos, sin = self.rope_tables(batch.end, q.device)
         norms = [tensors.get(f"{prefix}.{name}.weight") for name in ("q_norm", "k_norm")]
         norms = [t if t is None else t.to(torch.bfloat16).contiguous() for t in norms]
         q, k = ops.paged_append(q, k, v, cos, sin, batch.positions, batch.slots, k_pages, v_pages,
@@ -536,8 +539,6 @@ class BatchedAttention:
         if sinks is not None:
             sinks = sinks.to(torch.bfloat16).contiguous()
         if chunks:
-            tables, lengths, rows = batch.sequences()
-            plan = batch.plan(cfg, window, first, weights is not None)
             if weights is None:
                 context = ops.chunk_attention(q, k_pages, v_pages, tables, lengths, plan, sinks)
             else:

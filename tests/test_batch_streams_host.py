@@ -61,6 +61,22 @@ def test_other_streams_wait_for_what_the_first_layer_made(notes):
     assert b.plan(CONFIG, 16, 0) is windowed and ("wait", 0, "event of 7") in notes.log
 
 
+def test_a_batch_that_cannot_be_planned_stores_nothing(notes, monkeypatch):
+    cache = paged_kv.PagedKVCache("cpu", 1, 2, 64, 40, 16, weighted=(2, 200))
+    appended = []
+
+    def none(*args):
+        raise ValueError("too many blocks")
+
+    monkeypatch.setattr(ops, "attention_plan", none)
+    monkeypatch.setattr(ops, "paged_append", lambda *x, **kw: appended.append(x))
+    at = "model.layers.0.self_attn"
+    tensors = {f"{at}.{n}_proj.weight": torch.zeros(rows, 256).bfloat16() for n, rows in (("q", 256), ("k", 128), ("v", 128), ("o", 256))}
+    with pytest.raises(ValueError, match="too many blocks"):
+        paged_kv.BatchedAttention(CONFIG).forward(0, torch.zeros(1, 256).bfloat16(), tensors, batch(), cache)
+    assert not appended
+
+
 def test_a_capture_waits_for_nothing_and_makes_nothing(notes):
     b = batch()
     notes.capturing = True
