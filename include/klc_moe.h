@@ -585,8 +585,9 @@ int klc_attn_batch(const klc_attn_batch_args* args, void* stream);
  * or many), the last of the lengths[s] keys that the sequence has in the pages
  * of row s of tables (int32 [n_seq][table_width]); their rows of q follow one
  * another, sequence by sequence.  The token at key i sees the keys j <= i, and
- * with a window those with j > i - window or j < first.  q, softmax and
- * rounding as klc_attn_batch; out [tokens][n_heads][head_dim] bfloat16.  lse
+ * with a window those with j > i - window or j < first.  q and softmax as
+ * klc_attn_batch, probabilities rounded to kv_dtype as there (for the product
+ * with the values and its normaliser; all else is float32); out [tokens][n_heads][head_dim] bfloat16.  lse
  * (float32 [tokens][n_heads], or NULL) receives the logs of the normalisers,
  * the sink's part in them, of the probabilities before they are rounded: -inf
  * for a row without a key or sink.  A row without a key is zero; a length past
@@ -624,8 +625,8 @@ int klc_attn_chunk(const klc_attn_chunk_args* args, void* stream);
  * key j of sequence s, the sum over its new tokens that see the key and the
  * query heads of the KV head of exp(scale * q . k - lse), lse as klc_attn_chunk
  * wrote it for the same q: added for the keys that were there before the new
- * tokens, set for the new ones.  Sums over a call's rows are float64, in the
- * same order every time.  Window, first, lengths and tables as
+ * tokens, set for the new ones.  Of a call's rows 16 at a time are summed in
+ * float32 and those sums in float64, in the same order every time.  Window, first, lengths and tables as
  * klc_attn_chunk's, n_heads and n_kv the plan's.  A key that a new token sees
  * gets NaN if it is in a page outside [0, n_pages), or if its sequence's length
  * passes table_width * page_size, as which it then counts; what no new token

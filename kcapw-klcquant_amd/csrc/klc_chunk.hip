@@ -19,14 +19,14 @@
 //
 // What bounds it (64 heads over 8 of size 64 unless said): wide items by LDS
 // reads, 96 bytes a clock of the 128 it has with three workgroups a CU, and
-// the exponentials.  6,000 tokens over 2,000 beside 64 steps, 582 us (0.85
-// PFLOP/s), 8,192 over none 638 (0.86; 64 rows a wave, half the reads at two
-// waves a SIMD: 673 and 677 on one card), 2,000 over 16,000 of 32 heads of size
-// 128 575 (0.97).  Twelve suffixes of 50 to 100 over 2,000 to 4,000 take 84,
-// 464 items on 256 CUs, each waiting for itself.  Steps by HBM: 200 of a
-// window of 1,024 and 4 first tokens 92 us (4.6 TB/s), 256 of 2,000 155 (5.1);
-// eight of 700 keys take 12, the chain of item, length, page numbers and six
-// tiles a wave.
+// the exponentials.  6,000 tokens over 2,000 beside 64 steps, 573 to 590 us by
+// the card (0.84 PFLOP/s), 8,192 over none 631 (0.87; 64 rows a wave, half the
+// reads at two waves a SIMD: 673 and 677 on one card), 2,000 over 16,000 of 32
+// heads of size 128 576 to 588 (0.96).  Twelve suffixes of 50 to 100 over 2,000
+// to 4,000 take 85, 464 items on 256 CUs, each waiting for itself.  Steps by
+// HBM: 200 of a window of 1,024 and 4 first tokens 93 us (4.6 TB/s), 256 of
+// 2,000 156 (5.1); eight of 700 keys take 12, the chain of item, length, page
+// numbers and six tiles a wave.
 #include <math.h>
 
 #include <algorithm>
@@ -45,8 +45,8 @@ constexpr int kNarrowRows = 32;
 __host__ __device__ constexpr int pair_rows(int dim) { return dim <= 64 ? 64 : kNarrowRows; }
 constexpr int kJoinRows = 16;    // of one workgroup
 constexpr int kRecord = 8;       // int32 of an item and of a join
-// LDS of a workgroup: three fit a CU, past head size 64 two (with two of size 64 6,000 tokens beside 64 steps take 700 us,
-// with three 647)
+// LDS of a workgroup: three fit a CU, past head size 64 two (of size 64, with the loads of the time, 6,000 tokens over 2,000
+// beside 64 steps took 700 us with two and 647 with three)
 template <int DP>
 constexpr int kChunkLds = (DP == 64 ? 48 : 64) * 1024;
 
@@ -667,7 +667,8 @@ double makespan(std::vector<double>& costs, int64_t servers) {
   return last;
 }
 
-// How long a plan takes: two workgroups a CU, of one KV head's share of the chip.
+// How long a plan takes, on one KV head's share of the chip.  It only has to tell cuts apart: two workgroups a CU count as
+// side by side for every head size, and what the third of sizes up to 64 takes from them is in RowTile::shared.
 double duration(const std::vector<RowTile>& tiles, int64_t n_kv, int64_t dim) {
   std::vector<double> alone, shared;
   bool joins = false;

@@ -15,7 +15,8 @@
 // the moves and the recent keys.
 //
 // What bounds it (8 KV heads of size 64): many lists by HBM, 36 layers of three
-// sequences of up to 6,001 keys cut to 1,500 in 103 us (545 MB, 5.3 TB/s); few
+// sequences of up to 6,001 keys cut to 1,500 in 104 to 110 us by the card (545
+// MB, 5.0 to 5.2 TB/s, a large copy's rate); few
 // by that chain of steps, eight sequences of up to 2,064 keys cut to 2,000 in
 // one layer in 13.  Weights held in registers between the steps, and the recent
 // keys read ahead of the moves, changed neither.

@@ -9,7 +9,8 @@
 // A wave keeps 64 keys in registers as the matrix instruction's columns, and
 // rows come past in tiles of 32 through LDS, for the four waves of a
 // workgroup: a lane has 16 rows of its one key, so that the sums over rows
-// never leave it but at the end.  A list made on the host has the workgroups:
+// never leave it but at the end, 16 at a time in float32 and those sums in
+// float64.  A list made on the host has the workgroups:
 // a block of keys that new tokens see, and a part of the rows that see it.
 // Parts' float64 sums are added by a second launch, in their order.
 //
@@ -307,7 +308,7 @@ __global__ __launch_bounds__(kWave * kWaves, DP == 64 ? 4 : 3) void key_weights_
   bool more = true;
 #pragma unroll 1
   for (int grown = 0; more; ++grown) {
-    // the arguments and the item are read again for every block: held over the work on one, up to 60 scalars spill
+    // the arguments and the item are read again for every block: held over the work on one, 28 to 62 scalars spill
     int workgroup = blockIdx.x;
     uintptr_t args = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(workgroup), "+s"(args));

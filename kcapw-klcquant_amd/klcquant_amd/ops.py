@@ -704,7 +704,8 @@ def chunk_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     one behind the other; they are the last of the ``lengths[s]`` keys (int32 ``[S]``) of the pages ``tables[s]`` (int32
     ``[S, width]``).  A token sees the keys up to itself, or with the plan's window the last ones and the first; other
     arguments as :func:`batch_attention`.  Returns bf16 ``[T, n_heads, D]``, with ``want_lse`` also float32 ``[T,
-    n_heads]``, the logs of the softmax normalisers.  ``lengths`` may have grown since the plan was made, as in a
+    n_heads]``, the logs of the softmax normalisers.  Probabilities are rounded to the pages' type for the product with the
+    values, as :func:`batch_attention`'s, and to no fewer than 32 bits for those logs.  ``lengths`` may have grown since the plan was made, as in a
     captured step that is replayed; the counts are the plan's."""
     dev, stride, n_pages, page, width = _check_plan(q, k_pages, v_pages, tables, lengths, plan)
     sink_ptr, _, scale = _check_heads(sinks, plan.n_heads, plan.n_kv, None, scale, plan.head_dim, dev)
@@ -739,7 +740,7 @@ def add_key_weights(q: torch.Tensor, lse: torch.Tensor, k_pages: torch.Tensor, t
                     scale: float | None = None) -> None:
     """Adds to float32 ``weights [R, n_kv, capacity]`` what the new tokens' softmax gives every key of their sequence, summed
     over the tokens and the query heads of each KV head (klc_attn_key_weights); the new tokens' own keys start at the
-    sum.  ``q``, ``lse`` (float32 ``[T, n_heads]``) and the other arguments are :func:`chunk_attention`'s; sequence s has
+    sum.  Of the rows 16 at a time are summed in float32, those sums in float64.  ``q``, ``lse`` (float32 ``[T, n_heads]``) and the other arguments are :func:`chunk_attention`'s; sequence s has
     row ``rows[s]`` (int32 ``[S]``, distinct), and ``capacity`` at least its keys."""
     dev, stride, n_pages, page, width = _check_plan(q, k_pages, k_pages, tables, lengths, plan)
     if not _plain(lse, torch.float32, (plan.tokens, plan.n_heads), dev.index):

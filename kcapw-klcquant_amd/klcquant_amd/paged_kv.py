@@ -286,7 +286,8 @@ class PagedBatch:
     _made: dict = field(default_factory=dict, repr=False)
 
     def sequences(self) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-        """Of each sequence its pages (int32 ``[sequences, pages]``), its keys and its number, on the device."""
+        """Of each sequence its pages (int32 ``[sequences, pages]``), its keys and its number, on the device: what layers by
+        sequences read, and captured ones read again at every replay."""
         def make():
             if self.positions.is_cuda and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("a batch's arrays cannot be copied while a graph is captured: call sequences() and plan() before")
@@ -402,7 +403,9 @@ class PagedKVCache:
     def evict(self, seqs, keep: int, recent: int = 0, first: int = 0) -> list[int]:
         """Cuts those of ``seqs`` with more than ``keep`` keys to as many, in every layer and KV head by itself: the
         ``first`` and the last ``recent`` ones stay, and of the others those of the largest weights (ops.evict_keys).
-        Returns the sequences that were cut.  New tokens go on at their positions in the whole text.  A window counts
+        Returns the sequences that were cut.  Pages of the kept part that others hold too are copied first, to free ones:
+        RuntimeError, and nothing done, where there are too few of them, though the cut itself might free others (its keys
+        move within the pages, which are read to its end).  New tokens go on at their positions in the whole text.  A window counts
         keys that are held: layers with one need ``recent`` of at least it.  What layers see beside one are the keys at the
         start: a ``first`` below their ``first_tokens`` is refused, and so is such a layer on a sequence that was cut with
         one before.  Batches made before are void."""
@@ -493,8 +496,9 @@ class BatchedAttention:
         """Whether a batch with tokens behind cached ones goes by sequences rather than row by row: if any has several.
         Short suffixes behind a long prefix that all share do better by rows, for which it is read once (64 heads over
         8 of size 64, us by rows and by sequences: 64 behind 8,192 tokens 2 each 49 and 85, 8 each 159 and 126; 8 behind
-        8,192 2 each 18 and 26; 200 behind 1,000 2 each 38 and 42; 66 behind 960 2 each 23 and 20), and a captured graph,
-        which may be replayed with other ``tables`` and ``lengths`` of the rows, keeps to them."""
+        8,192 2 each 18 and 26; 200 behind 1,000 2 each 38 and 42).  The prefix's length itself is no part of the rule,
+        which costs a few us where it is short and the sequences are few (66 behind 960 2 each 23 and 20).  A captured
+        graph, which may be replayed with other ``tables`` and ``lengths`` of the rows, keeps to them."""
         count = batch.starts.shape[0] - 1
         if batch.tokens == count or not batch.host or torch.cuda.is_current_stream_capturing():
             return False
