@@ -299,6 +299,8 @@ class PagedBatch:
         """The division of its tokens' attention over the cache, for all layers with this window; without ``key_weights``
         for those of a cache that keeps none."""
         key = (config.num_heads, config.num_kv_heads, config.head_dim, window, first, key_weights)
+        if not key_weights and (*key[:5], True) in self._made:  # made for more: as good
+            key = (*key[:5], True)
 
         def make():
             made = ops.attention_plan(self.host["counts"], self.host["keys"], *key[:5], self.positions.device, key_weights)

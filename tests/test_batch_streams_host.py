@@ -61,6 +61,14 @@ def test_other_streams_wait_for_what_the_first_layer_made(notes):
     assert b.plan(CONFIG, 16, 0) is windowed and ("wait", 0, "event of 7") in notes.log
 
 
+def test_a_plan_with_key_weights_does_without_them_too(notes):
+    b = batch()
+    both = b.plan(CONFIG, 16, 4)  # as a caller makes it before a capture
+    assert b.plan(CONFIG, 16, 4, False) is both is b.plan(CONFIG, 16, 4, True)
+    bare = b.plan(CONFIG, None, 0, False)
+    assert b.plan(CONFIG, None, 0) is not bare
+
+
 def test_a_batch_that_cannot_be_planned_stores_nothing(notes, monkeypatch):
     cache = paged_kv.PagedKVCache("cpu", 1, 2, 64, 40, 16, weighted=(2, 200))
     appended = []
