@@ -56,7 +56,7 @@ def test_other_streams_wait_for_what_the_first_layer_made(notes):
     assert b.plan(CONFIG, None, 0) is plan and notes.log == [("wait", 7, "event of 0"), ("uses", 7, "plan None")]
     del notes.log[:]
     windowed = b.plan(CONFIG, 16, 0)  # made on this one
-    assert notes.log == [("record", 7)] and windowed is not plan and b.plan(CONFIG, 16, 0, False) is not windowed
+    assert notes.log == [("record", 7)] and windowed is not plan and b.plan(CONFIG, 16, 0, False) is windowed
     notes.now = 0
     assert b.plan(CONFIG, 16, 0) is windowed and ("wait", 0, "event of 7") in notes.log
 
