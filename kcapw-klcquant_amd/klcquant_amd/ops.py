@@ -656,7 +656,7 @@ def attention_plan(counts, lengths, n_heads: int, n_kv: int, head_dim: int, wind
 
     room = 64 * (counts.size + 64)  # mostly enough: what does not fit is planned once more
     if key_weights:
-        room += 8 * (int(lengths.sum(dtype=np.int64) >> 8) + counts.size + 1024)
+        room += 8 * min(int(lengths.sum(dtype=np.int64) >> 8) + counts.size + 1024, 1 << 18)
     while True:
         host = torch.empty(room, dtype=torch.int32, pin_memory=True)
         checked("klc_attn_plan", lib.klc_attn_plan(counts.ctypes.data, lengths.ctypes.data, *shape, window, first, host.data_ptr(),

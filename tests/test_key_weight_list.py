@@ -165,6 +165,10 @@ def test_refusals():
                    dict(heads=7), dict(kv=0), dict(heads=8192), dict(window=-1), dict(window=1 << 30), dict(first=1),
                    dict(window=4, first=-1), dict(window=4, first=1 << 29)):
         refused(**change)
+    refused(heads=4096, kv=1, n_seq=1)  # not this plan's sequences
+    keep, plan[0] = plan[0], 1
+    refused()
+    plan[0] = keep
     for bad in ([2, 9000], [5000, 0], [5000, -1], [1 << 29, 9000]):
         lengths[:] = bad
         refused()
