@@ -106,3 +106,45 @@ def test_a_plan_without_key_weights(gpu):
     assert torch.equal(ops.chunk_attention(c.q, c.k, c.v, c.table, c.lengths, plan), c.run())
     with pytest.raises(ValueError, match="key_weights"):
         ops.add_key_weights(c.q, lse, c.k, c.table, c.lengths, plan, torch.zeros((1, 2, 128), device=gpu), int32([0], gpu))
+
+
+@pytest.mark.parametrize("window,first", [(None, 0), (100, 4)])
+def test_captured_and_replayed_over_many_blocks(gpu, window, first):
+    """A graph whose sequences grow past the blocks of keys that its list was made for: as a list made for each length."""
+    counts, keys = [1, 300], [2400, 2600]
+    c = Case(gpu, "fp16", 16, 4, 64, 64, counts, keys, window, first)
+    rows = int32([1, 0], gpu)
+    lengths = [[200 + 700 * i, 310 + 700 * i] for i in range(4)]
+    weights = torch.zeros((2, 4, 2688), device=gpu)
+    c.lengths.copy_(int32(lengths[0], gpu))
+    plan = ops.attention_plan(counts, lengths[0], 16, 4, 64, window, first)
+    _, lse = ops.chunk_attention(c.q, c.k, c.v, c.table, c.lengths, plan, want_lse=True)
+    ops.add_key_weights(c.q, lse, c.k, c.table, c.lengths, plan, weights, rows)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _, lse = ops.chunk_attention(c.q, c.k, c.v, c.table, c.lengths, plan, want_lse=True)
+        ops.add_key_weights(c.q, lse, c.k, c.table, c.lengths, plan, weights, rows)
+    for now in (lengths[1], lengths[3], lengths[0], lengths[2]):
+        c.lengths.copy_(int32(now, gpu))
+        weights.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = weights.clone()
+        again = ops.attention_plan(counts, now, 16, 4, 64, window, first)
+        want, norm = torch.zeros_like(weights), ops.chunk_attention(c.q, c.k, c.v, c.table, c.lengths, again, want_lse=True)[1]
+        ops.add_key_weights(c.q, norm, c.k, c.table, c.lengths, again, want, rows)
+        # the logs by other parts of the keys, 2^-20 of each weight, and sums of the same float32 sums in float64
+        assert torch.isfinite(got).all() and got.any() and torch.allclose(got, want, rtol=1e-5, atol=1e-30)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("factor", [2.0 ** 60, 2.0 ** -60])
+def test_queries_of_all_sizes(gpu, dtype, factor):
+    """A power of two more in the queries and less in the scale changes no bit of the weights."""
+    c = Case(gpu, dtype, 8, 2, 64, 16, [3, 40], [50, 390])
+    _, lse = c.run(want_lse=True)
+    rows, weights = int32([0, 1], gpu), torch.zeros((2, 2, 2, 400), device=gpu)
+    ops.add_key_weights(c.q, lse, c.k, c.table, c.lengths, c.plan, weights[0], rows)
+    ops.add_key_weights(c.q * factor, lse, c.k, c.table, c.lengths, c.plan, weights[1], rows, scale=c.scale / factor)
+    assert weights[0].any() and torch.equal(weights[0], weights[1])
