@@ -373,8 +373,9 @@ extern "C" int klc_attn_weight_list(const int32_t* plan, const int64_t* sizes, c
               KLC_ERR_ARGUMENT, "klc_attn_weight_list: %lld sequences, heads %lld / %lld, window %lld, %lld first tokens",
               (long long)n_seq, (long long)n_heads, (long long)n_kv, (long long)window, (long long)first);
   const int64_t at = sizes[8], records = sizes[9], g = n_heads / n_kv;
-  KLC_REQUIRE(plan[0] == 0 && plan[n_seq] == sizes[1] && sizes[1] * g < ((int64_t)1 << 30) && records >= n_seq && at > n_seq && at + records * kPartRecord == sizes[0], KLC_ERR_ARGUMENT,
-              "klc_attn_weight_list: not a plan of %lld sequences", (long long)n_seq);
+  KLC_REQUIRE(plan[0] == 0 && plan[n_seq] == sizes[1] && sizes[1] * g < ((int64_t)1 << 30) && records >= n_seq && at > n_seq &&
+                  at + records * kPartRecord == sizes[0],
+              KLC_ERR_ARGUMENT, "klc_attn_weight_list: not a plan of %lld sequences", (long long)n_seq);
   for (int64_t s = 0; s < n_seq; ++s)
     KLC_REQUIRE(plan[s + 1] > plan[s] && lengths[s] >= plan[s + 1] - plan[s] && lengths[s] < (1 << 29), KLC_ERR_ARGUMENT,
                 "klc_attn_weight_list: sequence %lld of %d new tokens among %d (at least one, below 2^29)", (long long)s,

@@ -617,13 +617,14 @@ class AttentionPlan:
 
 
 def attention_plan(counts, lengths, n_heads: int, n_kv: int, head_dim: int, window: int | None = None, first: int = 0,
-                   device: torch.device | str = "cuda", key_weights: bool = True) -> AttentionPlan:
+                   device: torch.device | str = "cuda", key_weights: bool | None = None) -> AttentionPlan:
     """The plan of a batch (klc_attn_plan) for :func:`chunk_attention` and :func:`add_key_weights`, on the host from the
     sequences' ``counts`` of new tokens and ``lengths``, the keys up to and with them (sequences of whole numbers; one
     copy to ``device``, on its current stream: calls on other streams have to wait for it).  Made once for all layers of
-    a kind: ``window`` and ``first`` (tokens at the start that stay visible beside it) are the layers'.  Without
-    ``key_weights`` it is for :func:`chunk_attention` alone.  For a captured step whose sequences grow between replays it
-    is best made with the longest ``lengths`` that they will have."""
+    a kind: ``window`` and ``first`` (tokens at the start that stay visible beside it) are the layers'.  With ``key_weights``
+    False it is for :func:`chunk_attention` alone, and with None if the keys are too many for the other (True: ValueError
+    then).  For a captured step whose sequences grow between replays it is best made with the longest ``lengths`` that they
+    will have."""
     counts, lengths = (np.asarray(x) for x in (counts, lengths))
     if counts.ndim != 1 or counts.shape != lengths.shape or counts.size == 0:
         raise ValueError(f"counts and lengths must be one number a sequence, got shapes {counts.shape} and {lengths.shape}")
@@ -655,23 +656,29 @@ def attention_plan(counts, lengths, n_heads: int, n_kv: int, head_dim: int, wind
             raise nat.KlcError(name, int(rc), nat.last_error())
 
     room = 64 * (counts.size + 64)  # mostly enough: what does not fit is planned once more
-    if key_weights:
+    if key_weights is not False:
         room += 8 * min(int(lengths.sum(dtype=np.int64) >> 8) + counts.size + 1024, 1 << 18)
     while True:
         host = torch.empty(room, dtype=torch.int32, pin_memory=True)
         checked("klc_attn_plan", lib.klc_attn_plan(counts.ctypes.data, lengths.ctypes.data, *shape, window, first, host.data_ptr(),
                                                    room, sizes.ctypes.data))
         end = int(sizes[0])
-        at_list = end // 8 * 8 + (4 if end % 8 <= 4 else 12) if key_weights else None
-        if key_weights and at_list <= room:
-            checked("klc_attn_weight_list",
-                    lib.klc_attn_weight_list(host.data_ptr(), sizes.ctypes.data, lengths.ctypes.data, *shape[:3], window, first,
-                                             host.data_ptr() + 4 * at_list, room - at_list, list_sizes.ctypes.data))
-        if key_weights:
-            end = at_list + int(list_sizes[0])
-        if end <= room and (not key_weights or list_sizes[0]):
+        at_list = None
+        if key_weights is not False:
+            at_list = end // 8 * 8 + (4 if end % 8 <= 4 else 12)  # four values behind a multiple of 8
+            if at_list > room:
+                room = 2 * at_list
+                continue
+            rc = lib.klc_attn_weight_list(host.data_ptr(), sizes.ctypes.data, lengths.ctypes.data, *shape[:3], window, first,
+                                          host.data_ptr() + 4 * at_list, room - at_list, list_sizes.ctypes.data)
+            if rc == nat.KLC_ERR_ARGUMENT and key_weights is None:
+                at_list = None
+            else:
+                checked("klc_attn_weight_list", rc)
+                end = at_list + int(list_sizes[0])
+        if end <= room:
             break
-        room = 2 * end
+        room = end
     data = host[:end].to(device, non_blocking=True)
     return AttentionPlan(data, sizes, shape, window, first, at_list, list_sizes)
 
@@ -705,8 +712,8 @@ def chunk_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``[S, width]``).  A token sees the keys up to itself, or with the plan's window the last ones and the first; other
     arguments as :func:`batch_attention`.  Returns bf16 ``[T, n_heads, D]``, with ``want_lse`` also float32 ``[T,
     n_heads]``, the logs of the softmax normalisers.  Probabilities are rounded to the pages' type for the product with the
-    values, as :func:`batch_attention`'s, and to no fewer than 32 bits for those logs.  ``lengths`` may have grown since the plan was made, as in a
-    captured step that is replayed; the counts are the plan's."""
+    values, as :func:`batch_attention`'s; for those logs they are float32.  ``lengths`` may have grown since the plan was
+    made, as in a captured step that is replayed; the counts are the plan's."""
     dev, stride, n_pages, page, width = _check_plan(q, k_pages, v_pages, tables, lengths, plan)
     sink_ptr, _, scale = _check_heads(sinks, plan.n_heads, plan.n_kv, None, scale, plan.head_dim, dev)
     out = _result("out", out, q, dev)
@@ -740,8 +747,9 @@ def add_key_weights(q: torch.Tensor, lse: torch.Tensor, k_pages: torch.Tensor, t
                     scale: float | None = None) -> None:
     """Adds to float32 ``weights [R, n_kv, capacity]`` what the new tokens' softmax gives every key of their sequence, summed
     over the tokens and the query heads of each KV head (klc_attn_key_weights); the new tokens' own keys start at the
-    sum.  Of the rows 16 at a time are summed in float32, those sums in float64.  ``q``, ``lse`` (float32 ``[T, n_heads]``) and the other arguments are :func:`chunk_attention`'s; sequence s has
-    row ``rows[s]`` (int32 ``[S]``, distinct), and ``capacity`` at least its keys."""
+    sum.  Of the rows 16 at a time are summed in float32, those sums in float64.  ``q``, ``lse`` (float32 ``[T,
+    n_heads]``) and the other arguments are :func:`chunk_attention`'s; sequence s has row ``rows[s]`` (int32 ``[S]``,
+    distinct), and ``capacity`` at least its keys."""
     dev, stride, n_pages, page, width = _check_plan(q, k_pages, k_pages, tables, lengths, plan)
     if not _plain(lse, torch.float32, (plan.tokens, plan.n_heads), dev.index):
         _check_gpu("lse", lse, torch.float32, 2)
@@ -752,7 +760,7 @@ def add_key_weights(q: torch.Tensor, lse: torch.Tensor, k_pages: torch.Tensor, t
         raise ValueError(f"weights of {n_kv} KV heads for {plan.n_kv}")
     _, _, scale = _check_heads(None, plan.n_heads, n_kv, None, scale, plan.head_dim, dev)
     if plan.at_list is None:
-        raise ValueError("a plan without key weights: make it with key_weights=True")
+        raise ValueError("a plan without key weights: key_weights=False, or too many keys for them")
     nbytes = 2048 * plan.list_parts * n_kv
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None  # of this call alone
     _call("klc_attn_key_weights",

@@ -146,8 +146,8 @@ class PageTable:
         batch of these tokens, sequence by sequence: ``positions`` and ``slots`` of the tokens, ``starts`` of the
         sequences' runs, ``prefix`` (full pages that all share, in front), and for every token the pages behind them
         (``tables``) and the tokens in those up to itself (``lengths``).  ``fresh``: no sequence had tokens, and what
-        tells of earlier ones is empty.  Of the sequences: ``seqs``, ``counts``, ``keys`` with the new ones, ``pages`` and ``firsts``, the
-        tokens at their starts that evictions have left in place."""
+        tells of earlier ones is empty.  Of the sequences: ``seqs``, ``counts``, ``keys`` with the new
+        ones, ``pages`` and ``firsts``, the tokens at their starts that evictions have left in place."""
         at = self._check(seqs)
         counts = np.broadcast_to(np.asarray(counts), at.shape)
         if counts.dtype.kind not in "iu" or (counts <= 0).any():
@@ -407,10 +407,10 @@ class PagedKVCache:
         ``first`` and the last ``recent`` ones stay, and of the others those of the largest weights (ops.evict_keys).
         Returns the sequences that were cut.  Pages of the kept part that others hold too are copied first, to free ones:
         RuntimeError, and nothing done, where there are too few of them, though the cut itself might free others (its keys
-        move within the pages, which are read to its end).  New tokens go on at their positions in the whole text.  A window counts
-        keys that are held: layers with one need ``recent`` of at least it.  What layers see beside one are the keys at the
-        start: a ``first`` below their ``first_tokens`` is refused, and so is such a layer on a sequence that was cut with
-        one before.  Batches made before are void."""
+        move within the pages, which are read to its end).  New tokens go on at their positions in the whole text.  A
+        window counts keys that are held: layers with one need ``recent`` of at least it.  What layers see beside one are
+        the keys at the start: a ``first`` below their ``first_tokens`` is refused, and so is such a layer on a sequence
+        that was cut with one before.  Batches made before are void."""
         if self.weights is None:
             raise ValueError("a cache without weights: give `weighted` when it is made")
         keep, recent, first = operator.index(keep), operator.index(recent), operator.index(first)

@@ -18,5 +18,10 @@ def test_long_sequences(monkeypatch):
     monkeypatch.setattr(torch, "empty", noted)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     with pytest.raises(ValueError, match="too many"):  # 2^29 keys of each of 64 sequences: 134 million blocks
-        ops.attention_plan([1] * 64, [(1 << 29) - 1] * 64, 8, 8, 64)
+        ops.attention_plan([1] * 64, [(1 << 29) - 1] * 64, 8, 8, 64, key_weights=True)
     assert asked and max(asked) <= 1 << 23
+    monkeypatch.setattr(torch.Tensor, "to", lambda t, *x, **kw: t)
+    for key_weights in (None, False):  # attention alone
+        plan = ops.attention_plan([1] * 64, [(1 << 29) - 1] * 64, 8, 8, 64, key_weights=key_weights)
+        assert plan.at_list is None and plan.items >= 64
+    assert ops.attention_plan([1] * 64, [100000] * 64, 8, 8, 64).list_items == 64 * 391
