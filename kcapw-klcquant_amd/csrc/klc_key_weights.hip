@@ -421,11 +421,14 @@ extern "C" int klc_attn_weight_list(const int32_t* plan, const int64_t* sizes, c
     list_sizes[1] = items, list_sizes[2] = joins, list_sizes[3] = parts_held;
     if (list_sizes[0] > capacity) return KLC_OK;
     for (int64_t s = 0, sum = 0; s < n_seq; ++s) sum += std::exchange(scratch[s], sum);
-    // the first parts of joined blocks, which the second launch takes too, their other parts, and what is not joined
+    // Each sequence's blocks begin one further on, or where blocks and CUs agree in number one CU would have the same block
+    // of all of them (64 steps of 1,000 to 2,000 keys listed for 2,048: 26.4 us instead of 29.2).  In order: the first
+    // parts of joined blocks, which the second launch takes too, their other parts, and what is not joined.
     int32_t *first_parts = list, *other_parts = first_parts + joins * kListRecord, *whole = other_parts + others * kListRecord;
     walk([&](const int32_t* rec, bool head, int64_t blocks, int parts, int64_t place) {
       int32_t*& to = parts == 1 ? whole : rec[1] == 0 ? first_parts : other_parts;
-      for (int64_t b = 0; b < blocks; ++b) {
+      for (int64_t i = 0; i < blocks; ++i) {
+        const int64_t b = (i + rec[0]) % blocks;
         const int32_t item[kListRecord] = {rec[0], rec[1], parts, ListPlace::of(head, b == blocks - 1, b),
                                            parts == 1 ? 0 : (int32_t)(place + b * parts + rec[1]), plan[rec[0]],
                                            plan[rec[0] + 1] - plan[rec[0]], least};
