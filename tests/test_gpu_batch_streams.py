@@ -55,3 +55,38 @@ def test_a_layer_beside_the_first(gpu, weighted):
         got = run(True)
         assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(got, want))
     assert math.isfinite(float(cache.pool.float().sum()))
+
+
+def test_a_step_captured_without_a_run(gpu):
+    """A weighted cache's step, captured once its arrays and plans are made and never run before: each replay adds its
+    tokens' weights once, as eager steps of a twin do."""
+    from test_gpu_long_conversations import WINDOWS, Run
+
+    runs = [Run(gpu, "fp16", 64, 12, first_tokens=3) for _ in range(2)]
+    for run in runs:
+        run.generator.manual_seed(1)
+        assert [run.add(), run.add()] == [0, 1]
+        run.extend([0, 1], [70, 66])
+    run, twin = runs
+    batch, other = run.cache.extend([0, 1]), twin.cache.extend([0, 1])
+    hidden = torch.randn((2, run.config.hidden_size), device=gpu).bfloat16()
+    batch.sequences()
+    for window in WINDOWS:
+        batch.plan(run.config, window, 3 if window else 0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = [run.layer.forward(i, hidden, run.tensors, batch, run.cache, WINDOWS[i]) for i in range(2)]
+    for step in range(4):
+        if step:
+            new, other = run.cache.extend([0, 1]), twin.cache.extend([0, 1])
+            for name in ("positions", "slots"):
+                getattr(batch, name).copy_(getattr(new, name))
+            for mine, theirs in zip(batch.sequences(), new.sequences()):
+                mine.copy_(theirs)
+            hidden.copy_(torch.randn_like(hidden))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = [twin.layer.forward(i, hidden, twin.tensors, other, twin.cache, WINDOWS[i]) for i in range(2)]
+        assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(outs, want))
+        assert torch.equal(run.cache.weights.nan_to_num(nan=-1.0), twin.cache.weights.nan_to_num(nan=-1.0))
